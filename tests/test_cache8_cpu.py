@@ -1,0 +1,110 @@
+"""What the 8-bit cache's entry points refuse, before anything is launched (no GPU), and the plain forms' own arithmetic."""
+import math
+
+import pytest
+import torch
+
+from plain import cache8_plain as plain
+
+from turboquant_cpp_b200.kernels import KernelError, cache8
+
+H, G, D, PAGE = 4, 2, 32, 64
+
+
+def _i(values):
+    return torch.tensor(values, dtype=torch.int32)
+
+
+def _state(**other):
+    codes, scales, weights = cache8.storage(3, G, PAGE, D, "cpu", weights=True)
+    s = dict(codes=codes, scales=scales, weights=weights, table=_i([[0, 1]]), cu=_i([0, 2]), held=_i([5]), qkv=torch.zeros(2, (H + 2 * G) * D),
+             q=torch.zeros(2, H, D), out=torch.zeros(2, H * D), cos=torch.zeros(9, D // 2), sin=torch.zeros(9, D // 2), bias=None, positions=_i([5, 6]),
+             new_table=_i([[2]]), lengths=_i([70]), budget=32, recent=4, page=PAGE, hd=D, window=0)
+    s.update(other)
+    return s
+
+
+def _write(s):
+    cache8.write_rows8(s["qkv"], s["bias"], s["cos"], s["sin"], "half", s["positions"], s["cu"], s["held"], s["table"], s["page"], s["q"], s["codes"], s["scales"],
+                       H, G, s["hd"], 2)
+
+
+def _attend(s):
+    cache8.attention8(s["q"], s["codes"], s["scales"], s["cu"], s["held"], s["table"], s["page"], s["window"], 0.1, s["out"], H, G, s["hd"], 2, 7, weights=s["weights"])
+
+
+def _evict(s):
+    cache8.evict8(s["codes"], s["scales"], s["weights"], s["lengths"], s["table"], s["new_table"], s["page"], s["budget"], s["recent"])
+
+
+BAD_CACHE = [dict(codes=torch.zeros(3, 2, G, PAGE, D)), dict(codes=torch.zeros(3, 2, G, 48, D, dtype=torch.uint8).view(torch.float8_e4m3fn)),
+             dict(scales=torch.zeros(3, 2, G, 4)), dict(scales=torch.zeros(3, 2, G, 8, dtype=torch.uint8)), dict(table=_i([0, 1])),
+             dict(table=torch.zeros(1, 2, dtype=torch.int64))]
+
+
+@pytest.mark.parametrize("call", [_write, _attend, _evict])
+@pytest.mark.parametrize("bad", range(len(BAD_CACHE)))
+def test_a_cache_of_other_shapes_is_refused(call, bad):
+    with pytest.raises(KernelError):
+        call(_state(**BAD_CACHE[bad]))
+
+
+@pytest.mark.parametrize("bad", [dict(cu=_i([0, 1, 2])), dict(held=_i([5, 5])), dict(held=torch.tensor([5])), dict(cu=torch.tensor([0, 2])), dict(positions=_i([5])),
+                                 dict(positions=torch.tensor([5, 6])), dict(q=torch.zeros(2, H, D, dtype=torch.bfloat16)), dict(q=torch.zeros(1, H, D)), dict(sin=None),
+                                 dict(cos=torch.zeros(9, D)), dict(cos=torch.zeros(9, D // 2, dtype=torch.float64)), dict(bias=torch.zeros(D)),
+                                 dict(qkv=torch.zeros(2, (H + G) * D))])
+def test_steps_that_do_not_fit_are_not_written(bad):
+    with pytest.raises(KernelError):
+        _write(_state(**bad))
+
+
+@pytest.mark.parametrize("bad", [dict(cu=_i([0, 1, 2])), dict(held=_i([5, 5])), dict(held=torch.tensor([5])), dict(out=torch.zeros(2, H * D, dtype=torch.bfloat16)),
+                                 dict(out=torch.zeros(2, D)), dict(q=torch.zeros(2, H, 16)), dict(weights=torch.zeros(3, G, PAGE, dtype=torch.float64)),
+                                 dict(weights=torch.zeros(3, H, PAGE))])
+def test_steps_that_do_not_fit_are_not_attended(bad):
+    with pytest.raises(KernelError):
+        _attend(_state(**bad))
+
+
+@pytest.mark.parametrize("bad", [dict(lengths=_i([70, 70])), dict(lengths=torch.tensor([70])), dict(new_table=_i([2])), dict(new_table=_i([[2], [1]])), dict(budget=65),
+                                 dict(budget=0, recent=0), dict(recent=33), dict(recent=-1), dict(new_table=torch.tensor([[2]]))])
+def test_evictions_that_do_not_fit_are_refused(bad):
+    with pytest.raises(KernelError):
+        _evict(_state(**bad))
+
+
+@pytest.mark.parametrize("call", [_write, _attend, _evict])
+def test_there_is_no_cpu_path(call):
+    with pytest.raises(KernelError):
+        call(_state())
+
+
+@pytest.mark.parametrize("page_size,head_dim", [(64, 24), (64, 272), (64, 0), (8, 64), (40, 64)])
+def test_sizes_the_cache_does_not_take(page_size, head_dim):
+    with pytest.raises(KernelError):
+        cache8.storage(2, 1, page_size, head_dim, "cpu")
+
+
+@pytest.mark.parametrize("top,b", [(0.0, 1), (448.0, 127), (448.5, 128), (896.0, 128), (1.0, 119), (3.4e38, 247), (1e-45, 1), (2.0 ** -126 * 448, 1), (2.0 ** -125 * 448, 2)])
+def test_the_byte_is_the_smallest_that_holds_the_largest_magnitude(top, b):
+    top = float(torch.tensor(top))
+    assert plain.byte_of(top) == b
+    assert top <= 448 * 2.0 ** (b - 127) and (b == 1 or top > 448 * 2.0 ** (b - 128))
+
+
+def test_plain_codes_round_to_the_nearest():
+    x = torch.linspace(-448, 448, 4001)
+    got = plain.encode(x, 127).view(torch.float8_e4m3fn).double()
+    every = torch.arange(256, dtype=torch.uint8).view(torch.float8_e4m3fn).double()
+    every = every[torch.isfinite(every)]
+    best = (x.double()[:, None] - every).abs().amin(1)
+    assert torch.equal((x.double() - got).abs(), best)
+    assert plain.encode(torch.tensor([math.inf, -math.inf, math.nan]), 127).tolist() == [0x7f] * 3
+
+
+def test_plain_choice_of_rows():
+    nan = math.nan
+    assert plain.kept_places([1.0, 3.0, 2.0, 0.0], 2, 1) == [1, 3]
+    assert plain.kept_places([1.0, 1.0, 1.0, 0.0], 3, 1) == [0, 1, 3]
+    assert plain.kept_places([nan, 0.0, nan, -1.0], 2, 0) == [1, 3]
+    assert plain.kept_places([5.0, 1.0], 4, 1) == [0, 1]

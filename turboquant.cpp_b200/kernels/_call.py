@@ -57,6 +57,13 @@ def check(lib_name: str, rc: int, kernels: int = 1) -> None:
         raise KernelError(lib.tq_last_error().decode("utf-8", "replace") or f"{lib_name}: error {rc}")
 
 
+def on_current_device(*tensors: Optional[torch.Tensor]) -> None:
+    """Launches go to the current device's stream: tensors of another GPU are refused instead of read from there."""
+    used = {t.get_device() for t in tensors if t is not None and t.is_cuda}
+    if used and used != {_raw_device() if _raw_device is not None else torch.cuda.current_device()}:
+        raise KernelError(f"tensors lie on GPU {', '.join(map(str, sorted(used)))}, the current device is {torch.cuda.current_device()}")
+
+
 def ints(*values) -> map:
     """Whole numbers of any integer type (numpy's among them) as the plain ints that ctypes passes on without a declaration."""
     return map(index, values)
