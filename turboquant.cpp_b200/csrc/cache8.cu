@@ -1,15 +1,11 @@
-// The 8-bit key/value cache: a step's rows into its pages, and attention over them (layout and codes: cache8.cuh).
+// The 8-bit key/value cache: a step's rows into its pages (layout and codes: cache8.cuh).
 //
-//   tq_write8       bias + rotary encoding on the fused projection; queries to a buffer, keys and values as codes into the pages
-//   tq_attention8   softmax(scale q.K) V over the cache, causal, with an optional window; the log2 of each row's denominator on the side
-//   tq_weigh8       the softmax weights that every cached row received, added up over a step's rows and a key/value head's query heads
+//   tq_write8   bias + rotary encoding on the fused projection; queries to a buffer, keys and values as codes into the pages
 #include "cache8.cuh"
 
 TQ_DEFINE_LAST_ERROR
 
 namespace {
-
-constexpr float LOG2E = 1.4426950408889634f;
 
 // eight consecutive elements as float32
 __device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&f)[8]) {
@@ -170,85 +166,6 @@ __global__ void __launch_bounds__(256) write8_kernel(const TA* __restrict__ qkv,
     if (lane == 0) *byte = (uint8_t)b;
 }
 
-// ---------------------------------------------------------------------------------------
-// Attention, the plain way: a block per (row, query head), its warps share the keys, a lane holds every 32nd element.
-// ---------------------------------------------------------------------------------------
-template <typename TA>
-__global__ void __launch_bounds__(128) attention8_kernel(const TA* __restrict__ q, Cache8 c, const int* __restrict__ cu_seqlens, const int* __restrict__ held,
-                                                         int window, float scale, TA* __restrict__ out, float* __restrict__ lse, int nh) {
-    tq_grid_wait();                    // everything below may read what the previous kernel wrote
-    tq_grid_launch_dependents();
-    constexpr int E = C8_MAX_HEAD_DIM / 32;
-    __shared__ float s_o[4][C8_MAX_HEAD_DIM], s_m[4], s_l[4];
-    const int seq = blockIdx.z, r = blockIdx.x, h = blockIdx.y, t_begin = cu_seqlens[seq];
-    if (r >= cu_seqlens[seq + 1] - t_begin) return;
-    const int t = t_begin + r, place = held[seq] + r, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, hd = c.hd, g = h / (nh / c.nkv);
-    float qv[E], o[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-        qv[e] = lane + 32 * e < hd ? tq_to_float(q[((size_t)t * nh + h) * hd + lane + 32 * e]) * (scale * LOG2E) : 0.f;
-        o[e] = 0.f;
-    }
-    float m = -INFINITY, l = 0.f;
-    for (int p = (window > 0 ? max(0, place + 1 - window) : 0) + warp; p <= place; p += 4) {
-        const int page = c.page_of(seq, p), row = p % c.page_size;
-        const uint8_t* k = c.codes + c.codes_at(page, 0, g) + (size_t)row * hd;
-        const uint8_t* v = c.codes + c.codes_at(page, 1, g) + (size_t)row * hd;
-        float s = 0.f;
-#pragma unroll
-        for (int e = 0; e < E; ++e) if (lane + 32 * e < hd) s += qv[e] * c8_float(k[lane + 32 * e]);
-        s = tq_warp_sum(s) * c8_scale(c.scales[c.scales_at(page, 0, g) + row / C8_BLOCK]);
-        const float mn = fmaxf(m, s), old = m == -INFINITY ? 0.f : exp2f(m - mn), w = exp2f(s - mn), sv = w * c8_scale(c.scales[c.scales_at(page, 1, g) + row / C8_BLOCK]);
-        l = l * old + w;
-#pragma unroll
-        for (int e = 0; e < E; ++e) if (lane + 32 * e < hd) o[e] = o[e] * old + sv * c8_float(v[lane + 32 * e]);
-        m = mn;
-    }
-#pragma unroll
-    for (int e = 0; e < E; ++e) s_o[warp][lane + 32 * e] = o[e];
-    if (lane == 0) { s_m[warp] = m; s_l[warp] = l; }
-    __syncthreads();
-    const float M = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
-    float f[4], L = 0.f;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) { f[w] = s_m[w] == -INFINITY ? 0.f : exp2f(s_m[w] - M); L += f[w] * s_l[w]; }
-    for (int d = threadIdx.x; d < hd; d += blockDim.x)
-        out[((size_t)t * nh + h) * hd + d] = tq_from_float<TA>((s_o[0][d] * f[0] + s_o[1][d] * f[1] + s_o[2][d] * f[2] + s_o[3][d] * f[3]) / L);
-    if (lse != nullptr && threadIdx.x == 0) lse[(size_t)t * nh + h] = M + log2f(L);
-}
-
-// Sums of weights, the plain way: a warp per cached row of a key/value head, which walks the step's rows that see it.  One writer per
-// sum and a fixed order: the same bits every time.
-template <typename TA>
-__global__ void __launch_bounds__(128) weigh8_kernel(const TA* __restrict__ q, Cache8 c, const int* __restrict__ cu_seqlens, const int* __restrict__ held,
-                                                     int window, float scale, const float* __restrict__ lse, float* __restrict__ weights, int nh) {
-    tq_grid_wait();                    // everything below may read what the previous kernel wrote
-    tq_grid_launch_dependents();
-    constexpr int E = C8_MAX_HEAD_DIM / 32;
-    const int seq = blockIdx.z, g = blockIdx.y, lane = threadIdx.x & 31, hd = c.hd, per = nh / c.nkv;
-    const int p = blockIdx.x * 4 + (threadIdx.x >> 5), t_begin = cu_seqlens[seq], run = cu_seqlens[seq + 1] - t_begin, start = held[seq];
-    if (run <= 0 || p >= start + run || (window > 0 && p + window <= start)) return;     // no row of the step sees it
-    const int page = c.page_of(seq, p), row = p % c.page_size;
-    const uint8_t* k = c.codes + c.codes_at(page, 0, g) + (size_t)row * hd;
-    float kv[E];
-    const float ks = c8_scale(c.scales[c.scales_at(page, 0, g) + row / C8_BLOCK]) * (scale * LOG2E);
-#pragma unroll
-    for (int e = 0; e < E; ++e) kv[e] = lane + 32 * e < hd ? c8_float(k[lane + 32 * e]) : 0.f;
-    float sum = 0.f;
-    for (int r = max(0, p - start); r < run && (window <= 0 || start + r - p < window); ++r)
-        for (int h = g * per; h < (g + 1) * per; ++h) {
-            const size_t at = (size_t)(t_begin + r) * nh + h;
-            float s = 0.f;
-#pragma unroll
-            for (int e = 0; e < E; ++e) if (lane + 32 * e < hd) s += tq_to_float(q[at * hd + lane + 32 * e]) * kv[e];
-            sum += exp2f(tq_warp_sum(s) * ks - lse[at]);
-        }
-    if (lane == 0) {
-        float* w = weights + ((size_t)page * c.nkv + g) * c.page_size + row;
-        *w = (p < start ? *w : 0.f) + sum;
-    }
-}
-
 }  // namespace
 
 // qkv [T, (nh + 2 nkv) * hd]; bias as long as a row, or null; cos and sin [positions, hd / 2] float32, or null; q_out [T, nh, hd].
@@ -272,36 +189,5 @@ TQ_EXPORT int tq_write8(const void* qkv, int act_dtype, const void* bias, int bi
         if (max_q_len == 1) tq_launch(grid, warps * 32, 0, stream)(write8_kernel<TA, TB, 1>, (const TA*)qkv, (const TB*)bias, a, (TA*)q_out, c);
         else tq_launch(grid, warps * 32, 0, stream)(write8_kernel<TA, TB, 4>, (const TA*)qkv, (const TB*)bias, a, (TA*)q_out, c)));
     TQ_CHECK_LAUNCH("write8");
-    return 0;
-}
-
-// q [T, nh, hd], out [T, nh * hd]; place i sees j <= i with window == 0 or i - j < window.  lse [T, nh] float32 or null.
-TQ_EXPORT int tq_attention8(const void* q, const void* codes, const void* scales, int act_dtype, const int* cu_seqlens, const int* held,
-                            const int* page_table, int table_stride, int page_size, int window, float scale, void* out, float* lse, int n_pages,
-                            int n_seqs, int max_q_len, int nh, int nkv, int hd, cudaStream_t stream) {
-    if (n_seqs == 0 || max_q_len == 0) return 0;
-    int rc = c8_check("attention8", codes, scales, page_size, n_pages, nkv, hd, table_stride);
-    if (rc) return rc;
-    TQ_REQUIRE(nh >= 1 && nh % nkv == 0 && nh <= 65535, "attention8: %d heads are not a multiple of %d key/value heads", nh, nkv);
-    TQ_REQUIRE(n_seqs <= 65535 && max_q_len >= 1 && window >= 0, "attention8: %d sequences, longest run %d, window %d", n_seqs, max_q_len, window);
-    const Cache8 c{(uint8_t*)codes, (uint8_t*)scales, page_table, table_stride, page_size, n_pages, nkv, hd};
-    TQ_DISPATCH(act_dtype, TA, tq_launch(dim3(max_q_len, nh, n_seqs), 128, 0, stream)(attention8_kernel<TA>, (const TA*)q, c, cu_seqlens, held, window, scale, (TA*)out, lse, nh));
-    TQ_CHECK_LAUNCH("attention8");
-    return 0;
-}
-
-// weights of places below held[s] grow by, those of the step's own rows become, the sum over the step's rows and the head's query heads of
-// 2^(scale log2(e) q.k - lse).  max_kv_len: at least the longest held[s] + run.
-TQ_EXPORT int tq_weigh8(const void* q, const void* codes, const void* scales, int act_dtype, const int* cu_seqlens, const int* held,
-                        const int* page_table, int table_stride, int page_size, int window, float scale, const float* lse, float* weights, int n_pages,
-                        int n_seqs, int max_kv_len, int nh, int nkv, int hd, cudaStream_t stream) {
-    if (n_seqs == 0 || max_kv_len == 0) return 0;
-    int rc = c8_check("weigh8", codes, scales, page_size, n_pages, nkv, hd, table_stride);
-    if (rc) return rc;
-    TQ_REQUIRE(nh >= 1 && nh % nkv == 0 && nkv <= 65535, "weigh8: %d heads are not a multiple of %d key/value heads", nh, nkv);
-    TQ_REQUIRE(n_seqs <= 65535 && max_kv_len >= 1 && window >= 0, "weigh8: %d sequences, %d places, window %d", n_seqs, max_kv_len, window);
-    const Cache8 c{(uint8_t*)codes, (uint8_t*)scales, page_table, table_stride, page_size, n_pages, nkv, hd};
-    TQ_DISPATCH(act_dtype, TA, tq_launch(dim3((max_kv_len + 3) / 4, nkv, n_seqs), 128, 0, stream)(weigh8_kernel<TA>, (const TA*)q, c, cu_seqlens, held, window, scale, lse, weights, nh));
-    TQ_CHECK_LAUNCH("weigh8");
     return 0;
 }

@@ -1,4 +1,4 @@
-"""A key/value cache in 8 bits whose length can be bounded (csrc/cache8.cu, csrc/evict.cu).
+"""A key/value cache in 8 bits whose length can be bounded (csrc/cache8.cu, csrc/attention8.cu, csrc/evict.cu).
 
 An element is an e4m3 code times 2^(b - 127), b one byte for 16 consecutive rows of a (page, plane, key/value head): the smallest power of
 two, of those from 2^-126 on, under which the largest finite magnitude of the 16 rows is at most 448.  A block that takes rows in
@@ -15,14 +15,14 @@ are int32 on the device; every place a call reads or writes needs its page, and 
 The launches go to the current stream, allocate their scratch from torch's allocator and can be captured into CUDA graphs."""
 from __future__ import annotations
 
-from ctypes import c_float
+from ctypes import c_float, c_void_p
 from typing import Optional, Tuple
 
 import torch
 
 from ..csrc.build import load_kernel
 from ._call import KernelError, check, code, ints, on_current_device, ptr, stream, want_f32, want_int32
-from .attention import PAIRING
+from .attention import PAIRING, resident_ctas
 
 BLOCK = 16
 MAX_HEAD_DIM = 256
@@ -93,6 +93,21 @@ def write_rows8(qkv: torch.Tensor, bias: Optional[torch.Tensor], cos: Optional[t
         codes.shape[0], n, *ints(max_q_len, n_heads, n_kv_heads, head_dim), stream()))
 
 
+def ranges_for(tiles: int, blocks: int, resident: int) -> int:
+    """Ranges the keys of a tile of columns are cut into: as many as fill the CTAs the device runs at once, each of at least two blocks of
+    16 keys for its four warps; with more tiles than that, the count (up to 8) whose last wave is fullest, and one from four waves on."""
+    most = max(1, blocks // 8)
+    if tiles <= resident:
+        return max(1, min(most, resident // tiles))
+    if tiles >= 4 * resident:
+        return 1
+    fill = lambda n: tiles * n / (-(-tiles * n // resident) * resident)
+    return max(range(1, min(8, most) + 1), key=lambda n: (round(fill(n), 2), -n))
+
+
+SCORE_BYTES = 1 << 28        # scratch a decode step may take for scores
+
+
 def attention8(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, cu_seqlens: torch.Tensor, held: torch.Tensor,
                page_table: torch.Tensor, page_size: int, window: int, scale: float, out: torch.Tensor, n_heads: int, n_kv_heads: int,
                head_dim: int, max_q_len: int, max_kv_len: int, weights: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -106,18 +121,33 @@ def attention8(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, cu_se
     n = _check_step(cu_seqlens, held, page_table, "attention8")
     if q.numel() != T * n_heads * head_dim or out.numel() != q.numel() or out.dtype != q.dtype:
         raise KernelError(f"attention8: queries {tuple(q.shape)} {q.dtype} and output {tuple(out.shape)} {out.dtype} do not fit {n_heads} heads of {head_dim}")
-    if T == 0:
+    if T == 0 or n == 0 or max_q_len < 1:
         return out
     on_current_device(q, out, codes, scales, weights)
-    lse = torch.empty((T, n_heads), dtype=torch.float32, device=q.device) if weights is not None else None
-    lib = load_kernel("cache8")
-    check("cache8", lib.tq_attention8(
-        ptr(q), ptr(codes), ptr(scales), code(q.dtype), ptr(cu_seqlens), ptr(held), ptr(page_table), page_table.shape[1], *ints(page_size, window),
-        c_float(scale), ptr(out), ptr(lse), codes.shape[0], n, *ints(max_q_len, n_heads, n_kv_heads, head_dim), stream()))
-    if weights is not None:
-        check("cache8", lib.tq_weigh8(
-            ptr(q), ptr(codes), ptr(scales), code(q.dtype), ptr(cu_seqlens), ptr(held), ptr(page_table), page_table.shape[1], *ints(page_size, window),
-            c_float(scale), ptr(lse), ptr(weights), codes.shape[0], n, *ints(max_kv_len, n_heads, n_kv_heads, head_dim), stream()))
+    per = n_heads // n_kv_heads
+    columns = max_q_len * per
+    tiles = -(-columns // (16 if columns > 8 and head_dim <= 128 else 8)) * n_kv_heads * n
+    ranges = ranges_for(tiles, -(-max_kv_len // BLOCK), resident_ctas(q.device) * 3 // 4)
+    # one row a sequence: the first launch leaves its scores for the second one to add up, which moves 8 bytes a key and query head, where
+    # reading the keys again moves head_dim bytes a key
+    stride = -(-max_kv_len // BLOCK) * BLOCK
+    stored = weights is not None and max_q_len == 1 and 8 * per <= head_dim and 4 * T * n_heads * stride <= SCORE_BYTES
+    rows = T * n_heads
+    partial_floats = rows * ranges * (head_dim + 4) if ranges > 1 or stored else 0
+    scratch = torch.empty(partial_floats + (rows * stride if stored else 0) + (rows if weights is not None and not stored else 0), dtype=torch.float32,
+                          device=q.device) if weights is not None or partial_floats else None
+    at = 0 if scratch is None else scratch.data_ptr()
+    partial = at if partial_floats else None
+    rest = at + 4 * partial_floats
+    lib = load_kernel("attention8")
+    args = (ptr(q), ptr(codes), ptr(scales), code(q.dtype), ptr(cu_seqlens), ptr(held), ptr(page_table), page_table.shape[1], *ints(page_size, window), c_float(scale))
+    step = (codes.shape[0], n, *ints(max_q_len))
+    heads = (*ints(n_heads, n_kv_heads, head_dim), stream())
+    check("attention8", lib.tq_attention8(*args, ptr(out), c_void_p(partial), ranges, c_void_p(rest if weights is not None and not stored else None),
+                                          c_void_p(rest if stored else None), stride, ptr(weights) if stored else None, *ints(max_kv_len), *step, *heads),
+          kernels=2 if partial_floats else 1)
+    if weights is not None and not stored:
+        check("attention8", lib.tq_weigh8(*args, c_void_p(rest), ptr(weights), *step, *ints(max_kv_len), *heads))
     return out
 
 
