@@ -343,3 +343,15 @@ def test_a_sequence_from_its_prompt_through_evictions():
             held = budget
             turn += 1
     assert turn >= 2
+
+
+def test_a_small_scratch_takes_the_sequences_in_groups(monkeypatch):
+    from turboquant_cpp_b200.kernels import cache8
+    H, G, D, runs, held = 8, 2, 64, [60, 0, 33, 49, 1], [70, 9, 0, 200, 64]
+    table, pages = _pages([n + h for n, h in zip(runs, held)], 64)
+    codes, scales = _cache(pages, G, 64, D)
+    q = torch.randn(sum(runs), H, D).to(torch.bfloat16)
+    want, want_w = _attend(q, codes, scales, runs, held, table, 64, 0, 0.1, H, G, D, torch.zeros(pages, G, 64))
+    monkeypatch.setattr(cache8, "DENSE_BYTES", 2 * 2 * G * 64 * D * 2 * 4)          # two sequences of four pages
+    got, got_w = _attend(q, codes, scales, runs, held, table, 64, 0, 0.1, H, G, D, torch.zeros(pages, G, 64))
+    assert torch.equal(got, want) and torch.equal(got_w, want_w)

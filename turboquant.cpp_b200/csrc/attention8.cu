@@ -187,18 +187,12 @@ __device__ __forceinline__ int first_seen(int place, int window) { return window
 // lse: null, or [T * nh], log2 of the denominator (where there is no second launch).
 // ---------------------------------------------------------------------------------------
 template <typename TA, int HDP, int NT>
-__global__ void __launch_bounds__(WARPS * 32) attention8_kernel(const TA* __restrict__ q, Cache8 c, Step S, TA* __restrict__ out, float* __restrict__ partial,
-                                                                float* __restrict__ scores, int score_stride, float* __restrict__ lse) {
-    tq_grid_wait();                    // everything below may read what the previous kernel wrote
-    tq_grid_launch_dependents();
+__device__ __forceinline__ void attend_tile(const Tile& T, int range, int ranges, const TA* __restrict__ q, const Cache8& c, const Step& S, TA* __restrict__ out,
+                                            float* __restrict__ partial, float* __restrict__ scores, int score_stride, float* __restrict__ lse) {
     constexpr int NC = NT * 8, MT = HDP / 16;
-    const int ranges = gridDim.y, range = blockIdx.y;
     __shared__ Queries<TA, HDP, NT> Q;
     __shared__ float s_o[WARPS][NC][HDP + 4];
     __shared__ float s_stat[WARPS][NC][3];
-    const int tile_no = blockIdx.x / c.nkv;
-    const Tile T = tile_of(S, blockIdx.z, blockIdx.x - tile_no * c.nkv, c.nkv, tile_no, NC);
-    if (T.n <= 0) return;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, hd = c.hd;
     // this range's blocks of 16 keys
     const int place0 = T.start + T.row(0), place1 = T.start + T.row(T.n - 1);
@@ -417,6 +411,37 @@ __global__ void __launch_bounds__(WARPS * 32) attention8_kernel(const TA* __rest
     }
 }
 
+template <typename TA, int HDP, int NT>
+__global__ void __launch_bounds__(WARPS * 32) attention8_kernel(const TA* __restrict__ q, Cache8 c, Step S, TA* __restrict__ out, float* __restrict__ partial,
+                                                                float* __restrict__ scores, int score_stride, float* __restrict__ lse) {
+    tq_grid_wait();                    // everything below may read what the previous kernel wrote
+    tq_grid_launch_dependents();
+    const int tile_no = blockIdx.x / c.nkv;
+    const Tile T = tile_of(S, blockIdx.z, blockIdx.x - tile_no * c.nkv, c.nkv, tile_no, NT * 8);
+    if (T.n > 0) attend_tile<TA, HDP, NT>(T, blockIdx.y, gridDim.y, q, c, S, out, partial, scores, score_stride, lse);
+}
+
+// The prompt kernel gives values that a row may not see a weight of 0, which does not remove a NaN: key/value heads of sequences in whose pages
+// `lost` [n_seqs][nkv][pages] marks such values are done again here, all others cost a look at their marks.
+template <typename TA, int HDP, int NT>
+__global__ void __launch_bounds__(WARPS * 32) repair8_kernel(const TA* __restrict__ q, Cache8 c, Step S, TA* __restrict__ out, const uint8_t* __restrict__ lost,
+                                                             int lost_stride, int page_size) {
+    tq_grid_wait();                    // everything below may read what the previous kernel wrote
+    tq_grid_launch_dependents();
+    const int seq = blockIdx.z, g = blockIdx.y, start = S.held[seq], run = S.cu_seqlens[seq + 1] - S.cu_seqlens[seq];
+    if (run <= 0) return;
+    const uint8_t* marks = lost + ((size_t)seq * c.nkv + g) * lost_stride;
+    bool some = false;
+    for (int p = first_seen(start, S.window) / page_size + (int)threadIdx.x; p <= (start + run - 1) / page_size; p += WARPS * 32) some |= marks[p] != 0;
+    if (!__syncthreads_or(some)) return;
+    for (int tile_no = blockIdx.x; ; tile_no += gridDim.x) {
+        const Tile T = tile_of(S, seq, g, c.nkv, tile_no, NT * 8);
+        if (T.n <= 0) return;
+        __syncthreads();
+        attend_tile<TA, HDP, NT>(T, 0, 1, q, c, S, out, nullptr, nullptr, 0, nullptr);
+    }
+}
+
 // ---------------------------------------------------------------------------------------
 // The ranges of a row joined: block x = 0 of a (sequence, key/value head).  Further blocks add the row weights up from the scores the first
 // launch left, 128 places each.
@@ -612,6 +637,26 @@ TQ_EXPORT int tq_attention8(const void* q, const void* codes, const void* scales
     const int chunks = weights != nullptr ? (max_kv_len + 127) / 128 : 0;
     TQ_DISPATCH(act_dtype, TA, tq_launch(dim3(1 + chunks, nkv, n_seqs), 128, 0, stream)(join8_kernel<TA>, c, S, partial, ranges, (TA*)out, lse, scores, score_stride, weights));
     TQ_CHECK_LAUNCH("join8");
+    return 0;
+}
+
+// After a prompt kernel's launch over the same step (bfloat16, heads of 64 or 128): lost [n_seqs][nkv][lost_stride] marks the pages, counted
+// within a sequence, that hold a NaN among the values the step sees.
+TQ_EXPORT int tq_repair8(const void* q, const void* codes, const void* scales, const int* cu_seqlens, const int* held, const int* page_table, int table_stride,
+                         int page_size, int window, float scale, void* out, const void* lost, int lost_stride, int n_pages, int n_seqs, int nh, int nkv, int hd,
+                         cudaStream_t stream) {
+    if (n_seqs == 0) return 0;
+    int rc = c8_check("repair8", codes, scales, page_size, n_pages, nkv, hd, table_stride);
+    if (!rc) rc = check_step("repair8", nh, nkv, n_seqs, 1, window);
+    if (rc) return rc;
+    TQ_REQUIRE(hd == 64 || hd == 128, "repair8: head size %d", hd);
+    const Cache8 c{(uint8_t*)codes, (uint8_t*)scales, page_table, table_stride, page_size, n_pages, nkv, hd};
+    const Step S{cu_seqlens, held, nh, window, scale * LOG2E};
+    const int heads = nkv * n_seqs, each = heads >= 444 ? 1 : 444 / heads;
+    using TA = __nv_bfloat16;
+    if (hd == 64) tq_launch(dim3(each, nkv, n_seqs), WARPS * 32, 0, stream)(repair8_kernel<TA, 64, 2>, (const TA*)q, c, S, (TA*)out, (const uint8_t*)lost, lost_stride, page_size);
+    else tq_launch(dim3(each, nkv, n_seqs), WARPS * 32, 0, stream)(repair8_kernel<TA, 128, 2>, (const TA*)q, c, S, (TA*)out, (const uint8_t*)lost, lost_stride, page_size);
+    TQ_CHECK_LAUNCH("repair8");
     return 0;
 }
 

@@ -321,7 +321,7 @@ attention_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                          const __grid_constant__ Shape S, const int* __restrict__ cu_seqlens, const int* __restrict__ seq_start,
                          const int* __restrict__ page_table, const int* __restrict__ page_base,
                          const float* __restrict__ bias_t, const float* __restrict__ sink,
-                         __nv_bfloat16* __restrict__ out, int* __restrict__ status) {
+                         __nv_bfloat16* __restrict__ out, float* __restrict__ lse, int* __restrict__ status) {
     tq_grid_wait();                    // everything below may read what the previous kernel wrote
     using C = Cfg<DK, DV>;
     extern __shared__ uint8_t smem_raw[];
@@ -734,6 +734,7 @@ attention_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             if (sink != nullptr) l += ex2((floor_m - m) * to_log2);
             const float inv = 1.0f / l;
+            if (lse != nullptr && r < u.rows[slot]) lse[(size_t)(u.t0[slot] + r) * S.nh + h] = m * to_log2 + log2f(l);
             __nv_bfloat16* dst = out + ((size_t)(u.t0[slot] + r) * S.nh + h) * DV;
 #pragma unroll 1
             for (int c0 = 0; c0 < DV; c0 += 32) {
@@ -804,6 +805,7 @@ struct Args {
     const int *cu, *starts, *table, *page_base;
     const float *bias_t, *sink;
     void* out;
+    float* lse;
     int* status;
 };
 
@@ -818,7 +820,7 @@ int launch(const Maps& m, const Shape& S, const Args& a, cudaStream_t stream) {
     const int hs = S.pairing == PAIR_HEADS ? S.nh / 2 : S.nh, qs = S.pairing == PAIR_HEADS ? S.n_qt : (S.n_qt + 1) / 2;
     const int grid = qs * S.n_seqs * hs;
     tq_launch(grid, THREADS, C::SMEM_BYTES, stream)(kern, m.q, m.k, m.r, m.v, S, a.cu, a.starts, a.table, a.page_base, a.bias_t, a.sink,
-                                                   (__nv_bfloat16*)a.out, a.status);
+                                                   (__nv_bfloat16*)a.out, a.lse, a.status);
     TQ_CHECK_LAUNCH("attention_prefill");
     return 0;
 }
@@ -841,11 +843,11 @@ int check_common(const Shape& S, int T_, int max_q_len, const void* q, const voi
 // cu_seqlens [n_seqs+1]: rows of each sequence in q; seq_start [n_seqs]: position of each sequence's first row.
 // Position i sees j <= i with window == 0 or i - j < window or j < keep_first; with cell > 0 instead j <= i of its own
 // cell.  Scores times scale, capped (softcap > 0), plus bias_t [nh][far + 1] (or null) at distance min(i - j, far); sink
-// [nh] or null joins the denominator.  status: one int in device memory, set to 1 if a bounded wait ran out.
+// [nh] or null joins the denominator.  lse: null, or [T][nh], the base-2 logarithm of each row's denominator.  status: one int in device memory, set to 1 if a bounded wait ran out.
 TQ_EXPORT int tq_attention_prefill(const void* q, const void* cache, int planes, const int* cu_seqlens, const int* seq_start,
                                    const int* page_table, int table_stride, int page_size, int n_pages, int window, int keep_first,
                                    int cell, float scale, float softcap, const float* bias_t, int far, const float* sink, void* out,
-                                   int T_, int n_seqs, int max_q_len, int nh, int nkv, int dk, int dv, int* status, cudaStream_t stream) {
+                                   float* lse, int T_, int n_seqs, int max_q_len, int nh, int nkv, int dk, int dv, int* status, cudaStream_t stream) {
     if (T_ == 0 || n_seqs == 0) return 0;
     TQ_REQUIRE((dk == 64 || dk == 128) && (dv == 64 || dv == 128), "attention_prefill: key size %d or value size %d is not 64 or 128", dk, dv);
     TQ_REQUIRE(planes == 1 || (planes == 2 && dk == dv), "attention_prefill: %d planes of keys of %d and values of %d", planes, dk, dv);
@@ -865,7 +867,7 @@ TQ_EXPORT int tq_attention_prefill(const void* q, const void* cache, int planes,
     rc = make_map(&m.k, cache, (uint64_t)n_pages * S.kp, (uint64_t)(planes == 1 ? dk + dv : dk), PAGE);
     if (rc) return rc;
     m.r = m.v = m.k;
-    const Args a{cu_seqlens, seq_start, page_table, nullptr, bias_t, sink, out, status};
+    const Args a{cu_seqlens, seq_start, page_table, nullptr, bias_t, sink, out, lse, status};
     const bool shaped = planes == 1 || softcap > 0.f || bias_t != nullptr || !(scale > 0.f);     // (the other form compares unscaled scores)
 #define AP_CASE(DK_, DV_) if (dk == DK_ && dv == DV_) return shaped ? launch<DK_, DV_, true>(m, S, a, stream) : launch<DK_, DV_, false>(m, S, a, stream);
     AP_CASE(64, 64) AP_CASE(64, 128) AP_CASE(128, 64) AP_CASE(128, 128)
@@ -901,7 +903,7 @@ TQ_EXPORT int tq_attention_prefill_dense(const void* q, const void* kv, const vo
     m.r = m.v = m.k;
     if (rot) rc = make_map(&m.r, rot_rows, (uint64_t)rows, (uint64_t)rot_stride, PAGE);
     if (rc) return rc;
-    const Args a{cu_seqlens, seq_start, nullptr, page_base, nullptr, sink, out, status};
+    const Args a{cu_seqlens, seq_start, nullptr, page_base, nullptr, sink, out, nullptr, status};
 #define AP_CASE(DK_, DV_) if (dk == DK_ && dv == DV_) return launch<DK_, DV_, false>(m, S, a, stream);
     AP_CASE(64, 64) AP_CASE(64, 128) AP_CASE(128, 64) AP_CASE(128, 128) AP_CASE(192, 128)
 #undef AP_CASE

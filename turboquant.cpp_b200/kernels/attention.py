@@ -225,9 +225,9 @@ def prefill_rows(q: torch.Tensor, cache_layer: torch.Tensor, planes: int, cu_seq
                  page_table: torch.Tensor, page_size: int, window: int, scale: float, out: torch.Tensor, n_seqs: int, max_q_len: int,
                  n_heads: int, n_kv_heads: int, dk: int, dv: int, keep_first: int = 0, cell: int = 0, softcap: float = 0.0,
                  bias_t: Optional[torch.Tensor] = None, sink: Optional[torch.Tensor] = None,
-                 status: Optional[torch.Tensor] = None) -> torch.Tensor:
+                 status: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The tensor-core prompt kernel over a cache of two planes (keys, values) or one (rows [key | value]), with the
-    options of `kernels.bias_attention.attention_runs`."""
+    options of `kernels.bias_attention.attention_runs`.  lse [T, n_heads] float32: receives the base-2 logarithm of each row's denominator."""
     if status is None:
         from .gemm_tc import status_word
         status = status_word(q.device)
@@ -238,7 +238,7 @@ def prefill_rows(q: torch.Tensor, cache_layer: torch.Tensor, planes: int, cu_seq
     check("attention_prefill", load_kernel("attention_prefill").tq_attention_prefill(
         ptr(q), ptr(cache_layer), planes, ptr(cu_seqlens), ptr(seq_start), ptr(page_table), page_table.shape[1],
         *ints(page_size, cache_layer.shape[0], window, keep_first, cell), c_float(scale), c_float(softcap), ptr(bias_t),
-        0 if bias_t is None else bias_t.shape[1] - 1, ptr(sink), ptr(out),
+        0 if bias_t is None else bias_t.shape[1] - 1, ptr(sink), ptr(out), ptr(lse),
         *ints(q.shape[0], n_seqs, max_q_len, n_heads, n_kv_heads, dk, dv), ptr(status), stream()))
     return out
 

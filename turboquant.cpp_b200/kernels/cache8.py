@@ -1,4 +1,4 @@
-"""A key/value cache in 8 bits whose length can be bounded (csrc/cache8.cu, csrc/attention8.cu, csrc/evict.cu).
+"""A key/value cache in 8 bits whose length can be bounded (csrc/cache8.cu, csrc/attention8.cu, csrc/prompt8.cu, csrc/evict.cu).
 
 An element is an e4m3 code times 2^(b - 127), b one byte for 16 consecutive rows of a (page, plane, key/value head): the smallest power of
 two, of those from 2^-126 on, under which the largest finite magnitude of the 16 rows is at most 448.  A block that takes rows in
@@ -22,7 +22,7 @@ import torch
 
 from ..csrc.build import load_kernel
 from ._call import KernelError, check, code, ints, on_current_device, ptr, stream, want_f32, want_int32
-from .attention import PAIRING, resident_ctas
+from .attention import PAIRING, prefill_rows, prefill_usable, resident_ctas
 
 BLOCK = 16
 MAX_HEAD_DIM = 256
@@ -110,12 +110,14 @@ SCORE_BYTES = 1 << 28        # scratch a decode step may take for scores
 
 def attention8(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, cu_seqlens: torch.Tensor, held: torch.Tensor,
                page_table: torch.Tensor, page_size: int, window: int, scale: float, out: torch.Tensor, n_heads: int, n_kv_heads: int,
-               head_dim: int, max_q_len: int, max_kv_len: int, weights: Optional[torch.Tensor] = None) -> torch.Tensor:
+               head_dim: int, max_q_len: int, max_kv_len: int, weights: Optional[torch.Tensor] = None,
+               status: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Causal attention of the step's queries q [T, nh, hd] over the pages (the step's own rows are in them already): a row sees its
     sequence's places up to its own (window > 0: the last `window` of them), scores times `scale`; out [T, nh * hd] in q's type.
     max_q_len: the longest run; max_kv_len: at least the longest held + run.
     weights: the softmax weights that each cached row receives from the step's rows, summed over a key/value head's query heads, are
-    added to its sum; the sums of the step's own rows start with this step."""
+    added to its sum; the sums of the step's own rows start with this step.
+    status: the word in which the prompt kernel reports a wait that ran out (default: the device's, kernels.gemm_tc)."""
     T = q.shape[0]
     _check_cache(codes, scales, weights, page_table, page_size, n_kv_heads, head_dim)
     n = _check_step(cu_seqlens, held, page_table, "attention8")
@@ -124,6 +126,9 @@ def attention8(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, cu_se
     if T == 0 or n == 0 or max_q_len < 1:
         return out
     on_current_device(q, out, codes, scales, weights)
+    if max_q_len >= PROMPT_MIN_RUN and prefill_usable(q.dtype, head_dim, page_size):
+        return _attention8_prompt(q, codes, scales, cu_seqlens, held, page_table, page_size, window, scale, out, n_heads, n_kv_heads, head_dim,
+                                  max_q_len, max_kv_len, weights, status)
     per = n_heads // n_kv_heads
     columns = max_q_len * per
     tiles = -(-columns // (16 if columns > 8 and head_dim <= 128 else 8)) * n_kv_heads * n
@@ -148,6 +153,36 @@ def attention8(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, cu_se
           kernels=2 if partial_floats else 1)
     if weights is not None and not stored:
         check("attention8", lib.tq_weigh8(*args, c_void_p(rest), ptr(weights), *step, *ints(max_kv_len), *heads))
+    return out
+
+
+PROMPT_MIN_RUN = 48          # steps whose longest run is at least this go to the tensor-core prompt kernel, where it takes their sizes
+DENSE_BYTES = 1 << 30        # scratch a step may take for pages in bfloat16; sequences beyond it follow in further launches
+
+
+def _attention8_prompt(q, codes, scales, cu_seqlens, held, page_table, page_size, window, scale, out, n_heads, n_kv_heads, head_dim, max_q_len,
+                       max_kv_len, weights, status):
+    """The pages a step sees are expanded to bfloat16 pages of a scratch, exactly, and the prompt kernel of csrc/attention_prefill.cu reads those."""
+    T, n = q.shape[0], page_table.shape[0]
+    width = -(-max_kv_len // page_size)
+    page_bytes = 2 * n_kv_heads * page_size * head_dim * 2
+    group = max(1, min(n, DENSE_BYTES // (page_bytes * width)))
+    dense = torch.empty((group * width, 2, n_kv_heads, page_size, head_dim), dtype=torch.bfloat16, device=q.device)
+    table = torch.empty((group, width), dtype=torch.int32, device=q.device)
+    lost = torch.empty((group, n_kv_heads, width), dtype=torch.uint8, device=q.device)
+    lse = torch.empty((T, n_heads), dtype=torch.float32, device=q.device) if weights is not None else None
+    for i in range(0, n, group):
+        m = min(group, n - i)
+        cu, starts, pages, dtable = cu_seqlens[i:i + m + 1], held[i:i + m], page_table[i:i + m], table[:m]
+        cache = (ptr(codes), ptr(scales), ptr(cu), ptr(starts), ptr(pages), pages.shape[1], *ints(page_size, window))
+        check("prompt8", load_kernel("prompt8").tq_expand8(*cache, ptr(dense), ptr(table), ptr(lost), width, codes.shape[0], m, *ints(n_kv_heads, head_dim), stream()))
+        prefill_rows(q, dense, 2, cu, starts, dtable, page_size, window, scale, out, m, max_q_len, n_heads, n_kv_heads, head_dim, head_dim, status=status, lse=lse)
+        check("attention8", load_kernel("attention8").tq_repair8(
+            ptr(q), *cache, c_float(scale), ptr(out), ptr(lost), width, codes.shape[0], m, *ints(n_heads, n_kv_heads, head_dim), stream()))
+    if weights is not None:
+        check("attention8", load_kernel("attention8").tq_weigh8(
+            ptr(q), ptr(codes), ptr(scales), code(q.dtype), ptr(cu_seqlens), ptr(held), ptr(page_table), page_table.shape[1], *ints(page_size, window), c_float(scale),
+            ptr(lse), ptr(weights), codes.shape[0], n, *ints(max_q_len, max_kv_len, n_heads, n_kv_heads, head_dim), stream()))
     return out
 
 
