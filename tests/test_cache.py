@@ -127,3 +127,73 @@ def test_paged_cache_groups_state_and_tables():
     b = cache.open()
     assert b.slot == slot and float(cache.state[2][slot].abs().sum()) == 0.0     # the slot is used again, zeroed
     assert cache.bytes_per_token() == 3 * 2 * 2 * 16 * 4      # three entries keep keys and values
+
+
+# ---- sequences that give rows up --------------------------------------------------------------------------------------
+def test_moved_sequences_hold_fewer_rows_on_other_pages():
+    book = CacheBook([12, 12], [0, 0], page_size=64, max_slots=4)
+    book.keep_spare(130)                          # three pages a group set aside
+    assert [p.n_free for p in book.pools] == [9, 9]
+    book.check_invariants()
+    a, b = book.open(), book.open()
+    book.reserve_all([a, b], [250, 200])
+    book.commit(a, 250)
+    book.commit(b, 200)
+    assert (a.held, b.held) == (250, 200) and [p.n_free for p in book.pools] == [1, 1]
+    old = [list(p) for p in a.pages]
+    moves = book.take_for_moves(2, 130)           # one free page: only what is set aside
+    assert len(moves) == 1 and all(len(m) == 3 and not set(m) & set(o) for m, o in zip(moves[0], old))
+    book.moved(a, moves[0], 130)
+    assert (a.held, a.length) == (130, 250) and [len(s) for s in book.spare] == [3, 3] and [p.n_free for p in book.pools] == [2, 2]
+    book.check_invariants()
+    book.reserve(a, 62)                           # places 130 .. 191: the three pages it has
+    assert [len(p) for p in a.pages] == [3, 3]
+    book.commit(a, 62)
+    book.reserve(a, 1)
+    assert a.held == 192 and a.length == 312 and [len(p) for p in a.pages] == [4, 4]
+    book.check_invariants()
+    book.close(a)
+    moves = book.take_for_moves(5, 130)           # free pages serve further sequences of the same step
+    assert len(moves) == 2                        # 12 - 3 set aside - 4 of b's: 5 free, room for one more of three
+    book.moved(b, moves[0], 130)
+    for m in moves[1:]:
+        for g, pages in enumerate(m):
+            for p in pages:
+                book.pools[g].give_back(p)
+    book.check_invariants()
+    book.close(b)
+    assert [p.n_free for p in book.pools] == [9, 9]
+    with pytest.raises(CacheMisuse):
+        book.take_for_moves(1, 500)               # more than was set aside
+
+
+def test_batches_count_bounded_requests_by_what_they_come_to_hold():
+    from turboquant_cpp_b200.engine.generate import plan_batches
+    plan = lambda bounded: plan_batches([100, 100, 900, 10], 4000, 8, 2048, 8, 64, 8192, bounded)
+    assert plan(0) == [[0], [1], [2], [3]]
+    assert plan(256) == [[0, 1, 2, 3]]            # 256, 256, its prompt of 900, 256: 27 of 32 pages
+    assert plan_batches([100, 100], 20, 8, 256, 8, 64, 8192, 4096) == [[0, 1]]
+
+
+def test_options_that_an_engine_refuses(monkeypatch):
+    """Checked before anything is built: no GPU."""
+    import turboquant_cpp_b200 as tq
+    from conftest import TINY_A, TINY_B
+    import copy
+    import lumevik_util
+    make = lambda cfg: tq.build_model(cfg, "bfloat16")
+    check = lambda model, dtype, budget=0, recent=None: _engine_options(model, dtype, budget, recent)
+    odd = copy.deepcopy(TINY_A)
+    assert check(make(odd), "e4m3") is True and check(make(odd), "") is False and check(make(odd), "e4m3", 64) is True
+    assert check(make(TINY_B), "e4m3") is True
+    for model, dtype, budget, recent in ((make(odd), "int4", 0, None), (make(odd), "", 64, None), (make(odd), "e4m3", 64, 65), (make(odd), "e4m3", -1, None),
+                                         (make(TINY_B), "e4m3", 64, None), (make(next(iter(lumevik_util.CONFIGS.values()))), "e4m3", 0, None)):
+        with pytest.raises(ValueError):
+            check(model, dtype, budget, recent)
+
+
+def _engine_options(model, dtype, budget, recent):
+    from turboquant_cpp_b200.engine.step import Engine
+    e = Engine.__new__(Engine)
+    e.cache_budget, e.cache_recent = budget, budget // 4 if recent is None else recent
+    return e._cache_in_8_bits(model, dtype)

@@ -63,9 +63,15 @@ class Sequence_:
     def __init__(self, seq_id: int, slot: int, n_groups: int):
         self.id = seq_id
         self.slot = slot
-        self.length = 0
+        self.length = 0                  # tokens: the next one's position
+        self.evicted = 0                 # of them, those whose rows were given up
         self.pages: List[List[Optional[int]]] = [[] for _ in range(n_groups)]
         self.open = True
+
+    @property
+    def held(self) -> int:
+        """Rows the sequence holds in the cache: the place of its next token."""
+        return self.length - self.evicted
 
 
 class CacheBook:
@@ -81,6 +87,7 @@ class CacheBook:
         assert len(self.keep_first) == len(self.windows)
         self.pools = [IndexPool(n, f"page of group {g}") for g, n in enumerate(n_pages)]
         self.slots = IndexPool(max_slots, "sequence slot")
+        self.spare: List[List[int]] = [[] for _ in self.pools]      # pages no sequence holds, for moves (keep_spare)
         self._next_id = 0
         self.live: Dict[int, Sequence_] = {}
 
@@ -91,7 +98,7 @@ class CacheBook:
         return s
 
     def pages_needed(self, seq: Sequence_, n_new: int) -> List[int]:
-        total = -(-(seq.length + n_new) // self.page_size)
+        total = -(-(seq.held + n_new) // self.page_size)
         return [max(0, total - len(p)) for p in seq.pages]
 
     def reserve(self, seq: Sequence_, n_new: int) -> None:
@@ -101,7 +108,7 @@ class CacheBook:
         for g, c in enumerate(need):
             if c > self.pools[g].n_free:
                 raise CacheFull(f"sequence {seq.id} needs {c} more pages of {self.page_size} tokens in group {g} "
-                                f"for {seq.length}+{n_new} tokens, {self.pools[g].n_free} of {self.pools[g].n} are free")
+                                f"for {seq.held}+{n_new} tokens, {self.pools[g].n_free} of {self.pools[g].n} are free")
         for g, c in enumerate(need):
             seq.pages[g].extend(self.pools[g].take_many(c))
 
@@ -131,6 +138,38 @@ class CacheBook:
                     self.pools[g].give_back(seq.pages[g][i])
                     seq.pages[g][i] = None
 
+    # ---- eviction: a sequence's rows move to other pages, and there are fewer of them --------------
+    def keep_spare(self, rows: int) -> None:
+        """Sets pages for `rows` rows aside in every group, so that one sequence can always be moved."""
+        per = -(-int(rows) // self.page_size)
+        self.spare = [pool.take_many(per) for pool in self.pools]
+
+    def take_for_moves(self, n: int, rows: int) -> List[List[List[int]]]:
+        """New pages for `rows` rows each of up to n sequences (as many as the free pages allow, at least one): per sequence, per group.
+        Follow with `moved` for each of them."""
+        per = -(-int(rows) // self.page_size)
+        if any(len(s) < per for s in self.spare):
+            raise CacheMisuse(f"no pages for {rows} rows are set aside")
+        first = [s[:per] for s in self.spare]
+        self.spare = [s[per:] for s in self.spare]
+        out = [first]
+        while len(out) < n and all(pool.n_free >= per for pool in self.pools):
+            out.append([pool.take_many(per) for pool in self.pools])
+        return out
+
+    def moved(self, seq: Sequence_, pages: List[List[int]], rows: int) -> None:
+        """The sequence now holds `rows` rows, on these pages; its old ones are set aside again or free."""
+        self._check_open(seq)
+        per = len(pages[0]) if pages else 0
+        for g, new in enumerate(pages):
+            for p in seq.pages[g]:
+                if len(self.spare[g]) < per:
+                    self.spare[g].append(p)
+                else:
+                    self.pools[g].give_back(p)
+            seq.pages[g] = list(new)
+        seq.evicted = seq.length - rows
+
     def close(self, seq: Sequence_) -> None:
         self._check_open(seq)
         for g, pages in enumerate(seq.pages):
@@ -149,7 +188,7 @@ class CacheBook:
     def check_invariants(self) -> None:
         """Every page and slot is either free or held by exactly one live sequence."""
         for g, pool in enumerate(self.pools):
-            held = [p for s in self.live.values() for p in s.pages[g] if p is not None]
+            held = [p for s in self.live.values() for p in s.pages[g] if p is not None] + self.spare[g]
             if len(held) != len(set(held)):
                 raise AssertionError(f"group {g}: a page is held twice")
             if len(held) != pool.n_held:

@@ -12,6 +12,9 @@ its recurrent layers' fixed-size state in the same object, zeroed at creation
   windowed group gives pages back as they fall out of every later query's sight.
 * an entry's storage is one tensor [pages, planes, kv heads, page_size, head size]: two planes (K, V), or one
   for a mixer whose cached row serves as key and value.
+* in 8 bits (`eight_bits`) an entry's storage is codes and their blocks' bytes (kernels/cache8.py) and, where sequences are evicted by
+  it (`weights`), the attention weight every row has received.  A sequence that was evicted holds fewer rows than tokens: a row's
+  place in its pages is then no longer its position.
 * a sequence holds a *slot*: its row in every state tensor [max_slots, *shape].  The row is
   zeroed when the slot is taken.  Slots and pages are given back when the sequence is closed and
   are used again by later sequences.
@@ -23,6 +26,7 @@ from typing import Dict, List, Optional, Sequence, Tuple
 import numpy as np
 import torch
 
+from ..kernels.cache8 import evict8, storage as storage8
 from ..parts.base import KVNeed, LayerCache, StateNeed
 from .allocator import CacheBook, CacheFull, Sequence_
 
@@ -34,7 +38,7 @@ class PagedCache:
                  cache_of: Sequence[Optional[int]], max_tokens: int, dtype: torch.dtype, device,
                  max_slots: Optional[int] = None, page_size: int = PAGE_SIZE,
                  pages_per_group: Optional[Dict[KVNeed, int]] = None,
-                 embed_state_need: Optional[StateNeed] = None):
+                 embed_state_need: Optional[StateNeed] = None, eight_bits: bool = False, weights: bool = False):
         """kv_needs/state_needs/cache_of: one item per entry of the model's layer schedule.
         max_tokens: the most tokens live sequences hold together, each sequence's count rounded up
         to a multiple of page_size."""
@@ -63,16 +67,24 @@ class PagedCache:
         self.book = CacheBook(counts, [g.window for g in self.groups], self.page_size, self.max_slots,
                               keep_first=[g.keep_first for g in self.groups])
         self.kv: List[Optional[torch.Tensor]] = []
+        self.scales: List[Optional[torch.Tensor]] = [None] * len(kv_needs)
+        self.weights: List[Optional[torch.Tensor]] = [None] * len(kv_needs)
         for i, need in enumerate(kv_needs):
             if need is None or cache_of[i] is not None:
                 self.kv.append(None)
                 continue
             g = self.entry_group[i]
+            if eight_bits:
+                if need.planes != 2:
+                    raise ValueError("a cache in 8 bits keeps keys and values, not rows that serve as both")
+                codes, self.scales[i], self.weights[i] = storage8(counts[g], need.n_kv_heads, self.page_size, need.head_dim, self.device, weights)
+                self.kv.append(codes)
+                continue
             self.kv.append(torch.zeros((counts[g], need.planes, need.n_kv_heads, self.page_size, need.head_dim),
                                        dtype=dtype, device=self.device))
         for i, src in enumerate(cache_of):
             if src is not None:
-                self.kv[i] = self.kv[src]
+                self.kv[i], self.scales[i], self.weights[i] = self.kv[src], self.scales[src], self.weights[src]
         self.cache_of = list(cache_of)
         self.state: List[Optional[torch.Tensor]] = [
             None if n is None else torch.zeros((self.max_slots,) + tuple(n.shape), dtype=n.dtype, device=self.device)
@@ -119,11 +131,32 @@ class PagedCache:
             g = self.entry_group[i]
             out.append(LayerCache(kv=self.kv[i], page_table=None if g is None else device_tables[g],
                                   page_size=self.page_size, writes=self.cache_of[i] is None,
-                                  state=self.state[i]))
+                                  state=self.state[i], scales=self.scales[i], weights=self.weights[i]))
         return out
 
     def bytes_per_token(self) -> int:
         """Key/value bytes one token adds across all layers that keep a cache."""
-        el = torch.empty((), dtype=self.dtype).element_size()
-        return sum(t.shape[1] * t.shape[2] * t.shape[4] * el for i, t in enumerate(self.kv)
-                   if t is not None and self.cache_of[i] is None)
+        own = [i for i, t in enumerate(self.kv) if t is not None and self.cache_of[i] is None]
+        side = sum(t.numel() * t.element_size() for i in own for t in (self.scales[i], self.weights[i]) if t is not None)
+        tokens = self.kv[own[0]].shape[0] * self.page_size if own else 1
+        return sum(self.kv[i].shape[1] * self.kv[i].shape[2] * self.kv[i].shape[4] * self.kv[i].element_size() for i in own) + -(-side // tokens)
+
+    # ---- eviction -------------------------------------------------------------------------------
+    def evict(self, seqs: Sequence[Sequence_], budget: int, recent: int) -> None:
+        """The sequences keep `budget` rows in every key/value head of every layer (kernels.cache8.evict8), on pages of their own."""
+        todo = list(seqs)
+        while todo:
+            moves = self.book.take_for_moves(len(todo), budget)
+            now, todo = todo[:len(moves)], todo[len(moves):]
+            tables = self.page_tables(now)
+            fields = [np.array([s.held for s in now], dtype=np.int32)] + tables + [np.array([m[g] for m in moves], dtype=np.int32) for g in range(len(self.groups))]
+            sizes = [f.size for f in fields]
+            parts = torch.split(torch.from_numpy(np.concatenate([f.reshape(-1) for f in fields])).pin_memory().to(self.device, non_blocking=True), sizes)
+            for i, codes in enumerate(self.kv):
+                if codes is None or self.cache_of[i] is not None:
+                    continue
+                g = self.entry_group[i]
+                evict8(codes, self.scales[i], self.weights[i], parts[0], parts[1 + g].view(tables[g].shape),
+                       parts[1 + len(self.groups) + g].view(len(now), -1), self.page_size, budget, recent)
+            for s, m in zip(now, moves):
+                self.book.moved(s, m, min(s.held, budget))

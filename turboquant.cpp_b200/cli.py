@@ -3,7 +3,7 @@
     quant <model folder> | --random CONFIG.json [--seed-weights N]
           [-p "ids"]… [--tokens-file FILE] [-n max_tokens] [-T temperature] [-P top_p] [-s seed]
           [--ctx N] [--dtype bfloat16|float32] [--batch N] [--stop id]… [--rep-penalty F] [--rep-window N]
-          [--detect-loops] [--info] [--profile]
+          [--detect-loops] [--cache e4m3 [--cache-budget N [--cache-recent N]]] [--info] [--profile]
           [--bench-prefill] [--bench-memory]
 
 Names and meanings follow the reference where it has them: -p prompt (default "Hello" there; here
@@ -19,7 +19,9 @@ TQ_DEBUG_LAYERS=1 in the environment prints per-layer checksums of the residual 
 TQ_DEBUG_PREFILL does.  --rep-penalty and --rep-window set what the reference keeps as
 engine defaults without an option (1.1 over 32 tokens, include/turboquant/tq_engine.h:408-409); here
 the penalty is off unless asked for, and so is the reference's detector of repetition loops
-(--detect-loops; src/engine/tq_generate.c:610-630).  -j (threads) is accepted and ignored.  -p may be given several
+(--detect-loops; src/engine/tq_generate.c:610-630).  --cache e4m3 keeps keys and values in 8 bits,
+--cache-budget bounds the rows a request keeps of them by the attention they received, --cache-recent says how many of those
+are its newest.  -j (threads) is accepted and ignored.  -p may be given several
 times: the prompts run as batches.  Token ids go to stdout, one line per prompt; the summary
 "N tokens in X s (Y tok/s)" goes to stderr as the reference prints it (tools/quant.c:1371-1376).
 """
@@ -60,6 +62,9 @@ def main(argv=None) -> int:
     ap.add_argument("--rep-window", type=int, default=32)
     ap.add_argument("--detect-loops", action="store_true",
                     help="end a request whose last four tokens have come up three times before (the reference always does)")
+    ap.add_argument("--cache", choices=["e4m3"], default="", help="keep keys and values in 8 bits with a scale per 16 rows")
+    ap.add_argument("--cache-budget", type=int, default=0, help="most rows a request keeps of an 8-bit cache, by the attention they received (0: all)")
+    ap.add_argument("--cache-recent", type=int, default=None, help="of those, the newest (default: a quarter)")
     ap.add_argument("--info", action="store_true")
     ap.add_argument("--profile", action="store_true")
     ap.add_argument("--bench-prefill", action="store_true")
@@ -100,7 +105,7 @@ def main(argv=None) -> int:
     options = dict(temperature=args.temperature, top_p=args.top_p, max_tokens=args.max_tokens,
                    context_length=args.ctx, seed=seed, device=args.device, max_batch=args.batch,
                    stop_token_ids=args.stop, rep_penalty=args.rep_penalty, rep_window=args.rep_window,
-                   detect_loops=args.detect_loops)
+                   detect_loops=args.detect_loops, cache_dtype=args.cache, cache_budget=args.cache_budget, cache_recent=args.cache_recent)
     if raw is not None:
         from .engine.loading import random_model
         m = Model.from_model(random_model(raw, args.seed_weights, args.dtype, args.device), **options)

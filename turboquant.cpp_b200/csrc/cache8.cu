@@ -44,7 +44,7 @@ __device__ __forceinline__ void store8(float* p, const float (&f)[8]) {
 struct WriteArgs {
     const float *cos_t, *sin_t;
     const int *positions, *cu_seqlens, *held;
-    int nh, pairing, n_seqs;
+    int nh, pairing, written;          // written: the heads this launch takes (the queries alone, or all)
 };
 
 template <typename TA, typename TB, int KEPT>
@@ -52,7 +52,7 @@ __global__ void __launch_bounds__(256) write8_kernel(const TA* __restrict__ qkv,
     tq_grid_wait();                    // everything below may read what the previous kernel wrote
     tq_grid_launch_dependents();
     const int lane = threadIdx.x & 31, j = blockIdx.y * (blockDim.x >> 5) + (threadIdx.x >> 5), heads = a.nh + 2 * c.nkv;
-    if (j >= heads) return;
+    if (j >= a.written) return;
     const int seq = blockIdx.z, t_begin = a.cu_seqlens[seq], run = a.cu_seqlens[seq + 1] - t_begin;
     const int place0 = a.held[seq];
     const int block_start = (place0 / C8_BLOCK + (int)blockIdx.x) * C8_BLOCK;       // the unit's block, as a place
@@ -169,7 +169,7 @@ __global__ void __launch_bounds__(256) write8_kernel(const TA* __restrict__ qkv,
 }  // namespace
 
 // qkv [T, (nh + 2 nkv) * hd]; bias as long as a row, or null; cos and sin [positions, hd / 2] float32, or null; q_out [T, nh, hd].
-// max_q_len: the longest run (cu_seqlens, held [n_seqs]: device).  Rows behind cu_seqlens[n_seqs] are left alone.
+// max_q_len: the longest run (cu_seqlens, held [n_seqs]: device).  codes null: the queries only.  Rows behind cu_seqlens[n_seqs] are left alone.
 TQ_EXPORT int tq_write8(const void* qkv, int act_dtype, const void* bias, int bias_dtype, const float* cos_t, const float* sin_t, int pairing,
                         const int* positions, const int* cu_seqlens, const int* held, const int* page_table, int table_stride, int page_size,
                         void* q_out, void* codes, void* scales, int n_pages, int n_seqs, int max_q_len, int nh, int nkv, int hd, cudaStream_t stream) {
@@ -181,9 +181,9 @@ TQ_EXPORT int tq_write8(const void* qkv, int act_dtype, const void* bias, int bi
     TQ_REQUIRE(n_seqs <= 65535 && max_q_len >= 1, "write8: %d sequences, longest run %d", n_seqs, max_q_len);
     TQ_REQUIRE(((uintptr_t)qkv | (uintptr_t)bias | (uintptr_t)q_out | (uintptr_t)cos_t | (uintptr_t)sin_t) % 16 == 0, "write8: tensors must be 16-byte aligned");
     const Cache8 c{(uint8_t*)codes, (uint8_t*)scales, page_table, table_stride, page_size, n_pages, nkv, hd};
-    const WriteArgs a{cos_t, sin_t, positions, cu_seqlens, held, nh, pairing, n_seqs};
+    const WriteArgs a{cos_t, sin_t, positions, cu_seqlens, held, nh, pairing, codes != nullptr ? nh + 2 * nkv : nh};
     // a run of n rows touches at most (n + 14) / 16 + 1 blocks
-    const int units = max_q_len == 1 ? 1 : (max_q_len + 14) / C8_BLOCK + 1, heads = nh + 2 * nkv, warps = units * n_seqs >= 128 ? 8 : 2;
+    const int units = max_q_len == 1 ? 1 : (max_q_len + 14) / C8_BLOCK + 1, heads = a.written, warps = units * n_seqs >= 128 ? 8 : 2;
     const dim3 grid(units, (heads + warps - 1) / warps, n_seqs);
     TQ_DISPATCH(act_dtype, TA, TQ_DISPATCH(bias != nullptr ? bias_dtype : act_dtype, TB,
         if (max_q_len == 1) tq_launch(grid, warps * 32, 0, stream)(write8_kernel<TA, TB, 1>, (const TA*)qkv, (const TB*)bias, a, (TA*)q_out, c);

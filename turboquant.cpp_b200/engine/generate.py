@@ -78,9 +78,9 @@ class LoopDetector:
 
 
 def plan_batches(prompt_lens: Sequence[int], max_new_tokens: int, max_batch: int, capacity_tokens: int,
-                 max_slots: int, page_size: int, max_position: int) -> List[List[int]]:
+                 max_slots: int, page_size: int, max_position: int, bounded_rows: int = 0) -> List[List[int]]:
     """Splits requests, in order, into batches that fit the cache: a request is counted with the
-    most tokens it can come to hold, rounded up to whole pages."""
+    most tokens it can come to hold, rounded up to whole pages (bounded_rows > 0: no more than that beyond its prompt)."""
     if max_batch < 1:
         raise ValueError("max_batch must be at least 1")
     budget = capacity_tokens // page_size
@@ -92,7 +92,8 @@ def plan_batches(prompt_lens: Sequence[int], max_new_tokens: int, max_batch: int
             raise ValueError(f"request {i} has an empty prompt")
         if n > max_position:
             raise ValueError(f"request {i}: prompt of {n} tokens exceeds the model's {max_position} positions")
-        need = -(-min(n + max_new_tokens, max_position) // page_size)
+        need = min(n + max_new_tokens, max_position)
+        need = -(-(max(n, min(need, bounded_rows)) if bounded_rows > 0 else need) // page_size)
         if -(-n // page_size) > budget:
             raise CacheFull(f"request {i}: prompt of {n} tokens does not fit a cache of {capacity_tokens} tokens")
         need = min(need, budget)     # alone it may run until the cache is full
@@ -112,7 +113,7 @@ def generate(engine, sampler, prompts: Sequence[Sequence[int]], params: GenParam
     """Generates a continuation for every prompt.
 
     engine:   open(), close(seq), step(entries) -> logits rows, make_entry(seq, tokens, want),
-              capacity_tokens, max_slots, page_size, max_position; optionally can_step_ahead, step_ahead(seqs,
+              capacity_tokens, max_slots, page_size, max_position; optionally bounded_rows; optionally can_step_ahead, step_ahead(seqs,
               sampled tokens) -> logits rows, commit_ahead(), drop_ahead(), token_reader(n); optionally
               tokens_to_host(sampled tokens) -> list, which may raise if the step's kernels reported a fault (the
               tokens are then neither appended nor told)
@@ -134,7 +135,7 @@ def generate(engine, sampler, prompts: Sequence[Sequence[int]], params: GenParam
             r.finish_reason = "length"
         return results
     batches = plan_batches([len(p) for p in prompts], params.max_new_tokens, max_batch, engine.capacity_tokens,
-                           engine.max_slots, engine.page_size, engine.max_position)
+                           engine.max_slots, engine.page_size, engine.max_position, getattr(engine, "bounded_rows", 0))
     for batch in batches:
         stats.batches += 1
         live = {i: engine.open() for i in batch}

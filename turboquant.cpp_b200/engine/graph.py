@@ -26,7 +26,7 @@ class DecodeGraph:
         cache = engine.cache
         self.widths = [engine.table_width for _ in cache.groups]
         B = batch
-        sizes = [B, B, B, B + 1, B, B, B] + [B * w for w in self.widths]
+        sizes = [B, B, B, B + 1, B, B, B] + [B * w for w in self.widths] + [B]
         self.offsets = np.concatenate([[0], np.cumsum(sizes)]).astype(np.int64)
         total = int(self.offsets[-1])
         # two pinned staging buffers used in turn: a buffer is rewritten only after its copy has finished
@@ -41,7 +41,7 @@ class DecodeGraph:
             seq_start=parts[4], slots=parts[5], want_rows=parts[6], n_want=B, max_q_len=1,
             max_kv_len=engine.table_width * cache.page_size, act_dtype=engine.act_dtype, device=engine.device,
             host_q_lens=[1] * B, host_slots=[], debug={} if engine.record_routing else None, status=engine.status,
-            embed_state=cache.embed_state)
+            embed_state=cache.embed_state, held=parts[-1])
         for host in self.hosts:              # constant parts of the buffer
             h = host.numpy()
             h[:] = 0
@@ -63,6 +63,7 @@ class DecodeGraph:
         h[o[1]:o[2]] = lengths
         h[o[4]:o[5]] = lengths
         h[o[5]:o[6]] = [s.slot for s in seqs]
+        h[o[-2]:o[-1]] = [s.held for s in seqs]
         for g, w in enumerate(self.widths):
             t = h[o[7 + g]:o[8 + g]].reshape(B, w)
             for i, s in enumerate(seqs):

@@ -21,11 +21,12 @@ import os
 import numpy as np
 import torch
 
-from ..cache import CacheFull, PagedCache, Sequence_
+from ..cache import PAGE_SIZE, CacheFull, PagedCache, Sequence_
 from ..csrc.build import ensure_built, index_faults
 from ..kernels._call import KernelError
+from ..kernels.cache8 import check_sizes
 from ..kernels.gemm_tc import GAVE_UP, check_status
-from ..parts.base import StepContext
+from ..parts.base import Mixer, StepContext
 from .graph import DecodeGraphs
 
 
@@ -101,8 +102,13 @@ class Engine:
     """A model, its cache and the step function."""
 
     def __init__(self, model, max_tokens: int, max_slots: Optional[int] = None, device="cuda:0",
-                 use_graphs: Optional[bool] = None, record_routing: bool = False):
-        """record_routing: decode steps captured into CUDA graphs keep what the parts record into the step's
+                 use_graphs: Optional[bool] = None, record_routing: bool = False, cache_dtype: str = "",
+                 cache_budget: int = 0, cache_recent: Optional[int] = None):
+        """cache_dtype: "e4m3" keeps keys and values in 8 bits with a scale per 16 rows (kernels.cache8; models whose layers are all
+        plain attention), "" in the run's own type.  cache_budget > 0 (8-bit caches without windows): after a step, sequences that
+        hold `cache_budget` rows and a page more go back to that many, in every key/value head the last cache_recent (default a
+        quarter) and those that received the most attention; steps are then not launched ahead of their tokens.
+        record_routing: decode steps captured into CUDA graphs keep what the parts record into the step's
         `debug` (the experts chosen) in memory of the graph, so that setting `engine.debug = {}` before a step
         fills it from the very launches that generation replays; without it, a step with `debug` set runs
         outside the graphs."""
@@ -111,10 +117,17 @@ class Engine:
         if self.device.type != "cuda":
             raise RuntimeError("the engine runs on a CUDA device; there is no CPU path")
         self.act_dtype = model.dtype
+        self.cache_budget = int(cache_budget)
+        self.cache_recent = self.cache_budget // 4 if cache_recent is None else int(cache_recent)
+        eight = self._cache_in_8_bits(model, cache_dtype)
         ensure_built(model.kernels())
+        if self.cache_budget:
+            max_tokens = -(-max_tokens // PAGE_SIZE) * PAGE_SIZE + -(-self.cache_budget // PAGE_SIZE) * PAGE_SIZE      # one sequence's worth set aside
         self.cache = PagedCache(model.cache_needs(), model.state_needs(), [e.cache_of for e in model.schedule],
-                                max_tokens, self.act_dtype, self.device, max_slots=max_slots,
+                                max_tokens, self.act_dtype, self.device, max_slots=max_slots, eight_bits=eight, weights=self.cache_budget > 0,
                                 embed_state_need=model.embedding_state_need() if hasattr(model, "embedding_state_need") else None)
+        if self.cache_budget:
+            self.cache.book.keep_spare(self.cache_budget)
         self.debug: Optional[Dict[str, Any]] = None
         self.record_routing = bool(record_routing)
         # set by a kernel whose bounded wait ran out (one word per engine: a fault is seen by the engine it spoiled)
@@ -142,10 +155,41 @@ class Engine:
         self._ahead = None                       # (sequences, tokens each) of a step launched ahead, if any
         self._reader: Optional[TokenReader] = None
 
+    def _cache_in_8_bits(self, model, cache_dtype: str) -> bool:
+        """Checks the cache's options against the model and tells its mixers."""
+        if cache_dtype not in ("", "e4m3"):
+            raise ValueError(f"cache_dtype '{cache_dtype}': '' (the run's type) or 'e4m3'")
+        if self.cache_budget < 0 or (self.cache_budget and not 0 <= self.cache_recent <= self.cache_budget):
+            raise ValueError(f"a cache budget of {self.cache_budget} rows cannot keep the newest {self.cache_recent}")
+        if self.cache_budget and not cache_dtype:
+            raise ValueError("cache_budget needs a cache in 8 bits (cache_dtype='e4m3')")
+        blocks = getattr(model, "blocks", ())
+        mixers = [p for b in blocks for p in (b.parts() if hasattr(b, "parts") else [b]) if isinstance(p, Mixer)]
+        if cache_dtype:
+            needs = [n for n in model.cache_needs() if n is not None]
+            if not needs or any(b.cache_need() is not None and not any(isinstance(p, Mixer) for p in (b.parts() if hasattr(b, "parts") else ())) for b in blocks) \
+                    or not all(m.takes_cache8 for m in mixers if m.cache_need() is not None):
+                raise ValueError(f"{type(model).__name__}: layers that are not plain attention keep their cache in the run's type")
+            for n in needs:
+                check_sizes(PAGE_SIZE, n.head_dim)
+                if self.cache_budget and (n.window or n.keep_first):
+                    raise ValueError("cache_budget: layers with a window are bounded already")
+            if self.cache_budget and any(e.cache_of is not None for e in model.schedule):
+                raise ValueError("cache_budget: layers that read another layer's cache")
+        for m in mixers:
+            m.cache8 = bool(cache_dtype)
+        return bool(cache_dtype)
+
     # ---- what the generation loop asks -----------------------------------------------------------
     @property
     def capacity_tokens(self) -> int:
-        return min(p.n for p in self.cache.book.pools) * self.cache.page_size if self.cache.book.pools else 1 << 30
+        book = self.cache.book
+        return min(p.n - len(s) for p, s in zip(book.pools, book.spare)) * self.cache.page_size if book.pools else 1 << 30
+
+    @property
+    def bounded_rows(self) -> int:
+        """The most rows a sequence comes to hold after its prompt's step (0: as many as it has tokens)."""
+        return self.cache_budget + self.cache.page_size if self.cache_budget else 0
 
     @property
     def max_slots(self) -> int:
@@ -250,8 +294,9 @@ class Engine:
         positions = np.arange(T, dtype=np.int64) - cu[:-1][seq_of_token] + starts[seq_of_token]
         want = np.array([cu[i] + w for i, e in enumerate(entries) for w in e.want], dtype=np.int64)
         slots = np.array([e.seq.slot for e in entries], dtype=np.int64)
+        held = np.array([e.seq.held for e in entries], dtype=np.int64)
         tables = self.cache.page_tables([e.seq for e in entries])
-        fields = [tokens, positions, seq_of_token, cu, starts, slots, want] + [t.reshape(-1) for t in tables]
+        fields = [tokens, positions, seq_of_token, cu, starts, slots, want] + [t.reshape(-1) for t in tables] + [held]
         sizes = [f.size for f in fields]
         packed = torch.from_numpy(np.concatenate(fields).astype(np.int32))
         if packed.numel():
@@ -265,7 +310,7 @@ class Engine:
             max_q_len=int(q_lens.max()), max_kv_len=int((starts + q_lens).max()), act_dtype=self.act_dtype,
             device=self.device, host_q_lens=[int(n) for n in q_lens], host_slots=[int(s) for s in slots],
             host_seq_start=[int(s) for s in starts],
-            debug=self.debug, status=self.status, embed_state=self.cache.embed_state)
+            debug=self.debug, status=self.status, embed_state=self.cache.embed_state, held=parts[-1])
         return ctx, dev_tables
 
     def step(self, entries: Sequence[StepEntry]) -> Optional[torch.Tensor]:
@@ -289,9 +334,17 @@ class Engine:
             else:
                 ctx, dev_tables = self.build_context(entries)
                 logits = self.model.forward(ctx, self.cache.layer_caches(dev_tables))
+        self._commit(seqs, n_new)
+        return logits
+
+    def _commit(self, seqs, n_new) -> None:
         self.cache.commit(seqs, n_new)
         self.steps_run += 1
-        return logits
+        if self.cache_budget:
+            long = [s for s in seqs if s.held >= self.bounded_rows]
+            if long:
+                with torch.cuda.device(self.device):
+                    self.cache.evict(long, self.cache_budget, self.cache_recent)
 
     def _step_with_layer_dump(self, entries, seqs, n_new):
         import sys
@@ -308,16 +361,15 @@ class Engine:
                         print(f"[fwd]   L{layer} pos={pos} final x sum={sums[t]:.9f} sumabs={mags[t]:.9f}", file=sys.stderr)
         finally:
             self.debug = saved
-        self.cache.commit(seqs, n_new)
-        self.steps_run += 1
+        self._commit(seqs, n_new)
         return logits
 
     # ---- a decode step launched before its input tokens have reached the host --------------------------
     @property
     def can_step_ahead(self) -> bool:
         """Decode steps can be launched from tokens that are still on the device (CUDA graphs, no per-sequence
-        state that a dropped step would have changed)."""
-        return self.graphs is not None and self.debug is None and self._stateless and not self.layer_dump
+        state, sums of attention weights among it, that a dropped step would have changed)."""
+        return self.graphs is not None and self.debug is None and self._stateless and not self.layer_dump and not self.cache_budget
 
     def step_ahead(self, seqs: Sequence[Sequence_], tokens_dev: torch.Tensor) -> torch.Tensor:
         """Launches the decode step whose tokens are `tokens_dev` (int32, one per sequence, on the device: the
@@ -366,8 +418,7 @@ class Engine:
     def commit_ahead(self) -> None:
         seqs, n_new = self._ahead
         self._ahead = None
-        self.cache.commit(seqs, n_new)
-        self.steps_run += 1
+        self._commit(seqs, n_new)
 
     def drop_ahead(self) -> None:
         self._ahead = None

@@ -67,11 +67,18 @@ def _check_step(cu_seqlens, held, page_table, what: str) -> int:
 
 def write_rows8(qkv: torch.Tensor, bias: Optional[torch.Tensor], cos: Optional[torch.Tensor], sin: Optional[torch.Tensor], pairing: str,
                 positions: torch.Tensor, cu_seqlens: torch.Tensor, held: torch.Tensor, page_table: torch.Tensor, page_size: int,
-                q_out: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, n_heads: int, n_kv_heads: int, head_dim: int, max_q_len: int) -> None:
+                q_out: torch.Tensor, codes: Optional[torch.Tensor], scales: Optional[torch.Tensor], n_heads: int, n_kv_heads: int, head_dim: int,
+                max_q_len: int) -> None:
     """Bias and rotary encoding (by positions [T]; cos and sin [positions, head_dim / 2] float32 or None) on the fused projection qkv
-    [T, (nh + 2 nkv) * hd]; queries to q_out [T, nh, hd], keys and values as codes to their places.  max_q_len: the longest run."""
+    [T, (nh + 2 nkv) * hd]; queries to q_out [T, nh, hd], keys and values as codes to their places (codes and scales None: the queries
+    only, for layers that read another layer's cache).  max_q_len: the longest run."""
     T = qkv.shape[0]
-    _check_cache(codes, scales, None, page_table, page_size, n_kv_heads, head_dim)
+    if (codes is None) != (scales is None):
+        raise KernelError("write_rows8: codes and scales come together")
+    if codes is None:
+        check_sizes(page_size, head_dim)
+    else:
+        _check_cache(codes, scales, None, page_table, page_size, n_kv_heads, head_dim)
     n = _check_step(cu_seqlens, held, page_table, "write_rows8")
     want_int32(positions, "positions")
     if qkv.shape[1] != (n_heads + 2 * n_kv_heads) * head_dim or q_out.numel() != T * n_heads * head_dim or positions.numel() != T or q_out.dtype != qkv.dtype \
@@ -90,7 +97,7 @@ def write_rows8(qkv: torch.Tensor, bias: Optional[torch.Tensor], cos: Optional[t
     check("cache8", load_kernel("cache8").tq_write8(
         ptr(qkv), code(qkv.dtype), ptr(bias), 0 if bias is None else code(bias.dtype), ptr(cos), ptr(sin), PAIRING[pairing], ptr(positions),
         ptr(cu_seqlens), ptr(held), ptr(page_table), page_table.shape[1], page_size, ptr(q_out), ptr(codes), ptr(scales),
-        codes.shape[0], n, *ints(max_q_len, n_heads, n_kv_heads, head_dim), stream()))
+        0 if codes is None else codes.shape[0], n, *ints(max_q_len, n_heads, n_kv_heads, head_dim), stream()))
 
 
 def ranges_for(tiles: int, blocks: int, resident: int) -> int:

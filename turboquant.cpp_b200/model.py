@@ -26,32 +26,36 @@ class Model:
     def __init__(self, path: str, *, temperature: float = 0.7, top_p: float = 0.9, max_tokens: int = 256,
                  context_length: int = 0, seed: int = 42, dtype: str = "bfloat16", device: str = "cuda:0",
                  max_batch: int = 8, stop_token_ids: Optional[Sequence[int]] = None, rep_penalty: float = 1.0,
-                 rep_window: int = 32, detect_loops: bool = False):
+                 rep_window: int = 32, detect_loops: bool = False, cache_dtype: str = "", cache_budget: int = 0,
+                 cache_recent: Optional[int] = None):
         """path: folder with config.json and safetensors.  context_length: most tokens one request
         may hold (0: the model's max_position_embeddings, capped at 4096 as the reference caps its
         default context, src/engine/tq_model.c:2951).  The cache is sized for max_batch such requests.
         rep_penalty > 1 lowers the logits of a request's last rep_window tokens before each draw, as the
         reference does with 1.1 over 32 tokens (include/turboquant/tq_engine.h:408-409); 1 (the default
         here) leaves the logits alone.  detect_loops ends a request when its last four tokens have come up three
-        times among the 64 draws before, as the reference always does (src/engine/tq_generate.c:610-630)."""
+        times among the 64 draws before, as the reference always does (src/engine/tq_generate.c:610-630).
+        cache_dtype="e4m3" keeps keys and values in 8 bits; cache_budget > 0 bounds the rows a request keeps of them, cache_recent of
+        which are its newest (engine.Engine; models whose layers are all plain attention)."""
         if not os.path.isdir(path):
             raise FileNotFoundError(f"model folder '{path}' does not exist")
         self._setup(load_model(path, dtype, device), path, temperature, top_p, max_tokens, context_length, seed,
-                    device, max_batch, stop_token_ids, rep_penalty, rep_window, detect_loops)
+                    device, max_batch, stop_token_ids, rep_penalty, rep_window, detect_loops, cache_dtype, cache_budget, cache_recent)
 
     @classmethod
     def from_model(cls, model, *, temperature: float = 0.7, top_p: float = 0.9, max_tokens: int = 256,
                    context_length: int = 0, seed: int = 42, device: str = "cuda:0", max_batch: int = 8,
                    stop_token_ids: Optional[Sequence[int]] = None, rep_penalty: float = 1.0,
-                   rep_window: int = 32, detect_loops: bool = False) -> "Model":
+                   rep_window: int = 32, detect_loops: bool = False, cache_dtype: str = "", cache_budget: int = 0,
+                   cache_recent: Optional[int] = None) -> "Model":
         """Wraps a model that is already on the device (for instance one with random weights)."""
         self = cls.__new__(cls)
         self._setup(model, "", temperature, top_p, max_tokens, context_length, seed, device, max_batch, stop_token_ids,
-                    rep_penalty, rep_window, detect_loops)
+                    rep_penalty, rep_window, detect_loops, cache_dtype, cache_budget, cache_recent)
         return self
 
     def _setup(self, model, path, temperature, top_p, max_tokens, context_length, seed, device, max_batch,
-               stop_token_ids, rep_penalty=1.0, rep_window=32, detect_loops=False) -> None:
+               stop_token_ids, rep_penalty=1.0, rep_window=32, detect_loops=False, cache_dtype="", cache_budget=0, cache_recent=None) -> None:
         self._path = path
         self.rep_penalty, self.rep_window, self.detect_loops = float(rep_penalty), int(rep_window), bool(detect_loops)
         self.temperature, self.top_p, self.max_tokens, self.seed = temperature, top_p, max_tokens, seed
@@ -60,9 +64,10 @@ class Model:
         ctx = int(context_length) if context_length and context_length > 0 else min(self._model.max_position, 4096)
         self.context_length = min(ctx, self._model.max_position)
         page = PAGE_SIZE
+        cache = dict(cache_dtype=cache_dtype, cache_budget=cache_budget, cache_recent=cache_recent) if cache_dtype or cache_budget else {}
         per_request = -(-self.context_length // page) * page
         self._engine = Engine(self._model, max_tokens=per_request * self.max_batch, max_slots=max(self.max_batch, 1),
-                              device=device)
+                              device=device, **cache)
         eos = getattr(self._model.config, "eos_token_ids", ())
         self.stop_token_ids = tuple(stop_token_ids) if stop_token_ids is not None else tuple(eos)
         self.last_stats: Optional[GenStats] = None

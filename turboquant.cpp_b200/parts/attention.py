@@ -14,6 +14,7 @@ from typing import List, Optional
 import torch
 
 from ..kernels import attention as KA
+from ..kernels import cache8 as K8
 from ..kernels import elementwise as KE
 from ..kernels import gemv as KG
 from ..kernels.linear import linear
@@ -22,6 +23,7 @@ from .base import KVNeed, LayerCache, Mixer, PositionEncoding, StepContext, regi
 
 
 class AttentionMixer(Mixer):
+    takes_cache8 = True
     PREFILL_MIN_RUN = 48      # steps whose longest run of new tokens is at least this use the prompt kernel
 
     def __init__(self, prefix: str, hidden: int, n_heads: int, n_kv_heads: int, head_dim: int,
@@ -69,6 +71,10 @@ class AttentionMixer(Mixer):
             names.append("attention_prefill")
         if getattr(self, "run_dtype", None) == torch.float32 and self.head_dim in KA.F32_HEAD_DIMS:
             names.append("attention_f32")
+        if getattr(self, "cache8", False):
+            names += ["cache8", "attention8", "evict"]
+            if "attention_prefill" in names:
+                names.append("prompt8")
         return names + self.product_kernels(self.hidden, self.q_size)
 
     def cache_need(self) -> KVNeed:
@@ -77,7 +83,7 @@ class AttentionMixer(Mixer):
     def step_work(self, n_tokens, kv_tokens):
         wb = lambda w: 0 if w is None else w.numel() * w.element_size()
         proj = self.hidden * (self.q_size + 2 * self.kv_size) + self.q_size * self.hidden
-        kv_el = 2 if getattr(self, "run_dtype", None) == torch.bfloat16 else 4
+        kv_el = 1 + 1 / K8.BLOCK / self.head_dim if getattr(self, "cache8", False) else 2 if getattr(self, "run_dtype", None) == torch.bfloat16 else 4
         seen = min(kv_tokens, n_tokens * self.window) if self.window else kv_tokens
         return {"matmul": (wb(self.w_qkv) + wb(self.w_o), 2.0 * n_tokens * proj),
                 "attn": (2.0 * self.kv_size * kv_el * seen, 4.0 * self.q_size * seen)}
@@ -87,7 +93,7 @@ class AttentionMixer(Mixer):
         act = ctx.act_dtype
         q = torch.empty((T, self.n_heads, self.head_dim), dtype=act, device=xn.device)
         tables = self.position.tables() if self.position is not None else None
-        fused = (KG.fused_pays(xn, self.w_qkv) and (self.position is None or (tables is not None and tables[2] == "half"))
+        fused = (cache.scales is None and KG.fused_pays(xn, self.w_qkv) and (self.position is None or (tables is not None and tables[2] == "half"))
                  and (cache.kv is None or cache.kv.dtype == torch.bfloat16))
         if fused:
             # one or two tokens: the projection is a stream of its weights; bias, rotation and the cache write
@@ -108,6 +114,14 @@ class AttentionMixer(Mixer):
             rows = qkv.view(T, self.n_heads + 2 * self.n_kv_heads, self.head_dim)
             self.position.apply(rows[:, :self.n_heads], rows[:, self.n_heads:self.n_heads + self.n_kv_heads], ctx.positions)
         cos, sin, pairing = tables if tables is not None else (None, None, "half")
+        if cache.scales is not None:
+            held = ctx.held if ctx.held is not None else ctx.seq_start
+            K8.write_rows8(qkv, bias, cos, sin, pairing, ctx.positions, ctx.cu_seqlens, held, cache.page_table, cache.page_size, q,
+                           cache.kv if cache.writes else None, cache.scales if cache.writes else None, self.n_heads, self.n_kv_heads, self.head_dim, ctx.max_q_len)
+            o = K8.attention8(q, cache.kv, cache.scales, ctx.cu_seqlens, held, cache.page_table, cache.page_size, self.window, self.scale,
+                              torch.empty((T, self.q_size), dtype=act, device=xn.device), self.n_heads, self.n_kv_heads, self.head_dim, ctx.max_q_len,
+                              ctx.max_kv_len, weights=cache.weights, status=ctx.status)
+            return self._project(o, T, ctx)
         KA.qkv_rope_cache(qkv, bias, cos, sin, pairing, ctx.positions, ctx.seq_of_token, cache.page_table,
                           cache.page_size, q, cache.kv if cache.writes else None,
                           self.n_heads, self.n_kv_heads, self.head_dim)
@@ -141,6 +155,9 @@ class AttentionMixer(Mixer):
         else:
             KA.attention(q, cache.kv, ctx.positions, ctx.seq_of_token, cache.page_table, cache.page_size,
                          self.window, self.scale, o, self.n_heads, self.n_kv_heads, self.head_dim)
+        return self._project(o, T, ctx)
+
+    def _project(self, o: torch.Tensor, T: int, ctx: StepContext) -> torch.Tensor:
         if KG.pays(o, self.w_o):
             return KG.gemv(o, self.w_o, torch.empty((T, self.hidden), dtype=torch.float32, device=o.device))
         return linear(o, self.w_o, out_dtype=torch.float32, status=ctx.status)

@@ -70,6 +70,8 @@ class LayerCache:
     page_size: int = 0
     writes: bool = True                          # False: reads another entry's cache, writes nothing
     state: Optional[torch.Tensor] = None         # [max_slots, *StateNeed.shape]
+    scales: Optional[torch.Tensor] = None        # a cache in 8 bits (kernels.cache8): kv holds codes, this their blocks' bytes
+    weights: Optional[torch.Tensor] = None       # ... and this the attention weight each row has received, where sequences are evicted by it
 
 
 @dataclass
@@ -97,6 +99,8 @@ class StepContext:
     debug: Optional[Dict[str, Any]] = None      # tests: parts may record what they decided
     status: Optional[torch.Tensor] = None       # int32 [1]: kernels with bounded waits report here when one ran out
     embed_state: Optional[torch.Tensor] = None  # [max_slots, *shape]: the embedding's per-sequence state, if it keeps one
+    # [B] int32: cache rows each sequence held before this step, fewer than its positions where rows were evicted (None: seq_start)
+    held: Optional[torch.Tensor] = None
     # what a layer hands to later layers of the same step (the model empties it when a step starts): tensors over
     # the step's tokens under names the parts agree on, e.g. the values that later layers mix into their own
     carry: Dict[str, torch.Tensor] = field(default_factory=dict)
@@ -210,6 +214,9 @@ class PositionEncoding(Part):
 
 
 class Mixer(Part):
+    # whether forward reads and writes a cache in 8 bits (LayerCache.scales); an engine that keeps one sets `cache8` on its mixers before it
+    # builds their kernels
+    takes_cache8 = False
     runs_alone = False            # whether runs of many tokens go through a long kernel of few blocks that wants the GPU to itself
 
     def alone(self, ctx: StepContext) -> bool:
