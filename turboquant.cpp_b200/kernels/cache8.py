@@ -23,6 +23,7 @@ import torch
 from ..csrc.build import load_kernel
 from ._call import KernelError, check, code, ints, on_current_device, ptr, stream, want_f32, want_int32
 from .attention import PAIRING, prefill_rows, prefill_usable, resident_ctas
+from .gemm_tc import status_word
 
 BLOCK = 16
 MAX_HEAD_DIM = 256
@@ -171,6 +172,8 @@ def _attention8_prompt(q, codes, scales, cu_seqlens, held, page_table, page_size
                        max_kv_len, weights, status):
     """The pages a step sees are expanded to bfloat16 pages of a scratch, exactly, and the prompt kernel of csrc/attention_prefill.cu reads those."""
     T, n = q.shape[0], page_table.shape[0]
+    if status is None:
+        status = status_word(q.device)
     width = -(-max_kv_len // page_size)
     page_bytes = 2 * n_kv_heads * page_size * head_dim * 2
     group = max(1, min(n, DENSE_BYTES // (page_bytes * width)))
@@ -186,10 +189,10 @@ def _attention8_prompt(q, codes, scales, cu_seqlens, held, page_table, page_size
         prefill_rows(q, dense, 2, cu, starts, dtable, page_size, window, scale, out, m, max_q_len, n_heads, n_kv_heads, head_dim, head_dim, status=status, lse=lse)
         check("attention8", load_kernel("attention8").tq_repair8(
             ptr(q), *cache, c_float(scale), ptr(out), ptr(lost), width, codes.shape[0], m, *ints(n_heads, n_kv_heads, head_dim), stream()))
-    if weights is not None:
-        check("attention8", load_kernel("attention8").tq_weigh8(
-            ptr(q), ptr(codes), ptr(scales), code(q.dtype), ptr(cu_seqlens), ptr(held), ptr(page_table), page_table.shape[1], *ints(page_size, window), c_float(scale),
-            ptr(lse), ptr(weights), codes.shape[0], n, *ints(max_q_len, max_kv_len, n_heads, n_kv_heads, head_dim), stream()))
+        if weights is not None:
+            check("prompt8", load_kernel("prompt8").tq_weigh8_prompt(
+                ptr(q), ptr(dense), width, ptr(cu), ptr(starts), ptr(pages), pages.shape[1], *ints(window), c_float(scale), ptr(lse), ptr(weights),
+                codes.shape[0], T, m, *ints(max_kv_len, n_heads, n_kv_heads, head_dim), ptr(status), stream()))
     return out
 
 
