@@ -60,9 +60,9 @@ struct Step {
 struct Tile {
     int t_begin, run, start, per, first, n;           // n columns from number `first` on, counted row by row
     int seq, g;
-    __device__ __forceinline__ int row(int col) const { return (first + col) / per; }
+    __device__ __forceinline__ int row(int col) const { return per == 1 ? first + col : (first + col) / per; }
     __device__ __forceinline__ size_t query(int col, const Step& S) const {           // row of q as [T * nh]
-        const int c = first + col, r = c / per;
+        const int c = first + col, r = row(col);
         return (size_t)(t_begin + r) * S.nh + g * per + (c - r * per);
     }
 };
@@ -78,19 +78,32 @@ __device__ __forceinline__ Tile tile_of(const Step& S, int seq, int g, int nkv, 
     return t;
 }
 
-// The tile's queries in shared memory as right operands, [part][8 columns][step of 16 elements][lane], and each column's factor: score =
-// (sum of the products) * factor * 2^(key byte - 127).
-template <typename TA, int HDP, int NT> struct Queries {
-    static constexpr int PARTS = sizeof(TA) == 4 ? 2 : 1, STEPS = HDP / 16;
-    uint2 b[PARTS][NT][STEPS][32];
-    float factor[NT * 8], up[NT * 8];
-    __device__ void load(const TA* q, const Tile& t, const Step& S, int hd) {
+// Head sizes: HDP elements have registers; EXACT: the head has just that many (its offsets are then constants), else a multiple of 16 below.
+template <typename TA_, int HDP_, int NT_, bool EXACT_> struct Form {
+    using TA = TA_;
+    static constexpr int HDP = HDP_, NT = NT_, NC = NT * 8, MT = HDP / 16, STEPS = HDP / 16, PARTS = sizeof(TA) == 4 ? 2 : 1;
+    static constexpr bool EXACT = EXACT_, KEEP = NT * PARTS == 1 && HDP <= 128;       // KEEP: the queries stay in registers
+    static constexpr int KP = HDP / 64 * 2, VG = HDP > 128 ? 2 : 1, VB = HDP == 64 ? 8 : 16, STAGES = 3;
+    static constexpr int STAGE_BYTES = (KP * 16 + VG * 4 * VB) * 32, RING = WARPS * STAGES * STAGE_BYTES, SUMS = WARPS * NC * (HDP + 4) * 4;
+    static constexpr int SMEM = RING > SUMS ? RING : SUMS;
+    static constexpr int PER_SM = HDP > 128 ? 2 : HDP * NT > 128 ? 3 : 4;              // CTAs an SM holds (the registers' limit)
+};
+
+// The tile's queries in shared memory as right operands, [part][8 columns][step of 16 elements][lane], each column's factor (score =
+// (sum of the products) * factor * 2^(key byte - 127)), its row in q and its place (columns that are not there: place -1).
+template <class F> struct Queries {
+    uint2 b[F::PARTS][F::NT][F::STEPS][32];
+    float factor[F::NC], up[F::NC];
+    int place[F::NC];
+    size_t row[F::NC];
+    __device__ __forceinline__ void load(const typename F::TA* q, const Tile& t, const Step& S, int hd) {
         const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-        for (int c = warp; c < NT * 8; c += WARPS) {
+        for (int c = warp; c < F::NC; c += WARPS) {
             uint32_t top = 0;
+            size_t at = 0;
             if (c < t.n) {
-                const TA* row = q + t.query(c, S) * hd;
-                for (int d = lane; d < hd; d += 32) top = max(top, c8_magnitude(tq_to_float(row[d])));
+                at = t.query(c, S);
+                for (int d = lane; d < hd; d += 32) top = max(top, c8_magnitude(tq_to_float(q[at * hd + d])));
             }
             top = __reduce_max_sync(0xffffffffu, top);
             if (lane == 0) {
@@ -98,24 +111,26 @@ template <typename TA, int HDP, int NT> struct Queries {
                 const int shift = min(126, 14 - max((int)(top >> 23) - 127, -126));
                 up[c] = __uint_as_float((uint32_t)(127 + shift) << 23);
                 factor[c] = S.factor * __uint_as_float((uint32_t)(127 - shift) << 23);
+                place[c] = c < t.n ? t.start + t.row(c) : -1;
+                row[c] = at;
             }
         }
         __syncthreads();
-        for (int i = threadIdx.x; i < NT * STEPS * 32; i += WARPS * 32) {
-            const int l = i & 31, step = i / 32 % STEPS, nt = i / 32 / STEPS, c = nt * 8 + (l >> 2), d = (step / 4) * 64 + (l & 3) * 16 + (step & 3) * 4;
+        for (int i = threadIdx.x; i < F::NT * F::STEPS * 32; i += WARPS * 32) {
+            const int l = i & 31, step = i / 32 % F::STEPS, nt = i / 32 / F::STEPS, c = nt * 8 + (l >> 2), d = (step / 4) * 64 + (l & 3) * 16 + (step & 3) * 4;
             float f[4] = {0.f, 0.f, 0.f, 0.f};
             if (c < t.n && d < hd) {
-                const TA* row = q + t.query(c, S) * hd + d;
+                const typename F::TA* x = q + row[c] * hd + d;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) f[e] = tq_to_float(row[e]) * up[c];
+                for (int e = 0; e < 4; ++e) f[e] = tq_to_float(x[e]) * up[c];
             }
             const uint2 hi = make_uint2(half2_of(f[0], f[1]), half2_of(f[2], f[3]));
             b[0][nt][step][l] = hi;
-            if (PARTS == 2) {
+            if (F::PARTS == 2) {
                 const float2 x = float2_of(hi.x), y = float2_of(hi.y);
                 // (what is not finite stays in the first part alone)
                 auto left = [](float v, float h) { const float r = v - h; return fabsf(r) < INFINITY ? r : 0.f; };
-                b[PARTS - 1][nt][step][l] = make_uint2(half2_of(left(f[0], x.x), left(f[1], x.y)), half2_of(left(f[2], y.x), left(f[3], y.y)));
+                b[F::PARTS - 1][nt][step][l] = make_uint2(half2_of(left(f[0], x.x), left(f[1], x.y)), half2_of(left(f[2], y.x), left(f[3], y.y)));
             }
         }
         __syncthreads();
@@ -123,161 +138,223 @@ template <typename TA, int HDP, int NT> struct Queries {
 };
 
 // A lane's codes of a block of 16 keys: K rows lane / 4 and 8 more, 16 bytes of every 64; V rows 2 (lane % 4) and the next, and 8 more of both.
-template <int HDP> struct KeyRegs { uint4 k[HDP / 64][2]; };
-template <int HDP> struct ValueRegs { uint4 v[HDP > 128 ? 2 : 1][4]; };
+template <class F> struct KeyRegs { uint4 k[F::HDP / 64][2]; };
+template <class F> struct ValueRegs { uint4 v[F::VG][4]; };
 
-template <int HDP>
-__device__ __forceinline__ void load_keys(KeyRegs<HDP>& r, const uint8_t* rows, int hd) {
-    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-#pragma unroll
-    for (int j = 0; j < HDP / 64; ++j) {
-        const int d = j * 64 + t * 16;
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-            r.k[j][h] = d < hd ? __ldg(reinterpret_cast<const uint4*>(rows + (size_t)(g + 8 * h) * hd + d)) : make_uint4(0, 0, 0, 0);
-    }
+template <int B> __device__ __forceinline__ void copy_async(uint32_t to, const uint8_t* from, bool there) {
+    const int n = there ? B : 0;       // 0: zeros
+    if (B == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(n) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(to), "l"(from), "r"(n) : "memory");
 }
-template <int HDP>
-__device__ __forceinline__ void load_values(ValueRegs<HDP>& r, const uint8_t* rows, int hd) {
-    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+// A block on its way: a ring in shared memory in which every lane copies its own pieces and reads only those, so that it needs no barrier
+// and no bank is hit twice.  k, v: the block's first key and value row; at: the warp's stage (pieces lie 512 or 256 bytes apart).
+template <class F>
+__device__ __forceinline__ void copy_block(uint32_t at, const uint8_t* k, const uint8_t* v, int hd_) {
+    const int hd = F::EXACT ? F::HDP : hd_, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const uint8_t *kl = k + g * hd + t * 16, *vl = v + 2 * t * hd + g * F::VB;
+    at += lane * 16;
 #pragma unroll
-    for (int j = 0; j < (HDP > 128 ? 2 : 1); ++j)
+    for (int j = 0; j < F::HDP / 64; ++j)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const int row = 2 * t + (k & 1) + 8 * (k >> 1);
-            if (HDP == 64) {
-                const uint2 x = g * 8 < hd ? __ldg(reinterpret_cast<const uint2*>(rows + (size_t)row * hd + g * 8)) : make_uint2(0, 0);
-                r.v[j][k] = make_uint4(x.x, x.y, 0, 0);
-            } else {
-                const int d = j * 128 + g * 16;
-                r.v[j][k] = d < hd ? __ldg(reinterpret_cast<const uint4*>(rows + (size_t)row * hd + d)) : make_uint4(0, 0, 0, 0);
-            }
+        for (int h = 0; h < 2; ++h) {
+            const bool there = F::EXACT || j * 64 + t * 16 < hd;
+            copy_async<16>(at + (j * 2 + h) * 512, there ? kl + 8 * h * hd + j * 64 : k, there);
         }
+    at += F::KP * 512 - lane * (16 - F::VB);
+#pragma unroll
+    for (int j = 0; j < F::VG; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const bool there = F::EXACT || j * 128 + g * F::VB < hd;
+            copy_async<F::VB>(at + (j * 4 + r) * 32 * F::VB, there ? vl + ((r & 1) + 8 * (r >> 1)) * hd + j * 128 : v, there);
+        }
+}
+template <class F>
+__device__ __forceinline__ void take_block(KeyRegs<F>& kr, ValueRegs<F>& vr, const uint8_t* at) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int i = 0; i < F::KP; ++i) kr.k[i / 2][i % 2] = *reinterpret_cast<const uint4*>(at + i * 512 + lane * 16);
+#pragma unroll
+    for (int i = 0; i < F::VG * 4; ++i) {
+        const uint8_t* p = at + F::KP * 512 + i * 32 * F::VB + lane * F::VB;
+        if (F::HDP == 64) {
+            const uint2 x = *reinterpret_cast<const uint2*>(p);
+            vr.v[i / 4][i % 4] = make_uint4(x.x, x.y, 0, 0);
+        } else vr.v[i / 4][i % 4] = *reinterpret_cast<const uint4*>(p);
+    }
 }
 __device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 
-// Scores of a block: s[nt] = {key g column 2t, key g column 2t + 1, key g + 8 ..}, without their factors.
-template <typename TA, int HDP, int NT>
-__device__ __forceinline__ void products(float (&s)[NT][4], const KeyRegs<HDP>& r, const Queries<TA, HDP, NT>& Q) {
+// Sums of a block: s[nt] = {key g column 2t, key g column 2t + 1, key g + 8 ..}, without their factors.  One column tile: two chains of
+// products, added at the end.  kept: the lane's part of the queries, where they stay in registers.
+template <class F>
+__device__ __forceinline__ void products(float (&s)[F::NT][4], const KeyRegs<F>& r, const Queries<F>& Q, const uint2* kept) {
     const int lane = threadIdx.x & 31;
+    float odd[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+    for (int nt = 0; nt < F::NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
 #pragma unroll
-    for (int j = 0; j < HDP / 64; ++j)
+    for (int j = 0; j < F::HDP / 64; ++j)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const uint32_t x = word(r.k[j][0], i), y = word(r.k[j][1], i);
-            const uint32_t a0 = c8_half2(x & 0xffffu), a2 = c8_half2(x >> 16), a1 = c8_half2(y & 0xffffu), a3 = c8_half2(y >> 16);
+            uint32_t a0, a1, a2, a3;
+            c8_half4(word(r.k[j][0], i), a0, a2);
+            c8_half4(word(r.k[j][1], i), a1, a3);
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+            for (int nt = 0; nt < F::NT; ++nt)
 #pragma unroll
-                for (int p = 0; p < Queries<TA, HDP, NT>::PARTS; ++p) {
-                    const uint2 b = Q.b[p][nt][j * 4 + i][lane];
-                    mma(s[nt], a0, a1, a2, a3, b.x, b.y);
+                for (int p = 0; p < F::PARTS; ++p) {
+                    const uint2 b = F::KEEP ? kept[j * 4 + i] : Q.b[p][nt][j * 4 + i][lane];
+                    if (F::NT == 1 && ((i + p) & 1)) mma(odd, a0, a1, a2, a3, b.x, b.y);
+                    else mma(s[nt], a0, a1, a2, a3, b.x, b.y);
                 }
         }
+    if (F::NT == 1) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[0][i] += odd[i];
+    }
 }
 
-// Where a row of the step looks: the first and the last of its places.
+// Where a row of the step looks: the first of its places.
 __device__ __forceinline__ int first_seen(int place, int window) { return window > 0 ? max(0, place + 1 - window) : 0; }
+
+constexpr float LOWEST = -3.402823466e38f;       // a maximum over nothing
 
 // ---------------------------------------------------------------------------------------
 // A range of the keys for a tile of columns.  partial: null, or [T * nh][ranges][hd + 4] for a second launch: the unnormalised sum, the
 // maximum m' it is relative to, the denominator's maximum and the denominator.  scores: null, or [T * nh][score_stride], base-2 scores.
 // lse: null, or [T * nh], log2 of the denominator (where there is no second launch).
 // ---------------------------------------------------------------------------------------
-template <typename TA, int HDP, int NT>
-__device__ __forceinline__ void attend_tile(const Tile& T, int range, int ranges, const TA* __restrict__ q, const Cache8& c, const Step& S, TA* __restrict__ out,
-                                            float* __restrict__ partial, float* __restrict__ scores, int score_stride, float* __restrict__ lse) {
-    constexpr int NC = NT * 8, MT = HDP / 16;
-    __shared__ Queries<TA, HDP, NT> Q;
-    __shared__ float s_o[WARPS][NC][HDP + 4];
+template <class F>
+__device__ __forceinline__ void attend_tile(const Tile& T, int range, int ranges, const typename F::TA* __restrict__ q, const Cache8& c, const Step& S,
+                                            typename F::TA* __restrict__ out, float* __restrict__ partial, float* __restrict__ scores, int score_stride,
+                                            float* __restrict__ lse) {
+    constexpr int NT = F::NT, NC = F::NC, MT = F::MT, HDP = F::HDP;
+    extern __shared__ __align__(16) uint8_t ring[];
+    __shared__ Queries<F> Q;
     __shared__ float s_stat[WARPS][NC][3];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, hd = c.hd;
+    float (*s_o)[NC][HDP + 4] = reinterpret_cast<float (*)[NC][HDP + 4]>(ring);        // [WARPS], once the keys are through
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, hd = F::EXACT ? HDP : c.hd;
     // this range's blocks of 16 keys
     const int place0 = T.start + T.row(0), place1 = T.start + T.row(T.n - 1);
     const int block0 = first_seen(place0, S.window) / C8_BLOCK, blocks = place1 / C8_BLOCK + 1 - block0;
     const int each = (blocks + ranges * WARPS - 1) / (ranges * WARPS) * WARPS;
     const int from = block0 + range * each, to = min(from + each, block0 + blocks);
-    Q.load(q, T, S, hd);
 
-    int place_of[NT][2];               // the lane's columns' places (columns that are not there see nothing)
+    // The blocks the warp still has to ask for: column of the page table and block of that page; the page is looked up one block ahead.
+    const int per_page = c.page_size / C8_BLOCK;
+    int ask = from + warp, column = ask / per_page, inner = ask - column * per_page, slot = 0;
+    const int* pages = c.table + (size_t)T.seq * c.table_stride;
+    auto page_at = [&](int col) { return TQ_CHECKED(pages[TQ_CHECKED(col, c.table_stride, TQ_IDX_TABLE_COLUMN)], c.n_pages, TQ_IDX_PAGE); };
+    int page = ask < to ? page_at(column) : 0;
+    uint32_t kbs[F::STAGES - 1], vbs[F::STAGES - 1];      // the bytes of the blocks on their way, oldest first
+    const uint32_t mine = (uint32_t)__cvta_generic_to_shared(ring) + warp * (F::STAGES * F::STAGE_BYTES);
+    // (a page's codes stay below 2^31 bytes: head size, page size and heads as the launcher takes them)
+    const uint32_t plane = (uint32_t)c.nkv * c.page_size * hd, plane_scales = (uint32_t)c.nkv * per_page;
+    const uint8_t* codes_g = c.codes + (size_t)T.g * c.page_size * hd;
+    const uint8_t* scales_g = c.scales + (size_t)T.g * per_page;
+    auto next = [&](uint32_t& kb, uint32_t& vb) {
+        if (ask < to) {
+            const uint8_t* k = codes_g + (size_t)(uint32_t)page * (2u * plane) + (uint32_t)(inner * (C8_BLOCK * hd));
+            copy_block<F>(mine + slot * F::STAGE_BYTES, k, k + plane, hd);
+            const uint8_t* b8 = scales_g + (size_t)(uint32_t)page * (2u * plane_scales) + inner;
+            kb = __ldg(b8);
+            vb = __ldg(b8 + plane_scales);
+            ask += WARPS;
+            inner += WARPS;
+            const int was = column;
+            while (inner >= per_page) { inner -= per_page; ++column; }
+            if (column != was && ask < to) page = page_at(column);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        slot = slot + 1 == F::STAGES ? 0 : slot + 1;
+    };
+#pragma unroll
+    for (int i = 0; i < F::STAGES - 1; ++i) { kbs[i] = vbs[i] = 1; next(kbs[i], vbs[i]); }
+
+    Q.load(q, T, S, hd);
+    int place_of[NT][2];               // the lane's columns' places
     float f[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-            const int col = nt * 8 + 2 * t + j;
-            place_of[nt][j] = col < T.n ? T.start + T.row(col) : -1;
-            f[nt][j] = Q.factor[col];
+            place_of[nt][j] = Q.place[nt * 8 + 2 * t + j];
+            f[nt][j] = Q.factor[nt * 8 + 2 * t + j];
         }
+    uint2 kept[F::KEEP ? F::STEPS : 1];
+    if (F::KEEP) {
+#pragma unroll
+        for (int i = 0; i < F::STEPS; ++i) kept[F::KEEP ? i : 0] = Q.b[0][0][i][lane];
+    }
     float o[NT][MT][4], m[NT][2], mo[NT][2], l[NT][2];        // m: of the scores, mo: of scores and value scales
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
         for (int i = 0; i < MT; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
-        m[nt][0] = m[nt][1] = mo[nt][0] = mo[nt][1] = -INFINITY;
+        m[nt][0] = m[nt][1] = mo[nt][0] = mo[nt][1] = LOWEST;
         l[nt][0] = l[nt][1] = 0.f;
     }
-    KeyRegs<HDP> kr;
-    ValueRegs<HDP> vr;
-    uint32_t kb = 1, vb = 1;
-    auto fetch = [&](int b, int page, KeyRegs<HDP>& k, ValueRegs<HDP>& v) {
-        const int row = b * C8_BLOCK % c.page_size;
-        load_keys<HDP>(k, c.codes + c.codes_at(page, 0, T.g) + (size_t)row * hd, hd);
-        load_values<HDP>(v, c.codes + c.codes_at(page, 1, T.g) + (size_t)row * hd, hd);
-        kb = c.scales[c.scales_at(page, 0, T.g) + row / C8_BLOCK];
-        vb = c.scales[c.scales_at(page, 1, T.g) + row / C8_BLOCK];
-    };
-    int b = from + warp;
-    if (b < to) fetch(b, c.page_of(T.seq, b * C8_BLOCK), kr, vr);
-    int next_page = b + WARPS < to ? c.page_of(T.seq, (b + WARPS) * C8_BLOCK) : 0;
-    for (; b < to; b += WARPS) {
-        const KeyRegs<HDP> kc = kr;
-        const ValueRegs<HDP> vc = vr;
-        const float ks = c8_scale(kb), ve = (float)((int)vb - 127);
-        if (b + WARPS < to) {
-            fetch(b + WARPS, next_page, kr, vr);
-            next_page = b + 2 * WARPS < to ? c.page_of(T.seq, (b + 2 * WARPS) * C8_BLOCK) : 0;
-        }
+    int taken = 0;
+#pragma unroll 1
+    for (int b = from + warp; b < to; b += WARPS) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(F::STAGES - 2) : "memory");
+        KeyRegs<F> kc;
+        ValueRegs<F> vc;
+        take_block<F>(kc, vc, ring + warp * (F::STAGES * F::STAGE_BYTES) + taken * F::STAGE_BYTES);
+        taken = taken + 1 == F::STAGES ? 0 : taken + 1;
+        const float ks = c8_scale(kbs[0]), ve = (float)((int)vbs[0] - 127);
+#pragma unroll
+        for (int i = 0; i + 1 < F::STAGES - 1; ++i) { kbs[i] = kbs[i + 1]; vbs[i] = vbs[i + 1]; }
+        next(kbs[F::STAGES - 2], vbs[F::STAGES - 2]);
         float s[NT][4];
-        products<TA, HDP, NT>(s, kc, Q);
+        products<F>(s, kc, Q, kept);
         const int key = b * C8_BLOCK + g;
         // every column sees all 16 keys? (those that are not there may see them too: nobody reads their sums)
         const bool whole = b * C8_BLOCK + C8_BLOCK - 1 <= place0 && (S.window <= 0 || b * C8_BLOCK > place1 - S.window);
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int nt = 0; nt < NT; ++nt) {
+            const float f0 = f[nt][0] * ks, f1 = f[nt][1] * ks;
+            s[nt][0] *= f0; s[nt][1] *= f1; s[nt][2] *= f0; s[nt][3] *= f1;
+        }
+        if (!whole) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                s[nt][j] = s[nt][j] * (f[nt][j & 1] * ks);
-                const int p = place_of[nt][j & 1], k = key + 8 * (j >> 1);
-                if (!whole && (k > p || (S.window > 0 && k <= p - S.window))) s[nt][j] = -INFINITY;
-            }
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int p = place_of[nt][j & 1], k = key + 8 * (j >> 1);
+                    if (k > p || (S.window > 0 && k <= p - S.window)) s[nt][j] = -INFINITY;
+                }
+        }
         if (scores != nullptr) {
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const int col = nt * 8 + 2 * t + (j & 1);
-                    if (col < T.n && key + 8 * (j >> 1) < score_stride) scores[T.query(col, S) * score_stride + key + 8 * (j >> 1)] = s[nt][j];
+                    if (col < T.n && key + 8 * (j >> 1) < score_stride) scores[Q.row[col] * score_stride + key + 8 * (j >> 1)] = s[nt][j];
                 }
         }
         // the maxima grow now and then: found by all lanes of a column together when one of them sees a larger value
+        float top[NT][2];
         bool grows = false;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) grows |= s[nt][j] > m[nt][j & 1] || s[nt][j] + ve > mo[nt][j & 1];
+            for (int j = 0; j < 2; ++j) {
+                top[nt][j] = fmaxf(s[nt][j], s[nt][j + 2]);
+                grows |= top[nt][j] > m[nt][j] || top[nt][j] + ve > mo[nt][j];
+            }
         if (__any_sync(0xffffffffu, grows)) {
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    float top = fmaxf(s[nt][j], s[nt][j + 2]);
 #pragma unroll
-                    for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-                    const float mn = fmaxf(m[nt][j], top), mon = fmaxf(mo[nt][j], top + ve);
-                    if (mn > m[nt][j]) { l[nt][j] *= ex2(m[nt][j] - mn); m[nt][j] = mn; }
+                    for (int x = 4; x < 32; x <<= 1) top[nt][j] = fmaxf(top[nt][j], __shfl_xor_sync(0xffffffffu, top[nt][j], x));
+                    const float mn = fmaxf(m[nt][j], top[nt][j]), mon = fmaxf(mo[nt][j], top[nt][j] + ve);
+                    l[nt][j] *= ex2(m[nt][j] - mn);
+                    m[nt][j] = mn;
                     if (mon > mo[nt][j]) {
                         const float down = ex2(mo[nt][j] - mon);
 #pragma unroll
@@ -292,15 +369,14 @@ __device__ __forceinline__ void attend_tile(const Tile& T, int range, int ranges
             float w[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const float mr = m[nt][j & 1] == -INFINITY ? 0.f : m[nt][j & 1], mor = mo[nt][j & 1] == -INFINITY ? 0.f : mo[nt][j & 1];
-                l[nt][j & 1] += ex2(s[nt][j] - mr);
-                w[j] = ex2(s[nt][j] + ve - mor);
+                l[nt][j & 1] += ex2(s[nt][j] - m[nt][j & 1]);
+                w[j] = ex2(s[nt][j] + (ve - mo[nt][j & 1]));
             }
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const uint32_t hi = half2_of(w[2 * h], w[2 * h + 1]);
                 p_hi[nt][h] = transpose8x8(hi);
-                if (Queries<TA, HDP, NT>::PARTS == 2) {
+                if (F::PARTS == 2) {
                     const float2 x = float2_of(hi);
                     p_lo[nt][h] = transpose8x8(half2_of(w[2 * h] - x.x, w[2 * h + 1] - x.y));
                 }
@@ -308,21 +384,21 @@ __device__ __forceinline__ void attend_tile(const Tile& T, int range, int ranges
         }
         // Values no column may see come with a weight of 0, which does not remove a NaN: such codes are taken out of the product, and put
         // back as NaN into the sums of the columns that do see the key.
-        ValueRegs<HDP> vm = vc;
-        uint32_t lost[HDP > 128 ? 2 : 1][4] = {};             // of the lane's four rows: which of its 16 elements are NaN
+        uint32_t lost[F::VG][4] = {};                          // of the lane's four rows: which of its 16 elements are NaN
         bool some = false;
         if (!whole) {
 #pragma unroll
-            for (int j = 0; j < (HDP > 128 ? 2 : 1); ++j)
+            for (int j = 0; j < F::VG; ++j)
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    uint32_t* u = &vm.v[j][k].x;
+                    uint32_t u[4] = {vc.v[j][k].x, vc.v[j][k].y, vc.v[j][k].z, vc.v[j][k].w};
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const uint32_t hit = ((u[i] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;     // the top bit of every byte 0x7f or 0xff
                         lost[j][k] |= ((hit >> 7 & 1u) | (hit >> 14 & 2u) | (hit >> 21 & 4u) | (hit >> 28 & 8u)) << (4 * i);
                         u[i] &= ~((hit >> 7) * 0xffu);
                     }
+                    vc.v[j][k] = make_uint4(u[0], u[1], u[2], u[3]);
                     some |= lost[j][k] != 0;
                 }
             some = __any_sync(0xffffffffu, some);
@@ -331,15 +407,17 @@ __device__ __forceinline__ void attend_tile(const Tile& T, int range, int ranges
         for (int i = 0; i < MT; i += 2) {
             // words i / 2 of the lane's four rows: two steps of 16 elements
             const int j = HDP > 128 ? i / 8 : 0, wd = (i - 8 * j) / 2;
-            const uint32_t r0 = word(vm.v[j][0], wd), r1 = word(vm.v[j][1], wd), r2 = word(vm.v[j][2], wd), r3 = word(vm.v[j][3], wd);
-            const uint32_t x = __byte_perm(r0, r1, 0x5140), y = __byte_perm(r0, r1, 0x7362), z = __byte_perm(r2, r3, 0x5140), v = __byte_perm(r2, r3, 0x7362);
-            const uint32_t a0 = c8_half2(x & 0xffffu), a1 = c8_half2(x >> 16), a2 = c8_half2(z & 0xffffu), a3 = c8_half2(z >> 16);
-            const uint32_t e0 = c8_half2(y & 0xffffu), e1 = c8_half2(y >> 16), e2 = c8_half2(v & 0xffffu), e3 = c8_half2(v >> 16);
+            const uint32_t r0 = word(vc.v[j][0], wd), r1 = word(vc.v[j][1], wd), r2 = word(vc.v[j][2], wd), r3 = word(vc.v[j][3], wd);
+            uint32_t a0, a1, a2, a3, e0, e1, e2, e3;
+            c8_half4(__byte_perm(r0, r1, 0x5140), a0, a1);
+            c8_half4(__byte_perm(r2, r3, 0x5140), a2, a3);
+            c8_half4(__byte_perm(r0, r1, 0x7362), e0, e1);
+            c8_half4(__byte_perm(r2, r3, 0x7362), e2, e3);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
                 mma(o[nt][i], a0, a1, a2, a3, p_hi[nt][0], p_hi[nt][1]);
                 mma(o[nt][i + 1], e0, e1, e2, e3, p_hi[nt][0], p_hi[nt][1]);
-                if (Queries<TA, HDP, NT>::PARTS == 2) {
+                if (F::PARTS == 2) {
                     mma(o[nt][i], a0, a1, a2, a3, p_lo[nt][0], p_lo[nt][1]);
                     mma(o[nt][i + 1], e0, e1, e2, e3, p_lo[nt][0], p_lo[nt][1]);
                 }
@@ -348,11 +426,11 @@ __device__ __forceinline__ void attend_tile(const Tile& T, int range, int ranges
         if (some) {
 #pragma unroll 1
             for (int k16 = 0; k16 < C8_BLOCK; ++k16) {
-                const int owner = (lane & ~3) | ((k16 & 7) >> 1), slot = (k16 & 1) + 2 * (k16 >> 3);
+                const int owner = (lane & ~3) | ((k16 & 7) >> 1), slot16 = (k16 & 1) + 2 * (k16 >> 3);
 #pragma unroll
-                for (int j = 0; j < (HDP > 128 ? 2 : 1); ++j) {
-                    const uint32_t mine = slot == 0 ? lost[j][0] : slot == 1 ? lost[j][1] : slot == 2 ? lost[j][2] : lost[j][3];
-                    const uint32_t bits = __shfl_sync(0xffffffffu, mine, owner);
+                for (int j = 0; j < F::VG; ++j) {
+                    const uint32_t own = slot16 == 0 ? lost[j][0] : slot16 == 1 ? lost[j][1] : slot16 == 2 ? lost[j][2] : lost[j][3];
+                    const uint32_t bits = __shfl_sync(0xffffffffu, own, owner);
                     const int k = b * C8_BLOCK + k16;
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
@@ -370,14 +448,17 @@ __device__ __forceinline__ void attend_tile(const Tile& T, int range, int ranges
             }
         }
     }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();                   // every warp is through with its part of the ring
     // the warps' sums together
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
+            const int col = nt * 8 + 2 * t + j;
 #pragma unroll
             for (int x = 4; x < 32; x <<= 1) l[nt][j] += __shfl_xor_sync(0xffffffffu, l[nt][j], x);
-            const int col = nt * 8 + 2 * t + j;
+            if (col >= T.n) continue;
             if (g == 0) { s_stat[warp][col][0] = mo[nt][j]; s_stat[warp][col][1] = m[nt][j]; s_stat[warp][col][2] = l[nt][j]; }
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
@@ -387,16 +468,15 @@ __device__ __forceinline__ void attend_tile(const Tile& T, int range, int ranges
         }
     __syncthreads();
     for (int col = warp; col < T.n; col += WARPS) {
-        float mw[WARPS], M = -INFINITY, MO = -INFINITY, L = 0.f;
+        float mw[WARPS], M = LOWEST, MO = LOWEST, L = 0.f;
 #pragma unroll
         for (int w = 0; w < WARPS; ++w) { MO = fmaxf(MO, s_stat[w][col][0]); M = fmaxf(M, s_stat[w][col][1]); }
 #pragma unroll
         for (int w = 0; w < WARPS; ++w) {
-            mw[w] = s_stat[w][col][0] == -INFINITY ? 0.f : exp2f(s_stat[w][col][0] - MO);
-            // (a NaN in the denominator has to stay one)
-            L += s_stat[w][col][1] == -INFINITY ? s_stat[w][col][2] : s_stat[w][col][2] * exp2f(s_stat[w][col][1] - M);
+            mw[w] = exp2f(s_stat[w][col][0] - MO);
+            L += s_stat[w][col][2] * exp2f(s_stat[w][col][1] - M);
         }
-        const size_t at = T.query(col, S);
+        const size_t at = Q.row[col];
         float* pp = partial != nullptr ? partial + (at * ranges + range) * (hd + 4) : nullptr;
         const float norm = exp2f(MO - M) / L;
         for (int d = lane; d < hd; d += 32) {
@@ -404,28 +484,29 @@ __device__ __forceinline__ void attend_tile(const Tile& T, int range, int ranges
 #pragma unroll
             for (int w = 0; w < WARPS; ++w) sum += s_o[w][col][d] * mw[w];
             if (pp != nullptr) pp[d] = sum;
-            else out[at * hd + d] = tq_from_float<TA>(sum * norm);
+            else out[at * hd + d] = tq_from_float<typename F::TA>(sum * norm);
         }
         if (pp != nullptr && lane == 0) { pp[hd] = MO; pp[hd + 1] = M; pp[hd + 2] = L; }
         if (pp == nullptr && lse != nullptr && lane == 0) lse[at] = M + log2f(L);
     }
 }
 
-template <typename TA, int HDP, int NT>
-__global__ void __launch_bounds__(WARPS * 32) attention8_kernel(const TA* __restrict__ q, Cache8 c, Step S, TA* __restrict__ out, float* __restrict__ partial,
-                                                                float* __restrict__ scores, int score_stride, float* __restrict__ lse) {
+template <class F>
+__global__ void __launch_bounds__(WARPS * 32, F::PER_SM) attention8_kernel(const typename F::TA* __restrict__ q, Cache8 c, Step S, typename F::TA* __restrict__ out,
+                                                                                           float* __restrict__ partial, float* __restrict__ scores, int score_stride,
+                                                                                           float* __restrict__ lse) {
     tq_grid_wait();                    // everything below may read what the previous kernel wrote
     tq_grid_launch_dependents();
     const int tile_no = blockIdx.x / c.nkv;
-    const Tile T = tile_of(S, blockIdx.z, blockIdx.x - tile_no * c.nkv, c.nkv, tile_no, NT * 8);
-    if (T.n > 0) attend_tile<TA, HDP, NT>(T, blockIdx.y, gridDim.y, q, c, S, out, partial, scores, score_stride, lse);
+    const Tile T = tile_of(S, blockIdx.z, blockIdx.x - tile_no * c.nkv, c.nkv, tile_no, F::NC);
+    if (T.n > 0) attend_tile<F>(T, blockIdx.y, gridDim.y, q, c, S, out, partial, scores, score_stride, lse);
 }
 
 // The prompt kernel gives values that a row may not see a weight of 0, which does not remove a NaN: key/value heads of sequences in whose pages
 // `lost` [n_seqs][nkv][pages] marks such values are done again here, all others cost a look at their marks.
-template <typename TA, int HDP, int NT>
-__global__ void __launch_bounds__(WARPS * 32) repair8_kernel(const TA* __restrict__ q, Cache8 c, Step S, TA* __restrict__ out, const uint8_t* __restrict__ lost,
-                                                             int lost_stride, int page_size) {
+template <class F>
+__global__ void __launch_bounds__(WARPS * 32) repair8_kernel(const typename F::TA* __restrict__ q, Cache8 c, Step S, typename F::TA* __restrict__ out,
+                                                             const uint8_t* __restrict__ lost, int lost_stride, int page_size) {
     tq_grid_wait();                    // everything below may read what the previous kernel wrote
     tq_grid_launch_dependents();
     const int seq = blockIdx.z, g = blockIdx.y, start = S.held[seq], run = S.cu_seqlens[seq + 1] - S.cu_seqlens[seq];
@@ -435,10 +516,10 @@ __global__ void __launch_bounds__(WARPS * 32) repair8_kernel(const TA* __restric
     for (int p = first_seen(start, S.window) / page_size + (int)threadIdx.x; p <= (start + run - 1) / page_size; p += WARPS * 32) some |= marks[p] != 0;
     if (!__syncthreads_or(some)) return;
     for (int tile_no = blockIdx.x; ; tile_no += gridDim.x) {
-        const Tile T = tile_of(S, seq, g, c.nkv, tile_no, NT * 8);
+        const Tile T = tile_of(S, seq, g, c.nkv, tile_no, F::NC);
         if (T.n <= 0) return;
         __syncthreads();
-        attend_tile<TA, HDP, NT>(T, 0, 1, q, c, S, out, nullptr, nullptr, 0, nullptr);
+        attend_tile<F>(T, 0, 1, q, c, S, out, nullptr, nullptr, 0, nullptr);
     }
 }
 
@@ -457,14 +538,11 @@ __global__ void __launch_bounds__(128) join8_kernel(Cache8 c, Step S, const floa
     // the statistics of a row over its ranges
     auto stats = [&](size_t at, float& MO, float& M, float& L) {
         const float* p = partial + at * ranges * (hd + 4) + hd;
-        MO = -INFINITY; M = -INFINITY; L = 0.f;
+        MO = LOWEST; M = LOWEST; L = 0.f;
         for (int r = lane; r < ranges; r += 32) { MO = fmaxf(MO, p[(size_t)r * (hd + 4)]); M = fmaxf(M, p[(size_t)r * (hd + 4) + 1]); }
         MO = tq_warp_max(MO);
         M = tq_warp_max(M);
-        for (int r = lane; r < ranges; r += 32) {
-            const float mr = p[(size_t)r * (hd + 4) + 1], lr = p[(size_t)r * (hd + 4) + 2];
-            L += mr == -INFINITY ? lr : lr * exp2f(mr - M);
-        }
+        for (int r = lane; r < ranges; r += 32) L += p[(size_t)r * (hd + 4) + 2] * exp2f(p[(size_t)r * (hd + 4) + 1] - M);
         L = tq_warp_sum(L);
     };
     if (blockIdx.x == 0) {
@@ -478,10 +556,7 @@ __global__ void __launch_bounds__(128) join8_kernel(Cache8 c, Step S, const floa
             const float* p = partial + at * ranges * (hd + 4);
             for (int d = lane; d < hd; d += 32) {
                 float sum = 0.f;
-                for (int r = 0; r < ranges; ++r) {
-                    const float mr = p[(size_t)r * (hd + 4) + hd], v = p[(size_t)r * (hd + 4) + d];
-                    sum += mr == -INFINITY ? v : v * exp2f(mr - MO);
-                }
+                for (int r = 0; r < ranges; ++r) sum += p[(size_t)r * (hd + 4) + d] * exp2f(p[(size_t)r * (hd + 4) + hd] - MO);
                 out[at * hd + d] = tq_from_float<TA>(sum * norm);
             }
         }
@@ -515,12 +590,12 @@ __global__ void __launch_bounds__(128) join8_kernel(Cache8 c, Step S, const floa
 // Sums of weights from the queries and the keys again: a warp keeps a block of 16 keys in registers and walks the columns that see it, 8
 // or 16 at a time.  One writer per sum and a fixed order: the same bits every time.
 // ---------------------------------------------------------------------------------------
-template <typename TA, int HDP, int NT>
-__global__ void __launch_bounds__(WARPS * 32) weigh8_kernel(const TA* __restrict__ q, Cache8 c, Step S, const float* __restrict__ lse, float* __restrict__ weights) {
+template <class F>
+__global__ void __launch_bounds__(WARPS * 32) weigh8_kernel(const typename F::TA* __restrict__ q, Cache8 c, Step S, const float* __restrict__ lse, float* __restrict__ weights) {
     tq_grid_wait();                    // everything below may read what the previous kernel wrote
     tq_grid_launch_dependents();
-    constexpr int NC = NT * 8;
-    __shared__ Queries<TA, HDP, NT> Q;
+    constexpr int NT = F::NT, NC = F::NC;
+    __shared__ Queries<F> Q;
     const int seq = blockIdx.z, gh = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, hd = c.hd;
     Tile T = tile_of(S, seq, gh, c.nkv, 0, NC);
     const int key0 = blockIdx.x * WARPS * C8_BLOCK, last_key = key0 + WARPS * C8_BLOCK - 1;
@@ -529,13 +604,18 @@ __global__ void __launch_bounds__(WARPS * 32) weigh8_kernel(const TA* __restrict
     if (row0 >= row1) return;
     const int block = blockIdx.x * WARPS + warp, key = block * C8_BLOCK + g;
     const bool mine = block * C8_BLOCK < T.start + T.run && !(S.window > 0 && block * C8_BLOCK + C8_BLOCK - 1 + S.window <= T.start);
-    KeyRegs<HDP> kr = {};
+    KeyRegs<F> kr = {};
     float ks = 0.f;
     int page = 0;
     const int row = block * C8_BLOCK % c.page_size;
     if (mine) {
         page = c.page_of(seq, block * C8_BLOCK);
-        load_keys<HDP>(kr, c.codes + c.codes_at(page, 0, gh) + (size_t)row * hd, hd);
+        const uint8_t* k = c.codes + c.codes_at(page, 0, gh) + (size_t)row * hd;
+#pragma unroll
+        for (int j = 0; j < F::HDP / 64; ++j)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                if (j * 64 + t * 16 < hd) kr.k[j][h] = __ldg(reinterpret_cast<const uint4*>(k + (g + 8 * h) * hd + j * 64 + t * 16));
         ks = c8_scale(c.scales[c.scales_at(page, 0, gh) + row / C8_BLOCK]);
     }
     float sum[2] = {0.f, 0.f};
@@ -545,16 +625,21 @@ __global__ void __launch_bounds__(WARPS * 32) weigh8_kernel(const TA* __restrict
         __syncthreads();
         Q.load(q, T, S, hd);
         if (!mine) continue;
+        uint2 kept[F::KEEP ? F::STEPS : 1];
+        if (F::KEEP) {
+#pragma unroll
+            for (int i = 0; i < F::STEPS; ++i) kept[F::KEEP ? i : 0] = Q.b[0][0][i][lane];
+        }
         float s[NT][4];
-        products<TA, HDP, NT>(s, kr, Q);
+        products<F>(s, kr, Q, kept);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 const int col = nt * 8 + 2 * t + j;
                 if (col >= T.n) continue;
-                const int p = T.start + T.row(col);
-                const float f = Q.factor[col] * ks, L = lse[T.query(col, S)];
+                const int p = Q.place[col];
+                const float f = Q.factor[col] * ks, L = lse[Q.row[col]];
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const int k = key + 8 * h;
@@ -575,28 +660,43 @@ __global__ void __launch_bounds__(WARPS * 32) weigh8_kernel(const TA* __restrict
     }
 }
 
-template <typename TA, int HDP, int NT>
+template <class F>
+int launch_repair8(const void* q, const Cache8& c, const Step& S, void* out, const void* lost, int lost_stride, int n_seqs, cudaStream_t stream) {
+    static std::atomic<unsigned long long> asked{0};
+    const cudaError_t e = tq_reserve_smem(repair8_kernel<F>, F::SMEM, asked);
+    if (e != cudaSuccess) TQ_FAIL(-1, "repair8: cannot reserve %d bytes of shared memory: %s", F::SMEM, cudaGetErrorString(e));
+    const int heads = c.nkv * n_seqs, each = heads >= 444 ? 1 : 444 / heads;
+    tq_launch(dim3(each, c.nkv, n_seqs), WARPS * 32, F::SMEM, stream)(repair8_kernel<F>, (const typename F::TA*)q, c, S, (typename F::TA*)out, (const uint8_t*)lost, lost_stride, c.page_size);
+    TQ_CHECK_LAUNCH("repair8");
+    return 0;
+}
+template <class F>
 int launch8(const void* q, const Cache8& c, const Step& S, void* out, float* partial, int ranges, float* scores, int score_stride, float* lse, int n_seqs,
             int max_q_len, cudaStream_t stream) {
-    const long long tiles = ((long long)max_q_len * (S.nh / c.nkv) + NT * 8 - 1) / (NT * 8) * c.nkv;
+    const long long tiles = ((long long)max_q_len * (S.nh / c.nkv) + F::NC - 1) / F::NC * c.nkv;
     TQ_REQUIRE(tiles < (1ll << 31), "attention8: runs of %d rows", max_q_len);
-    tq_launch(dim3((unsigned)tiles, ranges, n_seqs), WARPS * 32, 0, stream)(attention8_kernel<TA, HDP, NT>, (const TA*)q, c, S, (TA*)out, partial, scores, score_stride, lse);
+    static std::atomic<unsigned long long> asked{0};
+    const cudaError_t e = tq_reserve_smem(attention8_kernel<F>, F::SMEM, asked);
+    if (e != cudaSuccess) TQ_FAIL(-1, "attention8: cannot reserve %d bytes of shared memory: %s", F::SMEM, cudaGetErrorString(e));
+    tq_launch(dim3((unsigned)tiles, ranges, n_seqs), WARPS * 32, F::SMEM, stream)(attention8_kernel<F>, (const typename F::TA*)q, c, S, (typename F::TA*)out, partial, scores, score_stride, lse);
     TQ_CHECK_LAUNCH("attention8");
     return 0;
 }
-template <typename TA, int HDP, int NT>
+template <class F>
 int launch_weigh8(const void* q, const Cache8& c, const Step& S, const float* lse, float* weights, int n_seqs, int max_kv_len, cudaStream_t stream) {
     const int per_cta = WARPS * C8_BLOCK;
-    tq_launch(dim3((max_kv_len + per_cta - 1) / per_cta, c.nkv, n_seqs), WARPS * 32, 0, stream)(weigh8_kernel<TA, HDP, NT>, (const TA*)q, c, S, lse, weights);
+    tq_launch(dim3((max_kv_len + per_cta - 1) / per_cta, c.nkv, n_seqs), WARPS * 32, 0, stream)(weigh8_kernel<F>, (const typename F::TA*)q, c, S, lse, weights);
     TQ_CHECK_LAUNCH("weigh8");
     return 0;
 }
 // Two tiles of 8 columns where there are more than 8 (heads of up to 128: beyond, the sums of 16 columns do not fit the registers)
-#define C8_SIZES(columns, CALL)                                                                          \
-    do {                                                                                                 \
-        if (hd <= 64) { if ((columns) > 8) return CALL(64, 2); return CALL(64, 1); }                     \
-        if (hd <= 128) { if ((columns) > 8) return CALL(128, 2); return CALL(128, 1); }                  \
-        return CALL(256, 1);                                                                             \
+#define C8_FORMS(columns, CALL)                                                                                              \
+    do {                                                                                                                     \
+        if (hd == 128) { if ((columns) > 8) return CALL(128, 2, true); return CALL(128, 1, true); }                          \
+        if (hd == 64) { if ((columns) > 8) return CALL(64, 2, true); return CALL(64, 1, true); }                             \
+        if (hd < 64) { if ((columns) > 8) return CALL(64, 2, false); return CALL(64, 1, false); }                            \
+        if (hd < 128) { if ((columns) > 8) return CALL(128, 2, false); return CALL(128, 1, false); }                         \
+        return CALL(256, 1, false);                                                                                          \
     } while (0)
 
 int check_step(const char* what, int nh, int nkv, int n_seqs, int longest, int window) {
@@ -627,8 +727,8 @@ TQ_EXPORT int tq_attention8(const void* q, const void* codes, const void* scales
     const int columns = max_q_len * (nh / nkv);
     auto first = [&]() -> int {
         TQ_DISPATCH(act_dtype, TA,
-#define C8_CALL(HDP, NT) (launch8<TA, HDP, NT>(q, c, S, out, partial, ranges, scores, score_stride, partial == nullptr ? lse : nullptr, n_seqs, max_q_len, stream))
-            C8_SIZES(columns, C8_CALL));
+#define C8_CALL(HDP, NT, EXACT) (launch8<Form<TA, HDP, NT, EXACT>>(q, c, S, out, partial, ranges, scores, score_stride, partial == nullptr ? lse : nullptr, n_seqs, max_q_len, stream))
+            C8_FORMS(columns, C8_CALL));
 #undef C8_CALL
         return -2;
     };
@@ -652,12 +752,7 @@ TQ_EXPORT int tq_repair8(const void* q, const void* codes, const void* scales, c
     TQ_REQUIRE(hd == 64 || hd == 128, "repair8: head size %d", hd);
     const Cache8 c{(uint8_t*)codes, (uint8_t*)scales, page_table, table_stride, page_size, n_pages, nkv, hd};
     const Step S{cu_seqlens, held, nh, window, scale * LOG2E};
-    const int heads = nkv * n_seqs, each = heads >= 444 ? 1 : 444 / heads;
-    using TA = __nv_bfloat16;
-    if (hd == 64) tq_launch(dim3(each, nkv, n_seqs), WARPS * 32, 0, stream)(repair8_kernel<TA, 64, 2>, (const TA*)q, c, S, (TA*)out, (const uint8_t*)lost, lost_stride, page_size);
-    else tq_launch(dim3(each, nkv, n_seqs), WARPS * 32, 0, stream)(repair8_kernel<TA, 128, 2>, (const TA*)q, c, S, (TA*)out, (const uint8_t*)lost, lost_stride, page_size);
-    TQ_CHECK_LAUNCH("repair8");
-    return 0;
+    return hd == 64 ? launch_repair8<Form<__nv_bfloat16, 64, 2, true>>(q, c, S, out, lost, lost_stride, n_seqs, stream) : launch_repair8<Form<__nv_bfloat16, 128, 2, true>>(q, c, S, out, lost, lost_stride, n_seqs, stream);
 }
 
 // weights of places below held[s] grow by, those of the step's own rows become, the sum over the step's rows and the head's query heads of
@@ -673,8 +768,8 @@ TQ_EXPORT int tq_weigh8(const void* q, const void* codes, const void* scales, in
     const Step S{cu_seqlens, held, nh, window, scale * LOG2E};
     const int columns = max_q_len * (nh / nkv);
     TQ_DISPATCH(act_dtype, TA,
-#define C8_CALL(HDP, NT) (launch_weigh8<TA, HDP, NT>(q, c, S, lse, weights, n_seqs, max_kv_len, stream))
-        C8_SIZES(columns, C8_CALL));
+#define C8_CALL(HDP, NT, EXACT) (launch_weigh8<Form<TA, HDP, NT, false>>(q, c, S, lse, weights, n_seqs, max_kv_len, stream))
+        C8_FORMS(columns, C8_CALL));
 #undef C8_CALL
     return -2;
 }

@@ -62,11 +62,9 @@ __device__ __forceinline__ uint32_t c8_half2(uint32_t two) {
     asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(d) : "h"((uint16_t)two));
     return d;
 }
-__device__ __forceinline__ float c8_float(uint8_t code) {
-    const uint32_t h = c8_half2(code);
-    float f;
-    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tcvt.f32.f16 %0, l;\n\t}" : "=f"(f) : "r"(h));
-    return f;
+// Four codes as two float16 pairs
+__device__ __forceinline__ void c8_half4(uint32_t four, uint32_t& lo, uint32_t& hi) {
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}" : "=r"(lo), "=r"(hi) : "r"(four));
 }
 // Four codes rounded again after a factor of 2^-shift (half2 `factor`, both halves; shift at most 24, where everything is 0): the
 // product is exact in float16 down to 2^-24 and lies below half of e4m3's smallest step before it is not.

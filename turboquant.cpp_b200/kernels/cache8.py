@@ -139,8 +139,10 @@ def attention8(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, cu_se
                                   max_q_len, max_kv_len, weights, status)
     per = n_heads // n_kv_heads
     columns = max_q_len * per
-    tiles = -(-columns // (16 if columns > 8 and head_dim <= 128 else 8)) * n_kv_heads * n
-    ranges = ranges_for(tiles, -(-max_kv_len // BLOCK), resident_ctas(q.device) * 3 // 4)
+    wide = columns > 8 and head_dim <= 128                  # two tiles of 8 columns in one CTA
+    tiles = -(-columns // (16 if wide else 8)) * n_kv_heads * n
+    per_sm = 2 if head_dim > 128 else 3 if wide and head_dim > 64 else 4         # CTAs an SM holds
+    ranges = ranges_for(tiles, -(-max_kv_len // BLOCK), resident_ctas(q.device) // 4 * per_sm)
     # one row a sequence: the first launch leaves its scores for the second one to add up, which moves 8 bytes a key and query head, where
     # reading the keys again moves head_dim bytes a key
     stride = -(-max_kv_len // BLOCK) * BLOCK
