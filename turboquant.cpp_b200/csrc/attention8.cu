@@ -83,11 +83,14 @@ template <typename TA_, int HDP_, int NT_, bool EXACT_> struct Form {
     using TA = TA_;
     static constexpr int HDP = HDP_, NT = NT_, NC = NT * 8, MT = HDP / 16, STEPS = HDP / 16, PARTS = sizeof(TA) == 4 ? 2 : 1;
     static constexpr bool EXACT = EXACT_, KEEP = NT * PARTS == 1 && HDP <= 128;       // KEEP: the queries stay in registers
-    static constexpr int KP = HDP / 64 * 2, VG = HDP > 128 ? 2 : 1, VB = HDP == 64 ? 8 : 16, STAGES = 3;
-    static constexpr int STAGE_BYTES = (KP * 16 + VG * 4 * VB) * 32, RING = WARPS * STAGES * STAGE_BYTES, SUMS = WARPS * NC * (HDP + 4) * 4;
+    static constexpr int VG = HDP > 128 ? 2 : 1, STAGES = 3, STAGE_BYTES = 2 * C8_BLOCK * HDP, RING = WARPS * STAGES * STAGE_BYTES, SUMS = WARPS * NC * (HDP + 4) * 4;
     static constexpr int SMEM = RING > SUMS ? RING : SUMS;
     static constexpr int PER_SM = HDP > 128 ? 2 : HDP * NT > 128 ? 3 : 4;              // CTAs an SM holds (the registers' limit)
 };
+
+// Which 16 elements of a key row a lane's piece j is: a quarter of the lanes (t = lane % 4) holds each, two by two so that even and odd rows meet in
+// no bank (see Piece).
+template <int HDP> __device__ __forceinline__ int chunk_of(int j, int t) { return HDP == 64 ? t : 2 * t + (j & 1) + 8 * (j >> 1); }
 
 // The tile's queries in shared memory as right operands, [part][8 columns][step of 16 elements][lane], each column's factor (score =
 // (sum of the products) * factor * 2^(key byte - 127)), its row in q and its place (columns that are not there: place -1).
@@ -117,7 +120,7 @@ template <class F> struct Queries {
         }
         __syncthreads();
         for (int i = threadIdx.x; i < F::NT * F::STEPS * 32; i += WARPS * 32) {
-            const int l = i & 31, step = i / 32 % F::STEPS, nt = i / 32 / F::STEPS, c = nt * 8 + (l >> 2), d = (step / 4) * 64 + (l & 3) * 16 + (step & 3) * 4;
+            const int l = i & 31, step = i / 32 % F::STEPS, nt = i / 32 / F::STEPS, c = nt * 8 + (l >> 2), d = chunk_of<F::HDP>(step / 4, l & 3) * 16 + (step & 3) * 4;
             float f[4] = {0.f, 0.f, 0.f, 0.f};
             if (c < t.n && d < hd) {
                 const typename F::TA* x = q + row[c] * hd + d;
@@ -141,47 +144,47 @@ template <class F> struct Queries {
 template <class F> struct KeyRegs { uint4 k[F::HDP / 64][2]; };
 template <class F> struct ValueRegs { uint4 v[F::VG][4]; };
 
-template <int B> __device__ __forceinline__ void copy_async(uint32_t to, const uint8_t* from, bool there) {
-    const int n = there ? B : 0;       // 0: zeros
-    if (B == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(n) : "memory");
-    else asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(to), "l"(from), "r"(n) : "memory");
+// A block on its way, 16 rows of keys and of values in the warp's part of a ring in shared memory.  The copies take whole rows, 512 bytes an
+// instruction (with 64 bytes of every row, each lane copying what it reads, the copies alone took as long as everything together: 103 of
+// 114 us, 64 sequences of up to 2,048 keys, 16 heads); a row's 16-byte chunks are stored at their number xor the row's, so that neither the
+// reads of keys (8 lanes: two rows, four chunks of each) nor those of values (four rows, two chunks) meet in a bank.
+template <int HDP> __device__ __forceinline__ int place_in(int row, int chunk) {
+    return row * HDP + ((HDP == 64 ? chunk ^ ((row >> 1) & 3) : chunk ^ (row & 7)) * 16);
 }
-// A block on its way: a ring in shared memory in which every lane copies its own pieces and reads only those, so that it needs no barrier
-// and no bank is hit twice.  k, v: the block's first key and value row; at: the warp's stage (pieces lie 512 or 256 bytes apart).
+__device__ __forceinline__ void copy_async(uint32_t to, const uint8_t* from, bool there) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");       // 0: zeros
+}
 template <class F>
 __device__ __forceinline__ void copy_block(uint32_t at, const uint8_t* k, const uint8_t* v, int hd_) {
-    const int hd = F::EXACT ? F::HDP : hd_, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const uint8_t *kl = k + g * hd + t * 16, *vl = v + 2 * t * hd + g * F::VB;
-    at += lane * 16;
+    constexpr int CPR = F::HDP / 16, ROWS = 32 / CPR;          // chunks a row, rows an instruction
+    const int hd = F::EXACT ? F::HDP : hd_, lane = threadIdx.x & 31, row = lane / CPR, chunk = lane % CPR;
+    const bool there = F::EXACT || chunk * 16 < hd;
+    const uint32_t off = there ? row * hd + chunk * 16 : 0;
+#pragma unroll
+    for (int i = 0; i < C8_BLOCK / ROWS; ++i) {
+        const uint32_t to = at + place_in<F::HDP>(row + i * ROWS, chunk), from = off + (there ? i * ROWS * hd : 0);
+        copy_async(to, k + from, there);
+        copy_async(to + C8_BLOCK * F::HDP, v + from, there);
+    }
+}
+template <class F>
+__device__ __forceinline__ void take_block(KeyRegs<F>& kr, ValueRegs<F>& vr, const uint8_t* at) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 #pragma unroll
     for (int j = 0; j < F::HDP / 64; ++j)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const bool there = F::EXACT || j * 64 + t * 16 < hd;
-            copy_async<16>(at + (j * 2 + h) * 512, there ? kl + 8 * h * hd + j * 64 : k, there);
-        }
-    at += F::KP * 512 - lane * (16 - F::VB);
+        for (int h = 0; h < 2; ++h) kr.k[j][h] = *reinterpret_cast<const uint4*>(at + place_in<F::HDP>(g + 8 * h, chunk_of<F::HDP>(j, t)));
+    at += C8_BLOCK * F::HDP;
 #pragma unroll
     for (int j = 0; j < F::VG; ++j)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const bool there = F::EXACT || j * 128 + g * F::VB < hd;
-            copy_async<F::VB>(at + (j * 4 + r) * 32 * F::VB, there ? vl + ((r & 1) + 8 * (r >> 1)) * hd + j * 128 : v, there);
+            const int row = 2 * t + (r & 1) + 8 * (r >> 1);
+            if (F::HDP == 64) {
+                const uint2 x = *reinterpret_cast<const uint2*>(at + place_in<F::HDP>(row, g >> 1) + (g & 1) * 8);
+                vr.v[j][r] = make_uint4(x.x, x.y, 0, 0);
+            } else vr.v[j][r] = *reinterpret_cast<const uint4*>(at + place_in<F::HDP>(row, g + 8 * j));
         }
-}
-template <class F>
-__device__ __forceinline__ void take_block(KeyRegs<F>& kr, ValueRegs<F>& vr, const uint8_t* at) {
-    const int lane = threadIdx.x & 31;
-#pragma unroll
-    for (int i = 0; i < F::KP; ++i) kr.k[i / 2][i % 2] = *reinterpret_cast<const uint4*>(at + i * 512 + lane * 16);
-#pragma unroll
-    for (int i = 0; i < F::VG * 4; ++i) {
-        const uint8_t* p = at + F::KP * 512 + i * 32 * F::VB + lane * F::VB;
-        if (F::HDP == 64) {
-            const uint2 x = *reinterpret_cast<const uint2*>(p);
-            vr.v[i / 4][i % 4] = make_uint4(x.x, x.y, 0, 0);
-        } else vr.v[i / 4][i % 4] = *reinterpret_cast<const uint4*>(p);
-    }
 }
 __device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 
@@ -301,8 +304,10 @@ __device__ __forceinline__ void attend_tile(const Tile& T, int range, int ranges
         asm volatile("cp.async.wait_group %0;" ::"n"(F::STAGES - 2) : "memory");
         KeyRegs<F> kc;
         ValueRegs<F> vc;
+        __syncwarp();                  // each lane's copies of this block are there, so all of them
         take_block<F>(kc, vc, ring + warp * (F::STAGES * F::STAGE_BYTES) + taken * F::STAGE_BYTES);
         taken = taken + 1 == F::STAGES ? 0 : taken + 1;
+        __syncwarp();                  // all lanes have read the block before this one, whose place is filled next
         const float ks = c8_scale(kbs[0]), ve = (float)((int)vbs[0] - 127);
 #pragma unroll
         for (int i = 0; i + 1 < F::STAGES - 1; ++i) { kbs[i] = kbs[i + 1]; vbs[i] = vbs[i + 1]; }
@@ -615,7 +620,7 @@ __global__ void __launch_bounds__(WARPS * 32) weigh8_kernel(const typename F::TA
         for (int j = 0; j < F::HDP / 64; ++j)
 #pragma unroll
             for (int h = 0; h < 2; ++h)
-                if (j * 64 + t * 16 < hd) kr.k[j][h] = __ldg(reinterpret_cast<const uint4*>(k + (g + 8 * h) * hd + j * 64 + t * 16));
+                if (chunk_of<F::HDP>(j, t) * 16 < hd) kr.k[j][h] = __ldg(reinterpret_cast<const uint4*>(k + (g + 8 * h) * hd + chunk_of<F::HDP>(j, t) * 16));
         ks = c8_scale(c.scales[c.scales_at(page, 0, gh) + row / C8_BLOCK]);
     }
     float sum[2] = {0.f, 0.f};
