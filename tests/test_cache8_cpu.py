@@ -108,3 +108,27 @@ def test_plain_choice_of_rows():
     assert plain.kept_places([1.0, 1.0, 1.0, 0.0], 3, 1) == [0, 1, 3]
     assert plain.kept_places([nan, 0.0, nan, -1.0], 2, 0) == [1, 3]
     assert plain.kept_places([5.0, 1.0], 4, 1) == [0, 1]
+
+
+def test_declared_arguments_are_those_of_the_sources():
+    """A letter per argument: an address, a whole number or a float, as the entry points are written."""
+    import os
+    import re
+
+    from conftest import ROOT
+    csrc = os.path.join(ROOT, "turboquant.cpp_b200", "csrc")
+    text = "".join(open(os.path.join(csrc, f), encoding="utf-8").read() for f in ("cache8.cu", "attention8.cu", "prompt8.cu", "evict.cu"))
+    found = dict(re.findall(r"TQ_EXPORT int (tq_\w+)\((.*?)\)\s*\{", text, re.S))
+    assert set(found) == set(cache8._SIGNATURES)
+    for name, arguments in found.items():
+        kinds = ["p" if "*" in a or "cudaStream_t" in a else "f" if a.split()[0] == "float" else "i" for a in (x.strip() for x in arguments.split(","))]
+        assert "".join(kinds) == cache8._SIGNATURES[name], name
+
+
+def test_ranges_fill_the_device_and_no_more():
+    r = cache8.ranges_for
+    assert r(1024, 128, 592) == 1 and r(592, 2000, 592) == 1                # as many tiles as there is room for, or more
+    assert r(1, 3, 592) == 1                                              # a few keys: one turn of one CTA's warps
+    for tiles, blocks in ((16, 44), (32, 2031), (4, 8000), (128, 256), (600, 128)):
+        n = r(tiles, blocks, 592)
+        assert 1 < n <= min(64, blocks // 4) and (tiles > 592 or tiles * n <= 592)

@@ -529,61 +529,91 @@ __global__ void __launch_bounds__(WARPS * 32) repair8_kernel(const typename F::T
 }
 
 // ---------------------------------------------------------------------------------------
-// The ranges of a row joined: block x = 0 of a (sequence, key/value head).  Further blocks add the row weights up from the scores the first
-// launch left, 128 places each.
+// The ranges of a row joined, a block per row.  Blocks behind the rows' add the weights up from the scores the first launch left, 128 places
+// of a (sequence, key/value head) each.
 // ---------------------------------------------------------------------------------------
+constexpr int JOIN_RANGES = 64;
+
+// The statistics of row `at` of q, and each range's factor in s_f[0 .. ranges - 1]; by a warp, which then has them.
+__device__ __forceinline__ void join_stats(const float* __restrict__ partial, size_t at, int ranges, int hd, float& MO, float& M, float& L, float* s_f) {
+    const int lane = threadIdx.x & 31;
+    const float* p = partial + at * ranges * (hd + 4) + hd;
+    float mo[JOIN_RANGES / 32], m[JOIN_RANGES / 32], l[JOIN_RANGES / 32];
+    MO = LOWEST; M = LOWEST; L = 0.f;
+#pragma unroll
+    for (int i = 0; i < JOIN_RANGES / 32; ++i) {
+        const int r = lane + 32 * i;
+        mo[i] = m[i] = LOWEST;
+        l[i] = 0.f;
+        if (r < ranges) { mo[i] = p[(size_t)r * (hd + 4)]; m[i] = p[(size_t)r * (hd + 4) + 1]; l[i] = p[(size_t)r * (hd + 4) + 2]; }
+        MO = fmaxf(MO, mo[i]);
+        M = fmaxf(M, m[i]);
+    }
+    MO = tq_warp_max(MO);
+    M = tq_warp_max(M);
+#pragma unroll
+    for (int i = 0; i < JOIN_RANGES / 32; ++i) {
+        L += l[i] * exp2f(m[i] - M);
+        if (s_f != nullptr && lane + 32 * i < ranges) s_f[lane + 32 * i] = exp2f(mo[i] - MO);
+    }
+    L = tq_warp_sum(L);
+}
+
 template <typename TA>
-__global__ void __launch_bounds__(128) join8_kernel(Cache8 c, Step S, const float* __restrict__ partial, int ranges, TA* __restrict__ out,
+__global__ void __launch_bounds__(128) join8_kernel(Cache8 c, Step S, const float* __restrict__ partial, int ranges, TA* __restrict__ out, int rows,
                                                     float* __restrict__ lse, const float* __restrict__ scores, int score_stride, float* __restrict__ weights) {
     tq_grid_wait();                    // everything below may read what the previous kernel wrote
     tq_grid_launch_dependents();
+    __shared__ float s_f[JOIN_RANGES], s_lse[128];
     const int seq = blockIdx.z, g = blockIdx.y, per = S.nh / c.nkv, hd = c.hd, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int t_begin = S.cu_seqlens[seq], run = S.cu_seqlens[seq + 1] - t_begin, start = S.held[seq];
-    if (run <= 0) return;
-    // the statistics of a row over its ranges
-    auto stats = [&](size_t at, float& MO, float& M, float& L) {
-        const float* p = partial + at * ranges * (hd + 4) + hd;
-        MO = LOWEST; M = LOWEST; L = 0.f;
-        for (int r = lane; r < ranges; r += 32) { MO = fmaxf(MO, p[(size_t)r * (hd + 4)]); M = fmaxf(M, p[(size_t)r * (hd + 4) + 1]); }
-        MO = tq_warp_max(MO);
-        M = tq_warp_max(M);
-        for (int r = lane; r < ranges; r += 32) L += p[(size_t)r * (hd + 4) + 2] * exp2f(p[(size_t)r * (hd + 4) + 1] - M);
-        L = tq_warp_sum(L);
-    };
-    if (blockIdx.x == 0) {
-        for (int c0 = warp; c0 < run * per; c0 += 4) {
-            const int r0 = c0 / per;
-            const size_t at = (size_t)(t_begin + r0) * S.nh + g * per + (c0 - r0 * per);
+    const int t_begin = S.cu_seqlens[seq], run = S.cu_seqlens[seq + 1] - t_begin, columns = run * per;
+    auto query = [&](int col) { const int r = col / per; return (size_t)(t_begin + r) * S.nh + g * per + (col - r * per); };
+    if ((int)blockIdx.x < rows) {
+        if ((int)blockIdx.x >= columns) return;
+        const size_t at = query(blockIdx.x);
+        const float* p = partial + at * ranges * (hd + 4);
+        float v[2][8];                 // the first ranges' elements, asked for beside the statistics
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int r = 0; r < 8; ++r) v[h][r] = r < ranges && (int)threadIdx.x + 128 * h < hd ? p[(size_t)r * (hd + 4) + threadIdx.x + 128 * h] : 0.f;
+        if (warp == 0) {
             float MO, M, L;
-            stats(at, MO, M, L);
-            const float norm = exp2f(MO - M) / L;
-            if (lse != nullptr && lane == 0) lse[at] = M + log2f(L);
-            const float* p = partial + at * ranges * (hd + 4);
-            for (int d = lane; d < hd; d += 32) {
-                float sum = 0.f;
-                for (int r = 0; r < ranges; ++r) sum += p[(size_t)r * (hd + 4) + d] * exp2f(p[(size_t)r * (hd + 4) + hd] - MO);
-                out[at * hd + d] = tq_from_float<TA>(sum * norm);
+            join_stats(partial, at, ranges, hd, MO, M, L, s_f);
+            if (lane == 0) {
+                s_lse[0] = exp2f(MO - M) / L;
+                if (lse != nullptr) lse[at] = M + log2f(L);
             }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int d = threadIdx.x + 128 * h;
+            if (d >= hd) break;
+            float sum = 0.f;
+#pragma unroll
+            for (int r = 0; r < 8; ++r) if (r < ranges) sum += v[h][r] * s_f[r];
+#pragma unroll 8
+            for (int r = 8; r < ranges; ++r) sum += p[(size_t)r * (hd + 4) + d] * s_f[r];
+            out[at * hd + d] = tq_from_float<TA>(sum * s_lse[0]);
         }
         return;
     }
-    __shared__ float s_lse[128];
-    const int place = (blockIdx.x - 1) * 128 + threadIdx.x, columns = run * per;
-    if ((int)(blockIdx.x - 1) * 128 >= start + run) return;
+    const int start = S.held[seq], place0 = ((int)blockIdx.x - rows) * 128, place = place0 + (int)threadIdx.x;
+    if (run <= 0 || place0 >= start + run) return;
     float sum = 0.f;
     for (int c0 = 0; c0 < columns; c0 += 128) {
         __syncthreads();
         for (int x = warp; x < min(128, columns - c0); x += 4) {
-            const int r0 = (c0 + x) / per;
             float MO, M, L;
-            stats((size_t)(t_begin + r0) * S.nh + g * per + (c0 + x - r0 * per), MO, M, L);
+            join_stats(partial, query(c0 + x), ranges, hd, MO, M, L, nullptr);
             if (lane == 0) s_lse[x] = M + log2f(L);
         }
         __syncthreads();
         for (int x = 0; x < min(128, columns - c0); ++x) {
-            const int r0 = (c0 + x) / per, p = start + r0;
+            const int p = start + (c0 + x) / per;
             if (place > p || place >= score_stride || (S.window > 0 && place <= p - S.window)) continue;
-            sum += ex2(scores[((size_t)(t_begin + r0) * S.nh + g * per + (c0 + x - r0 * per)) * score_stride + place] - s_lse[x]);
+            sum += ex2(scores[query(c0 + x) * score_stride + place] - s_lse[x]);
         }
     }
     if (place >= start + run || (S.window > 0 && place + S.window <= start)) return;       // no row of the step sees it
@@ -724,7 +754,7 @@ TQ_EXPORT int tq_attention8(const void* q, const void* codes, const void* scales
     int rc = c8_check("attention8", codes, scales, page_size, n_pages, nkv, hd, table_stride);
     if (!rc) rc = check_step("attention8", nh, nkv, n_seqs, max_q_len, window);
     if (rc) return rc;
-    TQ_REQUIRE(ranges >= 1 && ranges <= 65535 && (ranges == 1 || partial != nullptr), "attention8: %d ranges need a buffer for their sums", ranges);
+    TQ_REQUIRE(ranges >= 1 && ranges <= JOIN_RANGES && (ranges == 1 || partial != nullptr), "attention8: %d ranges need a buffer for their sums", ranges);
     TQ_REQUIRE((scores == nullptr) == (weights == nullptr) && (scores == nullptr || (partial != nullptr && score_stride % 16 == 0 && score_stride >= max_kv_len)),
                "attention8: scores of %d places do not hold %d", score_stride, max_kv_len);
     const Cache8 c{(uint8_t*)codes, (uint8_t*)scales, page_table, table_stride, page_size, n_pages, nkv, hd};
@@ -740,7 +770,7 @@ TQ_EXPORT int tq_attention8(const void* q, const void* codes, const void* scales
     rc = first();
     if (rc || partial == nullptr) return rc;
     const int chunks = weights != nullptr ? (max_kv_len + 127) / 128 : 0;
-    TQ_DISPATCH(act_dtype, TA, tq_launch(dim3(1 + chunks, nkv, n_seqs), 128, 0, stream)(join8_kernel<TA>, c, S, partial, ranges, (TA*)out, lse, scores, score_stride, weights));
+    TQ_DISPATCH(act_dtype, TA, tq_launch(dim3(columns + chunks, nkv, n_seqs), 128, 0, stream)(join8_kernel<TA>, c, S, partial, ranges, (TA*)out, columns, lse, scores, score_stride, weights));
     TQ_CHECK_LAUNCH("join8");
     return 0;
 }

@@ -33,11 +33,13 @@ __device__ __forceinline__ void store8(float* p, const float (&f)[8]) {
 }
 
 // ---------------------------------------------------------------------------------------
-// The writer.  A unit is the rows a sequence brings into one block of 16; a warp takes one head of it, query heads among them, so that
-// nothing is shared between warps: the block's largest magnitude is one reduction over the warp's registers, and rows the block holds
-// already are rounded again by the same warp when its byte grows.  An item is eight rotation pairs of a row: 16 elements, two 16-byte
-// loads of bfloat16 and two 8-byte stores of codes.  KEPT items a lane stay in registers between the maximum and the codes (heads of up
-// to 128); longer heads are loaded twice, the second time from the caches.
+// The writer.  A unit is the rows a sequence brings into one block of 16, of one head, query heads among them.  An item is eight rotation
+// pairs of a row: 16 elements, two 16-byte loads of bfloat16 and two 8-byte stores of codes; a thread has one item, so that all of a unit's
+// loads are under way at once, and keeps it in registers between the block's largest magnitude (a reduction over the unit's threads) and
+// its codes.  Rows the block holds already are rounded again by the same threads when its byte grows.
+// Single tokens (RUNS false): a warp per unit.  Runs: head size threads per unit, rounded up to warps, so a thread for each of a whole
+// block's items.  A warp per unit there too, four items a lane in 103 registers, took 42 us for prompts of 682 + 1,365 + 2,049 tokens,
+// 16 + 16 + 16 heads of 128.
 // Products and sums of the rotation are rounded one by one: the codes are then a function of the inputs that any float32 program can
 // state, and a rounding to 4 bits never depends on which product was fused.
 // ---------------------------------------------------------------------------------------
@@ -47,38 +49,38 @@ struct WriteArgs {
     int nh, pairing, written;          // written: the heads this launch takes (the queries alone, or all)
 };
 
-template <typename TA, typename TB, int KEPT>
-__global__ void __launch_bounds__(256) write8_kernel(const TA* __restrict__ qkv, const TB* __restrict__ bias, WriteArgs a, TA* __restrict__ q_out, Cache8 c) {
+constexpr int WRITE_THREADS = 512;
+
+template <typename TA, typename TB, bool RUNS>
+__global__ void __launch_bounds__(WRITE_THREADS) write8_kernel(const TA* __restrict__ qkv, const TB* __restrict__ bias, WriteArgs a, TA* __restrict__ q_out, Cache8 c,
+                                                               int threads) {
     tq_grid_wait();                    // everything below may read what the previous kernel wrote
     tq_grid_launch_dependents();
-    const int lane = threadIdx.x & 31, j = blockIdx.y * (blockDim.x >> 5) + (threadIdx.x >> 5), heads = a.nh + 2 * c.nkv;
-    if (j >= a.written) return;
+    __shared__ uint32_t s_top[WRITE_THREADS / 32];
+    const int unit = threadIdx.x / threads, it = threadIdx.x - unit * threads, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int j = blockIdx.y * (blockDim.x / threads) + unit, heads = a.nh + 2 * c.nkv;
     const int seq = blockIdx.z, t_begin = a.cu_seqlens[seq], run = a.cu_seqlens[seq + 1] - t_begin;
     const int place0 = a.held[seq];
     const int block_start = (place0 / C8_BLOCK + (int)blockIdx.x) * C8_BLOCK;       // the unit's block, as a place
     const int first = max(block_start, place0), rows = min(block_start + C8_BLOCK, place0 + run) - first;
-    if (rows <= 0) return;
+    if (rows <= 0 || (!RUNS && j >= a.written)) return;              // (runs: the whole block of threads returns or stays)
     const int t0 = t_begin + first - place0, hd = c.hd, half = hd >> 1, groups = half >> 3, items = rows * groups;
-    const bool is_q = j < a.nh, rotated = j < a.nh + c.nkv && a.cos_t != nullptr;
-    const size_t width = (size_t)heads * hd;
-    const TA* src = qkv + (size_t)t0 * width + (size_t)j * hd;
-    const TB* b_row = bias != nullptr ? bias + (size_t)j * hd : nullptr;
-
-    // the item's 16 elements, rotated; lo: elements at ia.., hi: at ib..
-    auto item = [&](int it, float (&lo)[8], float (&hi)[8]) {
-        const int r = it / groups, i = (it - r * groups) * 8;
-        const TA* row = src + (size_t)r * width;
-        const int ia = a.pairing == 0 ? i : 2 * i, ib = a.pairing == 0 ? i + half : 2 * i + 8;
+    const bool mine = it < items && j < a.written, is_q = j < a.nh;
+    const int r = it / groups, i = (it - r * groups) * 8;
+    const int ia = a.pairing == 0 ? i : 2 * i, ib = a.pairing == 0 ? i + half : 2 * i + 8;       // where the item's two halves lie in the head
+    float lo[8] = {}, hi[8] = {};
+    if (mine) {
+        const TA* row = qkv + ((size_t)(t0 + r) * heads + j) * hd;
         load8(row + ia, lo);
         load8(row + ib, hi);
-        if (b_row != nullptr) {
+        if (bias != nullptr) {
             float x[8], y[8];
-            load8(b_row + ia, x);
-            load8(b_row + ib, y);
+            load8(bias + (size_t)j * hd + ia, x);
+            load8(bias + (size_t)j * hd + ib, y);
 #pragma unroll
             for (int e = 0; e < 8; ++e) { lo[e] += x[e]; hi[e] += y[e]; }
         }
-        if (rotated) {
+        if (j < a.nh + c.nkv && a.cos_t != nullptr) {
             const size_t at = (size_t)a.positions[t0 + r] * half + i;
             float cs[8], sn[8];
             load8(a.cos_t + at, cs);
@@ -101,69 +103,52 @@ __global__ void __launch_bounds__(256) write8_kernel(const TA* __restrict__ qkv,
                 }
             }
         }
-    };
-    if (is_q) {
-        TA* dst = q_out + ((size_t)t0 * a.nh + j) * hd;
-        for (int it = lane; it < items; it += 32) {
-            float lo[8], hi[8];
-            item(it, lo, hi);
-            const int r = it / groups, i = (it - r * groups) * 8;
-            TA* d = dst + (size_t)r * a.nh * hd;
-            store8(d + (a.pairing == 0 ? i : 2 * i), lo);
-            store8(d + (a.pairing == 0 ? i + half : 2 * i + 8), hi);
+        if (is_q) {
+            TA* d = q_out + ((size_t)(t0 + r) * a.nh + j) * hd;
+            store8(d + ia, lo);
+            store8(d + ib, hi);
         }
-        return;
     }
-    const int plane = j >= a.nh + c.nkv ? 1 : 0, g = j - a.nh - plane * c.nkv;
-    const int page = c.page_of(seq, first), row0 = block_start % c.page_size, old = first - block_start;
-    uint8_t* codes = c.codes + c.codes_at(page, plane, g) + (size_t)row0 * hd;
-    uint8_t* byte = c.scales + c.scales_at(page, plane, g) + row0 / C8_BLOCK;
-    const uint32_t was = old > 0 ? max((uint32_t)*byte, 1u) : 1u;
-    float lo[KEPT][8], hi[KEPT][8];
-    uint32_t top = 0;
-    auto largest = [&](const float (&x)[8], const float (&y)[8]) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) top = max(top, max(c8_magnitude(x[e]), c8_magnitude(y[e])));
-    };
-    // one lane's items; a head too long for its registers goes through the first of them one by one
-    const bool kept = items <= 32 * KEPT;
-    if (kept) {
-#pragma unroll
-        for (int k = 0; k < KEPT; ++k)
-            if (lane + 32 * k < items) { item(lane + 32 * k, lo[k], hi[k]); largest(lo[k], hi[k]); }
-    } else {
-        for (int it = lane; it < items; it += 32) { item(it, lo[0], hi[0]); largest(lo[0], hi[0]); }
+    if (a.written == a.nh) return;                                    // queries only
+    const int plane = j >= a.nh + c.nkv ? 1 : 0, g = j - a.nh - plane * c.nkv, row0 = block_start % c.page_size, old = first - block_start;
+    uint8_t *codes = nullptr, *byte = nullptr;
+    uint32_t was = 1, top = 0;
+    if (!is_q && j < a.written) {
+        const int page = c.page_of(seq, first);
+        codes = c.codes + c.codes_at(page, plane, g) + (size_t)row0 * hd;
+        byte = c.scales + c.scales_at(page, plane, g) + row0 / C8_BLOCK;
+        if (old > 0) was = max((uint32_t)*byte, 1u);                  // (by all of the unit's threads before one of them writes it)
     }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) top = max(top, max(c8_magnitude(lo[e]), c8_magnitude(hi[e])));
     top = __reduce_max_sync(0xffffffffu, top);
+    if (RUNS) {
+        if (lane == 0) s_top[warp] = top;
+        __syncthreads();
+        for (int w = unit * (threads / 32); w < (unit + 1) * (threads / 32); ++w) top = max(top, s_top[w]);
+    }
+    if (codes == nullptr) return;
     const uint32_t b = max(c8_byte(top), was);
-    const float inv = c8_inverse(b);
-    auto write = [&](int it, const float (&x)[8], const float (&y)[8]) {
-        const int r = it / groups, i = (it - r * groups) * 8;
+    if (mine) {
+        const float inv = c8_inverse(b);
         uint8_t* d = codes + (size_t)(old + r) * hd;
         uint32_t w[4];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-            w[e] = c8_encode2(x[4 * e] * inv, x[4 * e + 1] * inv) | (c8_encode2(x[4 * e + 2] * inv, x[4 * e + 3] * inv) << 16);
-            w[2 + e] = c8_encode2(y[4 * e] * inv, y[4 * e + 1] * inv) | (c8_encode2(y[4 * e + 2] * inv, y[4 * e + 3] * inv) << 16);
+            w[e] = c8_encode2(lo[4 * e] * inv, lo[4 * e + 1] * inv) | (c8_encode2(lo[4 * e + 2] * inv, lo[4 * e + 3] * inv) << 16);
+            w[2 + e] = c8_encode2(hi[4 * e] * inv, hi[4 * e + 1] * inv) | (c8_encode2(hi[4 * e + 2] * inv, hi[4 * e + 3] * inv) << 16);
         }
-        *reinterpret_cast<uint2*>(d + (a.pairing == 0 ? i : 2 * i)) = make_uint2(w[0], w[1]);
-        *reinterpret_cast<uint2*>(d + (a.pairing == 0 ? i + half : 2 * i + 8)) = make_uint2(w[2], w[3]);
-    };
-    if (kept) {
-#pragma unroll
-        for (int k = 0; k < KEPT; ++k)
-            if (lane + 32 * k < items) write(lane + 32 * k, lo[k], hi[k]);
-    } else {
-        for (int it = lane; it < items; it += 32) { item(it, lo[0], hi[0]); write(it, lo[0], hi[0]); }
+        *reinterpret_cast<uint2*>(d + ia) = make_uint2(w[0], w[1]);
+        *reinterpret_cast<uint2*>(d + ib) = make_uint2(w[2], w[3]);
     }
     if (b > was && old > 0) {
         const uint32_t factor = c8_shift_factor((int)min(b - was, 25u));
-        for (int v = lane; v < old * (hd / 16); v += 32) {
+        for (int v = it; v < old * (hd / 16); v += threads) {
             uint4* p = reinterpret_cast<uint4*>(codes) + v;
             *p = c8_shift16(*p, factor);
         }
     }
-    if (lane == 0) *byte = (uint8_t)b;
+    if (it == 0) *byte = (uint8_t)b;
 }
 
 }  // namespace
@@ -183,11 +168,13 @@ TQ_EXPORT int tq_write8(const void* qkv, int act_dtype, const void* bias, int bi
     const Cache8 c{(uint8_t*)codes, (uint8_t*)scales, page_table, table_stride, page_size, n_pages, nkv, hd};
     const WriteArgs a{cos_t, sin_t, positions, cu_seqlens, held, nh, pairing, codes != nullptr ? nh + 2 * nkv : nh};
     // a run of n rows touches at most (n + 14) / 16 + 1 blocks
-    const int units = max_q_len == 1 ? 1 : (max_q_len + 14) / C8_BLOCK + 1, heads = a.written, warps = units * n_seqs >= 128 ? 8 : 2;
-    const dim3 grid(units, (heads + warps - 1) / warps, n_seqs);
+    const bool runs = max_q_len > 1;
+    const int units = runs ? (max_q_len + 14) / C8_BLOCK + 1 : 1, threads = runs ? (hd + 31) / 32 * 32 : 32;
+    const int side = runs ? WRITE_THREADS / threads : n_seqs >= 32 ? 8 : 2;              // units a block takes side by side
+    const dim3 grid(units, (a.written + side - 1) / side, n_seqs);
     TQ_DISPATCH(act_dtype, TA, TQ_DISPATCH(bias != nullptr ? bias_dtype : act_dtype, TB,
-        if (max_q_len == 1) tq_launch(grid, warps * 32, 0, stream)(write8_kernel<TA, TB, 1>, (const TA*)qkv, (const TB*)bias, a, (TA*)q_out, c);
-        else tq_launch(grid, warps * 32, 0, stream)(write8_kernel<TA, TB, 4>, (const TA*)qkv, (const TB*)bias, a, (TA*)q_out, c)));
+        if (runs) tq_launch(grid, side * threads, 0, stream)(write8_kernel<TA, TB, true>, (const TA*)qkv, (const TB*)bias, a, (TA*)q_out, c, threads);
+        else tq_launch(grid, side * threads, 0, stream)(write8_kernel<TA, TB, false>, (const TA*)qkv, (const TB*)bias, a, (TA*)q_out, c, threads)));
     TQ_CHECK_LAUNCH("write8");
     return 0;
 }

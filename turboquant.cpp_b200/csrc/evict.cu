@@ -17,16 +17,20 @@ __device__ __forceinline__ uint32_t rank_of(float w) {
 }
 
 // ---------------------------------------------------------------------------------------
-// Selection: a block per (key/value head, sequence) finds the rank of the last row that stays, a byte at a time from the highest (a
-// histogram of the rows that agree in the bytes found), then lists the rows above it and, of those equal to it, the first ones.
+// Selection: a block per (key/value head, sequence) finds the rank of the last row that stays, 11, 11 and 10 bits at a time from the highest
+// (a histogram of the rows that agree in the bits found), then lists the rows above it and, of those equal to it, the first ones.  The
+// ranks are read once, through the page table, and stay in shared memory as far as they fit (`cached` of them).
 // ---------------------------------------------------------------------------------------
-constexpr int SELECT_THREADS = 1024;
+constexpr int SELECT_THREADS = 1024, SELECT_WARPS = SELECT_THREADS / 32, BINS = 2048;
+constexpr int SELECT_MOST = 48 * 1024;             // ranks a block keeps, 192 KB
 
 __global__ void __launch_bounds__(SELECT_THREADS) evict8_select_kernel(const float* __restrict__ weights, const int* __restrict__ lengths, const int* __restrict__ table,
-                                                                       int table_stride, int page_size, int n_pages, int nkv, int budget, int recent, int* __restrict__ kept) {
+                                                                       int table_stride, int page_size, int n_pages, int nkv, int budget, int recent, int cached,
+                                                                       int* __restrict__ kept) {
     tq_grid_wait();                    // everything below may read what the previous kernel wrote
     tq_grid_launch_dependents();
-    __shared__ int s_hist[256], s_pick[2], s_sum[2][SELECT_THREADS / 32];
+    extern __shared__ uint32_t s_rank[];
+    __shared__ int s_hist[BINS], s_pick[2], s_warp[2][SELECT_WARPS];
     const int g = blockIdx.x, seq = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int n = max(0, min(lengths[seq], table_stride * page_size));
     int* list = kept + ((size_t)seq * nkv + g) * budget;
@@ -38,99 +42,114 @@ __global__ void __launch_bounds__(SELECT_THREADS) evict8_select_kernel(const flo
     for (int j = tid; j < recent; j += SELECT_THREADS) list[want + j] = rest + j;
     if (want == 0) return;
     const int* pages = table + (size_t)seq * table_stride;
-    auto rank_at = [&](int p) {
+    auto read = [&](int p) {
         const int page = TQ_CHECKED(pages[p / page_size], n_pages, TQ_IDX_PAGE);
         return rank_of(weights[((size_t)page * nkv + g) * page_size + p % page_size]);
     };
-    uint32_t prefix = 0;
-    int missing = want;                                               // rows still to be found among those that agree with the prefix
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        if (tid < 256) s_hist[tid] = 0;
+    auto rank_at = [&](int p) { return p < cached ? s_rank[p] : read(p); };
+#pragma unroll 4
+    for (int p = tid; p < min(rest, cached); p += SELECT_THREADS) s_rank[p] = read(p);
+    uint32_t prefix = 0, known = 0;                                   // the bits found and which they are
+    int missing = want;                                               // rows still to be found among those that agree with them
+    for (int pass = 0; pass < 3; ++pass) {
+        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : BINS;
+        for (int x = tid; x < bins; x += SELECT_THREADS) s_hist[x] = 0;
         __syncthreads();
-        for (int p = tid; p < rest; p += SELECT_THREADS) {
-            const uint32_t k = rank_at(p);
-            if (shift == 24 || (k >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&s_hist[(k >> shift) & 255u], 1);
+        for (int p0 = 0; p0 < rest; p0 += SELECT_THREADS) {
+            const int p = p0 + tid;
+            const uint32_t k = p < rest ? rank_at(p) : 0u;
+            const bool counts = p < rest && (k & known) == prefix;
+            const int bin = counts ? (int)((k >> shift) & (uint32_t)(bins - 1)) : -1;
+            // the first lane's bin is counted once for all lanes that share it (rows that never received any weight are many)
+            const int lead = __shfl_sync(0xffffffffu, bin, 0);
+            const uint32_t same = __ballot_sync(0xffffffffu, bin == lead);
+            if (lead >= 0 && lane == 0) atomicAdd(&s_hist[lead], __popc(same));
+            if (bin >= 0 && bin != lead) atomicAdd(&s_hist[bin], 1);
         }
         __syncthreads();
-        if (warp == 0) {                                              // lane i: bins 255 - 8 i downwards
-            int sum = 0;
-            for (int j = 0; j < 8; ++j) sum += s_hist[255 - 8 * lane - j];
-            int above = sum;                                          // rows in the bins of this lane and those before it
-            for (int o = 1; o < 32; o <<= 1) {
-                const int v = __shfl_up_sync(0xffffffffu, above, o);
-                if (lane >= o) above += v;
-            }
-            const int before = above - sum;
-            if (before < missing && missing <= above) {
-                int left = missing - before, bin = 255 - 8 * lane;
-                while (s_hist[bin] < left) left -= s_hist[bin--];
-                s_pick[0] = bin;
-                s_pick[1] = left;
-            }
+        // a thread has one or two bins, thread 0 the highest: rows in them and, scanned over the block, in those above
+        const int each = bins / SELECT_THREADS, high = bins - 1 - each * tid;
+        const int sum = s_hist[high] + (each > 1 ? s_hist[high - 1] : 0);
+        int above = sum;
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, above, o);
+            if (lane >= o) above += v;
+        }
+        if (lane == 31) s_warp[0][warp] = above;
+        __syncthreads();
+        above += __reduce_add_sync(0xffffffffu, lane < warp ? s_warp[0][lane] : 0);
+        const int before = above - sum;
+        if (before < missing && missing <= above) {
+            const bool first = missing - before <= s_hist[high];
+            s_pick[0] = first ? high : high - 1;
+            s_pick[1] = missing - before - (first ? 0 : s_hist[high]);
         }
         __syncthreads();
         prefix |= (uint32_t)s_pick[0] << shift;
+        known |= (uint32_t)(bins - 1) << shift;
         missing = s_pick[1];
         __syncthreads();
     }
-    // rows above `prefix` stay, and the first `missing` of those equal to it
-    int base_above = 0, base_equal = 0;
-    for (int p0 = 0; p0 < rest; p0 += SELECT_THREADS) {
-        const int p = p0 + tid;
-        const uint32_t k = p < rest ? rank_at(p) : 0u;
-        const bool above = p < rest && k > prefix, equal = p < rest && k == prefix;
-        const uint32_t am = __ballot_sync(0xffffffffu, above), em = __ballot_sync(0xffffffffu, equal), below = (1u << lane) - 1u;
-        if (lane == 0) { s_sum[0][warp] = __popc(am); s_sum[1][warp] = __popc(em); }
-        __syncthreads();
-        int a = base_above + __popc(am & below), e = base_equal + __popc(em & below);
-        for (int w = 0; w < SELECT_THREADS / 32; ++w) {
-            if (w < warp) { a += s_sum[0][w]; e += s_sum[1][w]; }
-            base_above += s_sum[0][w];
-            base_equal += s_sum[1][w];
-        }
-        if (above || (equal && e < missing)) list[a + min(e, missing)] = p;
-        __syncthreads();
+    // rows above `prefix` stay, and the first `missing` of those equal to it: a warp has a stretch of the places
+    const int stretch = ((rest + SELECT_WARPS - 1) / SELECT_WARPS + 31) / 32 * 32, from = warp * stretch, to = min(from + stretch, rest);
+    int above = 0, equal = 0;
+    for (int p0 = from; p0 < to; p0 += 32) {
+        const uint32_t k = p0 + lane < to ? rank_at(p0 + lane) : 0u;
+        above += __popc(__ballot_sync(0xffffffffu, p0 + lane < to && k > prefix));
+        equal += __popc(__ballot_sync(0xffffffffu, p0 + lane < to && k == prefix));
+    }
+    if (lane == 0) { s_warp[0][warp] = above; s_warp[1][warp] = equal; }
+    __syncthreads();
+    int a = lane < warp ? s_warp[0][lane] : 0, e = lane < warp ? s_warp[1][lane] : 0;         // what the warps before found
+    a = __reduce_add_sync(0xffffffffu, a);
+    e = __reduce_add_sync(0xffffffffu, e);
+    for (int p0 = from; p0 < to; p0 += 32) {
+        const uint32_t k = p0 + lane < to ? rank_at(p0 + lane) : 0u, below = (1u << lane) - 1u;
+        const uint32_t am = __ballot_sync(0xffffffffu, p0 + lane < to && k > prefix), em = __ballot_sync(0xffffffffu, p0 + lane < to && k == prefix);
+        const int a1 = a + __popc(am & below), e1 = e + __popc(em & below);
+        if ((am >> lane & 1u) || ((em >> lane & 1u) && e1 < missing)) list[a1 + min(e1, missing)] = p0 + lane;
+        a += __popc(am);
+        e += __popc(em);
     }
 }
 
 // ---------------------------------------------------------------------------------------
-// Moving: a block per 16 rows of the list.  The new block's byte is the largest of its rows' bytes; rows of a smaller one are rounded again.
+// Moving: a warp per 16 rows of the list and plane.  The new block's byte is the largest of its rows' bytes; rows of a smaller one are rounded
+// again.  Nothing is shared between warps; a row's page, byte and place go from lane to lane by shuffles.
 // ---------------------------------------------------------------------------------------
-__global__ void __launch_bounds__(128) evict8_move_kernel(Cache8 c, float* __restrict__ weights, const int* __restrict__ kept, const int* __restrict__ new_table,
+__global__ void __launch_bounds__(256) evict8_move_kernel(Cache8 c, float* __restrict__ weights, const int* __restrict__ kept, const int* __restrict__ new_table,
                                                           int new_stride, int budget) {
     tq_grid_wait();                    // everything below may read what the previous kernel wrote
     tq_grid_launch_dependents();
-    __shared__ size_t s_from[2][C8_BLOCK];
-    __shared__ uint32_t s_byte[2][C8_BLOCK];
-    const int seq = blockIdx.z, g = blockIdx.y, first = blockIdx.x * C8_BLOCK, tid = threadIdx.x;
+    const int lane = threadIdx.x & 31, work = blockIdx.x * 8 + (threadIdx.x >> 5), plane = work & 1, first = (work >> 1) * C8_BLOCK, seq = blockIdx.z, g = blockIdx.y;
+    if (first >= budget) return;
     const int* list = kept + ((size_t)seq * c.nkv + g) * budget;
-    const int rows = min(C8_BLOCK, budget - first);
-    if (list[first] < 0) return;                                      // the list ends before this block
+    const int place = lane < C8_BLOCK && first + lane < budget ? list[first + lane] : -1;
     const int page = TQ_CHECKED(new_table[(size_t)seq * new_stride + TQ_CHECKED(first / c.page_size, new_stride, TQ_IDX_TABLE_COLUMN)], c.n_pages, TQ_IDX_PAGE);
+    if (__shfl_sync(0xffffffffu, place, 0) < 0) return;               // the list ends before this block
     const int row0 = first % c.page_size;
-    if (tid < 2 * C8_BLOCK) {
-        const int plane = tid / C8_BLOCK, r = tid % C8_BLOCK, place = r < rows ? list[first + r] : -1;
-        uint32_t byte = 0;
-        if (place >= 0) {
-            const int from = c.page_of(seq, place), row = place % c.page_size;
-            byte = c.scales[c.scales_at(from, plane, g) + row / C8_BLOCK];
-            s_from[plane][r] = c.codes_at(from, plane, g) + (size_t)row * c.hd;
-            if (plane == 0) weights[((size_t)page * c.nkv + g) * c.page_size + row0 + r] = weights[((size_t)from * c.nkv + g) * c.page_size + row];
-        }
-        uint32_t top = byte;
-        for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-        s_byte[plane][r] = place < 0 ? 256u : top - byte;             // how far the row's codes move; 256: no row
-        if (r == 0) c.scales[c.scales_at(page, plane, g) + row0 / C8_BLOCK] = (uint8_t)top;
+    unsigned long long from = 0;
+    uint32_t byte = 0;
+    if (place >= 0) {
+        const int old = c.page_of(seq, place), row = place % c.page_size;
+        from = c.codes_at(old, plane, g) + (size_t)row * c.hd;
+        byte = c.scales[c.scales_at(old, plane, g) + row / C8_BLOCK];
+        if (plane == 0) weights[((size_t)page * c.nkv + g) * c.page_size + row0 + lane] = weights[((size_t)old * c.nkv + g) * c.page_size + row];
     }
-    __syncthreads();
-    const int vecs = c.hd / 16;
-    for (int v = tid; v < 2 * C8_BLOCK * vecs; v += blockDim.x) {
-        const int plane = v / (C8_BLOCK * vecs), r = v / vecs % C8_BLOCK, at = v % vecs;
-        const uint32_t shift = s_byte[plane][r];
-        if (shift == 256u) continue;
-        uint4 x = *reinterpret_cast<const uint4*>(c.codes + s_from[plane][r] + at * 16);
-        if (shift) x = c8_shift16(x, c8_shift_factor((int)min(shift, 25u)));
-        *reinterpret_cast<uint4*>(c.codes + c.codes_at(page, plane, g) + (size_t)(row0 + r) * c.hd + at * 16) = x;
+    const uint32_t top = __reduce_max_sync(0xffffffffu, byte);
+    const int rows = __popc(__ballot_sync(0xffffffffu, place >= 0)), vecs = c.hd / 16;
+    if (lane == 0) c.scales[c.scales_at(page, plane, g) + row0 / C8_BLOCK] = (uint8_t)top;
+    uint8_t* to = c.codes + c.codes_at(page, plane, g) + (size_t)row0 * c.hd;
+#pragma unroll 4
+    for (int v0 = 0; v0 < C8_BLOCK * vecs; v0 += 32) {                // (16 rows: a multiple of 32 pieces or half of one)
+        const int v = v0 + lane, r = min(v / vecs, C8_BLOCK - 1), at = v - v / vecs * vecs;
+        const unsigned long long src = __shfl_sync(0xffffffffu, from, r);
+        const uint32_t shift = top - __shfl_sync(0xffffffffu, byte, r);
+        if (v < rows * vecs) {
+            uint4 x = *reinterpret_cast<const uint4*>(c.codes + src + at * 16);
+            if (shift) x = c8_shift16(x, c8_shift_factor((int)min(shift, 25u)));
+            *reinterpret_cast<uint4*>(to + (size_t)r * c.hd + at * 16) = x;
+        }
     }
 }
 
@@ -143,7 +162,11 @@ TQ_EXPORT int tq_evict8_select(const float* weights, const int* lengths, const i
     TQ_REQUIRE(budget >= 1 && recent >= 0 && recent <= budget, "evict8: %d newest of a budget of %d rows", recent, budget);
     TQ_REQUIRE(page_size >= 1 && table_stride >= 1 && nkv >= 1 && n_seqs <= 65535, "evict8: page size %d, tables %d wide, %d heads, %d sequences", page_size, table_stride, nkv, n_seqs);
     TQ_REQUIRE((long long)table_stride * page_size < (1ll << 31), "evict8: page tables of %d pages", table_stride);
-    tq_launch(dim3(nkv, n_seqs), SELECT_THREADS, 0, stream)(evict8_select_kernel, weights, lengths, page_table, table_stride, page_size, n_pages, nkv, budget, recent, kept);
+    const int cached = table_stride * page_size < SELECT_MOST ? table_stride * page_size : SELECT_MOST;
+    static TqSmemAsked asked;
+    const cudaError_t e = tq_grow_smem(evict8_select_kernel, (size_t)cached * 4, asked);
+    if (e != cudaSuccess) TQ_FAIL(-1, "evict8_select: cannot reserve %d bytes of shared memory: %s", cached * 4, cudaGetErrorString(e));
+    tq_launch(dim3(nkv, n_seqs), SELECT_THREADS, (size_t)cached * 4, stream)(evict8_select_kernel, weights, lengths, page_table, table_stride, page_size, n_pages, nkv, budget, recent, cached, kept);
     TQ_CHECK_LAUNCH("evict8_select");
     return 0;
 }
@@ -157,7 +180,7 @@ TQ_EXPORT int tq_evict8_move(void* codes, void* scales, float* weights, const in
     TQ_REQUIRE(budget >= 1 && (long long)new_stride * page_size >= budget, "evict8: %d new pages a sequence for a budget of %d rows", new_stride, budget);
     TQ_REQUIRE(n_seqs <= 65535 && nkv <= 65535, "evict8: %d sequences, %d heads", n_seqs, nkv);
     const Cache8 c{(uint8_t*)codes, (uint8_t*)scales, page_table, table_stride, page_size, n_pages, nkv, hd};
-    tq_launch(dim3((budget + C8_BLOCK - 1) / C8_BLOCK, nkv, n_seqs), 128, 0, stream)(evict8_move_kernel, c, weights, kept, new_table, new_stride, budget);
+    tq_launch(dim3(((budget + C8_BLOCK - 1) / C8_BLOCK * 2 + 7) / 8, nkv, n_seqs), 256, 0, stream)(evict8_move_kernel, c, weights, kept, new_table, new_stride, budget);
     TQ_CHECK_LAUNCH("evict8_move");
     return 0;
 }

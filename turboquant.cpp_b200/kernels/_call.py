@@ -57,11 +57,38 @@ def check(lib_name: str, rc: int, kernels: int = 1) -> None:
         raise KernelError(lib.tq_last_error().decode("utf-8", "replace") or f"{lib_name}: error {rc}")
 
 
+def declared(lib: ctypes.CDLL, name: str, signature: str):
+    """A launcher of a loaded kernel library with its argument types declared, which is cheaper to call than one that gets ctypes objects:
+    signature has a letter per argument, p for an address (an int or None), i for a whole number, f for a float."""
+    kinds = {"p": ctypes.c_void_p, "i": ctypes.c_int, "f": ctypes.c_float}
+    fn = getattr(lib, name)
+    fn.argtypes = [kinds[c] for c in signature]
+    return fn
+
+
+def address(t: Optional[torch.Tensor]) -> Optional[int]:
+    """What `ptr` gives, as a plain int for launchers with declared arguments."""
+    if t is None:
+        return None
+    if not (t.is_cuda and t.is_contiguous()):
+        ptr(t)                              # raises
+    return t.data_ptr()
+
+
+def raw_stream() -> int:
+    return _raw_stream(_raw_device()) if _raw_stream is not None and _raw_device is not None else torch.cuda.current_stream().cuda_stream
+
+
 def on_current_device(*tensors: Optional[torch.Tensor]) -> None:
     """Launches go to the current device's stream: tensors of another GPU are refused instead of read from there."""
-    used = {t.get_device() for t in tensors if t is not None and t.is_cuda}
-    if used and used != {_raw_device() if _raw_device is not None else torch.cuda.current_device()}:
-        raise KernelError(f"tensors lie on GPU {', '.join(map(str, sorted(used)))}, the current device is {torch.cuda.current_device()}")
+    here = -1
+    for t in tensors:
+        if t is None or not t.is_cuda:
+            continue
+        if here < 0:
+            here = _raw_device() if _raw_device is not None else torch.cuda.current_device()
+        if t.get_device() != here:
+            raise KernelError(f"a tensor lies on GPU {t.get_device()}, the current device is {here}")
 
 
 def ints(*values) -> map:

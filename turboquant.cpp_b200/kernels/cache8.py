@@ -15,18 +15,49 @@ are int32 on the device; every place a call reads or writes needs its page, and 
 The launches go to the current stream, allocate their scratch from torch's allocator and can be captured into CUDA graphs."""
 from __future__ import annotations
 
-from ctypes import c_float, c_void_p
+from functools import lru_cache
+from operator import index
 from typing import Optional, Tuple
 
 import torch
 
 from ..csrc.build import load_kernel
-from ._call import KernelError, check, code, ints, on_current_device, ptr, stream, want_f32, want_int32
+from ._call import KernelError, address, check, code, declared, on_current_device, raw_stream, want_f32, want_int32
 from .attention import PAIRING, prefill_rows, prefill_usable, resident_ctas
 from .gemm_tc import status_word
 
 BLOCK = 16
 MAX_HEAD_DIM = 256
+
+
+_SIGNATURES = {              # argument types of the entry points (_call.declared)
+    "tq_write8": "pipippipppp" "iippp" "iiiiii" "p", "tq_attention8": "pppippp" "iiifppi" "ppipi" "iiiiii" "p",
+    "tq_weigh8": "pppippp" "iiifpp" "iiiiiii" "p", "tq_repair8": "pppppp" "iiifppi" "iiiii" "p",
+    "tq_expand8": "ppppp" "iiipppi" "iiii" "p", "tq_weigh8_prompt": "ppippp" "iifpp" "iiiiiii" "pp",
+    "tq_evict8_select": "ppp" "iiiiiii" "pp", "tq_evict8_move": "ppppp" "ipi" "iiiiii" "p",
+}
+_entries = {}
+
+
+def _declare(lib, name: str):
+    fn = _entries[name] = declared(lib, name, _SIGNATURES[name])
+    return fn
+
+
+def _cache8(name: str):
+    return _entries.get(name) or _declare(load_kernel("cache8"), name)
+
+
+def _attention8(name: str):
+    return _entries.get(name) or _declare(load_kernel("attention8"), name)
+
+
+def _prompt8(name: str):
+    return _entries.get(name) or _declare(load_kernel("prompt8"), name)
+
+
+def _evict(name: str):
+    return _entries.get(name) or _declare(load_kernel("evict"), name)
 
 
 def storage(n_pages: int, n_kv_heads: int, page_size: int, head_dim: int, device, weights: bool = False
@@ -47,12 +78,16 @@ def check_sizes(page_size: int, head_dim: int) -> None:
 
 def _check_cache(codes, scales, weights, page_table, page_size, n_kv_heads, head_dim) -> None:
     pages = codes.shape[0]
-    if codes.dtype != torch.float8_e4m3fn or tuple(codes.shape) != (pages, 2, n_kv_heads, page_size, head_dim):
+    if codes.dtype != torch.float8_e4m3fn or codes.shape != (pages, 2, n_kv_heads, page_size, head_dim):
         raise KernelError(f"8-bit cache: codes must be float8_e4m3fn [pages, 2, {n_kv_heads}, {page_size}, {head_dim}], got {codes.dtype} {tuple(codes.shape)}")
-    if scales.dtype != torch.uint8 or tuple(scales.shape) != (pages, 2, n_kv_heads, page_size // BLOCK):
+    if scales.dtype != torch.uint8 or scales.shape != (pages, 2, n_kv_heads, page_size // BLOCK):
         raise KernelError(f"8-bit cache: scales must be uint8 [{pages}, 2, {n_kv_heads}, {page_size // BLOCK}], got {scales.dtype} {tuple(scales.shape)}")
-    if weights is not None and (weights.dtype != torch.float32 or tuple(weights.shape) != (pages, n_kv_heads, page_size)):
+    if weights is not None and (weights.dtype != torch.float32 or weights.shape != (pages, n_kv_heads, page_size)):
         raise KernelError(f"8-bit cache: weights must be float32 [{pages}, {n_kv_heads}, {page_size}], got {weights.dtype} {tuple(weights.shape)}")
+    _check_table(page_table)
+
+
+def _check_table(page_table) -> None:
     if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[1] < 1:
         raise KernelError(f"8-bit cache: the page table must be int32 [sequences, pages], got {page_table.dtype} {tuple(page_table.shape)}")
 
@@ -78,6 +113,7 @@ def write_rows8(qkv: torch.Tensor, bias: Optional[torch.Tensor], cos: Optional[t
         raise KernelError("write_rows8: codes and scales come together")
     if codes is None:
         check_sizes(page_size, head_dim)
+        _check_table(page_table)
     else:
         _check_cache(codes, scales, None, page_table, page_size, n_kv_heads, head_dim)
     n = _check_step(cu_seqlens, held, page_table, "write_rows8")
@@ -94,23 +130,25 @@ def write_rows8(qkv: torch.Tensor, bias: Optional[torch.Tensor], cos: Optional[t
             raise KernelError(f"write_rows8: cos and sin tables must be [positions, {head_dim // 2}]")
     if T == 0:
         return
-    on_current_device(qkv, q_out, codes, scales)
-    check("cache8", load_kernel("cache8").tq_write8(
-        ptr(qkv), code(qkv.dtype), ptr(bias), 0 if bias is None else code(bias.dtype), ptr(cos), ptr(sin), PAIRING[pairing], ptr(positions),
-        ptr(cu_seqlens), ptr(held), ptr(page_table), page_table.shape[1], page_size, ptr(q_out), ptr(codes), ptr(scales),
-        0 if codes is None else codes.shape[0], n, *ints(max_q_len, n_heads, n_kv_heads, head_dim), stream()))
+    on_current_device(qkv, q_out, codes, scales, page_table)
+    check("cache8", _cache8("tq_write8")(
+        address(qkv), code(qkv.dtype), address(bias), 0 if bias is None else code(bias.dtype), address(cos), address(sin), PAIRING[pairing], address(positions),
+        address(cu_seqlens), address(held), address(page_table), page_table.shape[1], page_size, address(q_out), address(codes), address(scales),
+        0 if codes is None else codes.shape[0], n, index(max_q_len), n_heads, n_kv_heads, head_dim, raw_stream()))
 
 
+MAX_RANGES = 64
+SETUP, JOIN = 1.5, 2.5       # what a CTA's begin and end, and the second launch, take in turns of its warps over blocks of keys
+
+
+@lru_cache(maxsize=4096)
 def ranges_for(tiles: int, blocks: int, resident: int) -> int:
-    """Ranges the keys of a tile of columns are cut into: as many as fill the CTAs the device runs at once, each of at least two blocks of
-    16 keys for its four warps; with more tiles than that, the count (up to 8) whose last wave is fullest, and one from four waves on."""
-    most = max(1, blocks // 8)
-    if tiles <= resident:
-        return max(1, min(most, resident // tiles))
-    if tiles >= 4 * resident:
-        return 1
-    fill = lambda n: tiles * n / (-(-tiles * n // resident) * resident)
-    return max(range(1, min(8, most) + 1), key=lambda n: (round(fill(n), 2), -n))
+    """Ranges the keys of a tile of columns are cut into, where the device runs `resident` CTAs at once and a CTA's four warps take a block of 16
+    keys each in turn: the count with the fewest turns.  (B200, 16 heads of 128, 64 sequences of up to 2,048 keys, 1,024 tiles: one
+    range 86 us, two 97, three 95, four 99.)"""
+    turns = lambda n: -(-tiles * n // resident) * (-(-blocks // (4 * n)) + SETUP) + (JOIN if n > 1 else 0.0)
+    most = max(1, min(MAX_RANGES, blocks // 4, max(8, resident // tiles)))
+    return min((n for n in (1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, most) if n <= most), key=lambda n: (turns(n), n))
 
 
 SCORE_BYTES = 1 << 28        # scratch a decode step may take for scores
@@ -133,7 +171,8 @@ def attention8(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, cu_se
         raise KernelError(f"attention8: queries {tuple(q.shape)} {q.dtype} and output {tuple(out.shape)} {out.dtype} do not fit {n_heads} heads of {head_dim}")
     if T == 0 or n == 0 or max_q_len < 1:
         return out
-    on_current_device(q, out, codes, scales, weights)
+    max_q_len, max_kv_len = index(max_q_len), index(max_kv_len)
+    on_current_device(q, out, codes, scales, weights, page_table)
     if max_q_len >= PROMPT_MIN_RUN and prefill_usable(q.dtype, head_dim, page_size):
         return _attention8_prompt(q, codes, scales, cu_seqlens, held, page_table, page_size, window, scale, out, n_heads, n_kv_heads, head_dim,
                                   max_q_len, max_kv_len, weights, status)
@@ -142,27 +181,28 @@ def attention8(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, cu_se
     wide = columns > 8 and head_dim <= 128                  # two tiles of 8 columns in one CTA
     tiles = -(-columns // (16 if wide else 8)) * n_kv_heads * n
     per_sm = 2 if head_dim > 128 else 3 if wide and head_dim > 64 else 4         # CTAs an SM holds
-    ranges = ranges_for(tiles, -(-max_kv_len // BLOCK), resident_ctas(q.device) // 4 * per_sm)
+    blocks = -(-max_kv_len // BLOCK)
+    ranges = ranges_for(tiles, blocks, resident_ctas(q.device) // 4 * per_sm)
     # one row a sequence: the first launch leaves its scores for the second one to add up, which moves 8 bytes a key and query head, where
     # reading the keys again moves head_dim bytes a key
-    stride = -(-max_kv_len // BLOCK) * BLOCK
-    stored = weights is not None and max_q_len == 1 and 8 * per <= head_dim and 4 * T * n_heads * stride <= SCORE_BYTES
-    rows = T * n_heads
+    stride, rows = blocks * BLOCK, T * n_heads
+    stored = weights is not None and max_q_len == 1 and 8 * per <= head_dim and 4 * rows * stride <= SCORE_BYTES
+    again = weights is not None and not stored
     partial_floats = rows * ranges * (head_dim + 4) if ranges > 1 or stored else 0
-    scratch = torch.empty(partial_floats + (rows * stride if stored else 0) + (rows if weights is not None and not stored else 0), dtype=torch.float32,
-                          device=q.device) if weights is not None or partial_floats else None
-    at = 0 if scratch is None else scratch.data_ptr()
-    partial = at if partial_floats else None
-    rest = at + 4 * partial_floats
-    lib = load_kernel("attention8")
-    args = (ptr(q), ptr(codes), ptr(scales), code(q.dtype), ptr(cu_seqlens), ptr(held), ptr(page_table), page_table.shape[1], *ints(page_size, window), c_float(scale))
-    step = (codes.shape[0], n, *ints(max_q_len))
-    heads = (*ints(n_heads, n_kv_heads, head_dim), stream())
-    check("attention8", lib.tq_attention8(*args, ptr(out), c_void_p(partial), ranges, c_void_p(rest if weights is not None and not stored else None),
-                                          c_void_p(rest if stored else None), stride, ptr(weights) if stored else None, *ints(max_kv_len), *step, *heads),
-          kernels=2 if partial_floats else 1)
-    if weights is not None and not stored:
-        check("attention8", lib.tq_weigh8(*args, c_void_p(rest), ptr(weights), *step, *ints(max_kv_len), *heads))
+    partial = rest = None
+    if weights is not None or partial_floats:
+        scratch = torch.empty(partial_floats + (rows * stride if stored else 0) + (rows if again else 0), dtype=torch.float32, device=q.device)
+        rest = scratch.data_ptr() + 4 * partial_floats
+        if partial_floats:
+            partial = scratch.data_ptr()
+    step = (address(q), address(codes), address(scales), code(q.dtype), address(cu_seqlens), address(held), address(page_table), page_table.shape[1],
+            page_size, window, scale)
+    heads = (n_heads, n_kv_heads, head_dim, raw_stream())
+    check("attention8", _attention8("tq_attention8")(
+        *step, address(out), partial, ranges, rest if again else None, rest if stored else None, stride, address(weights) if stored else None, max_kv_len,
+        codes.shape[0], n, max_q_len, *heads), kernels=2 if partial_floats else 1)
+    if again:
+        check("attention8", _attention8("tq_weigh8")(*step, rest, address(weights), codes.shape[0], n, max_q_len, max_kv_len, *heads))
     return out
 
 
@@ -186,15 +226,15 @@ def _attention8_prompt(q, codes, scales, cu_seqlens, held, page_table, page_size
     for i in range(0, n, group):
         m = min(group, n - i)
         cu, starts, pages, dtable = cu_seqlens[i:i + m + 1], held[i:i + m], page_table[i:i + m], table[:m]
-        cache = (ptr(codes), ptr(scales), ptr(cu), ptr(starts), ptr(pages), pages.shape[1], *ints(page_size, window))
-        check("prompt8", load_kernel("prompt8").tq_expand8(*cache, ptr(dense), ptr(table), ptr(lost), width, codes.shape[0], m, *ints(n_kv_heads, head_dim), stream()))
+        cache = (address(codes), address(scales), address(cu), address(starts), address(pages), pages.shape[1], page_size, window)
+        check("prompt8", _prompt8("tq_expand8")(*cache, address(dense), address(table), address(lost), width, codes.shape[0], m, n_kv_heads, head_dim, raw_stream()))
         prefill_rows(q, dense, 2, cu, starts, dtable, page_size, window, scale, out, m, max_q_len, n_heads, n_kv_heads, head_dim, head_dim, status=status, lse=lse)
-        check("attention8", load_kernel("attention8").tq_repair8(
-            ptr(q), *cache, c_float(scale), ptr(out), ptr(lost), width, codes.shape[0], m, *ints(n_heads, n_kv_heads, head_dim), stream()))
+        check("attention8", _attention8("tq_repair8")(
+            address(q), *cache, scale, address(out), address(lost), width, codes.shape[0], m, n_heads, n_kv_heads, head_dim, raw_stream()))
         if weights is not None:
-            check("prompt8", load_kernel("prompt8").tq_weigh8_prompt(
-                ptr(q), ptr(dense), width, ptr(cu), ptr(starts), ptr(pages), pages.shape[1], *ints(window), c_float(scale), ptr(lse), ptr(weights),
-                codes.shape[0], T, m, *ints(max_kv_len, n_heads, n_kv_heads, head_dim), ptr(status), stream()))
+            check("prompt8", _prompt8("tq_weigh8_prompt")(
+                address(q), address(dense), width, address(cu), address(starts), address(pages), pages.shape[1], window, scale, address(lse), address(weights),
+                codes.shape[0], T, m, max_kv_len, n_heads, n_kv_heads, head_dim, address(status), raw_stream()))
     return out
 
 
@@ -216,12 +256,12 @@ def evict8(codes: torch.Tensor, scales: torch.Tensor, weights: torch.Tensor, len
         raise KernelError(f"evict8: {n} page tables, {lengths.numel()} lengths and new tables {tuple(new_table.shape)} for a budget of {budget} rows do not fit together")
     if not 0 <= recent <= budget or budget < 1:
         raise KernelError(f"evict8: cannot keep the newest {recent} rows of a budget of {budget}")
-    on_current_device(codes, scales, weights)
+    on_current_device(codes, scales, weights, page_table, new_table)
     kept = torch.empty((n, n_kv_heads, budget), dtype=torch.int32, device=codes.device)
-    lib = load_kernel("evict")
-    check("evict", lib.tq_evict8_select(
-        ptr(weights), ptr(lengths), ptr(page_table), page_table.shape[1], *ints(page_size, codes.shape[0], n, n_kv_heads, budget, recent), ptr(kept), stream()))
-    check("evict", lib.tq_evict8_move(
-        ptr(codes), ptr(scales), ptr(weights), ptr(kept), ptr(page_table), page_table.shape[1], ptr(new_table), new_table.shape[1],
-        *ints(page_size, codes.shape[0], n, n_kv_heads, head_dim, budget), stream()))
+    width, pages = page_table.shape[1], codes.shape[0]
+    check("evict", _evict("tq_evict8_select")(
+        address(weights), address(lengths), address(page_table), width, page_size, pages, n, n_kv_heads, budget, recent, address(kept), raw_stream()))
+    check("evict", _evict("tq_evict8_move")(
+        address(codes), address(scales), address(weights), address(kept), address(page_table), width, address(new_table), new_table.shape[1],
+        page_size, pages, n, n_kv_heads, head_dim, budget, raw_stream()))
     return kept
