@@ -617,7 +617,7 @@ __global__ void __launch_bounds__(128) join8_kernel(Cache8 c, Step S, const floa
         }
     }
     if (place >= start + run || (S.window > 0 && place + S.window <= start)) return;       // no row of the step sees it
-    float* w = weights + ((size_t)c.page_of(seq, place) * c.nkv + g) * c.page_size + place % c.page_size;
+    float* w = weights + ((size_t)c.page_of(seq, place) * c.nkv + g) * c.page_size + c.row(place);
     *w = (place < start ? *w : 0.f) + sum;
 }
 
@@ -642,7 +642,7 @@ __global__ void __launch_bounds__(WARPS * 32) weigh8_kernel(const typename F::TA
     KeyRegs<F> kr = {};
     float ks = 0.f;
     int page = 0;
-    const int row = block * C8_BLOCK % c.page_size;
+    const int row = c.row(block * C8_BLOCK);
     if (mine) {
         page = c.page_of(seq, block * C8_BLOCK);
         const uint8_t* k = c.codes + c.codes_at(page, 0, gh) + (size_t)row * hd;
@@ -757,7 +757,7 @@ TQ_EXPORT int tq_attention8(const void* q, const void* codes, const void* scales
     TQ_REQUIRE(ranges >= 1 && ranges <= JOIN_RANGES && (ranges == 1 || partial != nullptr), "attention8: %d ranges need a buffer for their sums", ranges);
     TQ_REQUIRE((scores == nullptr) == (weights == nullptr) && (scores == nullptr || (partial != nullptr && score_stride % 16 == 0 && score_stride >= max_kv_len)),
                "attention8: scores of %d places do not hold %d", score_stride, max_kv_len);
-    const Cache8 c{(uint8_t*)codes, (uint8_t*)scales, page_table, table_stride, page_size, n_pages, nkv, hd};
+    const Cache8 c = c8_cache(codes, scales, page_table, table_stride, page_size, n_pages, nkv, hd);
     const Step S{cu_seqlens, held, nh, window, scale * LOG2E};
     const int columns = max_q_len * (nh / nkv);
     auto first = [&]() -> int {
@@ -785,7 +785,7 @@ TQ_EXPORT int tq_repair8(const void* q, const void* codes, const void* scales, c
     if (!rc) rc = check_step("repair8", nh, nkv, n_seqs, 1, window);
     if (rc) return rc;
     TQ_REQUIRE(hd == 64 || hd == 128, "repair8: head size %d", hd);
-    const Cache8 c{(uint8_t*)codes, (uint8_t*)scales, page_table, table_stride, page_size, n_pages, nkv, hd};
+    const Cache8 c = c8_cache(codes, scales, page_table, table_stride, page_size, n_pages, nkv, hd);
     const Step S{cu_seqlens, held, nh, window, scale * LOG2E};
     return hd == 64 ? launch_repair8<Form<__nv_bfloat16, 64, 2, true>>(q, c, S, out, lost, lost_stride, n_seqs, stream) : launch_repair8<Form<__nv_bfloat16, 128, 2, true>>(q, c, S, out, lost, lost_stride, n_seqs, stream);
 }
@@ -799,7 +799,7 @@ TQ_EXPORT int tq_weigh8(const void* q, const void* codes, const void* scales, in
     int rc = c8_check("weigh8", codes, scales, page_size, n_pages, nkv, hd, table_stride);
     if (!rc) rc = check_step("weigh8", nh, nkv, n_seqs, max_kv_len, window);
     if (rc) return rc;
-    const Cache8 c{(uint8_t*)codes, (uint8_t*)scales, page_table, table_stride, page_size, n_pages, nkv, hd};
+    const Cache8 c = c8_cache(codes, scales, page_table, table_stride, page_size, n_pages, nkv, hd);
     const Step S{cu_seqlens, held, nh, window, scale * LOG2E};
     const int columns = max_q_len * (nh / nkv);
     TQ_DISPATCH(act_dtype, TA,

@@ -7,29 +7,65 @@ TQ_DEFINE_LAST_ERROR
 
 namespace {
 
-// eight consecutive elements as float32
-__device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&f)[8]) {
+// Eight consecutive elements as float32, in pairs for the packed operations.
+struct Eight { tq_f32x2 p[4]; };
+__device__ __forceinline__ Eight load8(const __nv_bfloat16* p) {
     const uint4 v = *reinterpret_cast<const uint4*>(p);
     const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+    Eight r;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) { f[2 * i] = __uint_as_float(u[i] << 16); f[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u); }
+    for (int i = 0; i < 4; ++i) r.p[i] = tq_pack2(__uint_as_float(u[i] << 16), __uint_as_float(u[i] & 0xffff0000u));
+    return r;
 }
-__device__ __forceinline__ void load8(const float* p, float (&f)[8]) {
+__device__ __forceinline__ Eight load8(const float* p) {
     const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+    return Eight{{tq_pack2(a.x, a.y), tq_pack2(a.z, a.w), tq_pack2(b.x, b.y), tq_pack2(b.z, b.w)}};
 }
-__device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&f)[8]) {
+__device__ __forceinline__ void store8(__nv_bfloat16* p, const Eight& f) {
     uint32_t u[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+        const float2 x = tq_unpack2(f.p[i]);
+        const __nv_bfloat162 h = __floats2bfloat162_rn(x.x, x.y);
         u[i] = *reinterpret_cast<const uint32_t*>(&h);
     }
     *reinterpret_cast<uint4*>(p) = make_uint4(u[0], u[1], u[2], u[3]);
 }
-__device__ __forceinline__ void store8(float* p, const float (&f)[8]) {
-    *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]);
-    *reinterpret_cast<float4*>(p + 4) = make_float4(f[4], f[5], f[6], f[7]);
+__device__ __forceinline__ void store8(float* p, const Eight& f) {
+    const float2 a = tq_unpack2(f.p[0]), b = tq_unpack2(f.p[1]), c = tq_unpack2(f.p[2]), d = tq_unpack2(f.p[3]);
+    *reinterpret_cast<float4*>(p) = make_float4(a.x, a.y, b.x, b.y);
+    *reinterpret_cast<float4*>(p + 4) = make_float4(c.x, c.y, d.x, d.y);
+}
+// the larger of `top` and the magnitudes of eight elements; NaN does not count
+__device__ __forceinline__ float magnitude8(const Eight& f, float top) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 x = tq_unpack2(f.p[i]);
+        asm("max.f32 %0, %1, %2, %3;" : "=f"(top) : "f"(top), "f"(fabsf(x.x)), "f"(fabsf(x.y)));
+    }
+    return top;
+}
+// the same over the finite elements alone
+__device__ __forceinline__ float finite8(const Eight& f, float top) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 x = tq_unpack2(f.p[i]);
+        top = fmaxf(top, fmaxf(__uint_as_float(c8_magnitude(x.x)), __uint_as_float(c8_magnitude(x.y))));
+    }
+    return top;
+}
+// eight elements as codes; infinite: some of the unit's elements may be (the conversion makes NaN of NaN, but 448 of them)
+__device__ __forceinline__ uint2 encode8(const Eight& f, tq_f32x2 inv, bool infinite) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 x = tq_unpack2(tq_mul2(f.p[i], inv));
+        uint16_t d;
+        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(d) : "f"(x.y), "f"(x.x));
+        w[i] = d;
+        if (infinite) w[i] = c8_encode2(x.x, x.y);
+    }
+    return make_uint2(__byte_perm(w[0], w[1], 0x5410), __byte_perm(w[2], w[3], 0x5410));
 }
 
 // ---------------------------------------------------------------------------------------
@@ -51,12 +87,14 @@ struct WriteArgs {
 
 constexpr int WRITE_THREADS = 512;
 
-template <typename TA, typename TB, bool RUNS>
+// HD: the head size, or 0 where it is known at the launch only
+template <typename TA, typename TB, bool RUNS, int HD>
 __global__ void __launch_bounds__(WRITE_THREADS) write8_kernel(const TA* __restrict__ qkv, const TB* __restrict__ bias, WriteArgs a, TA* __restrict__ q_out, Cache8 c,
-                                                               int threads) {
+                                                               int threads_) {
     tq_grid_wait();                    // everything below may read what the previous kernel wrote
     tq_grid_launch_dependents();
-    __shared__ uint32_t s_top[WRITE_THREADS / 32];
+    __shared__ float s_top[WRITE_THREADS / 32];
+    const int hd = HD ? HD : c.hd, threads = !RUNS ? 32 : HD ? HD : threads_;
     const int unit = threadIdx.x / threads, it = threadIdx.x - unit * threads, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int j = blockIdx.y * (blockDim.x / threads) + unit, heads = a.nh + 2 * c.nkv;
     const int seq = blockIdx.z, t_begin = a.cu_seqlens[seq], run = a.cu_seqlens[seq + 1] - t_begin;
@@ -64,42 +102,51 @@ __global__ void __launch_bounds__(WRITE_THREADS) write8_kernel(const TA* __restr
     const int block_start = (place0 / C8_BLOCK + (int)blockIdx.x) * C8_BLOCK;       // the unit's block, as a place
     const int first = max(block_start, place0), rows = min(block_start + C8_BLOCK, place0 + run) - first;
     if (rows <= 0 || (!RUNS && j >= a.written)) return;              // (runs: the whole block of threads returns or stays)
-    const int t0 = t_begin + first - place0, hd = c.hd, half = hd >> 1, groups = half >> 3, items = rows * groups;
+    const int t0 = t_begin + first - place0, half = hd >> 1, groups = half >> 3, items = rows * groups;
     const bool mine = it < items && j < a.written, is_q = j < a.nh;
     const int r = it / groups, i = (it - r * groups) * 8;
     const int ia = a.pairing == 0 ? i : 2 * i, ib = a.pairing == 0 ? i + half : 2 * i + 8;       // where the item's two halves lie in the head
-    float lo[8] = {}, hi[8] = {};
+    Eight lo = {}, hi = {};
     if (mine) {
         const TA* row = qkv + ((size_t)(t0 + r) * heads + j) * hd;
-        load8(row + ia, lo);
-        load8(row + ib, hi);
-        if (bias != nullptr) {
-            float x[8], y[8];
-            load8(bias + (size_t)j * hd + ia, x);
-            load8(bias + (size_t)j * hd + ib, y);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) { lo[e] += x[e]; hi[e] += y[e]; }
-        }
-        if (j < a.nh + c.nkv && a.cos_t != nullptr) {
+        const bool rotated = j < a.nh + c.nkv && a.cos_t != nullptr;
+        lo = load8(row + ia);
+        hi = load8(row + ib);
+        Eight cs = {}, sn = {};
+        if (rotated) {
             const size_t at = (size_t)a.positions[t0 + r] * half + i;
-            float cs[8], sn[8];
-            load8(a.cos_t + at, cs);
-            load8(a.sin_t + at, sn);
-            if (a.pairing == 0) {
+            cs = load8(a.cos_t + at);
+            sn = load8(a.sin_t + at);
+        }
+        if (bias != nullptr) {
+            const Eight x = load8(bias + (size_t)j * hd + ia), y = load8(bias + (size_t)j * hd + ib);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float u = lo[e], v = hi[e];
-                    lo[e] = __fsub_rn(__fmul_rn(u, cs[e]), __fmul_rn(v, sn[e]));
-                    hi[e] = __fadd_rn(__fmul_rn(u, sn[e]), __fmul_rn(v, cs[e]));
-                }
-            } else {
+            for (int e = 0; e < 4; ++e) { lo.p[e] = tq_add2(lo.p[e], x.p[e]); hi.p[e] = tq_add2(hi.p[e], y.p[e]); }
+        }
+        if (rotated) {
+            // interleaved: the pairs' first elements together and their second ones, and back
+            auto sort = [](Eight& x, Eight& y) {
+                const float2 p[8] = {tq_unpack2(x.p[0]), tq_unpack2(x.p[1]), tq_unpack2(x.p[2]), tq_unpack2(x.p[3]),
+                                     tq_unpack2(y.p[0]), tq_unpack2(y.p[1]), tq_unpack2(y.p[2]), tq_unpack2(y.p[3])};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) { x.p[e] = tq_pack2(p[2 * e].x, p[2 * e + 1].x); y.p[e] = tq_pack2(p[2 * e].y, p[2 * e + 1].y); }
+            };
+            if (a.pairing != 0) sort(lo, hi);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                // (the packed product and sum came out fused, their .rn notwithstanding)
+                const float2 u = tq_unpack2(lo.p[e]), v = tq_unpack2(hi.p[e]), x = tq_unpack2(cs.p[e]), y = tq_unpack2(sn.p[e]);
+                lo.p[e] = tq_pack2(__fsub_rn(__fmul_rn(u.x, x.x), __fmul_rn(v.x, y.x)), __fsub_rn(__fmul_rn(u.y, x.y), __fmul_rn(v.y, y.y)));
+                hi.p[e] = tq_pack2(__fadd_rn(__fmul_rn(u.x, y.x), __fmul_rn(v.x, x.x)), __fadd_rn(__fmul_rn(u.y, y.y), __fmul_rn(v.y, x.y)));
+            }
+            if (a.pairing != 0) {
+                const Eight u = lo, v = hi;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const float u = lo[2 * e], v = lo[2 * e + 1], x = hi[2 * e], y = hi[2 * e + 1];
-                    lo[2 * e] = __fsub_rn(__fmul_rn(u, cs[e]), __fmul_rn(v, sn[e]));
-                    lo[2 * e + 1] = __fadd_rn(__fmul_rn(u, sn[e]), __fmul_rn(v, cs[e]));
-                    hi[2 * e] = __fsub_rn(__fmul_rn(x, cs[e + 4]), __fmul_rn(y, sn[e + 4]));
-                    hi[2 * e + 1] = __fadd_rn(__fmul_rn(x, sn[e + 4]), __fmul_rn(y, cs[e + 4]));
+                    const float2 x = tq_unpack2(u.p[e]), y = tq_unpack2(v.p[e]);
+                    Eight& to = e < 2 ? lo : hi;
+                    to.p[2 * (e & 1)] = tq_pack2(x.x, y.x);
+                    to.p[2 * (e & 1) + 1] = tq_pack2(x.y, y.y);
                 }
             }
         }
@@ -110,36 +157,38 @@ __global__ void __launch_bounds__(WRITE_THREADS) write8_kernel(const TA* __restr
         }
     }
     if (a.written == a.nh) return;                                    // queries only
-    const int plane = j >= a.nh + c.nkv ? 1 : 0, g = j - a.nh - plane * c.nkv, row0 = block_start % c.page_size, old = first - block_start;
+    const int plane = j >= a.nh + c.nkv ? 1 : 0, g = j - a.nh - plane * c.nkv, row0 = c.row(block_start), old = first - block_start;
     uint8_t *codes = nullptr, *byte = nullptr;
-    uint32_t was = 1, top = 0;
+    uint32_t was = 1;
     if (!is_q && j < a.written) {
         const int page = c.page_of(seq, first);
         codes = c.codes + c.codes_at(page, plane, g) + (size_t)row0 * hd;
         byte = c.scales + c.scales_at(page, plane, g) + row0 / C8_BLOCK;
         if (old > 0) was = max((uint32_t)*byte, 1u);                  // (by all of the unit's threads before one of them writes it)
     }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) top = max(top, max(c8_magnitude(lo[e]), c8_magnitude(hi[e])));
-    top = __reduce_max_sync(0xffffffffu, top);
-    if (RUNS) {
-        if (lane == 0) s_top[warp] = top;
-        __syncthreads();
-        for (int w = unit * (threads / 32); w < (unit + 1) * (threads / 32); ++w) top = max(top, s_top[w]);
+    // over the unit's threads
+    auto over_unit = [&](float top) {
+        top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));       // magnitudes: ordered as integers are
+        if (RUNS) {
+            if (lane == 0) s_top[warp] = top;
+            __syncthreads();
+            for (int w = unit * (threads / 32); w < (unit + 1) * (threads / 32); ++w) top = fmaxf(top, s_top[w]);
+        }
+        return top;
+    };
+    float top = over_unit(magnitude8(hi, magnitude8(lo, 0.f)));
+    const bool infinite = top == INFINITY;
+    if (RUNS ? __syncthreads_or(infinite) : infinite) {
+        const float finite = over_unit(finite8(hi, finite8(lo, 0.f)));
+        if (infinite) top = finite;
     }
     if (codes == nullptr) return;
-    const uint32_t b = max(c8_byte(top), was);
+    const uint32_t b = max(c8_byte(__float_as_uint(top)), was);
     if (mine) {
         const float inv = c8_inverse(b);
         uint8_t* d = codes + (size_t)(old + r) * hd;
-        uint32_t w[4];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            w[e] = c8_encode2(lo[4 * e] * inv, lo[4 * e + 1] * inv) | (c8_encode2(lo[4 * e + 2] * inv, lo[4 * e + 3] * inv) << 16);
-            w[2 + e] = c8_encode2(hi[4 * e] * inv, hi[4 * e + 1] * inv) | (c8_encode2(hi[4 * e + 2] * inv, hi[4 * e + 3] * inv) << 16);
-        }
-        *reinterpret_cast<uint2*>(d + ia) = make_uint2(w[0], w[1]);
-        *reinterpret_cast<uint2*>(d + ib) = make_uint2(w[2], w[3]);
+        *reinterpret_cast<uint2*>(d + ia) = encode8(lo, tq_pack2(inv, inv), infinite);
+        *reinterpret_cast<uint2*>(d + ib) = encode8(hi, tq_pack2(inv, inv), infinite);
     }
     if (b > was && old > 0) {
         const uint32_t factor = c8_shift_factor((int)min(b - was, 25u));
@@ -165,7 +214,7 @@ TQ_EXPORT int tq_write8(const void* qkv, int act_dtype, const void* bias, int bi
     TQ_REQUIRE((cos_t == nullptr) == (sin_t == nullptr), "write8: cos and sin tables come together");
     TQ_REQUIRE(n_seqs <= 65535 && max_q_len >= 1, "write8: %d sequences, longest run %d", n_seqs, max_q_len);
     TQ_REQUIRE(((uintptr_t)qkv | (uintptr_t)bias | (uintptr_t)q_out | (uintptr_t)cos_t | (uintptr_t)sin_t) % 16 == 0, "write8: tensors must be 16-byte aligned");
-    const Cache8 c{(uint8_t*)codes, (uint8_t*)scales, page_table, table_stride, page_size, n_pages, nkv, hd};
+    const Cache8 c = c8_cache(codes, scales, page_table, table_stride, page_size, n_pages, nkv, hd);
     const WriteArgs a{cos_t, sin_t, positions, cu_seqlens, held, nh, pairing, codes != nullptr ? nh + 2 * nkv : nh};
     // a run of n rows touches at most (n + 14) / 16 + 1 blocks
     const bool runs = max_q_len > 1;
@@ -173,8 +222,9 @@ TQ_EXPORT int tq_write8(const void* qkv, int act_dtype, const void* bias, int bi
     const int side = runs ? WRITE_THREADS / threads : n_seqs >= 32 ? 8 : 2;              // units a block takes side by side
     const dim3 grid(units, (a.written + side - 1) / side, n_seqs);
     TQ_DISPATCH(act_dtype, TA, TQ_DISPATCH(bias != nullptr ? bias_dtype : act_dtype, TB,
-        if (runs) tq_launch(grid, side * threads, 0, stream)(write8_kernel<TA, TB, true>, (const TA*)qkv, (const TB*)bias, a, (TA*)q_out, c, threads);
-        else tq_launch(grid, side * threads, 0, stream)(write8_kernel<TA, TB, false>, (const TA*)qkv, (const TB*)bias, a, (TA*)q_out, c, threads)));
+        auto kernel = runs ? (hd == 128 ? write8_kernel<TA, TB, true, 128> : hd == 64 ? write8_kernel<TA, TB, true, 64> : write8_kernel<TA, TB, true, 0>)
+                           : (hd == 128 ? write8_kernel<TA, TB, false, 128> : write8_kernel<TA, TB, false, 0>);
+        tq_launch(grid, side * threads, 0, stream)(kernel, (const TA*)qkv, (const TB*)bias, a, (TA*)q_out, c, threads)));
     TQ_CHECK_LAUNCH("write8");
     return 0;
 }

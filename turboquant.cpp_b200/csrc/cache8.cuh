@@ -21,8 +21,11 @@ struct Cache8 {
     uint8_t* scales;
     const int* table;
     int table_stride, page_size, n_pages, nkv, hd;
+    int page_shift;                    // page_size = 2^page_shift, or -1 (a division a place was much of what the small kernels did)
+    __device__ __forceinline__ int column(int place) const { return page_shift >= 0 ? place >> page_shift : place / page_size; }
+    __device__ __forceinline__ int row(int place) const { return page_shift >= 0 ? place & (page_size - 1) : place % page_size; }
     __device__ __forceinline__ int page_of(int seq, int place) const {
-        return TQ_CHECKED(table[(size_t)seq * table_stride + TQ_CHECKED(place / page_size, table_stride, TQ_IDX_TABLE_COLUMN)], n_pages, TQ_IDX_PAGE);
+        return TQ_CHECKED(table[(size_t)seq * table_stride + TQ_CHECKED(column(place), table_stride, TQ_IDX_TABLE_COLUMN)], n_pages, TQ_IDX_PAGE);
     }
     // first code of a (page, plane, head); offsets pass 32 bits in a large cache
     __device__ __forceinline__ size_t codes_at(int page, int plane, int g) const {
@@ -84,6 +87,12 @@ __device__ __forceinline__ uint32_t c8_shift_factor(int shift) {
 }
 __device__ __forceinline__ uint4 c8_shift16(uint4 v, uint32_t factor) {
     return make_uint4(c8_shift4(v.x, factor), c8_shift4(v.y, factor), c8_shift4(v.z, factor), c8_shift4(v.w, factor));
+}
+
+inline Cache8 c8_cache(const void* codes, const void* scales, const int* table, int table_stride, int page_size, int n_pages, int nkv, int hd) {
+    int shift = 0;
+    while ((1 << shift) < page_size) ++shift;
+    return Cache8{(uint8_t*)codes, (uint8_t*)scales, table, table_stride, page_size, n_pages, nkv, hd, (1 << shift) == page_size ? shift : -1};
 }
 
 inline int c8_check(const char* what, const void* codes, const void* scales, int page_size, int n_pages, int nkv, int hd, int table_stride) {

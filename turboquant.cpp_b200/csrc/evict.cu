@@ -24,16 +24,15 @@ __device__ __forceinline__ uint32_t rank_of(float w) {
 constexpr int SELECT_THREADS = 1024, SELECT_WARPS = SELECT_THREADS / 32, BINS = 2048;
 constexpr int SELECT_MOST = 48 * 1024;             // ranks a block keeps, 192 KB
 
-__global__ void __launch_bounds__(SELECT_THREADS) evict8_select_kernel(const float* __restrict__ weights, const int* __restrict__ lengths, const int* __restrict__ table,
-                                                                       int table_stride, int page_size, int n_pages, int nkv, int budget, int recent, int cached,
-                                                                       int* __restrict__ kept) {
+__global__ void __launch_bounds__(SELECT_THREADS) evict8_select_kernel(Cache8 c, const float* __restrict__ weights, const int* __restrict__ lengths, int budget, int recent,
+                                                                       int cached, int* __restrict__ kept) {
     tq_grid_wait();                    // everything below may read what the previous kernel wrote
     tq_grid_launch_dependents();
     extern __shared__ uint32_t s_rank[];
     __shared__ int s_hist[BINS], s_pick[2], s_warp[2][SELECT_WARPS];
     const int g = blockIdx.x, seq = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int n = max(0, min(lengths[seq], table_stride * page_size));
-    int* list = kept + ((size_t)seq * nkv + g) * budget;
+    const int n = max(0, min(lengths[seq], c.table_stride * c.page_size));
+    int* list = kept + ((size_t)seq * c.nkv + g) * budget;
     if (n <= budget) {
         for (int j = tid; j < budget; j += SELECT_THREADS) list[j] = j < n ? j : -1;
         return;
@@ -41,13 +40,9 @@ __global__ void __launch_bounds__(SELECT_THREADS) evict8_select_kernel(const flo
     const int rest = n - recent, want = budget - recent;              // of places 0 .. rest - 1 `want` stay
     for (int j = tid; j < recent; j += SELECT_THREADS) list[want + j] = rest + j;
     if (want == 0) return;
-    const int* pages = table + (size_t)seq * table_stride;
-    auto read = [&](int p) {
-        const int page = TQ_CHECKED(pages[p / page_size], n_pages, TQ_IDX_PAGE);
-        return rank_of(weights[((size_t)page * nkv + g) * page_size + p % page_size]);
-    };
+    auto read = [&](int p) { return rank_of(weights[((size_t)c.page_of(seq, p) * c.nkv + g) * c.page_size + c.row(p)]); };
     auto rank_at = [&](int p) { return p < cached ? s_rank[p] : read(p); };
-#pragma unroll 4
+#pragma unroll 8
     for (int p = tid; p < min(rest, cached); p += SELECT_THREADS) s_rank[p] = read(p);
     uint32_t prefix = 0, known = 0;                                   // the bits found and which they are
     int missing = want;                                               // rows still to be found among those that agree with them
@@ -114,43 +109,50 @@ __global__ void __launch_bounds__(SELECT_THREADS) evict8_select_kernel(const flo
 }
 
 // ---------------------------------------------------------------------------------------
-// Moving: a warp per 16 rows of the list and plane.  The new block's byte is the largest of its rows' bytes; rows of a smaller one are rounded
-// again.  Nothing is shared between warps; a row's page, byte and place go from lane to lane by shuffles.
+// Moving: a warp per 16 rows of the list, a lane for each row and plane on the way to its page and byte.  The new block's byte is the largest of
+// its rows' bytes; rows of a smaller one are rounded again.  Nothing is shared between warps.  (A warp per 64 rows and plane, which goes that
+// way once for four times as many: 37 us where this form's predecessor, a warp per 16 rows and plane, took 31: too few warps.)
 // ---------------------------------------------------------------------------------------
 __global__ void __launch_bounds__(256) evict8_move_kernel(Cache8 c, float* __restrict__ weights, const int* __restrict__ kept, const int* __restrict__ new_table,
                                                           int new_stride, int budget) {
     tq_grid_wait();                    // everything below may read what the previous kernel wrote
     tq_grid_launch_dependents();
-    const int lane = threadIdx.x & 31, work = blockIdx.x * 8 + (threadIdx.x >> 5), plane = work & 1, first = (work >> 1) * C8_BLOCK, seq = blockIdx.z, g = blockIdx.y;
+    const int lane = threadIdx.x & 31, plane = lane >> 4, r = lane & 15, first = (blockIdx.x * 8 + (threadIdx.x >> 5)) * C8_BLOCK, seq = blockIdx.z, g = blockIdx.y;
     if (first >= budget) return;
     const int* list = kept + ((size_t)seq * c.nkv + g) * budget;
-    const int place = lane < C8_BLOCK && first + lane < budget ? list[first + lane] : -1;
-    const int page = TQ_CHECKED(new_table[(size_t)seq * new_stride + TQ_CHECKED(first / c.page_size, new_stride, TQ_IDX_TABLE_COLUMN)], c.n_pages, TQ_IDX_PAGE);
-    if (__shfl_sync(0xffffffffu, place, 0) < 0) return;               // the list ends before this block
-    const int row0 = first % c.page_size;
+    const int place = first + r < budget ? list[first + r] : -1;
+    const int page = TQ_CHECKED(new_table[(size_t)seq * new_stride + TQ_CHECKED(c.column(first), new_stride, TQ_IDX_TABLE_COLUMN)], c.n_pages, TQ_IDX_PAGE);
+    const int rows = __popc(__ballot_sync(0xffffffffu, place >= 0) & 0xffffu), row0 = c.row(first), vecs = c.hd / 16;
+    if (rows == 0) return;                                            // the list ends before these
     unsigned long long from = 0;
     uint32_t byte = 0;
+    float weight = 0.f;
     if (place >= 0) {
-        const int old = c.page_of(seq, place), row = place % c.page_size;
+        const int old = c.page_of(seq, place), row = c.row(place);
         from = c.codes_at(old, plane, g) + (size_t)row * c.hd;
         byte = c.scales[c.scales_at(old, plane, g) + row / C8_BLOCK];
-        if (plane == 0) weights[((size_t)page * c.nkv + g) * c.page_size + row0 + lane] = weights[((size_t)old * c.nkv + g) * c.page_size + row];
+        if (plane == 0) weight = weights[((size_t)old * c.nkv + g) * c.page_size + row];
     }
-    const uint32_t top = __reduce_max_sync(0xffffffffu, byte);
-    const int rows = __popc(__ballot_sync(0xffffffffu, place >= 0)), vecs = c.hd / 16;
-    if (lane == 0) c.scales[c.scales_at(page, plane, g) + row0 / C8_BLOCK] = (uint8_t)top;
-    uint8_t* to = c.codes + c.codes_at(page, plane, g) + (size_t)row0 * c.hd;
-#pragma unroll 4
-    for (int v0 = 0; v0 < C8_BLOCK * vecs; v0 += 32) {                // (16 rows: a multiple of 32 pieces or half of one)
-        const int v = v0 + lane, r = min(v / vecs, C8_BLOCK - 1), at = v - v / vecs * vecs;
-        const unsigned long long src = __shfl_sync(0xffffffffu, from, r);
-        const uint32_t shift = top - __shfl_sync(0xffffffffu, byte, r);
-        if (v < rows * vecs) {
-            uint4 x = *reinterpret_cast<const uint4*>(c.codes + src + at * 16);
-            if (shift) x = c8_shift16(x, c8_shift_factor((int)min(shift, 25u)));
-            *reinterpret_cast<uint4*>(to + (size_t)r * c.hd + at * 16) = x;
+    const size_t to = c.codes_at(page, 0, g) + (size_t)row0 * c.hd, between = (size_t)c.nkv * c.page_size * c.hd;
+    uint32_t top = byte;
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const uint32_t shift = top - byte;
+    // pieces of 16 bytes: all rows of the keys, then of the values
+    const int pieces = C8_BLOCK * vecs;
+#pragma unroll 8
+    for (int v0 = 0; v0 < 2 * pieces; v0 += 32) {
+        const int v = v0 + lane, which = v / vecs, at = (v - which * vecs) * 16;        // which: row, 16 more for values
+        const unsigned long long src = __shfl_sync(0xffffffffu, from, which);
+        const uint32_t s = __shfl_sync(0xffffffffu, shift, which);
+        if ((which & 15) < rows) {
+            uint4 x = *reinterpret_cast<const uint4*>(c.codes + src + at);
+            if (s) x = c8_shift16(x, c8_shift_factor((int)min(s, 25u)));
+            *reinterpret_cast<uint4*>(c.codes + to + (which >> 4) * between + (size_t)(which & 15) * c.hd + at) = x;
         }
     }
+    if (r == 0) c.scales[c.scales_at(page, plane, g) + row0 / C8_BLOCK] = (uint8_t)top;
+    if (plane == 0 && place >= 0) weights[((size_t)page * c.nkv + g) * c.page_size + row0 + r] = weight;
 }
 
 }  // namespace
@@ -162,11 +164,12 @@ TQ_EXPORT int tq_evict8_select(const float* weights, const int* lengths, const i
     TQ_REQUIRE(budget >= 1 && recent >= 0 && recent <= budget, "evict8: %d newest of a budget of %d rows", recent, budget);
     TQ_REQUIRE(page_size >= 1 && table_stride >= 1 && nkv >= 1 && n_seqs <= 65535, "evict8: page size %d, tables %d wide, %d heads, %d sequences", page_size, table_stride, nkv, n_seqs);
     TQ_REQUIRE((long long)table_stride * page_size < (1ll << 31), "evict8: page tables of %d pages", table_stride);
+    const Cache8 c = c8_cache(nullptr, nullptr, page_table, table_stride, page_size, n_pages, nkv, 0);
     const int cached = table_stride * page_size < SELECT_MOST ? table_stride * page_size : SELECT_MOST;
     static TqSmemAsked asked;
     const cudaError_t e = tq_grow_smem(evict8_select_kernel, (size_t)cached * 4, asked);
     if (e != cudaSuccess) TQ_FAIL(-1, "evict8_select: cannot reserve %d bytes of shared memory: %s", cached * 4, cudaGetErrorString(e));
-    tq_launch(dim3(nkv, n_seqs), SELECT_THREADS, (size_t)cached * 4, stream)(evict8_select_kernel, weights, lengths, page_table, table_stride, page_size, n_pages, nkv, budget, recent, cached, kept);
+    tq_launch(dim3(nkv, n_seqs), SELECT_THREADS, (size_t)cached * 4, stream)(evict8_select_kernel, c, weights, lengths, budget, recent, cached, kept);
     TQ_CHECK_LAUNCH("evict8_select");
     return 0;
 }
@@ -179,8 +182,8 @@ TQ_EXPORT int tq_evict8_move(void* codes, void* scales, float* weights, const in
     if (rc) return rc;
     TQ_REQUIRE(budget >= 1 && (long long)new_stride * page_size >= budget, "evict8: %d new pages a sequence for a budget of %d rows", new_stride, budget);
     TQ_REQUIRE(n_seqs <= 65535 && nkv <= 65535, "evict8: %d sequences, %d heads", n_seqs, nkv);
-    const Cache8 c{(uint8_t*)codes, (uint8_t*)scales, page_table, table_stride, page_size, n_pages, nkv, hd};
-    tq_launch(dim3(((budget + C8_BLOCK - 1) / C8_BLOCK * 2 + 7) / 8, nkv, n_seqs), 256, 0, stream)(evict8_move_kernel, c, weights, kept, new_table, new_stride, budget);
+    const Cache8 c = c8_cache(codes, scales, page_table, table_stride, page_size, n_pages, nkv, hd);
+    tq_launch(dim3(((budget + C8_BLOCK - 1) / C8_BLOCK + 7) / 8, nkv, n_seqs), 256, 0, stream)(evict8_move_kernel, c, weights, kept, new_table, new_stride, budget);
     TQ_CHECK_LAUNCH("evict8_move");
     return 0;
 }

@@ -244,7 +244,7 @@ TQ_EXPORT int tq_expand8(const void* codes, const void* scales, const int* cu_se
     if (rc) return rc;
     TQ_REQUIRE(page_size == PAGE && n_seqs <= 65535 && nkv <= 65535 && window >= 0, "expand8: page size %d, %d sequences, %d heads, window %d", page_size, n_seqs, nkv, window);
     TQ_REQUIRE((long long)n_seqs * width < (1ll << 31) && (uintptr_t)dense % 16 == 0, "expand8: %d pages for each of %d sequences", width, n_seqs);
-    const Cache8 c{(uint8_t*)codes, (uint8_t*)scales, page_table, table_stride, page_size, n_pages, nkv, hd};
+    const Cache8 c = c8_cache(codes, scales, page_table, table_stride, page_size, n_pages, nkv, hd);
     tq_launch(dim3(width, nkv, n_seqs), 256, 0, stream)(expand8_kernel, c, cu_seqlens, held, window, (uint4*)dense, dense_table, (uint8_t*)lost, width);
     TQ_CHECK_LAUNCH("expand8");
     return 0;
