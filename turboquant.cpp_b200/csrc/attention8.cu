@@ -55,6 +55,7 @@ struct Step {
     int nh, window;
     float factor;              // scale * log2(e)
 };
+constexpr int CLUSTER = 8;     // ranges of a row that join through one another's shared memory
 
 // A tile of columns: query heads of one key/value head and rows of one run.
 struct Tile {
@@ -226,16 +227,18 @@ constexpr float LOWEST = -3.402823466e38f;       // a maximum over nothing
 // ---------------------------------------------------------------------------------------
 // A range of the keys for a tile of columns.  partial: null, or [T * nh][ranges][hd + 4] for a second launch: the unnormalised sum, the
 // maximum m' it is relative to, the denominator's maximum and the denominator.  scores: null, or [T * nh][score_stride], base-2 scores.
-// lse: null, or [T * nh], log2 of the denominator (where there is no second launch).
+// lse: null, or [T * nh], log2 of the denominator (where there is no second launch).  Several ranges without `partial`: they are the CTAs of a
+// cluster, which join in their shared memory, each for its part of the result; with `weights` and scores each then adds up its own keys'
+// weights (the tile has all the columns of its sequence and head then).
 // ---------------------------------------------------------------------------------------
 template <class F>
 __device__ __forceinline__ void attend_tile(const Tile& T, int range, int ranges, const typename F::TA* __restrict__ q, const Cache8& c, const Step& S,
                                             typename F::TA* __restrict__ out, float* __restrict__ partial, float* __restrict__ scores, int score_stride,
-                                            float* __restrict__ lse) {
+                                            float* __restrict__ lse, float* __restrict__ weights) {
     constexpr int NT = F::NT, NC = F::NC, MT = F::MT, HDP = F::HDP;
     extern __shared__ __align__(16) uint8_t ring[];
     __shared__ Queries<F> Q;
-    __shared__ float s_stat[WARPS][NC][3];
+    __shared__ float s_stat[WARPS][NC][3], s_ranks[CLUSTER][NC][3], s_lse[NC];
     float (*s_o)[NC][HDP + 4] = reinterpret_cast<float (*)[NC][HDP + 4]>(ring);        // [WARPS], once the keys are through
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, hd = F::EXACT ? HDP : c.hd;
     // this range's blocks of 16 keys
@@ -481,6 +484,17 @@ __device__ __forceinline__ void attend_tile(const Tile& T, int range, int ranges
             mw[w] = exp2f(s_stat[w][col][0] - MO);
             L += s_stat[w][col][2] * exp2f(s_stat[w][col][1] - M);
         }
+        if (ranges > 1 && partial == nullptr) {
+            for (int d = lane; d < hd; d += 32) {
+                float sum = 0.f;
+#pragma unroll
+                for (int w = 0; w < WARPS; ++w) sum += s_o[w][col][d] * mw[w];
+                s_o[0][col][d] = sum;
+            }
+            __syncwarp();
+            if (lane == 0) { s_stat[0][col][0] = MO; s_stat[0][col][1] = M; s_stat[0][col][2] = L; }
+            continue;
+        }
         const size_t at = Q.row[col];
         float* pp = partial != nullptr ? partial + (at * ranges + range) * (hd + 4) : nullptr;
         const float norm = exp2f(MO - M) / L;
@@ -494,17 +508,62 @@ __device__ __forceinline__ void attend_tile(const Tile& T, int range, int ranges
         if (pp != nullptr && lane == 0) { pp[hd] = MO; pp[hd + 1] = M; pp[hd + 2] = L; }
         if (pp == nullptr && lse != nullptr && lane == 0) lse[at] = M + log2f(L);
     }
+    if (ranges == 1 || partial != nullptr) return;
+    __syncwarp();
+    // the cluster's sums together: statistics of all ranges first, then every CTA its part of the tile's results
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    auto remote = [](const float* own, int rank) {
+        uint32_t a;
+        float v;
+        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"((uint32_t)__cvta_generic_to_shared(own)), "r"(rank));
+        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+        return v;
+    };
+    for (int i = threadIdx.x; i < ranges * NC * 3; i += WARPS * 32)
+        if (i / 3 % NC < T.n) (&s_ranks[0][0][0])[i] = remote(&s_stat[0][0][0] + i % (NC * 3), i / (NC * 3));
+    __syncthreads();
+    for (int i = range * WARPS * 32 + threadIdx.x; i < T.n * hd; i += ranges * WARPS * 32) {
+        const int col = i / hd, d = i - col * hd;
+        float M = LOWEST, MO = LOWEST, L = 0.f, sum = 0.f;
+        for (int r = 0; r < ranges; ++r) { MO = fmaxf(MO, s_ranks[r][col][0]); M = fmaxf(M, s_ranks[r][col][1]); }
+#pragma unroll 8
+        for (int r = 0; r < ranges; ++r) {
+            L += s_ranks[r][col][2] * exp2f(s_ranks[r][col][1] - M);
+            sum += remote(&s_o[0][col][d], r) * exp2f(s_ranks[r][col][0] - MO);
+        }
+        out[Q.row[col] * hd + d] = tq_from_float<typename F::TA>(sum * (exp2f(MO - M) / L));
+        if (lse != nullptr && d == 0) lse[Q.row[col]] = M + log2f(L);
+    }
+    if (weights != nullptr) {
+        if (threadIdx.x < T.n) {
+            float M = LOWEST, L = 0.f;
+            for (int r = 0; r < ranges; ++r) M = fmaxf(M, s_ranks[r][threadIdx.x][1]);
+            for (int r = 0; r < ranges; ++r) L += s_ranks[r][threadIdx.x][2] * exp2f(s_ranks[r][threadIdx.x][1] - M);
+            s_lse[threadIdx.x] = M + log2f(L);
+        }
+        __syncthreads();
+        for (int k = from * C8_BLOCK + threadIdx.x; k < min(min(to * C8_BLOCK, place1 + 1), score_stride); k += WARPS * 32) {
+            if (S.window > 0 && k + S.window <= T.start) continue;                       // no row of the step sees it
+            float sum = 0.f;
+            for (int col = 0; col < T.n; ++col)
+                if (k <= Q.place[col] && (S.window <= 0 || k > Q.place[col] - S.window)) sum += ex2(scores[Q.row[col] * score_stride + k] - s_lse[col]);
+            float* w = weights + ((size_t)c.page_of(T.seq, k) * c.nkv + T.g) * c.page_size + c.row(k);
+            *w = (k < T.start ? *w : 0.f) + sum;
+        }
+    }
+    // nobody leaves while its sums are being read
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 template <class F>
 __global__ void __launch_bounds__(WARPS * 32, F::PER_SM) attention8_kernel(const typename F::TA* __restrict__ q, Cache8 c, Step S, typename F::TA* __restrict__ out,
                                                                                            float* __restrict__ partial, float* __restrict__ scores, int score_stride,
-                                                                                           float* __restrict__ lse) {
+                                                                                           float* __restrict__ lse, float* __restrict__ weights, int ranges) {
     tq_grid_wait();                    // everything below may read what the previous kernel wrote
     tq_grid_launch_dependents();
-    const int tile_no = blockIdx.x / c.nkv;
-    const Tile T = tile_of(S, blockIdx.z, blockIdx.x - tile_no * c.nkv, c.nkv, tile_no, F::NC);
-    if (T.n > 0) attend_tile<F>(T, blockIdx.y, gridDim.y, q, c, S, out, partial, scores, score_stride, lse);
+    const int tile = blockIdx.x / ranges, tile_no = tile / c.nkv;
+    const Tile T = tile_of(S, blockIdx.z, tile - tile_no * c.nkv, c.nkv, tile_no, F::NC);
+    if (T.n > 0) attend_tile<F>(T, blockIdx.x - tile * ranges, ranges, q, c, S, out, partial, scores, score_stride, lse, weights);
 }
 
 // The prompt kernel gives values that a row may not see a weight of 0, which does not remove a NaN: key/value heads of sequences in whose pages
@@ -524,7 +583,7 @@ __global__ void __launch_bounds__(WARPS * 32) repair8_kernel(const typename F::T
         const Tile T = tile_of(S, seq, g, c.nkv, tile_no, F::NC);
         if (T.n <= 0) return;
         __syncthreads();
-        attend_tile<F>(T, 0, 1, q, c, S, out, nullptr, nullptr, 0, nullptr);
+        attend_tile<F>(T, 0, 1, q, c, S, out, nullptr, nullptr, 0, nullptr, nullptr);
     }
 }
 
@@ -706,14 +765,16 @@ int launch_repair8(const void* q, const Cache8& c, const Step& S, void* out, con
     return 0;
 }
 template <class F>
-int launch8(const void* q, const Cache8& c, const Step& S, void* out, float* partial, int ranges, float* scores, int score_stride, float* lse, int n_seqs,
-            int max_q_len, cudaStream_t stream) {
+int launch8(const void* q, const Cache8& c, const Step& S, void* out, float* partial, int ranges, float* scores, int score_stride, float* lse, float* weights,
+            int n_seqs, int max_q_len, cudaStream_t stream) {
     const long long tiles = ((long long)max_q_len * (S.nh / c.nkv) + F::NC - 1) / F::NC * c.nkv;
-    TQ_REQUIRE(tiles < (1ll << 31), "attention8: runs of %d rows", max_q_len);
+    TQ_REQUIRE(tiles * ranges < (1ll << 31), "attention8: runs of %d rows", max_q_len);
     static std::atomic<unsigned long long> asked{0};
     const cudaError_t e = tq_reserve_smem(attention8_kernel<F>, F::SMEM, asked);
     if (e != cudaSuccess) TQ_FAIL(-1, "attention8: cannot reserve %d bytes of shared memory: %s", F::SMEM, cudaGetErrorString(e));
-    tq_launch(dim3((unsigned)tiles, ranges, n_seqs), WARPS * 32, F::SMEM, stream)(attention8_kernel<F>, (const typename F::TA*)q, c, S, (typename F::TA*)out, partial, scores, score_stride, lse);
+    TQ_REQUIRE(weights == nullptr || tiles == c.nkv, "attention8: a tile of %d columns does not hold %d query heads", F::NC, S.nh / c.nkv);
+    tq_launch(dim3((unsigned)(tiles * ranges), 1, n_seqs), WARPS * 32, F::SMEM, stream, partial == nullptr ? ranges : 1)(
+        attention8_kernel<F>, (const typename F::TA*)q, c, S, (typename F::TA*)out, partial, scores, score_stride, lse, weights, ranges);
     TQ_CHECK_LAUNCH("attention8");
     return 0;
 }
@@ -743,9 +804,10 @@ int check_step(const char* what, int nh, int nkv, int n_seqs, int longest, int w
 }  // namespace
 
 // q [T, nh, hd], out [T, nh * hd]; place i sees j <= i with window == 0 or i - j < window.  max_q_len: the longest run.  ranges > 1: the keys
-// of a row are cut into that many ranges, partial [T * nh * ranges * (hd + 4)].  lse [T, nh] float32 or null.  scores [T * nh,
-// score_stride] with weights [n_pages, nkv, page_size], or both null: the weights are added up by the second launch (any number of ranges
-// needs partial then); score_stride: a multiple of 16, at least the longest held[s] + run, max_kv_len.
+// of a row are cut into that many ranges, which join as a cluster (up to 8; partial null) or in a second launch (up to 64; partial
+// [T * nh * ranges * (hd + 4)]).  lse [T, nh] float32 or null.  scores [T * nh, score_stride] with weights [n_pages, nkv, page_size], or both
+// null: the weights are added up by whoever joins, so by clusters only of all of a key/value head's query heads, and of two ranges or more;
+// score_stride: a multiple of 16, at least the longest held[s] + run, max_kv_len.
 TQ_EXPORT int tq_attention8(const void* q, const void* codes, const void* scales, int act_dtype, const int* cu_seqlens, const int* held,
                             const int* page_table, int table_stride, int page_size, int window, float scale, void* out, float* partial, int ranges,
                             float* lse, float* scores, int score_stride, float* weights, int max_kv_len, int n_pages, int n_seqs, int max_q_len, int nh,
@@ -754,15 +816,15 @@ TQ_EXPORT int tq_attention8(const void* q, const void* codes, const void* scales
     int rc = c8_check("attention8", codes, scales, page_size, n_pages, nkv, hd, table_stride);
     if (!rc) rc = check_step("attention8", nh, nkv, n_seqs, max_q_len, window);
     if (rc) return rc;
-    TQ_REQUIRE(ranges >= 1 && ranges <= JOIN_RANGES && (ranges == 1 || partial != nullptr), "attention8: %d ranges need a buffer for their sums", ranges);
-    TQ_REQUIRE((scores == nullptr) == (weights == nullptr) && (scores == nullptr || (partial != nullptr && score_stride % 16 == 0 && score_stride >= max_kv_len)),
+    TQ_REQUIRE(ranges >= 1 && ranges <= (partial != nullptr ? JOIN_RANGES : CLUSTER), "attention8: %d ranges need a buffer for their sums", ranges);
+    TQ_REQUIRE((scores == nullptr) == (weights == nullptr) && (scores == nullptr || ((partial != nullptr || (ranges > 1 && max_q_len == 1)) && score_stride % 16 == 0 && score_stride >= max_kv_len)),
                "attention8: scores of %d places do not hold %d", score_stride, max_kv_len);
     const Cache8 c = c8_cache(codes, scales, page_table, table_stride, page_size, n_pages, nkv, hd);
     const Step S{cu_seqlens, held, nh, window, scale * LOG2E};
     const int columns = max_q_len * (nh / nkv);
     auto first = [&]() -> int {
         TQ_DISPATCH(act_dtype, TA,
-#define C8_CALL(HDP, NT, EXACT) (launch8<Form<TA, HDP, NT, EXACT>>(q, c, S, out, partial, ranges, scores, score_stride, partial == nullptr ? lse : nullptr, n_seqs, max_q_len, stream))
+#define C8_CALL(HDP, NT, EXACT) (launch8<Form<TA, HDP, NT, EXACT>>(q, c, S, out, partial, ranges, scores, score_stride, partial == nullptr ? lse : nullptr, partial == nullptr ? weights : nullptr, n_seqs, max_q_len, stream))
             C8_FORMS(columns, C8_CALL));
 #undef C8_CALL
         return -2;

@@ -1,8 +1,8 @@
 // Eviction from the 8-bit cache (layout and codes: cache8.cuh): sequences that hold more rows than a budget keep, in every key/value head,
 // the newest `recent` ones and, of the others, those whose accumulated attention weight is largest.
 //
-//   tq_evict8_select   which rows stay: per sequence and key/value head a list of places, ascending
-//   tq_evict8_move     the rows of such a list, their bytes and their sums of weights, to new pages
+//   tq_evict8   two launches: which rows stay, per sequence and key/value head a list of places, ascending; then the rows of the lists, their
+//               bytes and their sums of weights, to new pages
 #include "cache8.cuh"
 
 TQ_DEFINE_LAST_ERROR
@@ -157,32 +157,24 @@ __global__ void __launch_bounds__(256) evict8_move_kernel(Cache8 c, float* __res
 
 }  // namespace
 
-// lengths [n_seqs] (device): rows each sequence holds; kept [n_seqs, nkv, budget]: the places that stay, ascending, then -1.
-TQ_EXPORT int tq_evict8_select(const float* weights, const int* lengths, const int* page_table, int table_stride, int page_size, int n_pages, int n_seqs,
-                               int nkv, int budget, int recent, int* kept, cudaStream_t stream) {
-    if (n_seqs == 0) return 0;
-    TQ_REQUIRE(budget >= 1 && recent >= 0 && recent <= budget, "evict8: %d newest of a budget of %d rows", recent, budget);
-    TQ_REQUIRE(page_size >= 1 && table_stride >= 1 && nkv >= 1 && n_seqs <= 65535, "evict8: page size %d, tables %d wide, %d heads, %d sequences", page_size, table_stride, nkv, n_seqs);
-    TQ_REQUIRE((long long)table_stride * page_size < (1ll << 31), "evict8: page tables of %d pages", table_stride);
-    const Cache8 c = c8_cache(nullptr, nullptr, page_table, table_stride, page_size, n_pages, nkv, 0);
-    const int cached = table_stride * page_size < SELECT_MOST ? table_stride * page_size : SELECT_MOST;
-    static TqSmemAsked asked;
-    const cudaError_t e = tq_grow_smem(evict8_select_kernel, (size_t)cached * 4, asked);
-    if (e != cudaSuccess) TQ_FAIL(-1, "evict8_select: cannot reserve %d bytes of shared memory: %s", cached * 4, cudaGetErrorString(e));
-    tq_launch(dim3(nkv, n_seqs), SELECT_THREADS, (size_t)cached * 4, stream)(evict8_select_kernel, c, weights, lengths, budget, recent, cached, kept);
-    TQ_CHECK_LAUNCH("evict8_select");
-    return 0;
-}
-
-// The rows that `kept` lists, row j to place j of new_table's pages, which hold none of the listed rows.
-TQ_EXPORT int tq_evict8_move(void* codes, void* scales, float* weights, const int* kept, const int* page_table, int table_stride, const int* new_table,
-                             int new_stride, int page_size, int n_pages, int n_seqs, int nkv, int hd, int budget, cudaStream_t stream) {
+// lengths [n_seqs] (device): rows each sequence holds; kept [n_seqs, nkv, budget]: receives the places that stay, ascending, then -1.  Row j of
+// them goes to place j of new_table's pages, none of which holds any of these rows.
+TQ_EXPORT int tq_evict8(void* codes, void* scales, float* weights, const int* lengths, const int* page_table, int table_stride, const int* new_table, int new_stride,
+                        int page_size, int n_pages, int n_seqs, int nkv, int hd, int budget, int recent, int* kept, cudaStream_t stream) {
     if (n_seqs == 0) return 0;
     int rc = c8_check("evict8", codes, scales, page_size, n_pages, nkv, hd, table_stride);
     if (rc) return rc;
-    TQ_REQUIRE(budget >= 1 && (long long)new_stride * page_size >= budget, "evict8: %d new pages a sequence for a budget of %d rows", new_stride, budget);
+    TQ_REQUIRE(budget >= 1 && recent >= 0 && recent <= budget, "evict8: %d newest of a budget of %d rows", recent, budget);
+    TQ_REQUIRE((long long)new_stride * page_size >= budget, "evict8: %d new pages a sequence for a budget of %d rows", new_stride, budget);
     TQ_REQUIRE(n_seqs <= 65535 && nkv <= 65535, "evict8: %d sequences, %d heads", n_seqs, nkv);
+    TQ_REQUIRE((long long)table_stride * page_size < (1ll << 31), "evict8: page tables of %d pages", table_stride);
     const Cache8 c = c8_cache(codes, scales, page_table, table_stride, page_size, n_pages, nkv, hd);
+    const int cached = table_stride * page_size < SELECT_MOST ? table_stride * page_size : SELECT_MOST;
+    static TqSmemAsked asked;
+    const cudaError_t e = tq_grow_smem(evict8_select_kernel, (size_t)cached * 4, asked);
+    if (e != cudaSuccess) TQ_FAIL(-1, "evict8: cannot reserve %d bytes of shared memory: %s", cached * 4, cudaGetErrorString(e));
+    tq_launch(dim3(nkv, n_seqs), SELECT_THREADS, (size_t)cached * 4, stream)(evict8_select_kernel, c, weights, lengths, budget, recent, cached, kept);
+    TQ_CHECK_LAUNCH("evict8_select");
     tq_launch(dim3(((budget + C8_BLOCK - 1) / C8_BLOCK + 7) / 8, nkv, n_seqs), 256, 0, stream)(evict8_move_kernel, c, weights, kept, new_table, new_stride, budget);
     TQ_CHECK_LAUNCH("evict8_move");
     return 0;

@@ -3,7 +3,7 @@ from __future__ import annotations
 
 import ctypes
 from operator import index
-from typing import Optional
+from typing import List, Optional
 
 import torch
 
@@ -66,29 +66,23 @@ def declared(lib: ctypes.CDLL, name: str, signature: str):
     return fn
 
 
-def address(t: Optional[torch.Tensor]) -> Optional[int]:
-    """What `ptr` gives, as a plain int for launchers with declared arguments."""
-    if t is None:
-        return None
-    if not (t.is_cuda and t.is_contiguous()):
-        ptr(t)                              # raises
-    return t.data_ptr()
-
-
-def raw_stream() -> int:
-    return _raw_stream(_raw_device()) if _raw_stream is not None and _raw_device is not None else torch.cuda.current_stream().cuda_stream
-
-
-def on_current_device(*tensors: Optional[torch.Tensor]) -> None:
-    """Launches go to the current device's stream: tensors of another GPU are refused instead of read from there."""
-    here = -1
+def addresses(*tensors: Optional[torch.Tensor]) -> List[Optional[int]]:
+    """What `ptr` gives, as plain ints for launchers with declared arguments, and behind them the current stream.  Launches go to the current
+    device: tensors of another GPU are refused instead of read from there."""
+    if not tensors[0].is_cuda:
+        ptr(tensors[0])                     # raises
+    here = _raw_device() if _raw_device is not None else torch.cuda.current_device()
+    out: List[Optional[int]] = []
     for t in tensors:
-        if t is None or not t.is_cuda:
+        if t is None:
+            out.append(None)
             continue
-        if here < 0:
-            here = _raw_device() if _raw_device is not None else torch.cuda.current_device()
-        if t.get_device() != here:
+        if t.get_device() != here or not t.is_contiguous():
+            ptr(t)                          # raises, unless the device is the wrong one
             raise KernelError(f"a tensor lies on GPU {t.get_device()}, the current device is {here}")
+        out.append(t.data_ptr())
+    out.append(_raw_stream(here) if _raw_stream is not None else torch.cuda.current_stream().cuda_stream)
+    return out
 
 
 def ints(*values) -> map:

@@ -22,7 +22,7 @@ from typing import Optional, Tuple
 import torch
 
 from ..csrc.build import load_kernel
-from ._call import KernelError, address, check, code, declared, on_current_device, raw_stream, want_f32, want_int32
+from ._call import KernelError, addresses, check, code, declared, want_f32, want_int32
 from .attention import PAIRING, prefill_rows, prefill_usable, resident_ctas
 from .gemm_tc import status_word
 
@@ -34,7 +34,7 @@ _SIGNATURES = {              # argument types of the entry points (_call.declare
     "tq_write8": "pipippipppp" "iippp" "iiiiii" "p", "tq_attention8": "pppippp" "iiifppi" "ppipi" "iiiiii" "p",
     "tq_weigh8": "pppippp" "iiifpp" "iiiiiii" "p", "tq_repair8": "pppppp" "iiifppi" "iiiii" "p",
     "tq_expand8": "ppppp" "iiipppi" "iiii" "p", "tq_weigh8_prompt": "ppippp" "iifpp" "iiiiiii" "pp",
-    "tq_evict8_select": "ppp" "iiiiiii" "pp", "tq_evict8_move": "ppppp" "ipi" "iiiiii" "p",
+    "tq_evict8": "ppppp" "ipi" "iiiiiii" "pp",
 }
 _entries = {}
 
@@ -130,15 +130,16 @@ def write_rows8(qkv: torch.Tensor, bias: Optional[torch.Tensor], cos: Optional[t
             raise KernelError(f"write_rows8: cos and sin tables must be [positions, {head_dim // 2}]")
     if T == 0:
         return
-    on_current_device(qkv, q_out, codes, scales, page_table)
+    p_qkv, p_bias, p_cos, p_sin, p_positions, p_cu, p_held, p_table, p_q, p_codes, p_scales, at = addresses(
+        qkv, bias, cos, sin, positions, cu_seqlens, held, page_table, q_out, codes, scales)
     check("cache8", _cache8("tq_write8")(
-        address(qkv), code(qkv.dtype), address(bias), 0 if bias is None else code(bias.dtype), address(cos), address(sin), PAIRING[pairing], address(positions),
-        address(cu_seqlens), address(held), address(page_table), page_table.shape[1], page_size, address(q_out), address(codes), address(scales),
-        0 if codes is None else codes.shape[0], n, index(max_q_len), n_heads, n_kv_heads, head_dim, raw_stream()))
+        p_qkv, code(qkv.dtype), p_bias, 0 if bias is None else code(bias.dtype), p_cos, p_sin, PAIRING[pairing], p_positions, p_cu, p_held, p_table,
+        page_table.shape[1], page_size, p_q, p_codes, p_scales, 0 if codes is None else codes.shape[0], n, index(max_q_len), n_heads, n_kv_heads, head_dim, at))
 
 
-MAX_RANGES = 64
-SETUP, JOIN = 1.5, 2.5       # what a CTA's begin and end, and the second launch, take in turns of its warps over blocks of keys
+MAX_RANGES, CLUSTER = 64, 8
+# what a CTA's begin and end, the join of a cluster and that of a second launch take, in turns of a CTA's warps over blocks of keys
+SETUP, CLUSTER_JOIN, JOIN = 1.5, 1.0, 3.5
 
 
 @lru_cache(maxsize=4096)
@@ -146,9 +147,9 @@ def ranges_for(tiles: int, blocks: int, resident: int) -> int:
     """Ranges the keys of a tile of columns are cut into, where the device runs `resident` CTAs at once and a CTA's four warps take a block of 16
     keys each in turn: the count with the fewest turns.  (B200, 16 heads of 128, 64 sequences of up to 2,048 keys, 1,024 tiles: one
     range 86 us, two 97, three 95, four 99.)"""
-    turns = lambda n: -(-tiles * n // resident) * (-(-blocks // (4 * n)) + SETUP) + (JOIN if n > 1 else 0.0)
-    most = max(1, min(MAX_RANGES, blocks // 4, max(8, resident // tiles)))
-    return min((n for n in (1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, most) if n <= most), key=lambda n: (turns(n), n))
+    turns = lambda n: -(-tiles * n // resident) * (-(-blocks // (4 * n)) + SETUP) + (0.0 if n == 1 else CLUSTER_JOIN if n <= CLUSTER else JOIN)
+    most = max(1, min(MAX_RANGES, blocks // 4, max(CLUSTER, resident // tiles)))
+    return min((n for n in (1, 2, 3, 4, 5, 6, 7, 8, 12, 16, 24, 32, 48, most) if n <= most), key=lambda n: (turns(n), n))
 
 
 SCORE_BYTES = 1 << 28        # scratch a decode step may take for scores
@@ -172,37 +173,44 @@ def attention8(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, cu_se
     if T == 0 or n == 0 or max_q_len < 1:
         return out
     max_q_len, max_kv_len = index(max_q_len), index(max_kv_len)
-    on_current_device(q, out, codes, scales, weights, page_table)
     if max_q_len >= PROMPT_MIN_RUN and prefill_usable(q.dtype, head_dim, page_size):
         return _attention8_prompt(q, codes, scales, cu_seqlens, held, page_table, page_size, window, scale, out, n_heads, n_kv_heads, head_dim,
                                   max_q_len, max_kv_len, weights, status)
+    p_q, p_out, p_codes, p_scales, p_cu, p_held, p_table, p_weights, at = addresses(q, out, codes, scales, cu_seqlens, held, page_table, weights)
     per = n_heads // n_kv_heads
     columns = max_q_len * per
     wide = columns > 8 and head_dim <= 128                  # two tiles of 8 columns in one CTA
-    tiles = -(-columns // (16 if wide else 8)) * n_kv_heads * n
+    own_tiles = -(-columns // (16 if wide else 8))          # of a sequence and key/value head
     per_sm = 2 if head_dim > 128 else 3 if wide and head_dim > 64 else 4         # CTAs an SM holds
     blocks = -(-max_kv_len // BLOCK)
-    ranges = ranges_for(tiles, blocks, resident_ctas(q.device) // 4 * per_sm)
-    # one row a sequence: the first launch leaves its scores for the second one to add up, which moves 8 bytes a key and query head, where
-    # reading the keys again moves head_dim bytes a key
-    stride, rows = blocks * BLOCK, T * n_heads
-    stored = weights is not None and max_q_len == 1 and 8 * per <= head_dim and 4 * rows * stride <= SCORE_BYTES
-    again = weights is not None and not stored
-    partial_floats = rows * ranges * (head_dim + 4) if ranges > 1 or stored else 0
-    partial = rest = None
-    if weights is not None or partial_floats:
-        scratch = torch.empty(partial_floats + (rows * stride if stored else 0) + (rows if again else 0), dtype=torch.float32, device=q.device)
-        rest = scratch.data_ptr() + 4 * partial_floats
-        if partial_floats:
-            partial = scratch.data_ptr()
-    step = (address(q), address(codes), address(scales), code(q.dtype), address(cu_seqlens), address(held), address(page_table), page_table.shape[1],
-            page_size, window, scale)
-    heads = (n_heads, n_kv_heads, head_dim, raw_stream())
+    ranges = ranges_for(own_tiles * n_kv_heads * n, blocks, resident_ctas(q.device) // 4 * per_sm)
+    partial = again = scores = None
+    stride = 0
+    joins = ranges > CLUSTER                                # in a second launch
+    if weights is not None:
+        # one row a sequence: scores are left for whoever joins the ranges, to be added up, which moves 8 bytes a key and query head, where reading
+        # the keys again moves head_dim bytes a key
+        stride, rows = blocks * BLOCK, T * n_heads
+        stored = max_q_len == 1 and 8 * per <= head_dim and 4 * rows * stride <= SCORE_BYTES
+        joins |= stored and (ranges == 1 or own_tiles > 1)
+        sums = rows * ranges * (head_dim + 4) if joins else 0
+        scratch = torch.empty(sums + (rows * stride if stored else rows), dtype=torch.float32, device=q.device)
+        partial = scratch.data_ptr() if joins else None
+        if stored:
+            scores = scratch.data_ptr() + 4 * sums
+        else:
+            again = scratch.data_ptr() + 4 * sums           # the rows' denominators, for a launch that reads the keys again
+    elif joins:
+        scratch = torch.empty(T * n_heads * ranges * (head_dim + 4), dtype=torch.float32, device=q.device)
+        partial = scratch.data_ptr()
+    dtype, width, pages = code(q.dtype), page_table.shape[1], codes.shape[0]
     check("attention8", _attention8("tq_attention8")(
-        *step, address(out), partial, ranges, rest if again else None, rest if stored else None, stride, address(weights) if stored else None, max_kv_len,
-        codes.shape[0], n, max_q_len, *heads), kernels=2 if partial_floats else 1)
-    if again:
-        check("attention8", _attention8("tq_weigh8")(*step, rest, address(weights), codes.shape[0], n, max_q_len, max_kv_len, *heads))
+        p_q, p_codes, p_scales, dtype, p_cu, p_held, p_table, width, page_size, window, scale, p_out, partial, ranges, again, scores, stride,
+        p_weights if scores is not None else None, max_kv_len, pages, n, max_q_len, n_heads, n_kv_heads, head_dim, at), kernels=2 if joins else 1)
+    if again is not None:
+        check("attention8", _attention8("tq_weigh8")(
+            p_q, p_codes, p_scales, dtype, p_cu, p_held, p_table, width, page_size, window, scale, again, p_weights, pages, n, max_q_len, max_kv_len,
+            n_heads, n_kv_heads, head_dim, at))
     return out
 
 
@@ -223,18 +231,21 @@ def _attention8_prompt(q, codes, scales, cu_seqlens, held, page_table, page_size
     table = torch.empty((group, width), dtype=torch.int32, device=q.device)
     lost = torch.empty((group, n_kv_heads, width), dtype=torch.uint8, device=q.device)
     lse = torch.empty((T, n_heads), dtype=torch.float32, device=q.device) if weights is not None else None
+    p_q, p_out, p_codes, p_scales, p_dense, p_tables, p_lost, p_lse, p_weights, p_status, at = addresses(
+        q, out, codes, scales, dense, table, lost, lse, weights, status)
+    pages = codes.shape[0]
     for i in range(0, n, group):
         m = min(group, n - i)
-        cu, starts, pages, dtable = cu_seqlens[i:i + m + 1], held[i:i + m], page_table[i:i + m], table[:m]
-        cache = (address(codes), address(scales), address(cu), address(starts), address(pages), pages.shape[1], page_size, window)
-        check("prompt8", _prompt8("tq_expand8")(*cache, address(dense), address(table), address(lost), width, codes.shape[0], m, n_kv_heads, head_dim, raw_stream()))
-        prefill_rows(q, dense, 2, cu, starts, dtable, page_size, window, scale, out, m, max_q_len, n_heads, n_kv_heads, head_dim, head_dim, status=status, lse=lse)
-        check("attention8", _attention8("tq_repair8")(
-            address(q), *cache, scale, address(out), address(lost), width, codes.shape[0], m, n_heads, n_kv_heads, head_dim, raw_stream()))
+        cu, starts, own_pages = cu_seqlens[i:i + m + 1], held[i:i + m], page_table[i:i + m]
+        p_cu, p_held, p_table, _ = addresses(cu, starts, own_pages)
+        cache = (p_codes, p_scales, p_cu, p_held, p_table, page_table.shape[1], page_size, window)
+        check("prompt8", _prompt8("tq_expand8")(*cache, p_dense, p_tables, p_lost, width, pages, m, n_kv_heads, head_dim, at))
+        prefill_rows(q, dense, 2, cu, starts, table[:m], page_size, window, scale, out, m, max_q_len, n_heads, n_kv_heads, head_dim, head_dim, status=status, lse=lse)
+        check("attention8", _attention8("tq_repair8")(p_q, *cache, scale, p_out, p_lost, width, pages, m, n_heads, n_kv_heads, head_dim, at))
         if weights is not None:
             check("prompt8", _prompt8("tq_weigh8_prompt")(
-                address(q), address(dense), width, address(cu), address(starts), address(pages), pages.shape[1], window, scale, address(lse), address(weights),
-                codes.shape[0], T, m, max_kv_len, n_heads, n_kv_heads, head_dim, address(status), raw_stream()))
+                p_q, p_dense, width, p_cu, p_held, p_table, page_table.shape[1], window, scale, p_lse, p_weights, pages, T, m, max_kv_len,
+                n_heads, n_kv_heads, head_dim, p_status, at))
     return out
 
 
@@ -256,12 +267,9 @@ def evict8(codes: torch.Tensor, scales: torch.Tensor, weights: torch.Tensor, len
         raise KernelError(f"evict8: {n} page tables, {lengths.numel()} lengths and new tables {tuple(new_table.shape)} for a budget of {budget} rows do not fit together")
     if not 0 <= recent <= budget or budget < 1:
         raise KernelError(f"evict8: cannot keep the newest {recent} rows of a budget of {budget}")
-    on_current_device(codes, scales, weights, page_table, new_table)
+    p_codes, p_scales, p_weights, p_lengths, p_table, p_new, at = addresses(codes, scales, weights, lengths, page_table, new_table)
     kept = torch.empty((n, n_kv_heads, budget), dtype=torch.int32, device=codes.device)
-    width, pages = page_table.shape[1], codes.shape[0]
-    check("evict", _evict("tq_evict8_select")(
-        address(weights), address(lengths), address(page_table), width, page_size, pages, n, n_kv_heads, budget, recent, address(kept), raw_stream()))
-    check("evict", _evict("tq_evict8_move")(
-        address(codes), address(scales), address(weights), address(kept), address(page_table), width, address(new_table), new_table.shape[1],
-        page_size, pages, n, n_kv_heads, head_dim, budget, raw_stream()))
+    check("evict", _evict("tq_evict8")(
+        p_codes, p_scales, p_weights, p_lengths, p_table, page_table.shape[1], p_new, new_table.shape[1], page_size, codes.shape[0], n, n_kv_heads, head_dim,
+        budget, recent, kept.data_ptr(), at), kernels=2)
     return kept
