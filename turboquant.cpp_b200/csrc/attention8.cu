@@ -224,21 +224,42 @@ __device__ __forceinline__ int first_seen(int place, int window) { return window
 
 constexpr float LOWEST = -3.402823466e38f;       // a maximum over nothing
 
+// Scores of a step of single rows lie by key, a key's columns side by side in the next power of two (at most 16, or a multiple of 16).
+__host__ __device__ __forceinline__ int score_columns(int per) { return per <= 2 ? per : per <= 4 ? 4 : per <= 8 ? 8 : (per + 15) / 16 * 16; }
+// The sum over a key's columns of 2^(score - lse)
+__device__ __forceinline__ float weight_of(const float* __restrict__ scores, const float* lse, int per) {
+    float sum = 0.f;
+    if (per <= 2) {
+        sum = ex2(scores[0] - lse[0]);
+        if (per == 2) sum += ex2(scores[1] - lse[1]);
+        return sum;
+    }
+    for (int c = 0; c < per; c += 4) {
+        const float4 v = *reinterpret_cast<const float4*>(scores + c);
+        sum += ex2(v.x - lse[c]);
+        if (c + 1 < per) sum += ex2(v.y - lse[c + 1]);
+        if (c + 2 < per) sum += ex2(v.z - lse[c + 2]);
+        if (c + 3 < per) sum += ex2(v.w - lse[c + 3]);
+    }
+    return sum;
+}
+
 // ---------------------------------------------------------------------------------------
 // A range of the keys for a tile of columns.  partial: null, or [T * nh][ranges][hd + 4] for a second launch: the unnormalised sum, the
-// maximum m' it is relative to, the denominator's maximum and the denominator.  scores: null, or [T * nh][score_stride], base-2 scores.
+// maximum m' it is relative to, the denominator's maximum and the denominator.  scores: null, or (runs of one row) the base-2 scores of the
+// tile's `per` columns, [n_seqs * nkv][score_stride][score_columns(per)].
 // lse: null, or [T * nh], log2 of the denominator (where there is no second launch).  Several ranges without `partial`: they are the CTAs of a
 // cluster, which join in their shared memory, each for its part of the result; with `weights` and scores each then adds up its own keys'
 // weights (the tile has all the columns of its sequence and head then).
 // ---------------------------------------------------------------------------------------
-template <class F>
+template <class F, bool CLUSTERED>
 __device__ __forceinline__ void attend_tile(const Tile& T, int range, int ranges, const typename F::TA* __restrict__ q, const Cache8& c, const Step& S,
                                             typename F::TA* __restrict__ out, float* __restrict__ partial, float* __restrict__ scores, int score_stride,
                                             float* __restrict__ lse, float* __restrict__ weights) {
     constexpr int NT = F::NT, NC = F::NC, MT = F::MT, HDP = F::HDP;
     extern __shared__ __align__(16) uint8_t ring[];
     __shared__ Queries<F> Q;
-    __shared__ float s_stat[WARPS][NC][3], s_ranks[CLUSTER][NC][3], s_lse[NC];
+    __shared__ float s_stat[WARPS][NC][3], s_ranks[CLUSTERED ? CLUSTER : 1][NC][3], s_lse[NC];
     float (*s_o)[NC][HDP + 4] = reinterpret_cast<float (*)[NC][HDP + 4]>(ring);        // [WARPS], once the keys are through
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, hd = F::EXACT ? HDP : c.hd;
     // this range's blocks of 16 keys
@@ -301,6 +322,8 @@ __device__ __forceinline__ void attend_tile(const Tile& T, int range, int ranges
         m[nt][0] = m[nt][1] = mo[nt][0] = mo[nt][1] = LOWEST;
         l[nt][0] = l[nt][1] = 0.f;
     }
+    const int score_cols = score_columns(T.per);
+    float* own_scores = scores != nullptr ? scores + ((size_t)T.seq * c.nkv + T.g) * score_stride * score_cols : nullptr;
     int taken = 0;
 #pragma unroll 1
     for (int b = from + warp; b < to; b += WARPS) {
@@ -338,9 +361,12 @@ __device__ __forceinline__ void attend_tile(const Tile& T, int range, int ranges
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int col = nt * 8 + 2 * t + (j & 1);
-                    if (col < T.n && key + 8 * (j >> 1) < score_stride) scores[Q.row[col] * score_stride + key + 8 * (j >> 1)] = s[nt][j];
+                for (int h = 0; h < 2; ++h) {
+                    const int col = T.first + nt * 8 + 2 * t, k = key + 8 * h;
+                    if (nt * 8 + 2 * t >= T.n || k >= score_stride) continue;
+                    float* to = own_scores + (size_t)k * score_cols + col;
+                    if (score_cols > 1) *reinterpret_cast<float2*>(to) = make_float2(s[nt][2 * h], s[nt][2 * h + 1]);
+                    else *to = s[nt][2 * h];
                 }
         }
         // the maxima grow now and then: found by all lanes of a column together when one of them sees a larger value
@@ -484,7 +510,7 @@ __device__ __forceinline__ void attend_tile(const Tile& T, int range, int ranges
             mw[w] = exp2f(s_stat[w][col][0] - MO);
             L += s_stat[w][col][2] * exp2f(s_stat[w][col][1] - M);
         }
-        if (ranges > 1 && partial == nullptr) {
+        if (CLUSTERED) {
             for (int d = lane; d < hd; d += 32) {
                 float sum = 0.f;
 #pragma unroll
@@ -508,7 +534,7 @@ __device__ __forceinline__ void attend_tile(const Tile& T, int range, int ranges
         if (pp != nullptr && lane == 0) { pp[hd] = MO; pp[hd + 1] = M; pp[hd + 2] = L; }
         if (pp == nullptr && lse != nullptr && lane == 0) lse[at] = M + log2f(L);
     }
-    if (ranges == 1 || partial != nullptr) return;
+    if (!CLUSTERED) return;
     __syncwarp();
     // the cluster's sums together: statistics of all ranges first, then every CTA its part of the tile's results
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -542,20 +568,21 @@ __device__ __forceinline__ void attend_tile(const Tile& T, int range, int ranges
             s_lse[threadIdx.x] = M + log2f(L);
         }
         __syncthreads();
-        for (int k = from * C8_BLOCK + threadIdx.x; k < min(min(to * C8_BLOCK, place1 + 1), score_stride); k += WARPS * 32) {
-            if (S.window > 0 && k + S.window <= T.start) continue;                       // no row of the step sees it
-            float sum = 0.f;
-            for (int col = 0; col < T.n; ++col)
-                if (k <= Q.place[col] && (S.window <= 0 || k > Q.place[col] - S.window)) sum += ex2(scores[Q.row[col] * score_stride + k] - s_lse[col]);
+        // (the step has one row of the sequence: it sees up to its own place)
+        const int last = min(min(to * C8_BLOCK, place1 + 1), score_stride);
+#pragma unroll 2
+        for (int k = from * C8_BLOCK + threadIdx.x; k < last; k += WARPS * 32) {
+            if (S.window > 0 && k + S.window <= T.start) continue;
             float* w = weights + ((size_t)c.page_of(T.seq, k) * c.nkv + T.g) * c.page_size + c.row(k);
-            *w = (k < T.start ? *w : 0.f) + sum;
+            const float was = k < T.start ? *w : 0.f;
+            *w = was + weight_of(own_scores + (size_t)k * score_cols, s_lse, T.per);
         }
     }
     // nobody leaves while its sums are being read
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-template <class F>
+template <class F, bool CLUSTERED>
 __global__ void __launch_bounds__(WARPS * 32, F::PER_SM) attention8_kernel(const typename F::TA* __restrict__ q, Cache8 c, Step S, typename F::TA* __restrict__ out,
                                                                                            float* __restrict__ partial, float* __restrict__ scores, int score_stride,
                                                                                            float* __restrict__ lse, float* __restrict__ weights, int ranges) {
@@ -563,7 +590,7 @@ __global__ void __launch_bounds__(WARPS * 32, F::PER_SM) attention8_kernel(const
     tq_grid_launch_dependents();
     const int tile = blockIdx.x / ranges, tile_no = tile / c.nkv;
     const Tile T = tile_of(S, blockIdx.z, tile - tile_no * c.nkv, c.nkv, tile_no, F::NC);
-    if (T.n > 0) attend_tile<F>(T, blockIdx.x - tile * ranges, ranges, q, c, S, out, partial, scores, score_stride, lse, weights);
+    if (T.n > 0) attend_tile<F, CLUSTERED>(T, blockIdx.x - tile * ranges, ranges, q, c, S, out, partial, scores, score_stride, lse, weights);
 }
 
 // The prompt kernel gives values that a row may not see a weight of 0, which does not remove a NaN: key/value heads of sequences in whose pages
@@ -583,7 +610,7 @@ __global__ void __launch_bounds__(WARPS * 32) repair8_kernel(const typename F::T
         const Tile T = tile_of(S, seq, g, c.nkv, tile_no, F::NC);
         if (T.n <= 0) return;
         __syncthreads();
-        attend_tile<F>(T, 0, 1, q, c, S, out, nullptr, nullptr, 0, nullptr, nullptr);
+        attend_tile<F, false>(T, 0, 1, q, c, S, out, nullptr, nullptr, 0, nullptr, nullptr);
     }
 }
 
@@ -623,7 +650,7 @@ __global__ void __launch_bounds__(128) join8_kernel(Cache8 c, Step S, const floa
                                                     float* __restrict__ lse, const float* __restrict__ scores, int score_stride, float* __restrict__ weights) {
     tq_grid_wait();                    // everything below may read what the previous kernel wrote
     tq_grid_launch_dependents();
-    __shared__ float s_f[JOIN_RANGES], s_lse[128];
+    __shared__ float s_f[JOIN_RANGES], s_lse[128 + 4];
     const int seq = blockIdx.z, g = blockIdx.y, per = S.nh / c.nkv, hd = c.hd, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int t_begin = S.cu_seqlens[seq], run = S.cu_seqlens[seq + 1] - t_begin, columns = run * per;
     auto query = [&](int col) { const int r = col / per; return (size_t)(t_begin + r) * S.nh + g * per + (col - r * per); };
@@ -658,24 +685,23 @@ __global__ void __launch_bounds__(128) join8_kernel(Cache8 c, Step S, const floa
         }
         return;
     }
+    // (the step has one row of the sequence: it sees up to its own place)
     const int start = S.held[seq], place0 = ((int)blockIdx.x - rows) * 128, place = place0 + (int)threadIdx.x;
-    if (run <= 0 || place0 >= start + run) return;
+    if (run <= 0 || place0 > start) return;
     float sum = 0.f;
-    for (int c0 = 0; c0 < columns; c0 += 128) {
+    for (int c0 = 0; c0 < per; c0 += 128) {
+        const int n = min(128, per - c0);
         __syncthreads();
-        for (int x = warp; x < min(128, columns - c0); x += 4) {
+        for (int x = warp; x < n; x += 4) {
             float MO, M, L;
             join_stats(partial, query(c0 + x), ranges, hd, MO, M, L, nullptr);
             if (lane == 0) s_lse[x] = M + log2f(L);
         }
         __syncthreads();
-        for (int x = 0; x < min(128, columns - c0); ++x) {
-            const int p = start + (c0 + x) / per;
-            if (place > p || place >= score_stride || (S.window > 0 && place <= p - S.window)) continue;
-            sum += ex2(scores[query(c0 + x) * score_stride + place] - s_lse[x]);
-        }
+        if (place <= start && place < score_stride)
+            sum += weight_of(scores + (((size_t)seq * c.nkv + g) * score_stride + place) * score_columns(per) + c0, s_lse, n);
     }
-    if (place >= start + run || (S.window > 0 && place + S.window <= start)) return;       // no row of the step sees it
+    if (place > start || place >= score_stride || (S.window > 0 && place + S.window <= start)) return;
     float* w = weights + ((size_t)c.page_of(seq, place) * c.nkv + g) * c.page_size + c.row(place);
     *w = (place < start ? *w : 0.f) + sum;
 }
@@ -769,12 +795,17 @@ int launch8(const void* q, const Cache8& c, const Step& S, void* out, float* par
             int n_seqs, int max_q_len, cudaStream_t stream) {
     const long long tiles = ((long long)max_q_len * (S.nh / c.nkv) + F::NC - 1) / F::NC * c.nkv;
     TQ_REQUIRE(tiles * ranges < (1ll << 31), "attention8: runs of %d rows", max_q_len);
-    static std::atomic<unsigned long long> asked{0};
-    const cudaError_t e = tq_reserve_smem(attention8_kernel<F>, F::SMEM, asked);
-    if (e != cudaSuccess) TQ_FAIL(-1, "attention8: cannot reserve %d bytes of shared memory: %s", F::SMEM, cudaGetErrorString(e));
     TQ_REQUIRE(weights == nullptr || tiles == c.nkv, "attention8: a tile of %d columns does not hold %d query heads", F::NC, S.nh / c.nkv);
-    tq_launch(dim3((unsigned)(tiles * ranges), 1, n_seqs), WARPS * 32, F::SMEM, stream, partial == nullptr ? ranges : 1)(
-        attention8_kernel<F>, (const typename F::TA*)q, c, S, (typename F::TA*)out, partial, scores, score_stride, lse, weights, ranges);
+    auto launch = [&](auto kernel, std::atomic<unsigned long long>& asked, int cluster) -> int {
+        const cudaError_t e = tq_reserve_smem(kernel, F::SMEM, asked);
+        if (e != cudaSuccess) TQ_FAIL(-1, "attention8: cannot reserve %d bytes of shared memory: %s", F::SMEM, cudaGetErrorString(e));
+        tq_launch(dim3((unsigned)(tiles * ranges), 1, n_seqs), WARPS * 32, F::SMEM, stream, cluster)(
+            kernel, (const typename F::TA*)q, c, S, (typename F::TA*)out, partial, scores, score_stride, lse, weights, ranges);
+        return 0;
+    };
+    static std::atomic<unsigned long long> asked{0}, asked_clustered{0};
+    const int rc = ranges > 1 && partial == nullptr ? launch(attention8_kernel<F, true>, asked_clustered, ranges) : launch(attention8_kernel<F, false>, asked, 1);
+    if (rc) return rc;
     TQ_CHECK_LAUNCH("attention8");
     return 0;
 }
@@ -806,8 +837,8 @@ int check_step(const char* what, int nh, int nkv, int n_seqs, int longest, int w
 // q [T, nh, hd], out [T, nh * hd]; place i sees j <= i with window == 0 or i - j < window.  max_q_len: the longest run.  ranges > 1: the keys
 // of a row are cut into that many ranges, which join as a cluster (up to 8; partial null) or in a second launch (up to 64; partial
 // [T * nh * ranges * (hd + 4)]).  lse [T, nh] float32 or null.  scores [T * nh, score_stride] with weights [n_pages, nkv, page_size], or both
-// null: the weights are added up by whoever joins, so by clusters only of all of a key/value head's query heads, and of two ranges or more;
-// score_stride: a multiple of 16, at least the longest held[s] + run, max_kv_len.
+// null: the weights of a step of single rows are added up by whoever joins, so by clusters only of all of a key/value head's query heads, and of
+// two ranges or more.  scores: [n_seqs * nkv, score_stride, score_columns(nh / nkv)], score_stride at least max_kv_len, the longest held[s] + run.
 TQ_EXPORT int tq_attention8(const void* q, const void* codes, const void* scales, int act_dtype, const int* cu_seqlens, const int* held,
                             const int* page_table, int table_stride, int page_size, int window, float scale, void* out, float* partial, int ranges,
                             float* lse, float* scores, int score_stride, float* weights, int max_kv_len, int n_pages, int n_seqs, int max_q_len, int nh,
@@ -817,7 +848,7 @@ TQ_EXPORT int tq_attention8(const void* q, const void* codes, const void* scales
     if (!rc) rc = check_step("attention8", nh, nkv, n_seqs, max_q_len, window);
     if (rc) return rc;
     TQ_REQUIRE(ranges >= 1 && ranges <= (partial != nullptr ? JOIN_RANGES : CLUSTER), "attention8: %d ranges need a buffer for their sums", ranges);
-    TQ_REQUIRE((scores == nullptr) == (weights == nullptr) && (scores == nullptr || ((partial != nullptr || (ranges > 1 && max_q_len == 1)) && score_stride % 16 == 0 && score_stride >= max_kv_len)),
+    TQ_REQUIRE((scores == nullptr) == (weights == nullptr) && (scores == nullptr || (max_q_len == 1 && (partial != nullptr || ranges > 1) && score_stride >= max_kv_len && (uintptr_t)scores % 16 == 0)),
                "attention8: scores of %d places do not hold %d", score_stride, max_kv_len);
     const Cache8 c = c8_cache(codes, scales, page_table, table_stride, page_size, n_pages, nkv, hd);
     const Step S{cu_seqlens, held, nh, window, scale * LOG2E};

@@ -139,7 +139,7 @@ def write_rows8(qkv: torch.Tensor, bias: Optional[torch.Tensor], cos: Optional[t
 
 MAX_RANGES, CLUSTER = 64, 8
 # what a CTA's begin and end, the join of a cluster and that of a second launch take, in turns of a CTA's warps over blocks of keys
-SETUP, CLUSTER_JOIN, JOIN = 1.5, 1.0, 3.5
+SETUP, CLUSTER_JOIN, JOIN = 1.5, 1.0, 6.0
 
 
 @lru_cache(maxsize=4096)
@@ -191,10 +191,11 @@ def attention8(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, cu_se
         # one row a sequence: scores are left for whoever joins the ranges, to be added up, which moves 8 bytes a key and query head, where reading
         # the keys again moves head_dim bytes a key
         stride, rows = blocks * BLOCK, T * n_heads
-        stored = max_q_len == 1 and 8 * per <= head_dim and 4 * rows * stride <= SCORE_BYTES
+        size = n * n_kv_heads * stride * (per if per <= 2 else 4 if per <= 4 else 8 if per <= 8 else -(-per // 16) * 16)
+        stored = max_q_len == 1 and 8 * per <= head_dim and 4 * size <= SCORE_BYTES
         joins |= stored and (ranges == 1 or own_tiles > 1)
         sums = rows * ranges * (head_dim + 4) if joins else 0
-        scratch = torch.empty(sums + (rows * stride if stored else rows), dtype=torch.float32, device=q.device)
+        scratch = torch.empty(sums + (size if stored else rows), dtype=torch.float32, device=q.device)
         partial = scratch.data_ptr() if joins else None
         if stored:
             scores = scratch.data_ptr() + 4 * sums
