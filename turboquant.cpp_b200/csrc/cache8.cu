@@ -106,6 +106,16 @@ __global__ void __launch_bounds__(WRITE_THREADS) write8_kernel(const TA* __restr
     const bool mine = it < items && j < a.written, is_q = j < a.nh;
     const int r = it / groups, i = (it - r * groups) * 8;
     const int ia = a.pairing == 0 ? i : 2 * i, ib = a.pairing == 0 ? i + half : 2 * i + 8;       // where the item's two halves lie in the head
+    // where the unit's codes go, and the byte of rows the block holds already, looked up beside the loads of the rows
+    const int plane = j >= a.nh + c.nkv ? 1 : 0, g = j - a.nh - plane * c.nkv, row0 = c.row(block_start), old = first - block_start;
+    uint8_t *codes = nullptr, *byte = nullptr;
+    uint32_t was = 1;
+    if (!is_q && j < a.written) {
+        const int page = c.page_of(seq, first);
+        codes = c.codes + c.codes_at(page, plane, g) + (size_t)row0 * hd;
+        byte = c.scales + c.scales_at(page, plane, g) + row0 / C8_BLOCK;
+        if (old > 0) was = max((uint32_t)*byte, 1u);                  // (by all of the unit's threads before one of them writes it)
+    }
     Eight lo = {}, hi = {};
     if (mine) {
         const TA* row = qkv + ((size_t)(t0 + r) * heads + j) * hd;
@@ -157,15 +167,6 @@ __global__ void __launch_bounds__(WRITE_THREADS) write8_kernel(const TA* __restr
         }
     }
     if (a.written == a.nh) return;                                    // queries only
-    const int plane = j >= a.nh + c.nkv ? 1 : 0, g = j - a.nh - plane * c.nkv, row0 = c.row(block_start), old = first - block_start;
-    uint8_t *codes = nullptr, *byte = nullptr;
-    uint32_t was = 1;
-    if (!is_q && j < a.written) {
-        const int page = c.page_of(seq, first);
-        codes = c.codes + c.codes_at(page, plane, g) + (size_t)row0 * hd;
-        byte = c.scales + c.scales_at(page, plane, g) + row0 / C8_BLOCK;
-        if (old > 0) was = max((uint32_t)*byte, 1u);                  // (by all of the unit's threads before one of them writes it)
-    }
     // over the unit's threads
     auto over_unit = [&](float top) {
         top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));       // magnitudes: ordered as integers are

@@ -140,15 +140,23 @@ __global__ void __launch_bounds__(256) evict8_move_kernel(Cache8 c, float* __res
     const uint32_t shift = top - byte;
     // pieces of 16 bytes: all rows of the keys, then of the values
     const int pieces = C8_BLOCK * vecs;
-#pragma unroll 8
-    for (int v0 = 0; v0 < 2 * pieces; v0 += 32) {
-        const int v = v0 + lane, which = v / vecs, at = (v - which * vecs) * 16;        // which: row, 16 more for values
-        const unsigned long long src = __shfl_sync(0xffffffffu, from, which);
-        const uint32_t s = __shfl_sync(0xffffffffu, shift, which);
-        if ((which & 15) < rows) {
-            uint4 x = *reinterpret_cast<const uint4*>(c.codes + src + at);
-            if (s) x = c8_shift16(x, c8_shift_factor((int)min(s, 25u)));
-            *reinterpret_cast<uint4*>(c.codes + to + (which >> 4) * between + (size_t)(which & 15) * c.hd + at) = x;
+    constexpr int BATCH = 8;               // all of them asked for before the first is stored (the compiler cannot know that they do not overlap)
+    for (int v0 = 0; v0 < 2 * pieces; v0 += 32 * BATCH) {
+        uint4 x[BATCH];
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i) {
+            const int v = v0 + 32 * i + lane, which = v / vecs, at = (v - which * vecs) * 16;        // which: row, 16 more for values
+            const unsigned long long src = __shfl_sync(0xffffffffu, from, which & 31);
+            if (v < 2 * pieces && (which & 15) < rows) x[i] = *reinterpret_cast<const uint4*>(c.codes + src + at);
+        }
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i) {
+            const int v = v0 + 32 * i + lane, which = v / vecs, at = (v - which * vecs) * 16;
+            const uint32_t s = __shfl_sync(0xffffffffu, shift, which & 31);
+            if (v < 2 * pieces && (which & 15) < rows) {
+                if (s) x[i] = c8_shift16(x[i], c8_shift_factor((int)min(s, 25u)));
+                *reinterpret_cast<uint4*>(c.codes + to + (which >> 4) * between + (size_t)(which & 15) * c.hd + at) = x[i];
+            }
         }
     }
     if (r == 0) c.scales[c.scales_at(page, plane, g) + row0 / C8_BLOCK] = (uint8_t)top;

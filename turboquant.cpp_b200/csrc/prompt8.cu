@@ -31,21 +31,40 @@ __global__ void __launch_bounds__(256) expand8_kernel(Cache8 c, const int* __res
     if (run <= 0 || n * PAGE > last || n < (window > 0 ? max(0, start + 1 - window) : 0) / PAGE) return;
     const int page = c.page_of(seq, n * PAGE), to = seq * width + n, vecs = c.hd / 16, rows = min(PAGE, last + 1 - n * PAGE);
     bool nan = false;
-    for (int i = threadIdx.x; i < 2 * PAGE * vecs; i += 256) {
-        const int plane = i / (PAGE * vecs), r = i / vecs % PAGE, v = i % vecs;
-        uint4 a = make_uint4(0, 0, 0, 0), b = a;
-        if (r < rows) {
-            const uint4 x = *reinterpret_cast<const uint4*>(c.codes + c.codes_at(page, plane, g) + (size_t)r * c.hd + v * 16);
-            const float s = c8_scale(c.scales[c.scales_at(page, plane, g) + r / C8_BLOCK]);
-            a = make_uint4(bf16x2_of(x.x & 0xffffu, s), bf16x2_of(x.x >> 16, s), bf16x2_of(x.y & 0xffffu, s), bf16x2_of(x.y >> 16, s));
-            b = make_uint4(bf16x2_of(x.z & 0xffffu, s), bf16x2_of(x.z >> 16, s), bf16x2_of(x.w & 0xffffu, s), bf16x2_of(x.w >> 16, s));
-            const uint32_t u[4] = {x.x, x.y, x.z, x.w};
+    const uint8_t* codes = c.codes + c.codes_at(page, 0, g);
+    const uint8_t* scales = c.scales + c.scales_at(page, 0, g);
+    const size_t plane_codes = (size_t)c.nkv * PAGE * c.hd, plane_scales = (size_t)c.nkv * (PAGE / C8_BLOCK);
+    constexpr int BATCH = 4;                   // pieces of 16 codes a thread asks for at a time
+    const int pieces = PAGE * vecs;
+    for (int i0 = threadIdx.x; i0 < 2 * pieces; i0 += 256 * BATCH) {
+        uint4 x[BATCH];
+        float s[BATCH];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) nan |= plane == 1 && (((u[k] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0;
+        for (int k = 0; k < BATCH; ++k) {
+            const int i = i0 + 256 * k, plane = i >= pieces, j = i - plane * pieces, r = j / vecs;
+            x[k] = make_uint4(0, 0, 0, 0);
+            s[k] = 1.f;
+            if (i < 2 * pieces && r < rows) {
+                x[k] = __ldg(reinterpret_cast<const uint4*>(codes + plane * plane_codes) + j);
+                s[k] = c8_scale(__ldg(scales + plane * plane_scales + r / C8_BLOCK));
+            }
         }
-        uint4* d = dense + (((size_t)to * 2 + plane) * c.nkv + g) * (PAGE * vecs * 2) + (size_t)r * vecs * 2 + v * 2;
-        d[0] = a;
-        d[1] = b;
+#pragma unroll
+        for (int k = 0; k < BATCH; ++k) {
+            const int i = i0 + 256 * k, plane = i >= pieces, j = i - plane * pieces;
+            if (i >= 2 * pieces) break;
+            const uint32_t u[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
+            uint32_t w[8];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                w[2 * e] = bf16x2_of(u[e] & 0xffffu, s[k]);
+                w[2 * e + 1] = bf16x2_of(u[e] >> 16, s[k]);
+                nan |= plane == 1 && (((u[e] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0;
+            }
+            uint4* d = dense + (((size_t)to * 2 + plane) * c.nkv + g) * (pieces * 2) + (size_t)j * 2;
+            d[0] = make_uint4(w[0], w[1], w[2], w[3]);
+            d[1] = make_uint4(w[4], w[5], w[6], w[7]);
+        }
     }
     const bool any = __syncthreads_or(nan);
     if (threadIdx.x == 0) {
