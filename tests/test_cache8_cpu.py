@@ -132,3 +132,19 @@ def test_ranges_fill_the_device_and_no_more():
     for tiles, blocks in ((16, 44), (32, 2031), (4, 8000), (128, 256), (600, 128)):
         n = r(tiles, blocks, 592)
         assert 1 < n <= min(64, blocks // 4) and (tiles > 592 or tiles * n <= 592)
+
+
+def test_prompt_units_are_cut_where_few_of_them_are_long():
+    from turboquant_cpp_b200.kernels.attention import prefill_pieces
+    cut = lambda *a: prefill_pieces(*a, 148)
+    assert cut(12000, 8, 2667, 2667, 16, 16, 128, 0) == (1, 0)             # more units than the device takes at once
+    assert cut(2048, 1, 2048, 2048, 16, 16, 128, 0) == (1, 0)              # nearly as many
+    assert cut(500, 1, 500, 500, 16, 16, 128, 0) == (1, 0)                 # few keys
+    assert cut(1000, 2, 667, 9668, 28, 4, 128, 4096) == (1, 0)
+    for args in ((500, 1, 500, 3500, 16, 16, 128, 0), (60, 1, 60, 5000, 28, 4, 128, 0), (64, 4, 16, 40000, 16, 16, 64, 0), (200, 1, 200, 9000, 8, 2, 64, 4096)):
+        pieces, pages = cut(*args)
+        keys = args[3] if not args[7] else args[7] + 256
+        assert pieces > 1 and pages % 2 == 0 and pages >= 8 and pieces * pages * 64 >= keys + 127
+        units = args[1] * args[4] * -(-args[2] // 256)
+        assert pieces * units <= 2 * 148
+    assert cut(1 << 20, 1, 256, 1 << 30, 1, 1, 128, 0) == (1, 0)           # more scratch than a step may take

@@ -24,6 +24,14 @@ STEPS = [([1], [0]), ([1], [15]), ([1], [16]), ([1], [700]), ([1, 1, 1], [63, 64
          ([50], [0]), ([48, 200], [0, 77]), ([130, 49], [300, 16])]
 
 
+@pytest.fixture(params=["by size", "prompt kernel"])
+def prompts(request, monkeypatch):
+    """Small steps go to the kernel of single tokens and short runs: with the second value, to the prompt kernel whatever their size."""
+    if request.param != "by size":
+        from turboquant_cpp_b200.kernels import cache8
+        monkeypatch.setattr(cache8, "PROMPT_WORK", 0)
+
+
 def _i(values):
     return torch.tensor(values, dtype=torch.int32, device=DEV)
 
@@ -143,7 +151,7 @@ def test_a_step_written_again_leaves_the_same_bits():
 @pytest.mark.parametrize("shape", SHAPES, ids=str)
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("step", range(len(STEPS)))
-def test_attention_and_sums_of_weights(shape, dtype, step):
+def test_attention_and_sums_of_weights(shape, dtype, step, prompts):
     (H, G, D), (runs, held) = shape, STEPS[step]
     window = (0, 40, 0, 1, 0, 100)[(step + SHAPES.index(shape)) % 6]
     page_size = (64, 32, 64, 16)[step % 4]
@@ -172,7 +180,7 @@ def test_attention_and_sums_of_weights(shape, dtype, step):
 
 @pytest.mark.parametrize("runs,held", [([1, 1], [200, 30]), ([60, 1], [0, 100])])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
-def test_what_lies_behind_a_row_does_not_reach_it(dtype, runs, held):
+def test_what_lies_behind_a_row_does_not_reach_it(dtype, runs, held, prompts):
     """Codes and bytes behind the last row (of pages used before) are NaN or the largest there are; the result keeps its bits."""
     H, G, D = 8, 2, 128
     table, pages = _pages([n + h for n, h in zip(runs, held)], 64)
@@ -194,7 +202,7 @@ def test_what_lies_behind_a_row_does_not_reach_it(dtype, runs, held):
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("runs", [[1], [70]])
-def test_a_value_that_is_not_finite_is_lost_where_it_is_seen(dtype, runs):
+def test_a_value_that_is_not_finite_is_lost_where_it_is_seen(dtype, runs, prompts):
     H, G, D, held = 4, 2, 128, [90]
     table, pages = _pages([held[0] + runs[0]], 64)
     codes, scales = _cache(pages, G, 64, D)
@@ -214,7 +222,7 @@ def test_a_value_that_is_not_finite_is_lost_where_it_is_seen(dtype, runs):
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("runs", [[1], [70]])
-def test_blocks_of_very_unequal_bytes(dtype, runs):
+def test_blocks_of_very_unequal_bytes(dtype, runs, prompts):
     """Values of 2^30 whose weight is next to nothing beside values of 1, and rows of queries up to 2^60 and down to 2^-60."""
     H, G, D, held = 2, 1, 64, [150]
     n = held[0] + runs[0]
@@ -259,7 +267,7 @@ def test_rows_behind_the_last_sequence_stay_and_a_graph_replays():
     assert torch.equal(out, out2) and torch.equal(w, w2)
 
 
-def test_sums_of_weights_are_the_same_bits_every_time():
+def test_sums_of_weights_are_the_same_bits_every_time(prompts):
     H, G, D, runs, held = 28, 4, 128, [1, 1, 90], [500, 63, 200]
     table, pages = _pages([n + h for n, h in zip(runs, held)], 64)
     codes, scales = _cache(pages, G, 64, D)
@@ -305,7 +313,7 @@ def test_eviction_keeps_the_rows_it_should(shape, kind, case):
 
 
 # ---- together -----------------------------------------------------------------------------------------------------------
-def test_a_sequence_from_its_prompt_through_evictions():
+def test_a_sequence_from_its_prompt_through_evictions(prompts):
     """Write, attend with sums, evict, go on: every step against the plain forms on the plain forms' own cache."""
     from turboquant_cpp_b200.kernels import cache8
     H, G, D, page_size, budget, recent = 6, 2, 64, 64, 96, 16
@@ -351,7 +359,36 @@ def test_a_small_scratch_takes_the_sequences_in_groups(monkeypatch):
     table, pages = _pages([n + h for n, h in zip(runs, held)], 64)
     codes, scales = _cache(pages, G, 64, D)
     q = torch.randn(sum(runs), H, D).to(torch.bfloat16)
+    monkeypatch.setattr(cache8, "PROMPT_WORK", 0)
     want, want_w = _attend(q, codes, scales, runs, held, table, 64, 0, 0.1, H, G, D, torch.zeros(pages, G, 64))
     monkeypatch.setattr(cache8, "DENSE_BYTES", 2 * 2 * G * 64 * D * 2 * 4)          # two sequences of four pages
     got, got_w = _attend(q, codes, scales, runs, held, table, 64, 0, 0.1, H, G, D, torch.zeros(pages, G, 64))
     assert torch.equal(got, want) and torch.equal(got_w, want_w)
+
+
+@pytest.mark.parametrize("shape", [(8, 2, 64), (16, 16, 128), (28, 4, 128), (9, 1, 128)], ids=str)
+@pytest.mark.parametrize("runs,held,window", [([48], [3000], 0), ([300, 129, 0, 1], [900, 1500, 7, 2000], 0), ([200], [2500], 700), ([1000], [0], 0), ([60, 400], [1300, 13], 200)])
+def test_prompts_whose_keys_are_cut_into_pieces(shape, runs, held, window, monkeypatch):
+    """Few units of many keys: pieces joined by a second launch; held to what whole units are held to, the sums of weights among it."""
+    from turboquant_cpp_b200.kernels import cache8
+    H, G, D = shape
+    # four or six pages a piece, whatever the rule says of these sizes; a walk may begin inside a piece's first page
+    pages_of = 4 + 2 * (H % 8 == 0)
+    monkeypatch.setattr(cache8, "PROMPT_WORK", 0)
+    monkeypatch.setattr(cache8, "prefill_pieces", lambda *a: (-(-(max(n + h for n, h in zip(runs, held)) + 64) // (64 * pages_of)), pages_of))
+    table, pages = _pages([n + h for n, h in zip(runs, held)], 64)
+    codes, scales = _cache(pages, G, 64, D, spread=1.0)
+    q = (torch.randn(sum(runs), H, D) * 1.5).to(torch.bfloat16)
+    scale = 1.0 / math.sqrt(D) / 4
+    weights = torch.rand(pages, G, 64)
+    want, mags, units, p = plain.attention(q, codes, scales, runs, held, table, 64, window, scale, H, G, D)
+    want_w = weights.double()
+    plain.add_weights(want_w, p, runs, held, table, 64, H, G)
+    got, got_w = _attend(q, codes, scales, runs, held, table, 64, window, scale, H, G, D, weights)
+    places = max(n + h for n, h in zip(runs, held))
+    top = float((codes.view(torch.float8_e4m3fn).float().abs() * torch.pow(2.0, scales.float() - 127).repeat_interleave(16, -1)[..., None]).max())
+    limit = _limit(torch.bfloat16, want, mags, units, D, places, top)
+    off = (got.double().view(want.shape) - want).abs()
+    assert bool((off <= limit).all()), float((off / limit).max())
+    rel = float(2.02 * ((D + 8) * 4 * U * units).max()) + (places + H // G * max(runs) + 16) * 4 * U
+    assert bool(((got_w.double() - want_w).abs() <= rel * want_w.abs() + 1e-30).all())

@@ -68,15 +68,20 @@ struct Shape {
                                                            // map_r, whose columns begin at r_col
     int table_stride, n_pages, window, keep_first, cell, far;
     float scale, softcap;
+    int splits, chunk, rows;                               // units cut along the keys: how many at most, pages of each (even), rows of q
 };
 enum { PAIR_HEADS, PAIR_ROWS };
 
 // Two tiles of 128 consecutive query tokens of one sequence, each of one query head.
-struct Unit { int seq, g, p0, first, kept, n_pages, n_tiles, h[2], t0[2], rows[2], p_first[2], n[2]; bool valid; };
+struct Unit { int seq, g, p0, first, kept, n_pages, n_tiles, h[2], t0[2], rows[2], p_first[2], n[2], split; bool valid, cut[2]; };
 
-// The query tile is the slowest index, last tiles (which see the most keys) first.
+// The query tile is the slowest index, last tiles (which see the most keys) first.  SPLIT: units whose keys are cut into S.splits pieces of
+// S.chunk pages, the fastest index.
+template <bool SPLIT>
 __device__ __forceinline__ Unit unit_of(int unit, const Shape& S, const int* cu_seqlens, const int* seq_start) {
     Unit u;
+    u.split = SPLIT ? unit % S.splits : 0;
+    if (SPLIT) unit /= S.splits;
     const int hs = S.pairing == PAIR_HEADS ? S.nh / 2 : S.nh;
     const int per = S.n_seqs * hs, x = unit / per, rem = unit - x * per;
     u.seq = rem / hs;
@@ -105,15 +110,22 @@ __device__ __forceinline__ Unit unit_of(int unit, const Shape& S, const int* cu_
         u.t0[s] = t_begin + q * BM;
         u.rows[s] = min(BM, run - q * BM);
         u.p_first[s] = start + q * BM;
-        const int pages = u.kept + (u.p_first[s] + u.rows[s] - 1) / PAGE - u.first + 1;
+        int pages = u.kept + (u.p_first[s] + u.rows[s] - 1) / PAGE - u.first + 1;
+        u.cut[s] = SPLIT && pages > S.chunk;
+        if (SPLIT) pages = max(0, min(pages - u.split * S.chunk, S.chunk));
         u.n[s] = q < 0 || !u.valid ? 0 : (pages + 1) / 2;
         if (u.n[s]) u.n_pages = max(u.n_pages, pages);
     }
     u.n_tiles = max(u.n[0], u.n[1]);
+    if (SPLIT) u.valid = u.valid && u.n_tiles > 0;
     return u;
 }
 // the n-th page a unit walks
-__device__ __forceinline__ int page_at(const Unit& u, int n) { return n < u.kept ? n : u.first + n - u.kept; }
+template <bool SPLIT>
+__device__ __forceinline__ int page_at(const Unit& u, const Shape& S, int n) {
+    if (SPLIT) n += u.split * S.chunk;
+    return n < u.kept ? n : u.first + n - u.kept;
+}
 
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return tq_unpack2(tq_fma2(tq_pack2(a.x, a.y), tq_pack2(b.x, b.y), tq_pack2(c.x, c.y))); }
 __device__ __forceinline__ float2 mul2(float2 a, float2 b) { return tq_unpack2(tq_mul2(tq_pack2(a.x, a.y), tq_pack2(b.x, b.y))); }
@@ -182,14 +194,16 @@ __device__ __forceinline__ void cap_scores(uint32_t (&v)[32], const CapSeries& s
 // ROWS: the form of attention over rows.  Scores may pass through a cap and/or a bias per distance, and a row's largest weight is
 // exactly one at the end of each tile; the other form (plain and latent attention) takes plain scores and keeps a maximum until it is
 // outgrown by 2^8.
-template <int DK, int DV, bool ROWS>
+// SPLIT: results of tiles whose keys are cut go to part [split][rows of q][nh][DV] float32, divided by their own sum, and the base-2 logarithm
+// of that sum to part_lse [split][rows][nh], for attention_prefill_join_kernel.
+template <int DK, int DV, bool ROWS, bool SPLIT>
 __global__ void __launch_bounds__(THREADS, 1)
 attention_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                          const __grid_constant__ CUtensorMap map_r, const __grid_constant__ CUtensorMap map_v,
                          const __grid_constant__ Shape S, const int* __restrict__ cu_seqlens, const int* __restrict__ seq_start,
                          const int* __restrict__ page_table, const int* __restrict__ page_base,
                          const float* __restrict__ bias_t, const float* __restrict__ sink,
-                         __nv_bfloat16* __restrict__ out, float* __restrict__ lse, int* __restrict__ status) {
+                         __nv_bfloat16* __restrict__ out, float* __restrict__ lse, float* __restrict__ part, float* __restrict__ part_lse, int* __restrict__ status) {
     tq_grid_wait();                    // everything below may read what the previous kernel wrote
     using C = Cfg<DK, DV>;
     extern __shared__ uint8_t smem_raw[];
@@ -292,7 +306,7 @@ attention_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             };
             // from a block on, the first whose unit exists (a short run has none at a late tile)
             auto settle = [&](int unit) -> int {
-                while (ok && unit >= 0 && !unit_of(unit, S, cu_seqlens, seq_start).valid) { ask(); unit = answer(); }
+                while (ok && unit >= 0 && !unit_of<SPLIT>(unit, S, cu_seqlens, seq_start).valid) { ask(); unit = answer(); }
                 return ok ? unit : -1;
             };
             auto hand_on = [&](int k, int unit) {
@@ -307,7 +321,7 @@ attention_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             hand_on(0, unit);
             for (int k = 0; ok && unit >= 0; ++k) {
                 int following = -1;
-                const Unit u = unit_of(unit, S, cu_seqlens, seq_start);
+                const Unit u = unit_of<SPLIT>(unit, S, cu_seqlens, seq_start);
                 auto load_q = [&](int s) {
                     if (!u.n[s]) return true;
                     // the products that read the slot's previous Q must be done
@@ -329,7 +343,7 @@ attention_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                     const int np = min(2, u.n_pages - 2 * i);
                     int page[2] = {0, 0};
                     for (int pg = 0; pg < np; ++pg) {
-                        const int n = page_at(u, 2 * i + pg);
+                        const int n = page_at<SPLIT>(u, S, 2 * i + pg);
                         page[pg] = page_table != nullptr
                             ? TQ_CHECKED(page_table[(size_t)u.seq * S.table_stride + TQ_CHECKED(n, S.table_stride, TQ_IDX_TABLE_COLUMN)], S.n_pages, TQ_IDX_PAGE)
                             : page_base[u.seq] + n;
@@ -387,7 +401,7 @@ attention_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             auto wait = [&](uint32_t bar, uint32_t parity) { return (bool)__all_sync(0xffffffffu, mbar_wait(bar, parity, &s_abort)); };
             auto next_unit = [&](Unit& u) {
                 const int unit = take_unit(taken++);
-                if (unit >= 0) u = unit_of(unit, S, cu_seqlens, seq_start);
+                if (unit >= 0) u = unit_of<SPLIT>(unit, S, cu_seqlens, seq_start);
                 return unit >= 0;
             };
             const uint64_t q_desc = desc_k_major(q_smem(0)), k_desc = desc_k_major(k_smem(0)), v_desc = desc_mn_major(v_smem(0), BN * 128);
@@ -462,7 +476,7 @@ attention_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         int tiles = 0, units = 0, taken = 0;
         bool ok = true;
         for (int unit = take_unit(taken++); ok && unit >= 0; unit = ok ? take_unit(taken++) : -1) {
-            const Unit u = unit_of(unit, S, cu_seqlens, seq_start);
+            const Unit u = unit_of<SPLIT>(unit, S, cu_seqlens, seq_start);
             const int n = u.n[slot];
             if (n == 0) continue;
             const int h = u.h[slot], p_first = u.p_first[slot], qpos = p_first + r, p_last = p_first + BM - 1;
@@ -475,7 +489,7 @@ attention_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             auto fetch_bias = [&](int i) {
 #pragma unroll
                 for (int j = 0; j < 6; ++j) {
-                    const int d = p_first + quarter * 32 - page_at(u, 2 * i + j / 3) * PAGE - (PAGE - 1) + (j % 3) * 32 + lane;
+                    const int d = p_first + quarter * 32 - page_at<SPLIT>(u, S, 2 * i + j / 3) * PAGE - (PAGE - 1) + (j % 3) * 32 + lane;
                     nb[j] = __ldg(bias + min(max(d, 0), S.far));
                 }
             };
@@ -533,7 +547,7 @@ attention_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
 #pragma unroll
                     for (int w = 0; w < CW; ++w) tmem_ld32(s_addr + (q + w) * 32, sv[w]);
                     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                    const int kq = page_at(u, 2 * i + (q >> 1)) * PAGE + (q & 1) * 32;   // position of the first of these keys
+                    const int kq = page_at<SPLIT>(u, S, 2 * i + (q >> 1)) * PAGE + (q & 1) * 32;   // position of the first of these keys
                     if (ROWS && x < 0) {
                         if (capped) cap_scores(sv[0], series);
                         if (bias != nullptr) {
@@ -601,15 +615,24 @@ attention_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             if (!ok) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             if (sink != nullptr) l += ex2((floor_m - m) * to_log2);
-            const float inv = 1.0f / l;
-            if (lse != nullptr && r < u.rows[slot]) lse[(size_t)(u.t0[slot] + r) * S.nh + h] = m * to_log2 + log2f(l);
+            const bool cut = SPLIT && u.cut[slot];
+            const float inv = SPLIT && l == 0.f ? 0.f : 1.0f / l;                    // (a row may see none of a split's keys)
+            const size_t piece = SPLIT ? ((size_t)u.split * S.rows + u.t0[slot] + r) * S.nh + h : 0;
+            if (cut && r < u.rows[slot]) part_lse[piece] = l == 0.f ? -INFINITY : m * to_log2 + log2f(l);
+            if (!cut && lse != nullptr && r < u.rows[slot]) lse[(size_t)(u.t0[slot] + r) * S.nh + h] = m * to_log2 + log2f(l);
             __nv_bfloat16* dst = out + ((size_t)(u.t0[slot] + r) * S.nh + h) * DV;
 #pragma unroll 1
             for (int c0 = 0; c0 < DV; c0 += 32) {
                 uint32_t ov[32];
                 tmem_ld32(acc + c0, ov);               // every lane takes part: the load is warp-wide
                 asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                if (r < u.rows[slot]) {
+                if (cut && r < u.rows[slot]) {
+#pragma unroll
+                    for (int d = 0; d < 32; d += 4)
+                        *reinterpret_cast<float4*>(part + piece * DV + c0 + d) = make_float4(__uint_as_float(ov[d]) * inv, __uint_as_float(ov[d + 1]) * inv,
+                                                                                 __uint_as_float(ov[d + 2]) * inv, __uint_as_float(ov[d + 3]) * inv);
+                }
+                if (!cut && r < u.rows[slot]) {
 #pragma unroll
                     for (int d = 0; d < 32; d += 8) {
                         uint32_t packed[4];
@@ -637,27 +660,69 @@ attention_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     if (threadIdx.x == 0 && s_abort) atomicExch(status, 1);
 }
 
+// The splits of a row joined (rows whose tile's keys were not cut are done): a block per row of a run, a warp per head.
+template <int DV>
+__global__ void __launch_bounds__(256) attention_prefill_join_kernel(const __grid_constant__ Shape S, const int* __restrict__ cu_seqlens, const int* __restrict__ seq_start,
+                                                                     const float* __restrict__ part, const float* __restrict__ part_lse,
+                                                                     __nv_bfloat16* __restrict__ out, float* __restrict__ lse) {
+    tq_grid_wait();                    // everything below may read what the previous kernel wrote
+    tq_grid_launch_dependents();
+    const int r = blockIdx.x, seq = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int t_begin = cu_seqlens[seq], run = cu_seqlens[seq + 1] - t_begin, start = seq_start[seq];
+    if (r >= run) return;
+    // the splits that hold keys of the row's tile, as unit_of counts them
+    const int tile = r / BM, first_tile = S.pairing == PAIR_HEADS ? tile : tile & ~1;
+    const int first = S.window > 0 ? max(0, start + first_tile * BM + 1 - S.window) / PAGE : 0;
+    const int pages = (start + min(run, (tile + 1) * BM) - 1) / PAGE - first + 1, n = (pages + S.chunk - 1) / S.chunk;
+    if (n <= 1) return;
+    for (int h = warp; h < S.nh; h += 8) {
+        const size_t at = (size_t)(t_begin + r) * S.nh + h, step = (size_t)S.rows * S.nh;
+        float top = -INFINITY, sum = 0.f, o[DV / 32] = {};
+        for (int x = 0; x < n; ++x) top = fmaxf(top, part_lse[x * step + at]);
+        for (int x = 0; x < n; ++x) {
+            const float w = ex2(part_lse[x * step + at] - top);
+            sum += w;
+            const float* p = part + (x * step + at) * DV + lane * (DV / 32);
+            if (DV == 128) {
+                const float4 v = *reinterpret_cast<const float4*>(p);
+                o[0] += w * v.x; o[1] += w * v.y; o[2 % (DV / 32)] += w * v.z; o[3 % (DV / 32)] += w * v.w;
+            } else {
+                const float2 v = *reinterpret_cast<const float2*>(p);
+                o[0] += w * v.x; o[1] += w * v.y;
+            }
+        }
+        const float inv = 1.0f / sum;
+        __nv_bfloat162 two[DV / 64];
+#pragma unroll
+        for (int e = 0; e < DV / 64; ++e) two[e] = __floats2bfloat162_rn(o[2 * e] * inv, o[2 * e + 1] * inv);
+        __nv_bfloat16* d = out + at * DV + lane * (DV / 32);
+        if (DV == 128) *reinterpret_cast<uint2*>(d) = *reinterpret_cast<const uint2*>(two);
+        else *reinterpret_cast<uint32_t*>(d) = *reinterpret_cast<const uint32_t*>(two);
+        if (lse != nullptr && lane == 0) lse[at] = top + log2f(sum);
+    }
+}
+
 struct Maps { CUtensorMap q, k, r, v; };
 struct Args {
     const int *cu, *starts, *table, *page_base;
     const float *bias_t, *sink;
     void* out;
-    float* lse;
+    float *lse, *part, *part_lse;
     int* status;
 };
 
-template <int DK, int DV, bool ROWS>
+template <int DK, int DV, bool ROWS, bool SPLIT = false>
 int launch(const Maps& m, const Shape& S, const Args& a, cudaStream_t stream) {
     using C = Cfg<DK, DV>;
-    auto kern = attention_prefill_kernel<DK, DV, ROWS>;
+    auto kern = attention_prefill_kernel<DK, DV, ROWS, SPLIT>;
     static std::atomic<unsigned long long> asked{0};
     const cudaError_t e = tq_reserve_smem(kern, C::SMEM_BYTES, asked);
     if (e != cudaSuccess) TQ_FAIL(-1, "attention_prefill: cannot reserve %d bytes of shared memory: %s", C::SMEM_BYTES, cudaGetErrorString(e));
     // a block per unit; those that run take over the ones that have not started
     const int hs = S.pairing == PAIR_HEADS ? S.nh / 2 : S.nh, qs = S.pairing == PAIR_HEADS ? S.n_qt : (S.n_qt + 1) / 2;
-    const int grid = qs * S.n_seqs * hs;
+    const int grid = qs * S.n_seqs * hs * (SPLIT ? S.splits : 1);
     tq_launch(grid, THREADS, C::SMEM_BYTES, stream)(kern, m.q, m.k, m.r, m.v, S, a.cu, a.starts, a.table, a.page_base, a.bias_t, a.sink,
-                                                   (__nv_bfloat16*)a.out, a.lse, a.status);
+                                                   (__nv_bfloat16*)a.out, a.lse, a.part, a.part_lse, a.status);
     TQ_CHECK_LAUNCH("attention_prefill");
     return 0;
 }
@@ -704,12 +769,47 @@ TQ_EXPORT int tq_attention_prefill(const void* q, const void* cache, int planes,
     rc = make_map(&m.k, cache, (uint64_t)n_pages * S.kp, (uint64_t)(planes == 1 ? dk + dv : dk), PAGE);
     if (rc) return rc;
     m.r = m.v = m.k;
-    const Args a{cu_seqlens, seq_start, page_table, nullptr, bias_t, sink, out, lse, status};
+    const Args a{cu_seqlens, seq_start, page_table, nullptr, bias_t, sink, out, lse, nullptr, nullptr, status};
     const bool shaped = planes == 1 || softcap > 0.f || bias_t != nullptr || !(scale > 0.f);     // (the other form compares unscaled scores)
 #define AP_CASE(DK_, DV_) if (dk == DK_ && dv == DV_) return shaped ? launch<DK_, DV_, true>(m, S, a, stream) : launch<DK_, DV_, false>(m, S, a, stream);
     AP_CASE(64, 64) AP_CASE(64, 128) AP_CASE(128, 64) AP_CASE(128, 128)
 #undef AP_CASE
     return -2;
+}
+
+// The same for plain scores (two planes, keys and values of one size, scale > 0) with every unit's keys cut into pieces of `chunk` pages (even),
+// at most `splits` of them: for steps whose longest unit would keep the device waiting.  part [splits, T, nh, dk] and part_lse [splits, T,
+// nh] float32 are scratch; a second launch joins.
+TQ_EXPORT int tq_attention_prefill_split(const void* q, const void* cache, const int* cu_seqlens, const int* seq_start, const int* page_table, int table_stride,
+                                         int page_size, int n_pages, int window, float scale, void* out, float* lse, float* part, float* part_lse,
+                                         int splits, int chunk, int T_, int n_seqs, int max_q_len, int nh, int nkv, int dk, int* status, cudaStream_t stream) {
+    if (T_ == 0 || n_seqs == 0) return 0;
+    TQ_REQUIRE(dk == 64 || dk == 128, "attention_prefill: key size %d is not 64 or 128", dk);
+    TQ_REQUIRE(page_size == PAGE, "attention_prefill: page size %d must be %d", page_size, PAGE);
+    TQ_REQUIRE(splits >= 1 && chunk >= 2 && chunk % 2 == 0 && scale > 0.f && part != nullptr && part_lse != nullptr, "attention_prefill: %d pieces of %d pages, scale %g",
+               splits, chunk, scale);
+    TQ_REQUIRE(n_seqs <= 65535 && (uintptr_t)part % 16 == 0, "attention_prefill: %d sequences", n_seqs);
+    Shape S{};
+    S.nh = nh; S.nkv = nkv; S.n_seqs = n_seqs; S.n_qt = (max_q_len + BM - 1) / BM;
+    S.kp = 2 * nkv * PAGE; S.kg = PAGE; S.v_plane = nkv * PAGE; S.k_blocks = dk / 64;
+    S.table_stride = table_stride; S.n_pages = n_pages; S.window = window; S.scale = scale;
+    S.splits = splits; S.chunk = chunk; S.rows = T_;
+    int rc = check_common(S, T_, max_q_len, q, cache, cache, out, status);
+    if (rc) return rc;
+    TQ_REQUIRE((long long)S.n_qt * n_seqs * nh * splits < (1ll << 30) && (long long)n_pages * S.kp < (1ll << 31), "attention_prefill: too many units of work or pages");
+    S.pairing = nh / nkv % 2 == 0 ? PAIR_HEADS : PAIR_ROWS;
+    Maps m;
+    rc = make_map(&m.q, q, (uint64_t)T_, (uint64_t)nh * dk, BM);
+    if (!rc) rc = make_map(&m.k, cache, (uint64_t)n_pages * S.kp, (uint64_t)dk, PAGE);
+    if (rc) return rc;
+    m.r = m.v = m.k;
+    const Args a{cu_seqlens, seq_start, page_table, nullptr, nullptr, nullptr, out, lse, part, part_lse, status};
+    rc = dk == 64 ? launch<64, 64, false, true>(m, S, a, stream) : launch<128, 128, false, true>(m, S, a, stream);
+    if (rc) return rc;
+    auto join = dk == 64 ? attention_prefill_join_kernel<64> : attention_prefill_join_kernel<128>;
+    tq_launch(dim3(max_q_len, n_seqs), 256, 0, stream)(join, S, cu_seqlens, seq_start, part, part_lse, (__nv_bfloat16*)out, lse);
+    TQ_CHECK_LAUNCH("attention_prefill_join");
+    return 0;
 }
 
 // The same over keys and values that lie densely: kv [rows, nh * (dim + dv)] bf16, a position's keys of all heads, then its
@@ -740,7 +840,7 @@ TQ_EXPORT int tq_attention_prefill_dense(const void* q, const void* kv, const vo
     m.r = m.v = m.k;
     if (rot) rc = make_map(&m.r, rot_rows, (uint64_t)rows, (uint64_t)rot_stride, PAGE);
     if (rc) return rc;
-    const Args a{cu_seqlens, seq_start, nullptr, page_base, nullptr, sink, out, nullptr, status};
+    const Args a{cu_seqlens, seq_start, nullptr, page_base, nullptr, sink, out, nullptr, nullptr, nullptr, status};
 #define AP_CASE(DK_, DV_) if (dk == DK_ && dv == DV_) return launch<DK_, DV_, false>(m, S, a, stream);
     AP_CASE(64, 64) AP_CASE(64, 128) AP_CASE(128, 64) AP_CASE(128, 128) AP_CASE(192, 128)
 #undef AP_CASE

@@ -85,11 +85,11 @@ struct WriteArgs {
     int nh, pairing, written;          // written: the heads this launch takes (the queries alone, or all)
 };
 
-constexpr int WRITE_THREADS = 512;
+constexpr int WRITE_THREADS = 256;      // (512: 35 us for the prompts above, 31.5; five blocks an SM instead of four: 29.8)
 
 // HD: the head size, or 0 where it is known at the launch only
 template <typename TA, typename TB, bool RUNS, int HD>
-__global__ void __launch_bounds__(WRITE_THREADS) write8_kernel(const TA* __restrict__ qkv, const TB* __restrict__ bias, WriteArgs a, TA* __restrict__ q_out, Cache8 c,
+__global__ void __launch_bounds__(WRITE_THREADS, RUNS && HD ? 5 : 1) write8_kernel(const TA* __restrict__ qkv, const TB* __restrict__ bias, WriteArgs a, TA* __restrict__ q_out, Cache8 c,
                                                                int threads_) {
     tq_grid_wait();                    // everything below may read what the previous kernel wrote
     tq_grid_launch_dependents();

@@ -243,6 +243,44 @@ def prefill_rows(q: torch.Tensor, cache_layer: torch.Tensor, planes: int, cu_seq
     return out
 
 
+SPLIT_MIN_TILES, SPLIT_FROM = 4, 16      # a piece of a unit's keys has at least this many tiles of 128, a unit that is cut this many
+SPLIT_BYTES = 1 << 28        # scratch a step may take for the pieces' results
+
+
+def prefill_pieces(n_tokens: int, n_seqs: int, max_q_len: int, max_kv_len: int, n_heads: int, n_kv_heads: int, head_dim: int, window: int, sms: int):
+    """(pieces, pages of each) into which the tensor-core prompt kernel's units (two query tiles that walk the same keys) are cut along the keys, or
+    (1, 0).  They are cut where the device takes two pieces of every unit and more at once: a short run behind a long history.  (B200,
+    16 heads of 128, 500 rows behind 3,500, 32 units: 92 us whole, 55 in pieces; 300 behind 2,000, 28 heads on 4: 56 and 52.  Where there are more pieces than SMs,
+    or a row's results in float32 for every piece, written and read, weigh as much as what is saved, it does not pay: 2,048 rows, 128 units, 53 us whole, 56 cut;
+    1,000 rows, 64 units of at most 8 tiles, 34 and 37.)"""
+    tiles = -(-max_q_len // 128)
+    units, own = (n_heads // 2 * tiles, 1) if n_heads // n_kv_heads % 2 == 0 else (n_heads * -(-tiles // 2), 2)
+    most = sms // (units * n_seqs)
+    longest = min(max_kv_len, window + own * 128) if window > 0 else max_kv_len
+    steps = -(-longest // 128) + 1                     # tiles of 128 keys; a walk may begin inside one
+    piece = max(SPLIT_MIN_TILES, -(-steps // max(most, 1)))
+    pieces = -(-steps // piece)
+    if most < 2 or steps < SPLIT_FROM or 4 * pieces * n_tokens * n_heads * (head_dim + 1) > SPLIT_BYTES:
+        return 1, 0
+    return pieces, 2 * piece
+
+
+def prefill_split(q: torch.Tensor, cache_layer: torch.Tensor, cu_seqlens: torch.Tensor, seq_start: torch.Tensor, page_table: torch.Tensor, page_size: int,
+                  window: int, scale: float, out: torch.Tensor, n_seqs: int, max_q_len: int, n_heads: int, n_kv_heads: int, head_dim: int, pieces: int, pages: int,
+                  status: torch.Tensor, lse: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """attention_prefill with every unit's keys cut into `pieces` of `pages` pages (prefill_pieces), joined by a second launch."""
+    T = q.shape[0]
+    if any(t.dtype != torch.bfloat16 for t in (q, cache_layer, out)) or any(t.dtype != torch.int32 for t in (cu_seqlens, seq_start, page_table)):
+        raise KernelError("attention_prefill: queries, cache and output must be bfloat16, cu_seqlens, seq_start and the page table int32")
+    scratch = torch.empty(pieces * T * n_heads * (head_dim + 1), dtype=torch.float32, device=q.device)
+    part, part_lse = scratch[:pieces * T * n_heads * head_dim], scratch[pieces * T * n_heads * head_dim:]
+    check("attention_prefill", load_kernel("attention_prefill").tq_attention_prefill_split(
+        ptr(q), ptr(cache_layer), ptr(cu_seqlens), ptr(seq_start), ptr(page_table), page_table.shape[1], *ints(page_size, cache_layer.shape[0], window),
+        c_float(scale), ptr(out), ptr(lse), ptr(part), ptr(part_lse), *ints(pieces, pages, T, n_seqs, max_q_len, n_heads, n_kv_heads, head_dim), ptr(status),
+        stream()), kernels=2)
+    return out
+
+
 def dense_usable(dtype: torch.dtype, dim: int, rot: int, vdim: int, page_size: int) -> bool:
     """Whether the tensor-core prompt kernel takes keys of dim + rot elements (the last rot shared by the heads) and values
     of vdim that lie densely."""

@@ -23,7 +23,7 @@ import torch
 
 from ..csrc.build import load_kernel
 from ._call import KernelError, addresses, check, code, declared, want_f32, want_int32
-from .attention import PAIRING, prefill_rows, prefill_usable, resident_ctas
+from .attention import PAIRING, prefill_pieces, prefill_rows, prefill_split, prefill_usable, resident_ctas
 from .gemm_tc import status_word
 
 BLOCK = 16
@@ -173,7 +173,7 @@ def attention8(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, cu_se
     if T == 0 or n == 0 or max_q_len < 1:
         return out
     max_q_len, max_kv_len = index(max_q_len), index(max_kv_len)
-    if max_q_len >= PROMPT_MIN_RUN and prefill_usable(q.dtype, head_dim, page_size):
+    if max_q_len >= PROMPT_MIN_RUN and prefill_usable(q.dtype, head_dim, page_size) and T * (max_kv_len - max_q_len // 2) * n_heads * head_dim >= PROMPT_WORK:
         return _attention8_prompt(q, codes, scales, cu_seqlens, held, page_table, page_size, window, scale, out, n_heads, n_kv_heads, head_dim,
                                   max_q_len, max_kv_len, weights, status)
     p_q, p_out, p_codes, p_scales, p_cu, p_held, p_table, p_weights, at = addresses(q, out, codes, scales, cu_seqlens, held, page_table, weights)
@@ -215,7 +215,11 @@ def attention8(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, cu_se
     return out
 
 
-PROMPT_MIN_RUN = 48          # steps whose longest run is at least this go to the tensor-core prompt kernel, where it takes their sizes
+# Steps whose longest run is at least this, and whose queries, heads, elements and the keys they see multiply to this much, go to the tensor-core
+# prompt kernel, where it takes their sizes.  (B200, us, csrc/attention8.cu and the prompt kernel's five launches: 128 rows behind 800, 16
+# heads of 128, 0.2e9: 22 and 31; 28 heads on 4, 0.4e9: 45 and 31; 64 behind 4,000, 16 heads, 0.5e9: 31 and 38; 128 behind 4,000, 1.1e9: 48 and 41;
+# 256 behind 4,000, 2.2e9: 130 and 46.)
+PROMPT_MIN_RUN, PROMPT_WORK = 48, 350_000_000
 DENSE_BYTES = 1 << 30        # scratch a step may take for pages in bfloat16; sequences beyond it follow in further launches
 
 
@@ -235,13 +239,19 @@ def _attention8_prompt(q, codes, scales, cu_seqlens, held, page_table, page_size
     p_q, p_out, p_codes, p_scales, p_dense, p_tables, p_lost, p_lse, p_weights, p_status, at = addresses(
         q, out, codes, scales, dense, table, lost, lse, weights, status)
     pages = codes.shape[0]
+    pieces, piece_pages = prefill_pieces(T, min(group, n), max_q_len, max_kv_len, n_heads, n_kv_heads, head_dim, window, resident_ctas(q.device) // 4) \
+        if scale > 0.0 else (1, 0)
     for i in range(0, n, group):
         m = min(group, n - i)
         cu, starts, own_pages = cu_seqlens[i:i + m + 1], held[i:i + m], page_table[i:i + m]
         p_cu, p_held, p_table, _ = addresses(cu, starts, own_pages)
         cache = (p_codes, p_scales, p_cu, p_held, p_table, page_table.shape[1], page_size, window)
         check("prompt8", _prompt8("tq_expand8")(*cache, p_dense, p_tables, p_lost, width, pages, m, n_kv_heads, head_dim, at))
-        prefill_rows(q, dense, 2, cu, starts, table[:m], page_size, window, scale, out, m, max_q_len, n_heads, n_kv_heads, head_dim, head_dim, status=status, lse=lse)
+        if pieces > 1:
+            prefill_split(q, dense, cu, starts, table[:m], page_size, window, scale, out, m, max_q_len, n_heads, n_kv_heads, head_dim, pieces, piece_pages,
+                          status, lse=lse)
+        else:
+            prefill_rows(q, dense, 2, cu, starts, table[:m], page_size, window, scale, out, m, max_q_len, n_heads, n_kv_heads, head_dim, head_dim, status=status, lse=lse)
         check("attention8", _attention8("tq_repair8")(p_q, *cache, scale, p_out, p_lost, width, pages, m, n_heads, n_kv_heads, head_dim, at))
         if weights is not None:
             check("prompt8", _prompt8("tq_weigh8_prompt")(
