@@ -22,7 +22,7 @@ from typing import Optional, Tuple
 import torch
 
 from ..csrc.build import load_kernel
-from ._call import KernelError, addresses, check, code, declared, want_f32, want_int32
+from ._call import KernelError, addresses, check, code, declared, want_int32
 from .attention import PAIRING, prefill_pieces, prefill_rows, prefill_split, prefill_usable, resident_ctas
 from .gemm_tc import status_word
 
@@ -76,29 +76,35 @@ def check_sizes(page_size: int, head_dim: int) -> None:
         raise KernelError(f"the 8-bit cache takes pages of a multiple of {BLOCK} rows; got {page_size}")
 
 
-def _check_cache(codes, scales, weights, page_table, page_size, n_kv_heads, head_dim) -> None:
-    pages = codes.shape[0]
-    if codes.dtype != torch.float8_e4m3fn or codes.shape != (pages, 2, n_kv_heads, page_size, head_dim):
-        raise KernelError(f"8-bit cache: codes must be float8_e4m3fn [pages, 2, {n_kv_heads}, {page_size}, {head_dim}], got {codes.dtype} {tuple(codes.shape)}")
-    if scales.dtype != torch.uint8 or scales.shape != (pages, 2, n_kv_heads, page_size // BLOCK):
+_E4M3, _U8, _F32, _I32 = torch.float8_e4m3fn, torch.uint8, torch.float32, torch.int32
+
+
+def _sizes(codes, scales, weights, page_table, page_size: int, n_kv_heads: int, head_dim: int) -> Tuple[int, int, int]:
+    """(pages, sequences, pages of a table) of a cache that fits together."""
+    shape, table = codes.shape, page_table.shape
+    pages = shape[0]
+    if (shape == (pages, 2, n_kv_heads, page_size, head_dim) and codes.dtype is _E4M3 and scales.dtype is _U8
+            and scales.shape == (pages, 2, n_kv_heads, page_size // BLOCK) and len(table) == 2 and page_table.dtype is _I32 and table[1] > 0
+            and (weights is None or (weights.dtype is _F32 and weights.shape == (pages, n_kv_heads, page_size)))):
+        return pages, table[0], table[1]
+    if codes.dtype is not _E4M3 or shape != (pages, 2, n_kv_heads, page_size, head_dim):
+        raise KernelError(f"8-bit cache: codes must be float8_e4m3fn [pages, 2, {n_kv_heads}, {page_size}, {head_dim}], got {codes.dtype} {tuple(shape)}")
+    if scales.dtype is not _U8 or scales.shape != (pages, 2, n_kv_heads, page_size // BLOCK):
         raise KernelError(f"8-bit cache: scales must be uint8 [{pages}, 2, {n_kv_heads}, {page_size // BLOCK}], got {scales.dtype} {tuple(scales.shape)}")
-    if weights is not None and (weights.dtype != torch.float32 or weights.shape != (pages, n_kv_heads, page_size)):
+    if weights is not None and (weights.dtype is not _F32 or weights.shape != (pages, n_kv_heads, page_size)):
         raise KernelError(f"8-bit cache: weights must be float32 [{pages}, {n_kv_heads}, {page_size}], got {weights.dtype} {tuple(weights.shape)}")
-    _check_table(page_table)
+    raise _bad_table(page_table)
 
 
-def _check_table(page_table) -> None:
-    if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[1] < 1:
-        raise KernelError(f"8-bit cache: the page table must be int32 [sequences, pages], got {page_table.dtype} {tuple(page_table.shape)}")
+def _bad_table(page_table) -> KernelError:
+    return KernelError(f"8-bit cache: the page table must be int32 [sequences, pages], got {page_table.dtype} {tuple(page_table.shape)}")
 
 
-def _check_step(cu_seqlens, held, page_table, what: str) -> int:
-    n = page_table.shape[0]
-    want_int32(cu_seqlens, "cu_seqlens")
-    want_int32(held, "held")
-    if cu_seqlens.numel() != n + 1 or held.numel() != n:
+def _check_step(cu_seqlens, held, n: int, what: str) -> None:
+    if not (cu_seqlens.dtype is _I32 and held.dtype is _I32 and cu_seqlens.numel() == n + 1 and held.numel() == n):
+        want_int32(cu_seqlens, "cu_seqlens")
+        want_int32(held, "held")
         raise KernelError(f"{what}: {n} page tables, {held.numel()} counts of held rows and {cu_seqlens.numel()} run borders do not fit together")
-    return n
 
 
 def write_rows8(qkv: torch.Tensor, bias: Optional[torch.Tensor], cos: Optional[torch.Tensor], sin: Optional[torch.Tensor], pairing: str,
@@ -108,33 +114,34 @@ def write_rows8(qkv: torch.Tensor, bias: Optional[torch.Tensor], cos: Optional[t
     """Bias and rotary encoding (by positions [T]; cos and sin [positions, head_dim / 2] float32 or None) on the fused projection qkv
     [T, (nh + 2 nkv) * hd]; queries to q_out [T, nh, hd], keys and values as codes to their places (codes and scales None: the queries
     only, for layers that read another layer's cache).  max_q_len: the longest run."""
-    T = qkv.shape[0]
-    if (codes is None) != (scales is None):
-        raise KernelError("write_rows8: codes and scales come together")
-    if codes is None:
+    T, columns = qkv.shape
+    if codes is None or scales is None:
+        if codes is not None or scales is not None:
+            raise KernelError("write_rows8: codes and scales come together")
         check_sizes(page_size, head_dim)
-        _check_table(page_table)
+        if page_table.dtype is not _I32 or page_table.dim() != 2 or page_table.shape[1] < 1:
+            raise _bad_table(page_table)
+        pages, (n, width) = 0, page_table.shape
     else:
-        _check_cache(codes, scales, None, page_table, page_size, n_kv_heads, head_dim)
-    n = _check_step(cu_seqlens, held, page_table, "write_rows8")
-    want_int32(positions, "positions")
-    if qkv.shape[1] != (n_heads + 2 * n_kv_heads) * head_dim or q_out.numel() != T * n_heads * head_dim or positions.numel() != T or q_out.dtype != qkv.dtype \
-            or (bias is not None and bias.numel() != qkv.shape[1]):
-        raise KernelError(f"write_rows8: projection {tuple(qkv.shape)} {qkv.dtype}, queries {tuple(q_out.shape)} {q_out.dtype} and {positions.numel()} positions do not fit together")
-    if (cos is None) != (sin is None):
-        raise KernelError("write_rows8: cos and sin tables come together")
-    if cos is not None:
-        want_f32(cos, "cos table")
-        want_f32(sin, "sin table")
-        if cos.shape[-1] != head_dim // 2 or cos.shape != sin.shape:
-            raise KernelError(f"write_rows8: cos and sin tables must be [positions, {head_dim // 2}]")
+        pages, n, width = _sizes(codes, scales, None, page_table, page_size, n_kv_heads, head_dim)
+    _check_step(cu_seqlens, held, n, "write_rows8")
+    dtype = qkv.dtype
+    if columns != (n_heads + 2 * n_kv_heads) * head_dim or q_out.numel() != T * n_heads * head_dim or q_out.dtype is not dtype \
+            or positions.numel() != T or positions.dtype is not _I32 or (bias is not None and bias.numel() != columns):
+        want_int32(positions, "positions")
+        raise KernelError(f"write_rows8: projection {tuple(qkv.shape)} {dtype}, queries {tuple(q_out.shape)} {q_out.dtype} and {positions.numel()} positions do not fit together")
+    if cos is not None or sin is not None:
+        if cos is None or sin is None:
+            raise KernelError("write_rows8: cos and sin tables come together")
+        if cos.dtype is not _F32 or sin.dtype is not _F32 or cos.shape != sin.shape or cos.shape[-1] != head_dim // 2:
+            raise KernelError(f"write_rows8: cos and sin tables must be float32 [positions, {head_dim // 2}]")
     if T == 0:
         return
     p_qkv, p_bias, p_cos, p_sin, p_positions, p_cu, p_held, p_table, p_q, p_codes, p_scales, at = addresses(
         qkv, bias, cos, sin, positions, cu_seqlens, held, page_table, q_out, codes, scales)
     check("cache8", _cache8("tq_write8")(
-        p_qkv, code(qkv.dtype), p_bias, 0 if bias is None else code(bias.dtype), p_cos, p_sin, PAIRING[pairing], p_positions, p_cu, p_held, p_table,
-        page_table.shape[1], page_size, p_q, p_codes, p_scales, 0 if codes is None else codes.shape[0], n, index(max_q_len), n_heads, n_kv_heads, head_dim, at))
+        p_qkv, code(dtype), p_bias, 0 if bias is None else code(bias.dtype), p_cos, p_sin, PAIRING[pairing], p_positions, p_cu, p_held, p_table,
+        width, page_size, p_q, p_codes, p_scales, pages, n, max_q_len, n_heads, n_kv_heads, head_dim, at))
 
 
 MAX_RANGES, CLUSTER = 64, 8
@@ -152,6 +159,17 @@ def ranges_for(tiles: int, blocks: int, resident: int) -> int:
     return min((n for n in (1, 2, 3, 4, 5, 6, 7, 8, 12, 16, 24, 32, 48, most) if n <= most), key=lambda n: (turns(n), n))
 
 
+_multiprocessors = {}
+
+
+def _sms(t: torch.Tensor) -> int:
+    """SMs of a tensor's device."""
+    i = t.get_device()
+    if i not in _multiprocessors:
+        _multiprocessors[i] = resident_ctas(t.device) // 4
+    return _multiprocessors[i]
+
+
 SCORE_BYTES = 1 << 28        # scratch a decode step may take for scores
 
 
@@ -165,15 +183,16 @@ def attention8(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, cu_se
     weights: the softmax weights that each cached row receives from the step's rows, summed over a key/value head's query heads, are
     added to its sum; the sums of the step's own rows start with this step.
     status: the word in which the prompt kernel reports a wait that ran out (default: the device's, kernels.gemm_tc)."""
-    T = q.shape[0]
-    _check_cache(codes, scales, weights, page_table, page_size, n_kv_heads, head_dim)
-    n = _check_step(cu_seqlens, held, page_table, "attention8")
-    if q.numel() != T * n_heads * head_dim or out.numel() != q.numel() or out.dtype != q.dtype:
-        raise KernelError(f"attention8: queries {tuple(q.shape)} {q.dtype} and output {tuple(out.shape)} {out.dtype} do not fit {n_heads} heads of {head_dim}")
+    T, dtype = q.shape[0], q.dtype
+    pages, n, width = _sizes(codes, scales, weights, page_table, page_size, n_kv_heads, head_dim)
+    _check_step(cu_seqlens, held, n, "attention8")
+    elements = T * n_heads * head_dim
+    if q.numel() != elements or out.numel() != elements or out.dtype is not dtype:
+        raise KernelError(f"attention8: queries {tuple(q.shape)} {dtype} and output {tuple(out.shape)} {out.dtype} do not fit {n_heads} heads of {head_dim}")
     if T == 0 or n == 0 or max_q_len < 1:
         return out
     max_q_len, max_kv_len = index(max_q_len), index(max_kv_len)
-    if max_q_len >= PROMPT_MIN_RUN and prefill_usable(q.dtype, head_dim, page_size) and T * (max_kv_len - max_q_len // 2) * n_heads * head_dim >= PROMPT_WORK:
+    if max_q_len >= PROMPT_MIN_RUN and prefill_usable(dtype, head_dim, page_size) and T * (max_kv_len - max_q_len // 2) * n_heads * head_dim >= PROMPT_WORK:
         return _attention8_prompt(q, codes, scales, cu_seqlens, held, page_table, page_size, window, scale, out, n_heads, n_kv_heads, head_dim,
                                   max_q_len, max_kv_len, weights, status)
     p_q, p_out, p_codes, p_scales, p_cu, p_held, p_table, p_weights, at = addresses(q, out, codes, scales, cu_seqlens, held, page_table, weights)
@@ -183,7 +202,7 @@ def attention8(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, cu_se
     own_tiles = -(-columns // (16 if wide else 8))          # of a sequence and key/value head
     per_sm = 2 if head_dim > 128 else 3 if wide and head_dim > 64 else 4         # CTAs an SM holds
     blocks = -(-max_kv_len // BLOCK)
-    ranges = ranges_for(own_tiles * n_kv_heads * n, blocks, resident_ctas(q.device) // 4 * per_sm)
+    ranges = ranges_for(own_tiles * n_kv_heads * n, blocks, _sms(q) * per_sm)
     partial = again = scores = None
     stride = 0
     joins = ranges > CLUSTER                                # in a second launch
@@ -204,13 +223,13 @@ def attention8(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, cu_se
     elif joins:
         scratch = torch.empty(T * n_heads * ranges * (head_dim + 4), dtype=torch.float32, device=q.device)
         partial = scratch.data_ptr()
-    dtype, width, pages = code(q.dtype), page_table.shape[1], codes.shape[0]
+    kind = code(dtype)
     check("attention8", _attention8("tq_attention8")(
-        p_q, p_codes, p_scales, dtype, p_cu, p_held, p_table, width, page_size, window, scale, p_out, partial, ranges, again, scores, stride,
+        p_q, p_codes, p_scales, kind, p_cu, p_held, p_table, width, page_size, window, scale, p_out, partial, ranges, again, scores, stride,
         p_weights if scores is not None else None, max_kv_len, pages, n, max_q_len, n_heads, n_kv_heads, head_dim, at), kernels=2 if joins else 1)
     if again is not None:
         check("attention8", _attention8("tq_weigh8")(
-            p_q, p_codes, p_scales, dtype, p_cu, p_held, p_table, width, page_size, window, scale, again, p_weights, pages, n, max_q_len, max_kv_len,
+            p_q, p_codes, p_scales, kind, p_cu, p_held, p_table, width, page_size, window, scale, again, p_weights, pages, n, max_q_len, max_kv_len,
             n_heads, n_kv_heads, head_dim, at))
     return out
 
@@ -239,7 +258,7 @@ def _attention8_prompt(q, codes, scales, cu_seqlens, held, page_table, page_size
     p_q, p_out, p_codes, p_scales, p_dense, p_tables, p_lost, p_lse, p_weights, p_status, at = addresses(
         q, out, codes, scales, dense, table, lost, lse, weights, status)
     pages = codes.shape[0]
-    pieces, piece_pages = prefill_pieces(T, min(group, n), max_q_len, max_kv_len, n_heads, n_kv_heads, head_dim, window, resident_ctas(q.device) // 4) \
+    pieces, piece_pages = prefill_pieces(T, min(group, n), max_q_len, max_kv_len, n_heads, n_kv_heads, head_dim, window, _sms(q)) \
         if scale > 0.0 else (1, 0)
     for i in range(0, n, group):
         m = min(group, n - i)
@@ -268,19 +287,21 @@ def evict8(codes: torch.Tensor, scales: torch.Tensor, weights: torch.Tensor, len
     largest byte of its rows, rows of a smaller one are rounded again; sums of weights move along.  The old pages are only read and must
     not be among the new ones; rows of the new pages behind a sequence's last stay as they were.  Returns the places that were kept,
     int32 [n_seqs, nkv, budget], -1 where there are fewer."""
-    n_kv_heads, head_dim = codes.shape[2], codes.shape[4]
-    _check_cache(codes, scales, weights, page_table, page_size, n_kv_heads, head_dim)
+    if codes.dim() != 5:
+        raise KernelError(f"8-bit cache: codes must be float8_e4m3fn [pages, 2, kv heads, page_size, head size], got {tuple(codes.shape)}")
+    _, _, n_kv_heads, _, head_dim = codes.shape
+    pages, n, width = _sizes(codes, scales, weights, page_table, page_size, n_kv_heads, head_dim)
     check_sizes(page_size, head_dim)
-    want_int32(lengths, "lengths")
-    want_int32(new_table, "new page table")
-    n = page_table.shape[0]
-    if lengths.numel() != n or new_table.dim() != 2 or new_table.shape[0] != n or new_table.shape[1] * page_size < budget:
+    if lengths.dtype is not _I32 or new_table.dtype is not _I32 or lengths.numel() != n or new_table.dim() != 2 or new_table.shape[0] != n \
+            or new_table.shape[1] * page_size < budget:
+        want_int32(lengths, "lengths")
+        want_int32(new_table, "new page table")
         raise KernelError(f"evict8: {n} page tables, {lengths.numel()} lengths and new tables {tuple(new_table.shape)} for a budget of {budget} rows do not fit together")
     if not 0 <= recent <= budget or budget < 1:
         raise KernelError(f"evict8: cannot keep the newest {recent} rows of a budget of {budget}")
     p_codes, p_scales, p_weights, p_lengths, p_table, p_new, at = addresses(codes, scales, weights, lengths, page_table, new_table)
     kept = torch.empty((n, n_kv_heads, budget), dtype=torch.int32, device=codes.device)
     check("evict", _evict("tq_evict8")(
-        p_codes, p_scales, p_weights, p_lengths, p_table, page_table.shape[1], p_new, new_table.shape[1], page_size, codes.shape[0], n, n_kv_heads, head_dim,
+        p_codes, p_scales, p_weights, p_lengths, p_table, width, p_new, new_table.shape[1], page_size, pages, n, n_kv_heads, head_dim,
         budget, recent, kept.data_ptr(), at), kernels=2)
     return kept
