@@ -73,6 +73,17 @@ def test_evictions_that_do_not_fit_are_refused(bad):
         _evict(_state(**bad))
 
 
+@pytest.mark.parametrize("heads", [(4, 3), (0, 2), (4, 0)])
+def test_heads_that_do_not_divide(heads):
+    codes, scales, _ = cache8.storage(3, heads[1], PAGE, D, "cpu")
+    s = _state()
+    with pytest.raises(KernelError):
+        cache8.attention8(torch.zeros(2, heads[0], D), codes, scales, s["cu"], s["held"], s["table"], PAGE, 0, 0.1, torch.zeros(2, heads[0] * D), *heads, D, 2, 7)
+    with pytest.raises(KernelError):
+        cache8.write_rows8(torch.zeros(2, (heads[0] + 2 * heads[1]) * D), None, None, None, "half", s["positions"], s["cu"], s["held"], s["table"], PAGE,
+                           torch.zeros(2, heads[0], D), codes, scales, *heads, D, 2)
+
+
 @pytest.mark.parametrize("call", [_write, _attend, _evict])
 def test_there_is_no_cpu_path(call):
     with pytest.raises(KernelError):
@@ -119,10 +130,16 @@ def test_declared_arguments_are_those_of_the_sources():
     csrc = os.path.join(ROOT, "turboquant.cpp_b200", "csrc")
     text = "".join(open(os.path.join(csrc, f), encoding="utf-8").read() for f in ("cache8.cu", "attention8.cu", "prompt8.cu", "evict.cu"))
     found = dict(re.findall(r"TQ_EXPORT int (tq_\w+)\((.*?)\)\s*\{", text, re.S))
-    assert set(found) == set(cache8._SIGNATURES)
-    for name, arguments in found.items():
-        kinds = ["p" if "*" in a or "cudaStream_t" in a else "f" if a.split()[0] == "float" else "i" for a in (x.strip() for x in arguments.split(","))]
-        assert "".join(kinds) == cache8._SIGNATURES[name], name
+    assert set(found) == set(cache8._SIGNATURES) | set(cache8._PACKED)
+    kind = lambda a: "p" if "*" in a or "cudaStream_t" in a else "f" if a.split()[0] == "float" else "i"
+    for name, signature in cache8._SIGNATURES.items():
+        assert "".join(kind(a.strip()) for a in found[name].split(",")) == signature, name
+    for name, layout in cache8._PACKED.items():
+        struct = re.search(r"c8_call<(\w+)>", text[text.index(f"TQ_EXPORT int {name}("):]).group(1)
+        members = re.search(r"struct " + struct + r" \{(.*?)\};", text, re.S).group(1)
+        kinds = "".join(kind(line) * (line.count(",") + 1) for line in (x.strip() for x in members.split(";")) if line)
+        want = "".join(c * int(n or 1) for n, c in re.findall(r"(\d*)([Pif])", layout))
+        assert kinds.replace("p", "P") == want, name
 
 
 def test_ranges_fill_the_device_and_no_more():

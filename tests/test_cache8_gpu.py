@@ -392,3 +392,36 @@ def test_prompts_whose_keys_are_cut_into_pieces(shape, runs, held, window, monke
     assert bool((off <= limit).all()), float((off / limit).max())
     rel = float(2.02 * ((D + 8) * 4 * U * units).max()) + (places + H // G * max(runs) + 16) * 4 * U
     assert bool(((got_w.double() - want_w).abs() <= rel * want_w.abs() + 1e-30).all())
+
+
+def test_calls_on_two_streams_at_once():
+    """Each call's scratch is its own: steps of two caches on two streams give what they give one after the other."""
+    from turboquant_cpp_b200.kernels import cache8
+    H, G, D = 28, 4, 128
+    jobs = []
+    for runs, held in (([1] * 6, [900, 40, 333, 1500, 64, 2]), ([1, 1, 60], [3000, 16, 500])):
+        table, pages = _pages([n + h for n, h in zip(runs, held)], 64)
+        codes, scales = _cache(pages, G, 64, D)
+        q = torch.randn(sum(runs), H, D).to(torch.bfloat16).to(DEV)
+        jobs.append([q, _on(codes), scales.to(DEV), _cu(runs), _i(held), table.to(DEV), max(runs), max(n + h for n, h in zip(runs, held)), torch.rand(pages, G, 64, device=DEV)])
+
+    def call(job, out, w):
+        q, codes, scales, cu, held, table, run, longest, _ = job
+        cache8.attention8(q, codes, scales, cu, held, table, 64, 0, 0.08, out, H, G, D, run, longest, weights=w)
+    want = []
+    for job in jobs:
+        out, w = torch.empty(job[0].shape[0], H * D, dtype=torch.bfloat16, device=DEV), job[8].clone()
+        call(job, out, w)
+        want.append((out, w))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in jobs]
+    got = [[(torch.empty_like(out), job[8].clone()) for _ in range(20)] for (out, _), job in zip(want, jobs)]
+    torch.cuda.synchronize()
+    for i in range(20):
+        for s, job, g in zip(streams, jobs, got):
+            with torch.cuda.stream(s):
+                call(job, *g[i])
+    torch.cuda.synchronize()
+    for (out, w), g in zip(want, got):
+        for a, b in g:
+            assert torch.equal(a, out) and torch.equal(b, w)

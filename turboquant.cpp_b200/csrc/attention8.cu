@@ -839,23 +839,35 @@ int check_step(const char* what, int nh, int nkv, int n_seqs, int longest, int w
 // [T * nh * ranges * (hd + 4)]).  lse [T, nh] float32 or null.  scores [T * nh, score_stride] with weights [n_pages, nkv, page_size], or both
 // null: the weights of a step of single rows are added up by whoever joins, so by clusters only of all of a key/value head's query heads, and of
 // two ranges or more.  scores: [n_seqs * nkv, score_stride, score_columns(nh / nkv)], score_stride at least max_kv_len, the longest held[s] + run.
-TQ_EXPORT int tq_attention8(const void* q, const void* codes, const void* scales, int act_dtype, const int* cu_seqlens, const int* held,
-                            const int* page_table, int table_stride, int page_size, int window, float scale, void* out, float* partial, int ranges,
-                            float* lse, float* scores, int score_stride, float* weights, int max_kv_len, int n_pages, int n_seqs, int max_q_len, int nh,
-                            int nkv, int hd, cudaStream_t stream) {
+struct Attention8Call {
+    const void *q, *codes, *scales;
+    const int *cu_seqlens, *held, *page_table;
+    void* out;
+    float *partial, *lse, *scores, *weights;
+    cudaStream_t stream;
+    int act_dtype, table_stride, page_size, window, ranges, score_stride, max_kv_len, n_pages, n_seqs, max_q_len, nh, nkv, hd;
+    float scale;
+};
+TQ_EXPORT int tq_attention8(const void* packed) {
+    const Attention8Call x = c8_call<Attention8Call>(packed);
+    const void* q = x.q;
+    float *partial = x.partial, *scores = x.scores, *weights = x.weights;
+    const int page_size = x.page_size, window = x.window, ranges = x.ranges, score_stride = x.score_stride, max_kv_len = x.max_kv_len, n_pages = x.n_pages,
+              n_seqs = x.n_seqs, max_q_len = x.max_q_len, nh = x.nh, nkv = x.nkv, hd = x.hd;
+    const float scale = x.scale;
     if (n_seqs == 0 || max_q_len == 0) return 0;
-    int rc = c8_check("attention8", codes, scales, page_size, n_pages, nkv, hd, table_stride);
+    int rc = c8_check("attention8", x.codes, x.scales, page_size, n_pages, nkv, hd, x.table_stride);
     if (!rc) rc = check_step("attention8", nh, nkv, n_seqs, max_q_len, window);
     if (rc) return rc;
     TQ_REQUIRE(ranges >= 1 && ranges <= (partial != nullptr ? JOIN_RANGES : CLUSTER), "attention8: %d ranges need a buffer for their sums", ranges);
     TQ_REQUIRE((scores == nullptr) == (weights == nullptr) && (scores == nullptr || (max_q_len == 1 && (partial != nullptr || ranges > 1) && score_stride >= max_kv_len && (uintptr_t)scores % 16 == 0)),
                "attention8: scores of %d places do not hold %d", score_stride, max_kv_len);
-    const Cache8 c = c8_cache(codes, scales, page_table, table_stride, page_size, n_pages, nkv, hd);
-    const Step S{cu_seqlens, held, nh, window, scale * LOG2E};
+    const Cache8 c = c8_cache(x.codes, x.scales, x.page_table, x.table_stride, page_size, n_pages, nkv, hd);
+    const Step S{x.cu_seqlens, x.held, nh, window, scale * LOG2E};
     const int columns = max_q_len * (nh / nkv);
     auto first = [&]() -> int {
-        TQ_DISPATCH(act_dtype, TA,
-#define C8_CALL(HDP, NT, EXACT) (launch8<Form<TA, HDP, NT, EXACT>>(q, c, S, out, partial, ranges, scores, score_stride, partial == nullptr ? lse : nullptr, partial == nullptr ? weights : nullptr, n_seqs, max_q_len, stream))
+        TQ_DISPATCH(x.act_dtype, TA,
+#define C8_CALL(HDP, NT, EXACT) (launch8<Form<TA, HDP, NT, EXACT>>(q, c, S, x.out, partial, ranges, scores, score_stride, partial == nullptr ? x.lse : nullptr, partial == nullptr ? weights : nullptr, n_seqs, max_q_len, x.stream))
             C8_FORMS(columns, C8_CALL));
 #undef C8_CALL
         return -2;
@@ -863,7 +875,7 @@ TQ_EXPORT int tq_attention8(const void* q, const void* codes, const void* scales
     rc = first();
     if (rc || partial == nullptr) return rc;
     const int chunks = weights != nullptr ? (max_kv_len + 127) / 128 : 0;
-    TQ_DISPATCH(act_dtype, TA, tq_launch(dim3(columns + chunks, nkv, n_seqs), 128, 0, stream)(join8_kernel<TA>, c, S, partial, ranges, (TA*)out, columns, lse, scores, score_stride, weights));
+    TQ_DISPATCH(x.act_dtype, TA, tq_launch(dim3(columns + chunks, nkv, n_seqs), 128, 0, x.stream)(join8_kernel<TA>, c, S, partial, ranges, (TA*)x.out, columns, x.lse, scores, score_stride, weights));
     TQ_CHECK_LAUNCH("join8");
     return 0;
 }

@@ -205,27 +205,37 @@ __global__ void __launch_bounds__(WRITE_THREADS, RUNS && HD ? 5 : 1) write8_kern
 
 // qkv [T, (nh + 2 nkv) * hd]; bias as long as a row, or null; cos and sin [positions, hd / 2] float32, or null; q_out [T, nh, hd].
 // max_q_len: the longest run (cu_seqlens, held [n_seqs]: device).  codes null: the queries only.  Rows behind cu_seqlens[n_seqs] are left alone.
-TQ_EXPORT int tq_write8(const void* qkv, int act_dtype, const void* bias, int bias_dtype, const float* cos_t, const float* sin_t, int pairing,
-                        const int* positions, const int* cu_seqlens, const int* held, const int* page_table, int table_stride, int page_size,
-                        void* q_out, void* codes, void* scales, int n_pages, int n_seqs, int max_q_len, int nh, int nkv, int hd, cudaStream_t stream) {
+struct Write8Call {
+    const void *qkv, *bias;
+    const float *cos_t, *sin_t;
+    const int *positions, *cu_seqlens, *held, *page_table;
+    void *q_out, *codes, *scales;
+    cudaStream_t stream;
+    int act_dtype, bias_dtype, pairing, table_stride, page_size, n_pages, n_seqs, max_q_len, nh, nkv, hd;
+};
+TQ_EXPORT int tq_write8(const void* packed) {
+    const Write8Call x = c8_call<Write8Call>(packed);
+    const void *qkv = x.qkv, *bias = x.bias, *codes = x.codes, *scales = x.scales;
+    const float *cos_t = x.cos_t, *sin_t = x.sin_t;
+    const int page_size = x.page_size, n_pages = x.n_pages, n_seqs = x.n_seqs, max_q_len = x.max_q_len, nh = x.nh, nkv = x.nkv, hd = x.hd;
     if (n_seqs == 0 || max_q_len == 0) return 0;
-    int rc = c8_check("write8", codes, scales, page_size, n_pages, nkv, hd, table_stride);
+    int rc = c8_check("write8", codes, scales, page_size, n_pages, nkv, hd, x.table_stride);
     if (rc) return rc;
     TQ_REQUIRE(nh >= 1 && nh % nkv == 0, "write8: %d heads are not a multiple of %d key/value heads", nh, nkv);
     TQ_REQUIRE((cos_t == nullptr) == (sin_t == nullptr), "write8: cos and sin tables come together");
     TQ_REQUIRE(n_seqs <= 65535 && max_q_len >= 1, "write8: %d sequences, longest run %d", n_seqs, max_q_len);
-    TQ_REQUIRE(((uintptr_t)qkv | (uintptr_t)bias | (uintptr_t)q_out | (uintptr_t)cos_t | (uintptr_t)sin_t) % 16 == 0, "write8: tensors must be 16-byte aligned");
-    const Cache8 c = c8_cache(codes, scales, page_table, table_stride, page_size, n_pages, nkv, hd);
-    const WriteArgs a{cos_t, sin_t, positions, cu_seqlens, held, nh, pairing, codes != nullptr ? nh + 2 * nkv : nh};
+    TQ_REQUIRE(((uintptr_t)qkv | (uintptr_t)bias | (uintptr_t)x.q_out | (uintptr_t)cos_t | (uintptr_t)sin_t) % 16 == 0, "write8: tensors must be 16-byte aligned");
+    const Cache8 c = c8_cache(codes, scales, x.page_table, x.table_stride, page_size, n_pages, nkv, hd);
+    const WriteArgs a{cos_t, sin_t, x.positions, x.cu_seqlens, x.held, nh, x.pairing, codes != nullptr ? nh + 2 * nkv : nh};
     // a run of n rows touches at most (n + 14) / 16 + 1 blocks
     const bool runs = max_q_len > 1;
     const int units = runs ? (max_q_len + 14) / C8_BLOCK + 1 : 1, threads = runs ? (hd + 31) / 32 * 32 : 32;
     const int side = runs ? WRITE_THREADS / threads : n_seqs >= 32 ? 8 : 2;              // units a block takes side by side
     const dim3 grid(units, (a.written + side - 1) / side, n_seqs);
-    TQ_DISPATCH(act_dtype, TA, TQ_DISPATCH(bias != nullptr ? bias_dtype : act_dtype, TB,
+    TQ_DISPATCH(x.act_dtype, TA, TQ_DISPATCH(bias != nullptr ? x.bias_dtype : x.act_dtype, TB,
         auto kernel = runs ? (hd == 128 ? write8_kernel<TA, TB, true, 128> : hd == 64 ? write8_kernel<TA, TB, true, 64> : write8_kernel<TA, TB, true, 0>)
                            : (hd == 128 ? write8_kernel<TA, TB, false, 128> : write8_kernel<TA, TB, false, 0>);
-        tq_launch(grid, side * threads, 0, stream)(kernel, (const TA*)qkv, (const TB*)bias, a, (TA*)q_out, c, threads)));
+        tq_launch(grid, side * threads, 0, x.stream)(kernel, (const TA*)qkv, (const TB*)bias, a, (TA*)x.q_out, c, threads)));
     TQ_CHECK_LAUNCH("write8");
     return 0;
 }

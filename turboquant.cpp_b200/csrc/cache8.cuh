@@ -9,6 +9,7 @@
 // Row t of sequence s lies at place held[s] + t - cu_seqlens[s]; place p in page table[s][p / page_size], row p % page_size.
 #pragma once
 #include <cuda_fp8.h>
+#include <string.h>
 #include "common.cuh"
 
 #define C8_BLOCK 16
@@ -87,6 +88,14 @@ __device__ __forceinline__ uint32_t c8_shift_factor(int shift) {
 }
 __device__ __forceinline__ uint4 c8_shift16(uint4 v, uint32_t factor) {
     return make_uint4(c8_shift4(v.x, factor), c8_shift4(v.y, factor), c8_shift4(v.z, factor), c8_shift4(v.w, factor));
+}
+
+// Entry points of calls that single steps make take one packed struct (addresses first, then whole numbers, then floats: no gaps), which costs
+// the caller a fifth of what two dozen arguments do; it is copied, since a Python bytes object need not be aligned for it.
+template <typename C> inline C c8_call(const void* packed) {
+    C c;
+    memcpy(&c, packed, sizeof(c));
+    return c;
 }
 
 inline Cache8 c8_cache(const void* codes, const void* scales, const int* table, int table_stride, int page_size, int n_pages, int nkv, int hd) {

@@ -167,23 +167,33 @@ __global__ void __launch_bounds__(256) evict8_move_kernel(Cache8 c, float* __res
 
 // lengths [n_seqs] (device): rows each sequence holds; kept [n_seqs, nkv, budget]: receives the places that stay, ascending, then -1.  Row j of
 // them goes to place j of new_table's pages, none of which holds any of these rows.
-TQ_EXPORT int tq_evict8(void* codes, void* scales, float* weights, const int* lengths, const int* page_table, int table_stride, const int* new_table, int new_stride,
-                        int page_size, int n_pages, int n_seqs, int nkv, int hd, int budget, int recent, int* kept, cudaStream_t stream) {
+struct Evict8Call {
+    void *codes, *scales;
+    float* weights;
+    const int *lengths, *page_table, *new_table;
+    int* kept;
+    cudaStream_t stream;
+    int table_stride, new_stride, page_size, n_pages, n_seqs, nkv, hd, budget, recent;
+};
+TQ_EXPORT int tq_evict8(const void* packed) {
+    const Evict8Call x = c8_call<Evict8Call>(packed);
+    const int* page_table = x.page_table;
+    const int table_stride = x.table_stride, page_size = x.page_size, n_pages = x.n_pages, n_seqs = x.n_seqs, nkv = x.nkv, hd = x.hd, budget = x.budget, recent = x.recent;
     if (n_seqs == 0) return 0;
-    int rc = c8_check("evict8", codes, scales, page_size, n_pages, nkv, hd, table_stride);
+    int rc = c8_check("evict8", x.codes, x.scales, page_size, n_pages, nkv, hd, table_stride);
     if (rc) return rc;
     TQ_REQUIRE(budget >= 1 && recent >= 0 && recent <= budget, "evict8: %d newest of a budget of %d rows", recent, budget);
-    TQ_REQUIRE((long long)new_stride * page_size >= budget, "evict8: %d new pages a sequence for a budget of %d rows", new_stride, budget);
+    TQ_REQUIRE((long long)x.new_stride * page_size >= budget, "evict8: %d new pages a sequence for a budget of %d rows", x.new_stride, budget);
     TQ_REQUIRE(n_seqs <= 65535 && nkv <= 65535, "evict8: %d sequences, %d heads", n_seqs, nkv);
     TQ_REQUIRE((long long)table_stride * page_size < (1ll << 31), "evict8: page tables of %d pages", table_stride);
-    const Cache8 c = c8_cache(codes, scales, page_table, table_stride, page_size, n_pages, nkv, hd);
+    const Cache8 c = c8_cache(x.codes, x.scales, page_table, table_stride, page_size, n_pages, nkv, hd);
     const int cached = table_stride * page_size < SELECT_MOST ? table_stride * page_size : SELECT_MOST;
     static TqSmemAsked asked;
     const cudaError_t e = tq_grow_smem(evict8_select_kernel, (size_t)cached * 4, asked);
     if (e != cudaSuccess) TQ_FAIL(-1, "evict8: cannot reserve %d bytes of shared memory: %s", cached * 4, cudaGetErrorString(e));
-    tq_launch(dim3(nkv, n_seqs), SELECT_THREADS, (size_t)cached * 4, stream)(evict8_select_kernel, c, weights, lengths, budget, recent, cached, kept);
+    tq_launch(dim3(nkv, n_seqs), SELECT_THREADS, (size_t)cached * 4, x.stream)(evict8_select_kernel, c, x.weights, x.lengths, budget, recent, cached, x.kept);
     TQ_CHECK_LAUNCH("evict8_select");
-    tq_launch(dim3(((budget + C8_BLOCK - 1) / C8_BLOCK + 7) / 8, nkv, n_seqs), 256, 0, stream)(evict8_move_kernel, c, weights, kept, new_table, new_stride, budget);
+    tq_launch(dim3(((budget + C8_BLOCK - 1) / C8_BLOCK + 7) / 8, nkv, n_seqs), 256, 0, x.stream)(evict8_move_kernel, c, x.weights, x.kept, x.new_table, x.new_stride, budget);
     TQ_CHECK_LAUNCH("evict8_move");
     return 0;
 }

@@ -9,7 +9,7 @@ several steps keeps the largest byte; the rows it held are then rounded again.  
     weights  [pages, kv heads, page_size] float32: the attention weight each row has received, where it is kept
 
 The step's rows are packed, sequence after sequence: rows cu_seqlens[s] .. cu_seqlens[s + 1] - 1 belong to sequence s, and row t lies at
-place held[s] + t - cu_seqlens[s], which is row place % page_size of page page_table[s, place / page_size].  A place is not a position:
+place held[s] + t - cu_seqlens[s], which is row place % page_size of page page_table[s, place / page_size].  A page belongs to one sequence of a call.  A place is not a position:
 a sequence that lost rows to `evict8` holds fewer than it has positions.  cu_seqlens [n_seqs + 1], held and page_table [n_seqs, width]
 are int32 on the device; every place a call reads or writes needs its page, and rows behind the last sequence are left as they were.
 The launches go to the current stream, allocate their scratch from torch's allocator and can be captured into CUDA graphs."""
@@ -22,7 +22,7 @@ from typing import Optional, Tuple
 import torch
 
 from ..csrc.build import load_kernel
-from ._call import KernelError, addresses, check, code, declared, want_int32
+from ._call import KernelError, addresses, check, code, declared, packed, want_int32
 from .attention import PAIRING, prefill_pieces, prefill_rows, prefill_split, prefill_usable, resident_ctas
 from .gemm_tc import status_word
 
@@ -30,17 +30,16 @@ BLOCK = 16
 MAX_HEAD_DIM = 256
 
 
-_SIGNATURES = {              # argument types of the entry points (_call.declared)
-    "tq_write8": "pipippipppp" "iippp" "iiiiii" "p", "tq_attention8": "pppippp" "iiifppi" "ppipi" "iiiiii" "p",
+_PACKED = {"tq_write8": "12P11i", "tq_attention8": "12P13if", "tq_evict8": "8P9i"}        # members of the entry points' structs (_call.packed)
+_SIGNATURES = {              # argument types of the others (_call.declared)
     "tq_weigh8": "pppippp" "iiifpp" "iiiiiii" "p", "tq_repair8": "pppppp" "iiifppi" "iiiii" "p",
     "tq_expand8": "ppppp" "iiipppi" "iiii" "p", "tq_weigh8_prompt": "ppippp" "iifpp" "iiiiiii" "pp",
-    "tq_evict8": "ppppp" "ipi" "iiiiiii" "pp",
 }
 _entries = {}
 
 
 def _declare(lib, name: str):
-    fn = _entries[name] = declared(lib, name, _SIGNATURES[name])
+    fn = _entries[name] = packed(lib, name, _PACKED[name]) if name in _PACKED else declared(lib, name, _SIGNATURES[name])
     return fn
 
 
@@ -126,6 +125,8 @@ def write_rows8(qkv: torch.Tensor, bias: Optional[torch.Tensor], cos: Optional[t
         pages, n, width = _sizes(codes, scales, None, page_table, page_size, n_kv_heads, head_dim)
     _check_step(cu_seqlens, held, n, "write_rows8")
     dtype = qkv.dtype
+    if n_kv_heads < 1 or n_heads < 1 or n_heads % n_kv_heads:
+        raise KernelError(f"write_rows8: {n_heads} heads are not a multiple of {n_kv_heads} key/value heads")
     if columns != (n_heads + 2 * n_kv_heads) * head_dim or q_out.numel() != T * n_heads * head_dim or q_out.dtype is not dtype \
             or positions.numel() != T or positions.dtype is not _I32 or (bias is not None and bias.numel() != columns):
         want_int32(positions, "positions")
@@ -140,8 +141,8 @@ def write_rows8(qkv: torch.Tensor, bias: Optional[torch.Tensor], cos: Optional[t
     p_qkv, p_bias, p_cos, p_sin, p_positions, p_cu, p_held, p_table, p_q, p_codes, p_scales, at = addresses(
         qkv, bias, cos, sin, positions, cu_seqlens, held, page_table, q_out, codes, scales)
     check("cache8", _cache8("tq_write8")(
-        p_qkv, code(dtype), p_bias, 0 if bias is None else code(bias.dtype), p_cos, p_sin, PAIRING[pairing], p_positions, p_cu, p_held, p_table,
-        width, page_size, p_q, p_codes, p_scales, pages, n, max_q_len, n_heads, n_kv_heads, head_dim, at))
+        p_qkv, p_bias, p_cos, p_sin, p_positions, p_cu, p_held, p_table, p_q, p_codes, p_scales, at,
+        code(dtype), 0 if bias is None else code(bias.dtype), PAIRING[pairing], width, page_size, pages, n, max_q_len, n_heads, n_kv_heads, head_dim))
 
 
 MAX_RANGES, CLUSTER = 64, 8
@@ -186,6 +187,8 @@ def attention8(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, cu_se
     T, dtype = q.shape[0], q.dtype
     pages, n, width = _sizes(codes, scales, weights, page_table, page_size, n_kv_heads, head_dim)
     _check_step(cu_seqlens, held, n, "attention8")
+    if n_kv_heads < 1 or n_heads < 1 or n_heads % n_kv_heads:
+        raise KernelError(f"attention8: {n_heads} heads are not a multiple of {n_kv_heads} key/value heads")
     elements = T * n_heads * head_dim
     if q.numel() != elements or out.numel() != elements or out.dtype is not dtype:
         raise KernelError(f"attention8: queries {tuple(q.shape)} {dtype} and output {tuple(out.shape)} {out.dtype} do not fit {n_heads} heads of {head_dim}")
@@ -203,8 +206,7 @@ def attention8(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, cu_se
     per_sm = 2 if head_dim > 128 else 3 if wide and head_dim > 64 else 4         # CTAs an SM holds
     blocks = -(-max_kv_len // BLOCK)
     ranges = ranges_for(own_tiles * n_kv_heads * n, blocks, _sms(q) * per_sm)
-    partial = again = scores = None
-    stride = 0
+    partial = again = scores = stride = 0
     joins = ranges > CLUSTER                                # in a second launch
     if weights is not None:
         # one row a sequence: scores are left for whoever joins the ranges, to be added up, which moves 8 bytes a key and query head, where reading
@@ -215,7 +217,7 @@ def attention8(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, cu_se
         joins |= stored and (ranges == 1 or own_tiles > 1)
         sums = rows * ranges * (head_dim + 4) if joins else 0
         scratch = torch.empty(sums + (size if stored else rows), dtype=torch.float32, device=q.device)
-        partial = scratch.data_ptr() if joins else None
+        partial = scratch.data_ptr() if joins else 0
         if stored:
             scores = scratch.data_ptr() + 4 * sums
         else:
@@ -225,9 +227,9 @@ def attention8(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, cu_se
         partial = scratch.data_ptr()
     kind = code(dtype)
     check("attention8", _attention8("tq_attention8")(
-        p_q, p_codes, p_scales, kind, p_cu, p_held, p_table, width, page_size, window, scale, p_out, partial, ranges, again, scores, stride,
-        p_weights if scores is not None else None, max_kv_len, pages, n, max_q_len, n_heads, n_kv_heads, head_dim, at), kernels=2 if joins else 1)
-    if again is not None:
+        p_q, p_codes, p_scales, p_cu, p_held, p_table, p_out, partial, again, scores, p_weights if scores else 0, at,
+        kind, width, page_size, window, ranges, stride, max_kv_len, pages, n, max_q_len, n_heads, n_kv_heads, head_dim, scale), kernels=2 if joins else 1)
+    if again:
         check("attention8", _attention8("tq_weigh8")(
             p_q, p_codes, p_scales, kind, p_cu, p_held, p_table, width, page_size, window, scale, again, p_weights, pages, n, max_q_len, max_kv_len,
             n_heads, n_kv_heads, head_dim, at))
@@ -302,6 +304,6 @@ def evict8(codes: torch.Tensor, scales: torch.Tensor, weights: torch.Tensor, len
     p_codes, p_scales, p_weights, p_lengths, p_table, p_new, at = addresses(codes, scales, weights, lengths, page_table, new_table)
     kept = torch.empty((n, n_kv_heads, budget), dtype=torch.int32, device=codes.device)
     check("evict", _evict("tq_evict8")(
-        p_codes, p_scales, p_weights, p_lengths, p_table, width, p_new, new_table.shape[1], page_size, pages, n, n_kv_heads, head_dim,
-        budget, recent, kept.data_ptr(), at), kernels=2)
+        p_codes, p_scales, p_weights, p_lengths, p_table, p_new, kept.data_ptr(), at, width, new_table.shape[1], page_size, pages, n, n_kv_heads, head_dim,
+        budget, recent), kernels=2)
     return kept
