@@ -707,76 +707,159 @@ __global__ void __launch_bounds__(128) join8_kernel(Cache8 c, Step S, const floa
 }
 
 // ---------------------------------------------------------------------------------------
-// Sums of weights from the queries and the keys again: a warp keeps a block of 16 keys in registers and walks the columns that see it, 8
-// or 16 at a time.  One writer per sum and a fixed order: the same bits every time.
+// Sums of weights from the queries and the keys again.  A CTA has KB blocks of 16 keys of a (sequence, key/value head); each of its four warps
+// holds all of them as left operands and walks every fourth tile of 8 columns that see them, whose queries go from memory straight to its
+// registers: no shared memory, no barrier but the one at the end, where the warps' sums meet in order.  One writer per sum: the same bits
+// every time.  (A warp per block and the columns one tile after another through shared memory: 588 rows of 8 heads of 256 484 us.)
 // ---------------------------------------------------------------------------------------
-template <class F>
+// sixteen elements of a row; the row's offset is a multiple of 16 elements
+__device__ __forceinline__ void load16(float (&x)[16], const __nv_bfloat16* p, bool aligned) {
+    if (aligned) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const uint4 v = __ldg(reinterpret_cast<const uint4*>(p) + h);
+            const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) { x[8 * h + 2 * e] = __uint_as_float(u[e] << 16); x[8 * h + 2 * e + 1] = __uint_as_float(u[e] & 0xffff0000u); }
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[e] = tq_to_float(p[e]);
+    }
+}
+__device__ __forceinline__ void load16(float (&x)[16], const float* p, bool aligned) {
+    if (aligned) {
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+            const float4 v = __ldg(reinterpret_cast<const float4*>(p) + h);
+            x[4 * h] = v.x; x[4 * h + 1] = v.y; x[4 * h + 2] = v.z; x[4 * h + 3] = v.w;
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[e] = p[e];
+    }
+}
+
+template <class F, int KB>
 __global__ void __launch_bounds__(WARPS * 32) weigh8_kernel(const typename F::TA* __restrict__ q, Cache8 c, Step S, const float* __restrict__ lse, float* __restrict__ weights) {
     tq_grid_wait();                    // everything below may read what the previous kernel wrote
     tq_grid_launch_dependents();
-    constexpr int NT = F::NT, NC = F::NC;
-    __shared__ Queries<F> Q;
+    using TA = typename F::TA;
+    constexpr int KEYS = KB * C8_BLOCK;
+    const bool aligned = ((uintptr_t)q & 15) == 0;
+    __shared__ float s_sum[WARPS][KEYS];
     const int seq = blockIdx.z, gh = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, hd = c.hd;
-    Tile T = tile_of(S, seq, gh, c.nkv, 0, NC);
-    const int key0 = blockIdx.x * WARPS * C8_BLOCK, last_key = key0 + WARPS * C8_BLOCK - 1;
+    const Tile T = tile_of(S, seq, gh, c.nkv, 0, 8);
+    const int key0 = blockIdx.x * KEYS, end = T.start + T.run;
     // rows of the run that see some of the CTA's keys
-    const int row0 = max(0, key0 - T.start), row1 = S.window > 0 ? min(T.run, last_key + S.window - T.start) : T.run;
+    const int row0 = max(0, key0 - T.start), row1 = S.window > 0 ? min(T.run, key0 + KEYS - 1 + S.window - T.start) : T.run;
     if (row0 >= row1) return;
-    const int block = blockIdx.x * WARPS + warp, key = block * C8_BLOCK + g;
-    const bool mine = block * C8_BLOCK < T.start + T.run && !(S.window > 0 && block * C8_BLOCK + C8_BLOCK - 1 + S.window <= T.start);
-    KeyRegs<F> kr = {};
-    float ks = 0.f;
-    int page = 0;
-    const int row = c.row(block * C8_BLOCK);
-    if (mine) {
-        page = c.page_of(seq, block * C8_BLOCK);
+    uint4 kr[KB][F::HDP / 64][2];
+    float ks[KB];
+#pragma unroll
+    for (int b = 0; b < KB; ++b) {
+        const int key = key0 + b * C8_BLOCK;
+        ks[b] = 0.f;
+        // blocks behind the last row, or whose pages may have been given back, have no page
+        const bool there = key < end && !(S.window > 0 && key + C8_BLOCK - 1 + S.window <= T.start);
+        const int page = there ? c.page_of(seq, key) : 0, row = c.row(key);
         const uint8_t* k = c.codes + c.codes_at(page, 0, gh) + (size_t)row * hd;
 #pragma unroll
         for (int j = 0; j < F::HDP / 64; ++j)
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-                if (chunk_of<F::HDP>(j, t) * 16 < hd) kr.k[j][h] = __ldg(reinterpret_cast<const uint4*>(k + (g + 8 * h) * hd + chunk_of<F::HDP>(j, t) * 16));
-        ks = c8_scale(c.scales[c.scales_at(page, 0, gh) + row / C8_BLOCK]);
+            for (int h = 0; h < 2; ++h) {
+                const int at = chunk_of<F::HDP>(j, t) * 16;
+                kr[b][j][h] = there && at < hd ? __ldg(reinterpret_cast<const uint4*>(k + (g + 8 * h) * hd + at)) : make_uint4(0, 0, 0, 0);
+            }
+        if (there) ks[b] = c8_scale(c.scales[c.scales_at(page, 0, gh) + row / C8_BLOCK]);
     }
-    float sum[2] = {0.f, 0.f};
-    const int all = row1 * T.per;
-    for (T.first = row0 * T.per; T.first < all; T.first += NC) {
-        T.n = min(NC, all - T.first);
-        __syncthreads();
-        Q.load(q, T, S, hd);
-        if (!mine) continue;
-        uint2 kept[F::KEEP ? F::STEPS : 1];
-        if (F::KEEP) {
+    float sum[KB][2] = {};
+    const int last = row1 * T.per;
+    for (int first = row0 * T.per + warp * 8; first < last; first += WARPS * 8) {
+        // the lane's column: its queries, scaled to a largest element between 2^14 and 2^15, and what its scores need
+        const int col = first + g;
+        const bool mine = col < last;
+        const size_t at = mine ? T.query(col, S) : 0;
+        float x[F::HDP / 64][16];
+        uint32_t top = 0;
 #pragma unroll
-            for (int i = 0; i < F::STEPS; ++i) kept[F::KEEP ? i : 0] = Q.b[0][0][i][lane];
+        for (int j = 0; j < F::HDP / 64; ++j) {
+            const int d = chunk_of<F::HDP>(j, t) * 16;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) x[j][e] = 0.f;
+            if (mine && d < hd) load16(x[j], q + at * hd + d, aligned);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) top = max(top, c8_magnitude(x[j][e]));
         }
-        float s[NT][4];
-        products<F>(s, kr, Q, kept);
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const int shift = min(126, 14 - max((int)(top >> 23) - 127, -126));
+        const float up = __uint_as_float((uint32_t)(127 + shift) << 23), factor = S.factor * __uint_as_float((uint32_t)(127 - shift) << 23);
+        const float minus = mine ? -lse[at] : 0.f;
+        const int place = mine ? T.start + T.row(col) : -1;               // (T.first is 0)
+        uint2 b0[F::HDP / 64][4], b1[F::PARTS == 2 ? F::HDP / 64 : 1][4];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int j = 0; j < F::HDP / 64; ++j)
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const int col = nt * 8 + 2 * t + j;
-                if (col >= T.n) continue;
-                const int p = Q.place[col];
-                const float f = Q.factor[col] * ks, L = lse[Q.row[col]];
+            for (int i = 0; i < 4; ++i) {
+                float v[4];
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int k = key + 8 * h;
-                    if (k <= p && (S.window <= 0 || k > p - S.window)) sum[h] += ex2(s[nt][j + 2 * h] * f - L);
+                for (int e = 0; e < 4; ++e) v[e] = x[j][4 * i + e] * up;
+                b0[j][i] = make_uint2(half2_of(v[0], v[1]), half2_of(v[2], v[3]));
+                if (F::PARTS == 2) {
+                    const float2 p = float2_of(b0[j][i].x), r = float2_of(b0[j][i].y);
+                    auto left = [](float a, float h) { const float d = a - h; return fabsf(d) < INFINITY ? d : 0.f; };
+                    b1[F::PARTS == 2 ? j : 0][i] = make_uint2(half2_of(left(v[0], p.x), left(v[1], p.y)), half2_of(left(v[2], r.x), left(v[3], r.y)));
                 }
             }
-    }
-    if (!mine) return;
+        // what the lane's two columns of results need, from the lanes that have them
+        float f[2], m[2];
+        int p[2];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 1);
-        sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 2);
-        const int k = key + 8 * h;
-        if (t == 0 && k < T.start + T.run && !(S.window > 0 && k + S.window <= T.start)) {
-            float* w = weights + ((size_t)page * c.nkv + gh) * c.page_size + row + g + 8 * h;
-            *w = (k < T.start ? *w : 0.f) + sum[h];
+        for (int j = 0; j < 2; ++j) {
+            const int from = (2 * t + j) * 4;
+            f[j] = __shfl_sync(0xffffffffu, factor, from);
+            m[j] = __shfl_sync(0xffffffffu, minus, from);
+            p[j] = __shfl_sync(0xffffffffu, place, from);
         }
+#pragma unroll
+        for (int b = 0; b < KB; ++b) {
+            float s[4] = {}, odd[4] = {};
+#pragma unroll
+            for (int j = 0; j < F::HDP / 64; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    uint32_t a0, a1, a2, a3;
+                    c8_half4(word(kr[b][j][0], i), a0, a2);
+                    c8_half4(word(kr[b][j][1], i), a1, a3);
+                    mma(i & 1 ? odd : s, a0, a1, a2, a3, b0[j][i].x, b0[j][i].y);
+                    if (F::PARTS == 2) mma(i & 1 ? s : odd, a0, a1, a2, a3, b1[F::PARTS == 2 ? j : 0][i].x, b1[F::PARTS == 2 ? j : 0][i].y);
+                }
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int k = key0 + b * C8_BLOCK + g + 8 * h;
+                    if (k <= p[j] && (S.window <= 0 || k > p[j] - S.window)) sum[b][h] += ex2(fmaf(s[j + 2 * h] + odd[j + 2 * h], f[j] * ks[b], m[j]));
+                }
+        }
+    }
+#pragma unroll
+    for (int b = 0; b < KB; ++b)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            sum[b][h] += __shfl_xor_sync(0xffffffffu, sum[b][h], 1);
+            sum[b][h] += __shfl_xor_sync(0xffffffffu, sum[b][h], 2);
+            if (t == 0) s_sum[warp][b * C8_BLOCK + g + 8 * h] = sum[b][h];
+        }
+    __syncthreads();
+    const int k = key0 + (int)threadIdx.x;
+    if (threadIdx.x < KEYS && k < end && !(S.window > 0 && k + S.window <= T.start)) {       // (others: no row of the step sees them)
+        float all = 0.f;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) all += s_sum[w][threadIdx.x];
+        float* w = weights + ((size_t)c.page_of(seq, k) * c.nkv + gh) * c.page_size + c.row(k);
+        *w = (k < T.start ? *w : 0.f) + all;
     }
 }
 
@@ -809,10 +892,10 @@ int launch8(const void* q, const Cache8& c, const Step& S, void* out, float* par
     TQ_CHECK_LAUNCH("attention8");
     return 0;
 }
-template <class F>
+template <class F, int KB>
 int launch_weigh8(const void* q, const Cache8& c, const Step& S, const float* lse, float* weights, int n_seqs, int max_kv_len, cudaStream_t stream) {
-    const int per_cta = WARPS * C8_BLOCK;
-    tq_launch(dim3((max_kv_len + per_cta - 1) / per_cta, c.nkv, n_seqs), WARPS * 32, 0, stream)(weigh8_kernel<F>, (const typename F::TA*)q, c, S, lse, weights);
+    const int per_cta = KB * C8_BLOCK;
+    tq_launch(dim3((max_kv_len + per_cta - 1) / per_cta, c.nkv, n_seqs), WARPS * 32, 0, stream)(weigh8_kernel<F, KB>, (const typename F::TA*)q, c, S, lse, weights);
     TQ_CHECK_LAUNCH("weigh8");
     return 0;
 }
@@ -899,17 +982,16 @@ TQ_EXPORT int tq_repair8(const void* q, const void* codes, const void* scales, c
 // 2^(score - lse).  max_kv_len: at least the longest held[s] + run.
 TQ_EXPORT int tq_weigh8(const void* q, const void* codes, const void* scales, int act_dtype, const int* cu_seqlens, const int* held,
                         const int* page_table, int table_stride, int page_size, int window, float scale, const float* lse, float* weights, int n_pages,
-                        int n_seqs, int max_q_len, int max_kv_len, int nh, int nkv, int hd, cudaStream_t stream) {
+                        int n_seqs, int max_kv_len, int nh, int nkv, int hd, cudaStream_t stream) {
     if (n_seqs == 0 || max_kv_len == 0) return 0;
     int rc = c8_check("weigh8", codes, scales, page_size, n_pages, nkv, hd, table_stride);
     if (!rc) rc = check_step("weigh8", nh, nkv, n_seqs, max_kv_len, window);
     if (rc) return rc;
     const Cache8 c = c8_cache(codes, scales, page_table, table_stride, page_size, n_pages, nkv, hd);
     const Step S{cu_seqlens, held, nh, window, scale * LOG2E};
-    const int columns = max_q_len * (nh / nkv);
     TQ_DISPATCH(act_dtype, TA,
-#define C8_CALL(HDP, NT, EXACT) (launch_weigh8<Form<TA, HDP, NT, false>>(q, c, S, lse, weights, n_seqs, max_kv_len, stream))
-        C8_FORMS(columns, C8_CALL));
-#undef C8_CALL
+        if (hd <= 64) return launch_weigh8<Form<TA, 64, 1, false>, 4>(q, c, S, lse, weights, n_seqs, max_kv_len, stream);
+        if (hd <= 128) return launch_weigh8<Form<TA, 128, 1, false>, 4>(q, c, S, lse, weights, n_seqs, max_kv_len, stream);
+        return launch_weigh8<Form<TA, 256, 1, false>, 2>(q, c, S, lse, weights, n_seqs, max_kv_len, stream));
     return -2;
 }

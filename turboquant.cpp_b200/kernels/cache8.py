@@ -32,7 +32,7 @@ MAX_HEAD_DIM = 256
 
 _PACKED = {"tq_write8": "12P11i", "tq_attention8": "12P13if", "tq_evict8": "8P9i"}        # members of the entry points' structs (_call.packed)
 _SIGNATURES = {              # argument types of the others (_call.declared)
-    "tq_weigh8": "pppippp" "iiifpp" "iiiiiii" "p", "tq_repair8": "pppppp" "iiifppi" "iiiii" "p",
+    "tq_weigh8": "pppippp" "iiifpp" "iiiiii" "p", "tq_repair8": "pppppp" "iiifppi" "iiiii" "p",
     "tq_expand8": "ppppp" "iiipppi" "iiii" "p", "tq_weigh8_prompt": "ppippp" "iifpp" "iiiiiii" "pp",
 }
 _entries = {}
@@ -231,7 +231,7 @@ def attention8(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, cu_se
         kind, width, page_size, window, ranges, stride, max_kv_len, pages, n, max_q_len, n_heads, n_kv_heads, head_dim, scale), kernels=2 if joins else 1)
     if again:
         check("attention8", _attention8("tq_weigh8")(
-            p_q, p_codes, p_scales, kind, p_cu, p_held, p_table, width, page_size, window, scale, again, p_weights, pages, n, max_q_len, max_kv_len,
+            p_q, p_codes, p_scales, kind, p_cu, p_held, p_table, width, page_size, window, scale, again, p_weights, pages, n, max_kv_len,
             n_heads, n_kv_heads, head_dim, at))
     return out
 
