@@ -425,3 +425,24 @@ def test_calls_on_two_streams_at_once():
     for (out, w), g in zip(want, got):
         for a, b in g:
             assert torch.equal(a, out) and torch.equal(b, w)
+
+
+@pytest.mark.parametrize("runs,held", [([1, 1], [5, 64]), ([20, 3], [0, 33])])
+def test_queries_alone(runs, held):
+    """A layer that reads another layer's cache writes its queries and nothing else."""
+    from turboquant_cpp_b200.kernels import cache8
+    H, G, D = 6, 2, 32
+    T = sum(runs)
+    table, pages = _pages([n + h for n, h in zip(runs, held)], 64)
+    codes, scales = _cache(pages, G, 64, D)
+    qkv, bias = torch.randn(T, (H + 2 * G) * D, device=DEV).to(torch.bfloat16), torch.randn((H + 2 * G) * D, device=DEV)
+    angle = torch.rand(300, D // 2, device=DEV) * 6.3
+    positions = torch.randint(0, 300, (T,), dtype=torch.int32, device=DEV)
+    both = []
+    for c, s in ((_on(codes), scales.to(DEV)), (None, None)):
+        q = torch.empty(T, H, D, dtype=torch.bfloat16, device=DEV)
+        cache8.write_rows8(qkv, bias, torch.cos(angle), torch.sin(angle), "half", positions, _cu(runs), _i(held), table.to(DEV), 64, q, c, s, H, G, D, max(runs))
+        both.append(q)
+    assert torch.equal(*both)
+    with pytest.raises(Exception):
+        cache8.write_rows8(qkv, bias, None, None, "half", positions, _cu(runs), _i(held), table.to(DEV), 64, both[0], None, scales.to(DEV), H, G, D, max(runs))

@@ -14,6 +14,7 @@ constexpr int PAGE = 64;
 // ---------------------------------------------------------------------------------------
 // A page of one key/value head, both planes.  e4m3 times a power of two is a bfloat16 value: nothing is rounded (below 2^-133 apart).  Rows
 // behind the sequence's last become zeros, since the prompt kernel reads whole pages; pages that hold a NaN among the values are marked.
+// Bound by memory: 12,000 rows of 16 heads of 128, 49 MB in and 98 MB out, some 20 us of the prompt's 168.
 // ---------------------------------------------------------------------------------------
 __device__ __forceinline__ uint32_t bf16x2_of(uint32_t two, float scale) {
     const uint32_t h = c8_half2(two);
@@ -78,7 +79,8 @@ __global__ void __launch_bounds__(256) expand8_kernel(Cache8 c, const int* __res
 // running maximum.  A CTA keeps 128 keys of one key/value head as the left operand and lets the query tiles that see them pass, so that a
 // thread holds one key's scores against 128 rows and adds them up in its own register: no reduction, no atomics, one writer per sum and a
 // fixed order.  Two accumulators in tensor memory, one for each of two groups of four warps: one group's exponentials (the bound: 16,384 a
-// tile at 16 a cycle and SM) run beside the other's product.  Two CTAs share an SM.
+// tile at 16 a cycle and SM) run beside the other's product.  Two CTAs share an SM.  A prompt of 2,048 rows, 16 heads of 128: 18 us (the CTA
+// of the first keys walks 16 tiles, the last one's one), where the same sums on mma.sync, each query tile converted for 64 keys, took 650.
 //   warp 0   TMA: the keys once, then query tiles through a ring      warp 1   owns tensor memory, issues S = K Q^T
 //   warps 2..5 and 6..9   every other tile each
 // ---------------------------------------------------------------------------------------

@@ -225,9 +225,9 @@ def prefill_rows(q: torch.Tensor, cache_layer: torch.Tensor, planes: int, cu_seq
                  page_table: torch.Tensor, page_size: int, window: int, scale: float, out: torch.Tensor, n_seqs: int, max_q_len: int,
                  n_heads: int, n_kv_heads: int, dk: int, dv: int, keep_first: int = 0, cell: int = 0, softcap: float = 0.0,
                  bias_t: Optional[torch.Tensor] = None, sink: Optional[torch.Tensor] = None,
-                 status: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None) -> torch.Tensor:
+                 status: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The tensor-core prompt kernel over a cache of two planes (keys, values) or one (rows [key | value]), with the
-    options of `kernels.bias_attention.attention_runs`.  lse [T, n_heads] float32: receives the base-2 logarithm of each row's denominator."""
+    options of `kernels.bias_attention.attention_runs`."""
     if status is None:
         from .gemm_tc import status_word
         status = status_word(q.device)
@@ -238,7 +238,7 @@ def prefill_rows(q: torch.Tensor, cache_layer: torch.Tensor, planes: int, cu_seq
     check("attention_prefill", load_kernel("attention_prefill").tq_attention_prefill(
         ptr(q), ptr(cache_layer), planes, ptr(cu_seqlens), ptr(seq_start), ptr(page_table), page_table.shape[1],
         *ints(page_size, cache_layer.shape[0], window, keep_first, cell), c_float(scale), c_float(softcap), ptr(bias_t),
-        0 if bias_t is None else bias_t.shape[1] - 1, ptr(sink), ptr(out), ptr(lse),
+        0 if bias_t is None else bias_t.shape[1] - 1, ptr(sink), ptr(out), None,
         *ints(q.shape[0], n_seqs, max_q_len, n_heads, n_kv_heads, dk, dv), ptr(status), stream()))
     return out
 
@@ -263,22 +263,6 @@ def prefill_pieces(n_tokens: int, n_seqs: int, max_q_len: int, max_kv_len: int, 
     if most < 2 or steps < SPLIT_FROM or 4 * pieces * n_tokens * n_heads * (head_dim + 1) > SPLIT_BYTES:
         return 1, 0
     return pieces, 2 * piece
-
-
-def prefill_split(q: torch.Tensor, cache_layer: torch.Tensor, cu_seqlens: torch.Tensor, seq_start: torch.Tensor, page_table: torch.Tensor, page_size: int,
-                  window: int, scale: float, out: torch.Tensor, n_seqs: int, max_q_len: int, n_heads: int, n_kv_heads: int, head_dim: int, pieces: int, pages: int,
-                  status: torch.Tensor, lse: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """attention_prefill with every unit's keys cut into `pieces` of `pages` pages (prefill_pieces), joined by a second launch."""
-    T = q.shape[0]
-    if any(t.dtype != torch.bfloat16 for t in (q, cache_layer, out)) or any(t.dtype != torch.int32 for t in (cu_seqlens, seq_start, page_table)):
-        raise KernelError("attention_prefill: queries, cache and output must be bfloat16, cu_seqlens, seq_start and the page table int32")
-    scratch = torch.empty(pieces * T * n_heads * (head_dim + 1), dtype=torch.float32, device=q.device)
-    part, part_lse = scratch[:pieces * T * n_heads * head_dim], scratch[pieces * T * n_heads * head_dim:]
-    check("attention_prefill", load_kernel("attention_prefill").tq_attention_prefill_split(
-        ptr(q), ptr(cache_layer), ptr(cu_seqlens), ptr(seq_start), ptr(page_table), page_table.shape[1], *ints(page_size, cache_layer.shape[0], window),
-        c_float(scale), ptr(out), ptr(lse), ptr(part), ptr(part_lse), *ints(pieces, pages, T, n_seqs, max_q_len, n_heads, n_kv_heads, head_dim), ptr(status),
-        stream()), kernels=2)
-    return out
 
 
 def dense_usable(dtype: torch.dtype, dim: int, rot: int, vdim: int, page_size: int) -> bool:

@@ -23,7 +23,7 @@ import torch
 
 from ..csrc.build import load_kernel
 from ._call import KernelError, addresses, check, code, declared, packed, want_int32
-from .attention import PAIRING, prefill_pieces, prefill_rows, prefill_split, prefill_usable, resident_ctas
+from .attention import PAIRING, prefill_pieces, prefill_usable, resident_ctas
 from .gemm_tc import status_word
 
 BLOCK = 16
@@ -34,6 +34,7 @@ _PACKED = {"tq_write8": "12P11i", "tq_attention8": "12P13if", "tq_evict8": "8P9i
 _SIGNATURES = {              # argument types of the others (_call.declared)
     "tq_weigh8": "pppippp" "iiifpp" "iiiiii" "p", "tq_repair8": "pppppp" "iiifppi" "iiiii" "p",
     "tq_expand8": "ppppp" "iiipppi" "iiii" "p", "tq_weigh8_prompt": "ppippp" "iifpp" "iiiiiii" "pp",
+    "tq_attention_prefill": "ppippp" "iiiiii" "ffpippp" "iiiiiii" "pp", "tq_attention_prefill_split": "ppppp" "iiiifpppp" "iiiiiiii" "pp",
 }
 _entries = {}
 
@@ -53,6 +54,10 @@ def _attention8(name: str):
 
 def _prompt8(name: str):
     return _entries.get(name) or _declare(load_kernel("prompt8"), name)
+
+
+def _attention_prefill(name: str):
+    return _entries.get(name) or _declare(load_kernel("attention_prefill"), name)
 
 
 def _evict(name: str):
@@ -247,36 +252,42 @@ DENSE_BYTES = 1 << 30        # scratch a step may take for pages in bfloat16; se
 def _attention8_prompt(q, codes, scales, cu_seqlens, held, page_table, page_size, window, scale, out, n_heads, n_kv_heads, head_dim, max_q_len,
                        max_kv_len, weights, status):
     """The pages a step sees are expanded to bfloat16 pages of a scratch, exactly, and the prompt kernel of csrc/attention_prefill.cu reads those."""
-    T, n = q.shape[0], page_table.shape[0]
+    T, (n, columns), pages = q.shape[0], page_table.shape, codes.shape[0]
     if status is None:
         status = status_word(q.device)
+    p_q, p_out, p_codes, p_scales, p_cu, p_held, p_table, p_weights, p_status, at = addresses(
+        q, out, codes, scales, cu_seqlens, held, page_table, weights, status)
     width = -(-max_kv_len // page_size)
     page_bytes = 2 * n_kv_heads * page_size * head_dim * 2
     group = max(1, min(n, DENSE_BYTES // (page_bytes * width)))
-    dense = torch.empty((group * width, 2, n_kv_heads, page_size, head_dim), dtype=torch.bfloat16, device=q.device)
-    table = torch.empty((group, width), dtype=torch.int32, device=q.device)
-    lost = torch.empty((group, n_kv_heads, width), dtype=torch.uint8, device=q.device)
-    lse = torch.empty((T, n_heads), dtype=torch.float32, device=q.device) if weights is not None else None
-    p_q, p_out, p_codes, p_scales, p_dense, p_tables, p_lost, p_lse, p_weights, p_status, at = addresses(
-        q, out, codes, scales, dense, table, lost, lse, weights, status)
-    pages = codes.shape[0]
-    pieces, piece_pages = prefill_pieces(T, min(group, n), max_q_len, max_kv_len, n_heads, n_kv_heads, head_dim, window, _sms(q)) \
-        if scale > 0.0 else (1, 0)
+    pieces, piece_pages = prefill_pieces(T, group, max_q_len, max_kv_len, n_heads, n_kv_heads, head_dim, window, _sms(q)) if scale > 0.0 else (1, 0)
+    # one allocation: the pages, the rows' denominators and the pieces' results (float32), the page table (int32), the pages' marks (bytes)
+    rows = T * n_heads
+    sizes = (group * width * page_bytes, 4 * rows if weights is not None else 0, 4 * rows * pieces * (head_dim + 1) if pieces > 1 else 0, 4 * group * width,
+             group * n_kv_heads * width)
+    scratch = torch.empty(sum(sizes) + 64, dtype=torch.uint8, device=q.device)
+    dense = scratch.data_ptr()
+    lse = dense + sizes[0]
+    part = -(-(lse + sizes[1]) // 16) * 16
+    tables = part + sizes[2]
+    lost = tables + sizes[3]
+    p_lse = lse if weights is not None else 0
     for i in range(0, n, group):
-        m = min(group, n - i)
-        cu, starts, own_pages = cu_seqlens[i:i + m + 1], held[i:i + m], page_table[i:i + m]
-        p_cu, p_held, p_table, _ = addresses(cu, starts, own_pages)
-        cache = (p_codes, p_scales, p_cu, p_held, p_table, page_table.shape[1], page_size, window)
-        check("prompt8", _prompt8("tq_expand8")(*cache, p_dense, p_tables, p_lost, width, pages, m, n_kv_heads, head_dim, at))
+        m, cu, starts, own = min(group, n - i), p_cu + 4 * i, p_held + 4 * i, p_table + 4 * i * columns
+        cache = (p_codes, p_scales, cu, starts, own, columns, page_size, window)
+        check("prompt8", _prompt8("tq_expand8")(*cache, dense, tables, lost, width, pages, m, n_kv_heads, head_dim, at))
         if pieces > 1:
-            prefill_split(q, dense, cu, starts, table[:m], page_size, window, scale, out, m, max_q_len, n_heads, n_kv_heads, head_dim, pieces, piece_pages,
-                          status, lse=lse)
+            check("attention_prefill", _attention_prefill("tq_attention_prefill_split")(
+                p_q, dense, cu, starts, tables, width, page_size, group * width, window, scale, p_out, p_lse, part, part + 4 * rows * pieces * head_dim,
+                pieces, piece_pages, T, m, max_q_len, n_heads, n_kv_heads, head_dim, p_status, at), kernels=2)
         else:
-            prefill_rows(q, dense, 2, cu, starts, table[:m], page_size, window, scale, out, m, max_q_len, n_heads, n_kv_heads, head_dim, head_dim, status=status, lse=lse)
-        check("attention8", _attention8("tq_repair8")(p_q, *cache, scale, p_out, p_lost, width, pages, m, n_heads, n_kv_heads, head_dim, at))
+            check("attention_prefill", _attention_prefill("tq_attention_prefill")(
+                p_q, dense, 2, cu, starts, tables, width, page_size, group * width, window, 0, 0, scale, 0.0, 0, 0, 0, p_out, p_lse, T, m, max_q_len,
+                n_heads, n_kv_heads, head_dim, head_dim, p_status, at))
+        check("attention8", _attention8("tq_repair8")(p_q, *cache, scale, p_out, lost, width, pages, m, n_heads, n_kv_heads, head_dim, at))
         if weights is not None:
             check("prompt8", _prompt8("tq_weigh8_prompt")(
-                p_q, p_dense, width, p_cu, p_held, p_table, page_table.shape[1], window, scale, p_lse, p_weights, pages, T, m, max_kv_len,
+                p_q, dense, width, cu, starts, own, columns, window, scale, p_lse, p_weights, pages, T, m, max_kv_len,
                 n_heads, n_kv_heads, head_dim, p_status, at))
     return out
 
