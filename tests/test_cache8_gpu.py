@@ -446,3 +446,48 @@ def test_queries_alone(runs, held):
     assert torch.equal(*both)
     with pytest.raises(Exception):
         cache8.write_rows8(qkv, bias, None, None, "half", positions, _cu(runs), _i(held), table.to(DEV), 64, both[0], None, scales.to(DEV), H, G, D, max(runs))
+
+
+@pytest.mark.parametrize("shape", [(28, 4, 128), (16, 16, 128), (8, 2, 64), (4, 2, 80), (3, 1, 256), (5, 1, 48)], ids=str)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("pairing,biased", [("half", True), ("interleaved", False), ("half", None)])
+def test_long_prompts_are_written_as_their_pieces_are(shape, dtype, pairing, biased):
+    """One step of long prompts, whose threads go through several heads, leaves the bits that steps of 48 rows leave: they end where a block does."""
+    from turboquant_cpp_b200.kernels import cache8
+    H, G, D = shape
+    runs, held, page_size = [1600, 3, 1, 700, 0, 33, 16, 900], [21, 0, 15, 16, 7, 31, 64, 5], 32
+    table, pages = _pages([n + h for n, h in zip(runs, held)], page_size)
+    codes, scales = _cache(pages, G, page_size, D)
+    T = sum(runs)
+    qkv = torch.randn(T, (H + 2 * G) * D, device=DEV) * torch.exp(2 * torch.randn(T, 1, device=DEV))
+    for value in (math.inf, -math.inf, math.nan):
+        qkv.view(-1)[torch.randint(0, qkv.numel(), (400,), device=DEV)] = value
+    qkv = qkv.to(dtype)
+    bias = None if biased is None else torch.randn((H + 2 * G) * D, device=DEV).to(torch.bfloat16 if biased else dtype)
+    angle = torch.rand(1000, D // 2, device=DEV) * 6.3
+    cos, sin = torch.cos(angle), torch.sin(angle)
+    positions = torch.randint(0, 1000, (T,), dtype=torch.int32, device=DEV)
+    dev_table = table.to(DEV)
+
+    def write(rows, runs, held, codes, scales, q):
+        cache8.write_rows8(qkv[rows].contiguous(), bias, cos, sin, pairing, positions[rows].contiguous(), _cu(runs), _i(held), dev_table, page_size, q, codes, scales,
+                           H, G, D, max(runs))
+
+    everything = torch.arange(T, device=DEV)
+    got_q, got_codes, got_scales = torch.empty(T, H, D, dtype=dtype, device=DEV), _on(codes), scales.to(DEV)
+    write(everything, runs, held, got_codes, got_scales, got_q)
+    alone = torch.empty_like(got_q)
+    write(everything, runs, held, None, None, alone)
+    want_q, want_codes, want_scales = torch.empty_like(got_q), _on(codes), scales.to(DEV)
+    starts, done = [sum(runs[:i]) for i in range(len(runs))], [0] * len(runs)
+    while done != runs:
+        now = [min(n - d, 48 - (h + d) % 16) for n, d, h in zip(runs, done, held)]
+        rows = torch.tensor([s + d + i for s, d, n in zip(starts, done, now) for i in range(n)], device=DEV)
+        q = torch.empty(len(rows), H, D, dtype=dtype, device=DEV)
+        write(rows, now, [h + d for h, d in zip(held, done)], want_codes, want_scales, q)
+        want_q[rows] = q
+        done = [d + n for d, n in zip(done, now)]
+    assert torch.equal(got_scales, want_scales)
+    assert torch.equal(got_codes.view(torch.uint8), want_codes.view(torch.uint8))
+    bits = torch.int16 if dtype == torch.bfloat16 else torch.int32
+    assert torch.equal(got_q.view(bits), want_q.view(bits)) and torch.equal(alone.view(bits), want_q.view(bits))

@@ -9,17 +9,28 @@ namespace {
 
 // Eight consecutive elements as float32, in pairs for the packed operations.
 struct Eight { tq_f32x2 p[4]; };
-__device__ __forceinline__ Eight load8(const __nv_bfloat16* p) {
-    const uint4 v = *reinterpret_cast<const uint4*>(p);
-    const uint32_t u[4] = {v.x, v.y, v.z, v.w};
-    Eight r;
+// the same as they lie in memory
+template <typename T> struct Raw;
+template <> struct Raw<__nv_bfloat16> {
+    uint4 v;
+    __device__ __forceinline__ void load(const __nv_bfloat16* p) { v = *reinterpret_cast<const uint4*>(p); }
+    __device__ __forceinline__ Eight wide() const {
+        const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+        Eight r;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) r.p[i] = tq_pack2(__uint_as_float(u[i] << 16), __uint_as_float(u[i] & 0xffff0000u));
-    return r;
-}
+        for (int i = 0; i < 4; ++i) r.p[i] = tq_pack2(__uint_as_float(u[i] << 16), __uint_as_float(u[i] & 0xffff0000u));
+        return r;
+    }
+};
+template <> struct Raw<float> {
+    float4 a, b;
+    __device__ __forceinline__ void load(const float* p) { a = *reinterpret_cast<const float4*>(p); b = *reinterpret_cast<const float4*>(p + 4); }
+    __device__ __forceinline__ Eight wide() const { return Eight{{tq_pack2(a.x, a.y), tq_pack2(a.z, a.w), tq_pack2(b.x, b.y), tq_pack2(b.z, b.w)}}; }
+};
 __device__ __forceinline__ Eight load8(const float* p) {
-    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-    return Eight{{tq_pack2(a.x, a.y), tq_pack2(a.z, a.w), tq_pack2(b.x, b.y), tq_pack2(b.z, b.w)}};
+    Raw<float> r;
+    r.load(p);
+    return r.wide();
 }
 __device__ __forceinline__ void store8(__nv_bfloat16* p, const Eight& f) {
     uint32_t u[4];
@@ -70,7 +81,7 @@ __device__ __forceinline__ uint2 encode8(const Eight& f, tq_f32x2 inv, bool infi
 
 // ---------------------------------------------------------------------------------------
 // The writer.  A unit is the rows a sequence brings into one block of 16, of one head, query heads among them.  An item is eight rotation
-// pairs of a row: 16 elements, two 16-byte loads of bfloat16 and two 8-byte stores of codes; a thread has one item, so that all of a unit's
+// pairs of a row: 16 elements, two 16-byte loads of bfloat16 and two 8-byte stores of codes; a thread has one item of a unit, so that all of its
 // loads are under way at once, and keeps it in registers between the block's largest magnitude (a reduction over the unit's threads) and
 // its codes.  Rows the block holds already are rounded again by the same threads when its byte grows.
 // Single tokens (RUNS false): a warp per unit.  Runs: head size threads per unit, rounded up to warps, so a thread for each of a whole
@@ -82,123 +93,150 @@ __device__ __forceinline__ uint2 encode8(const Eight& f, tq_f32x2 inv, bool infi
 struct WriteArgs {
     const float *cos_t, *sin_t;
     const int *positions, *cu_seqlens, *held;
-    int nh, pairing, written;          // written: the heads this launch takes (the queries alone, or all)
+    int nh, pairing, written, each;    // written: the heads this launch takes (the queries alone, or all); each: units a thread takes one after another
 };
 
-constexpr int WRITE_THREADS = 256;      // (512: 35 us for the prompts above, 31.5; five blocks an SM instead of four: 29.8)
+// Runs of many rows: a thread goes through the items of up to WRITE_EACH heads, so that the cosines and sines, twice the bytes of a bfloat16 item,
+// are fetched once, and the next item is on its way while one is worked on (prompts above, heads a thread: one 33 us, two 27, three 25.7, four
+// 25.5, six 26.8, eight 29.5; before, each head with its own cosines, 29.8).  Not where fewer than WRITE_FILL blocks would be left a turn.
+constexpr int WRITE_EACH = 4, WRITE_FILL = 148 * 4;
+constexpr int WRITE_THREADS = 256;
 
-// HD: the head size, or 0 where it is known at the launch only
+// HD: the head size, or 0 where it is known at the launch only.  Blocks an SM: of float32, whose items take twice the registers, 3 (4,096 rows of
+// 28 + 4 + 4 heads: 30.5 us, with the bias asked for ahead 34, and 39 with four blocks).  The bias of bfloat16 is asked for ahead (prompts above: 25.7
+// us, else 28).
 template <typename TA, typename TB, bool RUNS, int HD>
-__global__ void __launch_bounds__(WRITE_THREADS, RUNS && HD ? 5 : 1) write8_kernel(const TA* __restrict__ qkv, const TB* __restrict__ bias, WriteArgs a, TA* __restrict__ q_out, Cache8 c,
-                                                               int threads_) {
+__global__ void __launch_bounds__(WRITE_THREADS, RUNS ? HD == 128 && sizeof(TA) == 2 ? 4 : 3 : 1) write8_kernel(const TA* __restrict__ qkv, const TB* __restrict__ bias, WriteArgs a,
+                                                                                                                 TA* __restrict__ q_out, Cache8 c, int threads_) {
     tq_grid_wait();                    // everything below may read what the previous kernel wrote
     tq_grid_launch_dependents();
-    __shared__ float s_top[WRITE_THREADS / 32];
+    __shared__ float s_top[3][WRITE_THREADS / 32];
     const int hd = HD ? HD : c.hd, threads = !RUNS ? 32 : HD ? HD : threads_;
     const int unit = threadIdx.x / threads, it = threadIdx.x - unit * threads, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int j = blockIdx.y * (blockDim.x / threads) + unit, heads = a.nh + 2 * c.nkv;
+    const int side = RUNS && HD ? WRITE_THREADS / HD : blockDim.x / threads, warps = RUNS && HD ? WRITE_THREADS / 32 : blockDim.x / 32;
+    const int each = RUNS ? a.each : 1, j0 = blockIdx.y * side * each, heads = a.nh + 2 * c.nkv;
     const int seq = blockIdx.z, t_begin = a.cu_seqlens[seq], run = a.cu_seqlens[seq + 1] - t_begin;
     const int place0 = a.held[seq];
     const int block_start = (place0 / C8_BLOCK + (int)blockIdx.x) * C8_BLOCK;       // the unit's block, as a place
     const int first = max(block_start, place0), rows = min(block_start + C8_BLOCK, place0 + run) - first;
-    if (rows <= 0 || (!RUNS && j >= a.written)) return;              // (runs: the whole block of threads returns or stays)
+    if (rows <= 0 || (!RUNS && j0 + unit >= a.written)) return;      // (runs: the whole block of threads returns or stays)
     const int t0 = t_begin + first - place0, half = hd >> 1, groups = half >> 3, items = rows * groups;
-    const bool mine = it < items && j < a.written, is_q = j < a.nh;
     const int r = it / groups, i = (it - r * groups) * 8;
     const int ia = a.pairing == 0 ? i : 2 * i, ib = a.pairing == 0 ? i + half : 2 * i + 8;       // where the item's two halves lie in the head
-    // where the unit's codes go, and the byte of rows the block holds already, looked up beside the loads of the rows
-    const int plane = j >= a.nh + c.nkv ? 1 : 0, g = j - a.nh - plane * c.nkv, row0 = c.row(block_start), old = first - block_start;
-    uint8_t *codes = nullptr, *byte = nullptr;
-    uint32_t was = 1;
-    if (!is_q && j < a.written) {
-        const int page = c.page_of(seq, first);
-        codes = c.codes + c.codes_at(page, plane, g) + (size_t)row0 * hd;
-        byte = c.scales + c.scales_at(page, plane, g) + row0 / C8_BLOCK;
-        if (old > 0) was = max((uint32_t)*byte, 1u);                  // (by all of the unit's threads before one of them writes it)
+    const int row0 = c.row(block_start), old = first - block_start;
+    const TA* row = qkv + (size_t)(t0 + r) * heads * hd;
+    const bool inside = it < items;
+    Raw<TA> next_lo = {}, next_hi = {};
+    constexpr bool AHEAD = sizeof(TA) + sizeof(TB) == 4;             // the bias too
+    Raw<TB> bias_lo = {}, bias_hi = {};
+    auto ask = [&](int j) {
+        if (!inside || j >= a.written) return;
+        next_lo.load(row + j * hd + ia);
+        next_hi.load(row + j * hd + ib);
+        if (AHEAD && bias != nullptr) { bias_lo.load(bias + j * hd + ia); bias_hi.load(bias + j * hd + ib); }
+    };
+    ask(j0 + unit);
+    const int page = a.written > a.nh ? c.page_of(seq, first) : 0;
+    Eight cs = {}, sn = {};
+    if (inside && j0 + unit < a.nh + c.nkv && a.cos_t != nullptr) {
+        const size_t at = (size_t)a.positions[t0 + r] * half + i;
+        cs = load8(a.cos_t + at);
+        sn = load8(a.sin_t + at);
     }
-    Eight lo = {}, hi = {};
-    if (mine) {
-        const TA* row = qkv + ((size_t)(t0 + r) * heads + j) * hd;
-        const bool rotated = j < a.nh + c.nkv && a.cos_t != nullptr;
-        lo = load8(row + ia);
-        hi = load8(row + ib);
-        Eight cs = {}, sn = {};
-        if (rotated) {
-            const size_t at = (size_t)a.positions[t0 + r] * half + i;
-            cs = load8(a.cos_t + at);
-            sn = load8(a.sin_t + at);
+    for (int k = 0; k < each; ++k) {
+        const int j = j0 + k * side + unit;
+        if (RUNS && j0 + k * side >= a.written) break;
+        const bool mine = inside && j < a.written, is_q = j < a.nh;
+        // where the unit's codes go, and the byte of rows the block holds already
+        const int plane = j >= a.nh + c.nkv ? 1 : 0, g = j - a.nh - plane * c.nkv;
+        uint8_t *codes = nullptr, *byte = nullptr;
+        uint32_t was = 1;
+        if (!is_q && j < a.written) {
+            codes = c.codes + c.codes_at(page, plane, g) + (size_t)row0 * hd;
+            byte = c.scales + c.scales_at(page, plane, g) + row0 / C8_BLOCK;
+            if (old > 0) was = max((uint32_t)*byte, 1u);              // (by all of the unit's threads before one of them writes it)
         }
-        if (bias != nullptr) {
-            const Eight x = load8(bias + (size_t)j * hd + ia), y = load8(bias + (size_t)j * hd + ib);
+        Eight lo = next_lo.wide(), hi = next_hi.wide();
+        if (bias != nullptr && mine) {
+            Raw<TB> bias0 = bias_lo, bias1 = bias_hi;
+            if (!AHEAD) { bias0.load(bias + j * hd + ia); bias1.load(bias + j * hd + ib); }
+            const Eight x = bias0.wide(), y = bias1.wide();
 #pragma unroll
             for (int e = 0; e < 4; ++e) { lo.p[e] = tq_add2(lo.p[e], x.p[e]); hi.p[e] = tq_add2(hi.p[e], y.p[e]); }
         }
-        if (rotated) {
-            // interleaved: the pairs' first elements together and their second ones, and back
-            auto sort = [](Eight& x, Eight& y) {
-                const float2 p[8] = {tq_unpack2(x.p[0]), tq_unpack2(x.p[1]), tq_unpack2(x.p[2]), tq_unpack2(x.p[3]),
-                                     tq_unpack2(y.p[0]), tq_unpack2(y.p[1]), tq_unpack2(y.p[2]), tq_unpack2(y.p[3])};
+        if (RUNS && k + 1 < each) ask(j + side);                      // on its way while this one is worked on
+        if (mine) {
+            if (j < a.nh + c.nkv && a.cos_t != nullptr) {
+                // interleaved: the pairs' first elements together and their second ones, and back
+                auto sort = [](Eight& x, Eight& y) {
+                    const float2 p[8] = {tq_unpack2(x.p[0]), tq_unpack2(x.p[1]), tq_unpack2(x.p[2]), tq_unpack2(x.p[3]),
+                                         tq_unpack2(y.p[0]), tq_unpack2(y.p[1]), tq_unpack2(y.p[2]), tq_unpack2(y.p[3])};
 #pragma unroll
-                for (int e = 0; e < 4; ++e) { x.p[e] = tq_pack2(p[2 * e].x, p[2 * e + 1].x); y.p[e] = tq_pack2(p[2 * e].y, p[2 * e + 1].y); }
-            };
-            if (a.pairing != 0) sort(lo, hi);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                // (the packed product and sum came out fused, their .rn notwithstanding)
-                const float2 u = tq_unpack2(lo.p[e]), v = tq_unpack2(hi.p[e]), x = tq_unpack2(cs.p[e]), y = tq_unpack2(sn.p[e]);
-                lo.p[e] = tq_pack2(__fsub_rn(__fmul_rn(u.x, x.x), __fmul_rn(v.x, y.x)), __fsub_rn(__fmul_rn(u.y, x.y), __fmul_rn(v.y, y.y)));
-                hi.p[e] = tq_pack2(__fadd_rn(__fmul_rn(u.x, y.x), __fmul_rn(v.x, x.x)), __fadd_rn(__fmul_rn(u.y, y.y), __fmul_rn(v.y, x.y)));
-            }
-            if (a.pairing != 0) {
-                const Eight u = lo, v = hi;
+                    for (int e = 0; e < 4; ++e) { x.p[e] = tq_pack2(p[2 * e].x, p[2 * e + 1].x); y.p[e] = tq_pack2(p[2 * e].y, p[2 * e + 1].y); }
+                };
+                if (a.pairing != 0) sort(lo, hi);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const float2 x = tq_unpack2(u.p[e]), y = tq_unpack2(v.p[e]);
-                    Eight& to = e < 2 ? lo : hi;
-                    to.p[2 * (e & 1)] = tq_pack2(x.x, y.x);
-                    to.p[2 * (e & 1) + 1] = tq_pack2(x.y, y.y);
+                    // (the packed product and sum came out fused, their .rn notwithstanding)
+                    const float2 u = tq_unpack2(lo.p[e]), v = tq_unpack2(hi.p[e]), x = tq_unpack2(cs.p[e]), y = tq_unpack2(sn.p[e]);
+                    lo.p[e] = tq_pack2(__fsub_rn(__fmul_rn(u.x, x.x), __fmul_rn(v.x, y.x)), __fsub_rn(__fmul_rn(u.y, x.y), __fmul_rn(v.y, y.y)));
+                    hi.p[e] = tq_pack2(__fadd_rn(__fmul_rn(u.x, y.x), __fmul_rn(v.x, x.x)), __fadd_rn(__fmul_rn(u.y, y.y), __fmul_rn(v.y, x.y)));
+                }
+                if (a.pairing != 0) {
+                    const Eight u = lo, v = hi;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float2 x = tq_unpack2(u.p[e]), y = tq_unpack2(v.p[e]);
+                        Eight& to = e < 2 ? lo : hi;
+                        to.p[2 * (e & 1)] = tq_pack2(x.x, y.x);
+                        to.p[2 * (e & 1) + 1] = tq_pack2(x.y, y.y);
+                    }
                 }
             }
+            if (is_q) {
+                TA* d = q_out + ((size_t)(t0 + r) * a.nh + j) * hd;
+                store8(d + ia, lo);
+                store8(d + ib, hi);
+            }
         }
-        if (is_q) {
-            TA* d = q_out + ((size_t)(t0 + r) * a.nh + j) * hd;
-            store8(d + ia, lo);
-            store8(d + ib, hi);
+        // queries only (runs: all of the block's units, since the others' reductions are the block's)
+        if (RUNS ? min(j0 + (k + 1) * side, a.written) <= a.nh : is_q) continue;
+        // over the unit's threads; most: over the block's, where a block is several warps
+        float most;
+        auto over_unit = [&](float top, float* tops) {
+            top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));       // magnitudes: ordered as integers are
+            most = top;
+            if (RUNS) {
+                if (lane == 0) tops[warp] = top;
+                __syncthreads();
+                for (int w = 0; w < warps; ++w) most = fmaxf(most, tops[w]);
+                for (int w = unit * (threads / 32); w < (unit + 1) * (threads / 32); ++w) top = fmaxf(top, tops[w]);
+            }
+            return top;
+        };
+        float top = over_unit(mine ? magnitude8(hi, magnitude8(lo, 0.f)) : 0.f, s_top[k & 1]);       // (s_top's other half is read until the next barrier)
+        const bool infinite = top == INFINITY;
+        if (most == INFINITY) {
+            const float finite = over_unit(mine ? finite8(hi, finite8(lo, 0.f)) : 0.f, s_top[2]);
+            if (infinite) top = finite;
         }
-    }
-    if (a.written == a.nh) return;                                    // queries only
-    // over the unit's threads
-    auto over_unit = [&](float top) {
-        top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));       // magnitudes: ordered as integers are
-        if (RUNS) {
-            if (lane == 0) s_top[warp] = top;
-            __syncthreads();
-            for (int w = unit * (threads / 32); w < (unit + 1) * (threads / 32); ++w) top = fmaxf(top, s_top[w]);
+        if (codes == nullptr) continue;
+        const uint32_t b = max(c8_byte(__float_as_uint(top)), was);
+        if (mine) {
+            const float inv = c8_inverse(b);
+            uint8_t* d = codes + (size_t)(old + r) * hd;
+            *reinterpret_cast<uint2*>(d + ia) = encode8(lo, tq_pack2(inv, inv), infinite);
+            *reinterpret_cast<uint2*>(d + ib) = encode8(hi, tq_pack2(inv, inv), infinite);
         }
-        return top;
-    };
-    float top = over_unit(magnitude8(hi, magnitude8(lo, 0.f)));
-    const bool infinite = top == INFINITY;
-    if (RUNS ? __syncthreads_or(infinite) : infinite) {
-        const float finite = over_unit(finite8(hi, finite8(lo, 0.f)));
-        if (infinite) top = finite;
-    }
-    if (codes == nullptr) return;
-    const uint32_t b = max(c8_byte(__float_as_uint(top)), was);
-    if (mine) {
-        const float inv = c8_inverse(b);
-        uint8_t* d = codes + (size_t)(old + r) * hd;
-        *reinterpret_cast<uint2*>(d + ia) = encode8(lo, tq_pack2(inv, inv), infinite);
-        *reinterpret_cast<uint2*>(d + ib) = encode8(hi, tq_pack2(inv, inv), infinite);
-    }
-    if (b > was && old > 0) {
-        const uint32_t factor = c8_shift_factor((int)min(b - was, 25u));
-        for (int v = it; v < old * (hd / 16); v += threads) {
-            uint4* p = reinterpret_cast<uint4*>(codes) + v;
-            *p = c8_shift16(*p, factor);
+        if (b > was && old > 0) {
+            const uint32_t factor = c8_shift_factor((int)min(b - was, 25u));
+            for (int v = it; v < old * (hd / 16); v += threads) {
+                uint4* p = reinterpret_cast<uint4*>(codes) + v;
+                *p = c8_shift16(*p, factor);
+            }
         }
+        if (it == 0) *byte = (uint8_t)b;
     }
-    if (it == 0) *byte = (uint8_t)b;
 }
 
 }  // namespace
@@ -226,12 +264,14 @@ TQ_EXPORT int tq_write8(const void* packed) {
     TQ_REQUIRE(n_seqs <= 65535 && max_q_len >= 1, "write8: %d sequences, longest run %d", n_seqs, max_q_len);
     TQ_REQUIRE(((uintptr_t)qkv | (uintptr_t)bias | (uintptr_t)x.q_out | (uintptr_t)cos_t | (uintptr_t)sin_t) % 16 == 0, "write8: tensors must be 16-byte aligned");
     const Cache8 c = c8_cache(codes, scales, x.page_table, x.table_stride, page_size, n_pages, nkv, hd);
-    const WriteArgs a{cos_t, sin_t, x.positions, x.cu_seqlens, x.held, nh, x.pairing, codes != nullptr ? nh + 2 * nkv : nh};
+    WriteArgs a{cos_t, sin_t, x.positions, x.cu_seqlens, x.held, nh, x.pairing, codes != nullptr ? nh + 2 * nkv : nh, 1};
     // a run of n rows touches at most (n + 14) / 16 + 1 blocks
     const bool runs = max_q_len > 1;
     const int units = runs ? (max_q_len + 14) / C8_BLOCK + 1 : 1, threads = runs ? (hd + 31) / 32 * 32 : 32;
     const int side = runs ? WRITE_THREADS / threads : n_seqs >= 32 ? 8 : 2;              // units a block takes side by side
-    const dim3 grid(units, (a.written + side - 1) / side, n_seqs);
+    const long long blocks = (long long)units * ((a.written + side - 1) / side) * n_seqs;
+    a.each = runs ? (int)max(1ll, min((long long)WRITE_EACH, blocks / WRITE_FILL)) : 1;
+    const dim3 grid(units, (a.written + side * a.each - 1) / (side * a.each), n_seqs);
     TQ_DISPATCH(x.act_dtype, TA, TQ_DISPATCH(bias != nullptr ? x.bias_dtype : x.act_dtype, TB,
         auto kernel = runs ? (hd == 128 ? write8_kernel<TA, TB, true, 128> : hd == 64 ? write8_kernel<TA, TB, true, 64> : write8_kernel<TA, TB, true, 0>)
                            : (hd == 128 ? write8_kernel<TA, TB, false, 128> : write8_kernel<TA, TB, false, 0>);
