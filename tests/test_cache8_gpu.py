@@ -312,6 +312,52 @@ def test_eviction_keeps_the_rows_it_should(shape, kind, case):
     assert torch.equal(torch.nan_to_num(got_w.cpu().double(), nan=-7.0), torch.nan_to_num(want_w, nan=-7.0))
 
 
+@pytest.mark.parametrize("lengths,budget,recent", [([60000, 3000, 49300], 5000, 70), ([1023, 1024, 1025, 1100], 900, 0), ([4100, 8200, 2049], 1900, 130)])
+@pytest.mark.parametrize("close", [0, 3, 63, 64, 65, 900])
+@pytest.mark.parametrize("page_size", [48, 64])
+def test_rows_whose_weights_lie_close_together(lengths, budget, recent, close, page_size):
+    """`close` rows around the last that stays differ in the lowest bits alone, or not at all; sequences of more rows than a block keeps among them."""
+    from turboquant_cpp_b200.kernels import cache8
+    G, D = 2, 16
+    per = -(-budget // page_size)
+    table, pages = _pages(lengths, page_size, spare=per * len(lengths))
+    taken = set(table.flatten().tolist())
+    new_table = torch.tensor([p for p in range(pages) if p not in taken], dtype=torch.int32).view(len(lengths), per)
+    codes, scales = torch.zeros(pages, 2, G, page_size, D, dtype=torch.uint8), torch.full((pages, 2, G, page_size // 16), 127, dtype=torch.uint8)
+    w = torch.zeros(pages, G, page_size)
+    want = torch.full((len(lengths), G, budget), -1, dtype=torch.int32)
+    want_w = torch.zeros(len(lengths), G, budget)
+    for s, n in enumerate(lengths):
+        places = torch.arange(n)
+        for g in range(G):
+            mine = torch.exp(4 * torch.randn(n)).clamp(1e-30, 1e30)
+            rest, keep = max(0, n - recent), budget - recent
+            if close and n > budget and rest > close:
+                order = torch.randperm(rest)
+                above = max(0, keep - (close + 1) // 2)                   # rows above the close ones
+                mine[order[:above]] = 4.0 + mine[order[:above]]
+                mine[order[above:above + close]] = 1.0 + torch.randint(0, 2 * close, (min(close, rest - above),)).float() * 2.0 ** -23
+                mine[order[above + close:]] = 0.9 / (1.0 + mine[order[above + close:]])
+            w[table[s, places // page_size].long(), g, places % page_size] = mine
+            kept = plain.kept_places(mine.tolist(), budget, recent)
+            want[s, g, :len(kept)] = torch.tensor(kept, dtype=torch.int32)
+            want_w[s, g, :len(kept)] = mine[kept]
+    got_w = w.to(DEV)
+    kept = cache8.evict8(_on(codes), scales.to(DEV), got_w, _i(lengths), table.to(DEV), new_table.to(DEV), page_size, budget, recent)
+    assert torch.equal(kept.cpu(), want)
+    moved = got_w.cpu()[new_table.long()].transpose(1, 2).reshape(len(lengths), G, -1)[:, :, :budget]
+    assert torch.equal(torch.where(want >= 0, moved, 0.0), want_w)
+
+
+def test_eviction_refuses_weights_that_are_not_aligned():
+    from turboquant_cpp_b200.kernels import cache8
+    from turboquant_cpp_b200.kernels._call import KernelError
+    codes, scales = cache8.storage(4, 1, 16, 16, DEV)[:2]
+    weights = torch.zeros(4 * 16 + 1, device=DEV)[1:].view(4, 1, 16)
+    with pytest.raises(KernelError, match="16-byte aligned"):
+        cache8.evict8(codes, scales, weights, _i([20]), _i([0, 1]).view(1, 2), _i([2]).view(1, 1), 16, 16, 4)
+
+
 # ---- together -----------------------------------------------------------------------------------------------------------
 def test_a_sequence_from_its_prompt_through_evictions(prompts):
     """Write, attend with sums, evict, go on: every step against the plain forms on the plain forms' own cache."""

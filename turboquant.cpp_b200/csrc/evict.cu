@@ -17,20 +17,28 @@ __device__ __forceinline__ uint32_t rank_of(float w) {
 }
 
 // ---------------------------------------------------------------------------------------
-// Selection: a block per (key/value head, sequence) finds the rank of the last row that stays, 11, 11 and 10 bits at a time from the highest
-// (a histogram of the rows that agree in the bits found), then lists the rows above it and, of those equal to it, the first ones.  The
-// ranks are read once, through the page table, and stay in shared memory as far as they fit (`cached` of them).  32 sequences of about 7,000 rows,
-// 4 heads: 14.6 us, of them 4.5 for the reads (two dependent ones a row), 7.2 for the histograms, 2.9 for the lists: latencies of one block an SM.
+// Selection: a block per (key/value head, sequence) finds the rank of the last row that stays, 11 bits at a time from the highest in which the
+// ranks differ at all (a histogram of the rows that agree in the bits found; once a bin holds few rows they are compared one by one), then
+// lists the rows above it and, of those equal to it, the first ones.  Ranks are counted from the smallest one, so that the first histogram
+// spreads over its bins: with the 11 highest bits of the float a handful of bins took all rows, and the additions to them queued.  A thread
+// takes four consecutive rows of a page, one load of it and one of the page table; the ranks stay in shared memory as far as they fit (`cached` of them).
+// 32 sequences of about 7,000 rows, 4 heads: 9 us, of them 2 for the reads, 5 for the histograms, 2 for the lists: latencies of one block an SM
+// (row by row, bits from the top: 14.6).  Where a row a thread covers a sequence that is shorter (960 rows of 16 heads, with the moving: 8.8 us, by
+// fours 10.3; 1,600 rows 8.9 and 8.4).
 // ---------------------------------------------------------------------------------------
-constexpr int SELECT_THREADS = 1024, SELECT_WARPS = SELECT_THREADS / 32, BINS = 2048;
+constexpr int SELECT_THREADS = 1024, SELECT_WARPS = SELECT_THREADS / 32, DIGIT = 11, BINS = 1 << DIGIT;
+constexpr int FEW = 64;                 // rows of a bin that are told apart one by one
 constexpr int SELECT_MOST = 48 * 1024;             // ranks a block keeps, 192 KB
 
+template <int PER>
 __global__ void __launch_bounds__(SELECT_THREADS) evict8_select_kernel(Cache8 c, const float* __restrict__ weights, const int* __restrict__ lengths, int budget, int recent,
                                                                        int cached, int* __restrict__ kept) {
     tq_grid_wait();                    // everything below may read what the previous kernel wrote
     tq_grid_launch_dependents();
-    extern __shared__ uint32_t s_rank[];
-    __shared__ int s_hist[BINS], s_pick[2], s_warp[2][SELECT_WARPS];
+    constexpr int ROUND = PER * SELECT_THREADS;        // rows the block looks at at once
+    extern __shared__ __align__(16) uint32_t s_rank[];
+    __shared__ uint32_t s_few[FEW];
+    __shared__ int s_hist[BINS], s_pick[4], s_warp[2][SELECT_WARPS], s_own[SELECT_WARPS];
     const int g = blockIdx.x, seq = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int n = max(0, min(lengths[seq], c.table_stride * c.page_size));
     int* list = kept + ((size_t)seq * c.nkv + g) * budget;
@@ -41,31 +49,64 @@ __global__ void __launch_bounds__(SELECT_THREADS) evict8_select_kernel(Cache8 c,
     const int rest = n - recent, want = budget - recent;              // of places 0 .. rest - 1 `want` stay
     for (int j = tid; j < recent; j += SELECT_THREADS) list[want + j] = rest + j;
     if (want == 0) return;
-    auto read = [&](int p) { return rank_of(weights[((size_t)c.page_of(seq, p) * c.nkv + g) * c.page_size + c.row(p)]); };
-    auto rank_at = [&](int p) { return p < cached ? s_rank[p] : read(p); };
-#pragma unroll 8
-    for (int p = tid; p < min(rest, cached); p += SELECT_THREADS) s_rank[p] = read(p);
-    uint32_t prefix = 0, known = 0;                                   // the bits found and which they are
+    // the ranks of places p .. p + PER - 1: one page has all of them
+    struct alignas(4 * PER) Ranks { uint32_t k[PER]; };
+    auto read = [&](int p) {
+        const float* w = weights + ((size_t)c.page_of(seq, p) * c.nkv + g) * c.page_size + c.row(p);
+        Ranks f;
+        if constexpr (PER == 4) {
+            const float4 v = *reinterpret_cast<const float4*>(w);
+            f = {{rank_of(v.x), rank_of(v.y), rank_of(v.z), rank_of(v.w)}};
+        } else f = {{rank_of(*w)}};
+        return f;
+    };
+    auto ranks = [&](int p) { return p >= rest ? Ranks{} : p < cached ? *reinterpret_cast<const Ranks*>(s_rank + p) : read(p); };
+    uint32_t least = 0xffffffffu, most = 0u;
+    for (int p = PER * tid; p < rest; p += ROUND) {
+        const Ranks f = read(p);
+        if (p < cached) *reinterpret_cast<Ranks*>(s_rank + p) = f;
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+            if (p + i < rest) { least = min(least, f.k[i]); most = max(most, f.k[i]); }
+    }
+    least = __reduce_min_sync(0xffffffffu, least);
+    most = __reduce_max_sync(0xffffffffu, most);
+    if (lane == 0) { s_warp[0][warp] = (int)least; s_warp[1][warp] = (int)most; }
+    __syncthreads();
+    least = __reduce_min_sync(0xffffffffu, (uint32_t)s_warp[0][lane]);
+    most = __reduce_max_sync(0xffffffffu, (uint32_t)s_warp[1][lane]);
+    uint32_t found = 0;                                               // the rank of the last row that stays, less `least`: its highest bits
     int missing = want;                                               // rows still to be found among those that agree with them
-    for (int pass = 0; pass < 3; ++pass) {
-        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : BINS;
-        for (int x = tid; x < bins; x += SELECT_THREADS) s_hist[x] = 0;
+    for (int left = 32 - __clz(most - least); left > 0;) {            // bits not yet found
+        const int shift = max(left - DIGIT, 0);
+        *reinterpret_cast<int2*>(s_hist + 2 * tid) = make_int2(0, 0);
         __syncthreads();
-        for (int p0 = 0; p0 < rest; p0 += SELECT_THREADS) {
-            const int p = p0 + tid;
-            const uint32_t k = p < rest ? rank_at(p) : 0u;
-            const bool counts = p < rest && (k & known) == prefix;
-            const int bin = counts ? (int)((k >> shift) & (uint32_t)(bins - 1)) : -1;
-            // the first lane's bin is counted once for all lanes that share it (rows that never received any weight are many)
-            const int lead = __shfl_sync(0xffffffffu, bin, 0);
-            const uint32_t same = __ballot_sync(0xffffffffu, bin == lead);
-            if (lead >= 0 && lane == 0) atomicAdd(&s_hist[lead], __popc(same));
-            if (bin >= 0 && bin != lead) atomicAdd(&s_hist[bin], 1);
+        for (int p0 = 0; p0 < rest; p0 += ROUND) {
+            const int p = p0 + PER * tid;
+            const Ranks f = ranks(p);
+            uint32_t d[PER];
+            bool counts[PER], any = false;
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                d[i] = (f.k[i] - least) ^ found;                      // found: no bits below `left`
+                counts[i] = p + i < rest && (left == 32 || d[i] >> left == 0);
+                any |= counts[i];
+            }
+            if (!__any_sync(0xffffffffu, any)) continue;
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                const uint32_t lanes = __ballot_sync(0xffffffffu, counts[i]);
+                if (lanes == 0) continue;
+                // one lane's bin is counted once for all lanes that share it (rows that never received any weight are many)
+                const int bin = counts[i] ? (int)(d[i] >> shift) : -1, leader = __ffs(lanes) - 1, lead = __shfl_sync(0xffffffffu, bin, leader);
+                const uint32_t same = __ballot_sync(0xffffffffu, bin == lead);
+                if (lane == leader) atomicAdd(&s_hist[lead], __popc(same));
+                if (counts[i] && bin != lead) atomicAdd(&s_hist[bin], 1);
+            }
         }
         __syncthreads();
-        // a thread has one or two bins, thread 0 the highest: rows in them and, scanned over the block, in those above
-        const int each = bins / SELECT_THREADS, high = bins - 1 - each * tid;
-        const int sum = s_hist[high] + (each > 1 ? s_hist[high - 1] : 0);
+        // a thread has two bins, thread 0 the highest: rows in them and, scanned over the block, in those above
+        const int high = BINS - 1 - 2 * tid, in_high = s_hist[high], sum = in_high + s_hist[high - 1];
         int above = sum;
         for (int o = 1; o < 32; o <<= 1) {
             const int v = __shfl_up_sync(0xffffffffu, above, o);
@@ -76,44 +117,82 @@ __global__ void __launch_bounds__(SELECT_THREADS) evict8_select_kernel(Cache8 c,
         above += __reduce_add_sync(0xffffffffu, lane < warp ? s_warp[0][lane] : 0);
         const int before = above - sum;
         if (before < missing && missing <= above) {
-            const bool first = missing - before <= s_hist[high];
+            const bool first = missing - before <= in_high;
             s_pick[0] = first ? high : high - 1;
-            s_pick[1] = missing - before - (first ? 0 : s_hist[high]);
+            s_pick[1] = missing - before - (first ? 0 : in_high);
+            s_pick[2] = first ? in_high : sum - in_high;
+            s_pick[3] = 0;
         }
         __syncthreads();
-        prefix |= (uint32_t)s_pick[0] << shift;
-        known |= (uint32_t)(bins - 1) << shift;
+        found |= (uint32_t)s_pick[0] << shift;
         missing = s_pick[1];
+        left = shift;
+        if (missing == s_pick[2]) {                                   // all rows of the bin stay: those above `found` - 1 (it is not the lowest, or all of `rest` would stay)
+            found -= 1;
+            missing = 0;
+            break;
+        }
+        if (left > 0 && s_pick[2] <= FEW) {                           // the bin's rows, each compared to all
+            const int few = s_pick[2];
+            for (int p = PER * tid; p < rest; p += ROUND) {
+                const Ranks f = ranks(p);
+#pragma unroll
+                for (int i = 0; i < PER; ++i) {
+                    const uint32_t d = f.k[i] - least;
+                    if (p + i < rest && (d ^ found) >> left == 0) s_few[atomicAdd(&s_pick[3], 1)] = d;
+                }
+            }
+            __syncthreads();
+            if (tid < few) {
+                const uint32_t d = s_few[tid];
+                int higher = 0, equal = 0;
+                for (int i = 0; i < few; ++i) { higher += s_few[i] > d; equal += s_few[i] == d; }
+                if (higher < missing && missing <= higher + equal) { s_pick[0] = (int)d; s_pick[1] = missing - higher; }       // (rows of one rank write alike)
+            }
+            __syncthreads();
+            found = (uint32_t)s_pick[0];
+            missing = s_pick[1];
+            break;
+        }
+    }
+    const uint32_t last = least + found;
+    // rows above `last` stay, and the first `missing` of those equal to it: a scan over the block of how many of each a thread has, 16 bits each
+    int a = 0, e = 0;                                                 // those of the rounds before
+    for (int p0 = 0; p0 < rest; p0 += ROUND) {
+        const int p = p0 + PER * tid;
+        const Ranks f = ranks(p);
+        int own = 0;
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+            if (p + i < rest) own += f.k[i] > last ? 1 << 16 : f.k[i] == last ? 1 : 0;
+        int upto = own;
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += v;
+        }
+        if (lane == 31) s_own[warp] = upto;
         __syncthreads();
-    }
-    // rows above `prefix` stay, and the first `missing` of those equal to it: a warp has a stretch of the places
-    const int stretch = ((rest + SELECT_WARPS - 1) / SELECT_WARPS + 31) / 32 * 32, from = warp * stretch, to = min(from + stretch, rest);
-    int above = 0, equal = 0;
-    for (int p0 = from; p0 < to; p0 += 32) {
-        const uint32_t k = p0 + lane < to ? rank_at(p0 + lane) : 0u;
-        above += __popc(__ballot_sync(0xffffffffu, p0 + lane < to && k > prefix));
-        equal += __popc(__ballot_sync(0xffffffffu, p0 + lane < to && k == prefix));
-    }
-    if (lane == 0) { s_warp[0][warp] = above; s_warp[1][warp] = equal; }
-    __syncthreads();
-    int a = lane < warp ? s_warp[0][lane] : 0, e = lane < warp ? s_warp[1][lane] : 0;         // what the warps before found
-    a = __reduce_add_sync(0xffffffffu, a);
-    e = __reduce_add_sync(0xffffffffu, e);
-    for (int p0 = from; p0 < to; p0 += 32) {
-        const uint32_t k = p0 + lane < to ? rank_at(p0 + lane) : 0u, below = (1u << lane) - 1u;
-        const uint32_t am = __ballot_sync(0xffffffffu, p0 + lane < to && k > prefix), em = __ballot_sync(0xffffffffu, p0 + lane < to && k == prefix);
-        const int a1 = a + __popc(am & below), e1 = e + __popc(em & below);
-        if ((am >> lane & 1u) || ((em >> lane & 1u) && e1 < missing)) list[a1 + min(e1, missing)] = p0 + lane;
-        a += __popc(am);
-        e += __popc(em);
+        const int of_warp = s_own[lane], before = __reduce_add_sync(0xffffffffu, lane < warp ? of_warp : 0) + upto - own;
+        int a1 = a + (before >> 16), e1 = e + (before & 0xffff);
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            if (p + i >= rest) break;
+            if (f.k[i] > last) list[a1++ + min(e1, missing)] = p + i;
+            else if (f.k[i] == last && e1++ < missing) list[a1 + e1 - 1] = p + i;
+        }
+        const int all = __reduce_add_sync(0xffffffffu, of_warp);
+        a += all >> 16;
+        e += all & 0xffff;
+        __syncthreads();
     }
 }
 
 // ---------------------------------------------------------------------------------------
 // Moving: a warp per 16 rows of the list, a lane for each row and plane on the way to its page and byte.  The new block's byte is the largest of
 // its rows' bytes; rows of a smaller one are rounded again.  Nothing is shared between warps.  2,048 of about 7,000 rows of 32 sequences, 4 heads of 128:
-// 38 us for 134 MB, about the time of reading all of the old pages: 128 bytes in three of every 384.  (A warp per 64 rows and plane, which goes
-// that way once for four times as many, was slower by a fifth: too few warps.)
+// 36 us for 134 MB, about the time of reading all of the old pages: 128 bytes in three of every 384.  (A warp per 64 rows and plane, which goes
+// that way once for four times as many, was slower by a fifth: too few warps;
+// so was a warp that looked up two or four blocks' rows at once.  Rows that lie side by side take 27 us.)
 // ---------------------------------------------------------------------------------------
 __global__ void __launch_bounds__(256) evict8_move_kernel(Cache8 c, float* __restrict__ weights, const int* __restrict__ kept, const int* __restrict__ new_table,
                                                           int new_stride, int budget) {
@@ -188,12 +267,15 @@ TQ_EXPORT int tq_evict8(const void* packed) {
     TQ_REQUIRE((long long)x.new_stride * page_size >= budget, "evict8: %d new pages a sequence for a budget of %d rows", x.new_stride, budget);
     TQ_REQUIRE(n_seqs <= 65535 && nkv <= 65535, "evict8: %d sequences, %d heads", n_seqs, nkv);
     TQ_REQUIRE((long long)table_stride * page_size < (1ll << 31), "evict8: page tables of %d pages", table_stride);
+    TQ_REQUIRE((uintptr_t)x.weights % 16 == 0, "evict8: weights must be 16-byte aligned");
     const Cache8 c = c8_cache(x.codes, x.scales, page_table, table_stride, page_size, n_pages, nkv, hd);
     const int cached = table_stride * page_size < SELECT_MOST ? table_stride * page_size : SELECT_MOST;
-    static TqSmemAsked asked;
-    const cudaError_t e = tq_grow_smem(evict8_select_kernel, (size_t)cached * 4, asked);
+    const bool small = table_stride * page_size - recent <= SELECT_THREADS;
+    static TqSmemAsked asked[2];
+    const auto select = small ? evict8_select_kernel<1> : evict8_select_kernel<4>;
+    const cudaError_t e = tq_grow_smem(select, (size_t)cached * 4, asked[small]);
     if (e != cudaSuccess) TQ_FAIL(-1, "evict8: cannot reserve %d bytes of shared memory: %s", cached * 4, cudaGetErrorString(e));
-    tq_launch(dim3(nkv, n_seqs), SELECT_THREADS, (size_t)cached * 4, x.stream)(evict8_select_kernel, c, x.weights, x.lengths, budget, recent, cached, x.kept);
+    tq_launch(dim3(nkv, n_seqs), SELECT_THREADS, (size_t)cached * 4, x.stream)(select, c, x.weights, x.lengths, budget, recent, cached, x.kept);
     TQ_CHECK_LAUNCH("evict8_select");
     tq_launch(dim3(((budget + C8_BLOCK - 1) / C8_BLOCK + 7) / 8, nkv, n_seqs), 256, 0, x.stream)(evict8_move_kernel, c, x.weights, x.kept, x.new_table, x.new_stride, budget);
     TQ_CHECK_LAUNCH("evict8_move");
