@@ -7,9 +7,9 @@ TQ_DEFINE_LAST_ERROR
 
 namespace {
 
-// Eight consecutive elements as float32, in pairs for the packed operations.
-struct Eight { tq_f32x2 p[4]; };
-// the same as they lie in memory
+// Eight consecutive elements as they lie in memory, and as float32.  (Additions and products of pairs, as packed operations: 22.7 us,
+// single ones 23.0, for the prompts below; 2.26 and 2.09 for a token; 3.6 and 3.3 for four prompts of up to 1,000 rows, 16 + 4 + 4 heads of 64.)
+struct Eight { float v[8]; };
 template <typename T> struct Raw;
 template <> struct Raw<__nv_bfloat16> {
     uint4 v;
@@ -18,14 +18,14 @@ template <> struct Raw<__nv_bfloat16> {
         const uint32_t u[4] = {v.x, v.y, v.z, v.w};
         Eight r;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) r.p[i] = tq_pack2(__uint_as_float(u[i] << 16), __uint_as_float(u[i] & 0xffff0000u));
+        for (int i = 0; i < 4; ++i) { r.v[2 * i] = __uint_as_float(u[i] << 16); r.v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u); }
         return r;
     }
 };
 template <> struct Raw<float> {
     float4 a, b;
     __device__ __forceinline__ void load(const float* p) { a = *reinterpret_cast<const float4*>(p); b = *reinterpret_cast<const float4*>(p + 4); }
-    __device__ __forceinline__ Eight wide() const { return Eight{{tq_pack2(a.x, a.y), tq_pack2(a.z, a.w), tq_pack2(b.x, b.y), tq_pack2(b.z, b.w)}}; }
+    __device__ __forceinline__ Eight wide() const { return Eight{{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}}; }
 };
 __device__ __forceinline__ Eight load8(const float* p) {
     Raw<float> r;
@@ -36,47 +36,47 @@ __device__ __forceinline__ void store8(__nv_bfloat16* p, const Eight& f) {
     uint32_t u[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const float2 x = tq_unpack2(f.p[i]);
-        const __nv_bfloat162 h = __floats2bfloat162_rn(x.x, x.y);
+        const __nv_bfloat162 h = __floats2bfloat162_rn(f.v[2 * i], f.v[2 * i + 1]);
         u[i] = *reinterpret_cast<const uint32_t*>(&h);
     }
     *reinterpret_cast<uint4*>(p) = make_uint4(u[0], u[1], u[2], u[3]);
 }
 __device__ __forceinline__ void store8(float* p, const Eight& f) {
-    const float2 a = tq_unpack2(f.p[0]), b = tq_unpack2(f.p[1]), c = tq_unpack2(f.p[2]), d = tq_unpack2(f.p[3]);
-    *reinterpret_cast<float4*>(p) = make_float4(a.x, a.y, b.x, b.y);
-    *reinterpret_cast<float4*>(p + 4) = make_float4(c.x, c.y, d.x, d.y);
+    *reinterpret_cast<float4*>(p) = make_float4(f.v[0], f.v[1], f.v[2], f.v[3]);
+    *reinterpret_cast<float4*>(p + 4) = make_float4(f.v[4], f.v[5], f.v[6], f.v[7]);
 }
 // the larger of `top` and the magnitudes of eight elements; NaN does not count
 __device__ __forceinline__ float magnitude8(const Eight& f, float top) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float2 x = tq_unpack2(f.p[i]);
-        asm("max.f32 %0, %1, %2, %3;" : "=f"(top) : "f"(top), "f"(fabsf(x.x)), "f"(fabsf(x.y)));
-    }
+    for (int i = 0; i < 8; i += 2) asm("max.f32 %0, %1, %2, %3;" : "=f"(top) : "f"(top), "f"(fabsf(f.v[i])), "f"(fabsf(f.v[i + 1])));
     return top;
 }
 // the same over the finite elements alone
 __device__ __forceinline__ float finite8(const Eight& f, float top) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float2 x = tq_unpack2(f.p[i]);
-        top = fmaxf(top, fmaxf(__uint_as_float(c8_magnitude(x.x)), __uint_as_float(c8_magnitude(x.y))));
-    }
+    for (int i = 0; i < 8; ++i) top = fmaxf(top, __uint_as_float(c8_magnitude(f.v[i])));
     return top;
 }
-// eight elements as codes; infinite: some of the unit's elements may be (the conversion makes NaN of NaN, but 448 of them)
-__device__ __forceinline__ uint2 encode8(const Eight& f, tq_f32x2 inv, bool infinite) {
+// eight elements as codes; INFINITE: some may be infinite (the conversion makes NaN of NaN, but 448 of them)
+template <bool INFINITE> __device__ __forceinline__ uint2 encode8(const Eight& f, float inv) {
     uint32_t w[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const float2 x = tq_unpack2(tq_mul2(f.p[i], inv));
-        uint16_t d;
-        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(d) : "f"(x.y), "f"(x.x));
-        w[i] = d;
-        if (infinite) w[i] = c8_encode2(x.x, x.y);
+        const float x = f.v[2 * i] * inv, y = f.v[2 * i + 1] * inv;
+        if constexpr (INFINITE) w[i] = c8_encode2(x, y);
+        else {
+            uint16_t d;
+            asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(d) : "f"(y), "f"(x));
+            w[i] = d;
+        }
     }
     return make_uint2(__byte_perm(w[0], w[1], 0x5410), __byte_perm(w[2], w[3], 0x5410));
+}
+// products and sums rounded one by one
+__device__ __forceinline__ void rotate(float& u, float& v, float cs, float sn) {
+    const float x = __fsub_rn(__fmul_rn(u, cs), __fmul_rn(v, sn));
+    v = __fadd_rn(__fmul_rn(u, sn), __fmul_rn(v, cs));
+    u = x;
 }
 
 // ---------------------------------------------------------------------------------------
@@ -93,19 +93,20 @@ __device__ __forceinline__ uint2 encode8(const Eight& f, tq_f32x2 inv, bool infi
 struct WriteArgs {
     const float *cos_t, *sin_t;
     const int *positions, *cu_seqlens, *held;
-    int nh, pairing, written, each;    // written: the heads this launch takes (the queries alone, or all); each: units a thread takes one after another
+    int nh, written, each;    // written: the heads this launch takes (the queries alone, or all); each: units a thread takes one after another
 };
 
 // Runs of many rows: a thread goes through the items of up to WRITE_EACH heads, so that the cosines and sines, twice the bytes of a bfloat16 item,
 // are fetched once, and the next item is on its way while one is worked on (prompts above, heads a thread: one 33 us, two 27, three 25.7, four
-// 25.5, six 26.8, eight 29.5; before, each head with its own cosines, 29.8).  Not where fewer than WRITE_FILL blocks would be left a turn.
+// 25.5, six 26.8, eight 29.5).  Not where fewer than WRITE_FILL blocks would be left a turn.  Then 23.0, with the pairing known to the compiler and
+// the encoding of infinite elements in a branch of its own: instructions, 2.8 a cycle and busy SM, against 13 for the bytes.
 constexpr int WRITE_EACH = 4, WRITE_FILL = 148 * 4;
 constexpr int WRITE_THREADS = 256;
 
-// HD: the head size, or 0 where it is known at the launch only.  Blocks an SM: of float32, whose items take twice the registers, 3 (4,096 rows of
-// 28 + 4 + 4 heads: 30.5 us, with the bias asked for ahead 34, and 39 with four blocks).  The bias of bfloat16 is asked for ahead (prompts above: 25.7
-// us, else 28).
-template <typename TA, typename TB, bool RUNS, int HD>
+// PAIRING 0: element i of the first half with element i of the second; 1: neighbours.  HD: the head size, or 0 where it is known at the launch only.
+// Blocks an SM: of float32, whose items take twice the registers, 3 (4,096 rows of 28 + 4 + 4 heads: 30.5 us, with the bias asked for ahead 34, and
+// 39 with four blocks).  The bias of bfloat16 is asked for ahead (prompts above: 25.7 us, else 28).
+template <typename TA, typename TB, bool RUNS, int HD, int PAIRING>
 __global__ void __launch_bounds__(WRITE_THREADS, RUNS ? HD == 128 && sizeof(TA) == 2 ? 4 : 3 : 1) write8_kernel(const TA* __restrict__ qkv, const TB* __restrict__ bias, WriteArgs a,
                                                                                                                  TA* __restrict__ q_out, Cache8 c, int threads_) {
     tq_grid_wait();                    // everything below may read what the previous kernel wrote
@@ -122,7 +123,7 @@ __global__ void __launch_bounds__(WRITE_THREADS, RUNS ? HD == 128 && sizeof(TA) 
     if (rows <= 0 || (!RUNS && j0 + unit >= a.written)) return;      // (runs: the whole block of threads returns or stays)
     const int t0 = t_begin + first - place0, half = hd >> 1, groups = half >> 3, items = rows * groups;
     const int r = it / groups, i = (it - r * groups) * 8;
-    const int ia = a.pairing == 0 ? i : 2 * i, ib = a.pairing == 0 ? i + half : 2 * i + 8;       // where the item's two halves lie in the head
+    const int ia = PAIRING == 0 ? i : 2 * i, ib = PAIRING == 0 ? i + half : 2 * i + 8;       // where the item's two halves lie in the head
     const int row0 = c.row(block_start), old = first - block_start;
     const TA* row = qkv + (size_t)(t0 + r) * heads * hd;
     const bool inside = it < items;
@@ -162,35 +163,15 @@ __global__ void __launch_bounds__(WRITE_THREADS, RUNS ? HD == 128 && sizeof(TA) 
             if (!AHEAD) { bias0.load(bias + j * hd + ia); bias1.load(bias + j * hd + ib); }
             const Eight x = bias0.wide(), y = bias1.wide();
 #pragma unroll
-            for (int e = 0; e < 4; ++e) { lo.p[e] = tq_add2(lo.p[e], x.p[e]); hi.p[e] = tq_add2(hi.p[e], y.p[e]); }
+            for (int e = 0; e < 8; ++e) { lo.v[e] += x.v[e]; hi.v[e] += y.v[e]; }
         }
         if (RUNS && k + 1 < each) ask(j + side);                      // on its way while this one is worked on
         if (mine) {
             if (j < a.nh + c.nkv && a.cos_t != nullptr) {
-                // interleaved: the pairs' first elements together and their second ones, and back
-                auto sort = [](Eight& x, Eight& y) {
-                    const float2 p[8] = {tq_unpack2(x.p[0]), tq_unpack2(x.p[1]), tq_unpack2(x.p[2]), tq_unpack2(x.p[3]),
-                                         tq_unpack2(y.p[0]), tq_unpack2(y.p[1]), tq_unpack2(y.p[2]), tq_unpack2(y.p[3])};
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) { x.p[e] = tq_pack2(p[2 * e].x, p[2 * e + 1].x); y.p[e] = tq_pack2(p[2 * e].y, p[2 * e + 1].y); }
-                };
-                if (a.pairing != 0) sort(lo, hi);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    // (the packed product and sum came out fused, their .rn notwithstanding)
-                    const float2 u = tq_unpack2(lo.p[e]), v = tq_unpack2(hi.p[e]), x = tq_unpack2(cs.p[e]), y = tq_unpack2(sn.p[e]);
-                    lo.p[e] = tq_pack2(__fsub_rn(__fmul_rn(u.x, x.x), __fmul_rn(v.x, y.x)), __fsub_rn(__fmul_rn(u.y, x.y), __fmul_rn(v.y, y.y)));
-                    hi.p[e] = tq_pack2(__fadd_rn(__fmul_rn(u.x, y.x), __fmul_rn(v.x, x.x)), __fadd_rn(__fmul_rn(u.y, y.y), __fmul_rn(v.y, x.y)));
-                }
-                if (a.pairing != 0) {
-                    const Eight u = lo, v = hi;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float2 x = tq_unpack2(u.p[e]), y = tq_unpack2(v.p[e]);
-                        Eight& to = e < 2 ? lo : hi;
-                        to.p[2 * (e & 1)] = tq_pack2(x.x, y.x);
-                        to.p[2 * (e & 1) + 1] = tq_pack2(x.y, y.y);
-                    }
+                for (int e = 0; e < 8; ++e) {
+                    if (PAIRING == 0) rotate(lo.v[e], hi.v[e], cs.v[e], sn.v[e]);
+                    else rotate((e < 4 ? lo : hi).v[2 * (e & 3)], (e < 4 ? lo : hi).v[2 * (e & 3) + 1], cs.v[e], sn.v[e]);
                 }
             }
             if (is_q) {
@@ -225,8 +206,13 @@ __global__ void __launch_bounds__(WRITE_THREADS, RUNS ? HD == 128 && sizeof(TA) 
         if (mine) {
             const float inv = c8_inverse(b);
             uint8_t* d = codes + (size_t)(old + r) * hd;
-            *reinterpret_cast<uint2*>(d + ia) = encode8(lo, tq_pack2(inv, inv), infinite);
-            *reinterpret_cast<uint2*>(d + ib) = encode8(hi, tq_pack2(inv, inv), infinite);
+            if (!infinite) {
+                *reinterpret_cast<uint2*>(d + ia) = encode8<false>(lo, inv);
+                *reinterpret_cast<uint2*>(d + ib) = encode8<false>(hi, inv);
+            } else {
+                *reinterpret_cast<uint2*>(d + ia) = encode8<true>(lo, inv);
+                *reinterpret_cast<uint2*>(d + ib) = encode8<true>(hi, inv);
+            }
         }
         if (b > was && old > 0) {
             const uint32_t factor = c8_shift_factor((int)min(b - was, 25u));
@@ -264,7 +250,7 @@ TQ_EXPORT int tq_write8(const void* packed) {
     TQ_REQUIRE(n_seqs <= 65535 && max_q_len >= 1, "write8: %d sequences, longest run %d", n_seqs, max_q_len);
     TQ_REQUIRE(((uintptr_t)qkv | (uintptr_t)bias | (uintptr_t)x.q_out | (uintptr_t)cos_t | (uintptr_t)sin_t) % 16 == 0, "write8: tensors must be 16-byte aligned");
     const Cache8 c = c8_cache(codes, scales, x.page_table, x.table_stride, page_size, n_pages, nkv, hd);
-    WriteArgs a{cos_t, sin_t, x.positions, x.cu_seqlens, x.held, nh, x.pairing, codes != nullptr ? nh + 2 * nkv : nh, 1};
+    WriteArgs a{cos_t, sin_t, x.positions, x.cu_seqlens, x.held, nh, codes != nullptr ? nh + 2 * nkv : nh, 1};
     // a run of n rows touches at most (n + 14) / 16 + 1 blocks
     const bool runs = max_q_len > 1;
     const int units = runs ? (max_q_len + 14) / C8_BLOCK + 1 : 1, threads = runs ? (hd + 31) / 32 * 32 : 32;
@@ -273,9 +259,13 @@ TQ_EXPORT int tq_write8(const void* packed) {
     a.each = runs ? (int)max(1ll, min((long long)WRITE_EACH, blocks / WRITE_FILL)) : 1;
     const dim3 grid(units, (a.written + side * a.each - 1) / (side * a.each), n_seqs);
     TQ_DISPATCH(x.act_dtype, TA, TQ_DISPATCH(bias != nullptr ? x.bias_dtype : x.act_dtype, TB,
-        auto kernel = runs ? (hd == 128 ? write8_kernel<TA, TB, true, 128> : hd == 64 ? write8_kernel<TA, TB, true, 64> : write8_kernel<TA, TB, true, 0>)
-                           : (hd == 128 ? write8_kernel<TA, TB, false, 128> : write8_kernel<TA, TB, false, 0>);
-        tq_launch(grid, side * threads, 0, x.stream)(kernel, (const TA*)qkv, (const TB*)bias, a, (TA*)x.q_out, c, threads)));
+        const auto launch = [&](auto kernel) { tq_launch(grid, side * threads, 0, x.stream)(kernel, (const TA*)qkv, (const TB*)bias, a, (TA*)x.q_out, c, threads); };
+        const auto of_pairing = [&](auto pairing) {
+            constexpr int P = decltype(pairing)::value;
+            if (runs) launch(hd == 128 ? write8_kernel<TA, TB, true, 128, P> : hd == 64 ? write8_kernel<TA, TB, true, 64, P> : write8_kernel<TA, TB, true, 0, P>);
+            else launch(hd == 128 ? write8_kernel<TA, TB, false, 128, P> : write8_kernel<TA, TB, false, 0, P>);
+        };
+        if (x.pairing == 0) of_pairing(std::integral_constant<int, 0>()); else of_pairing(std::integral_constant<int, 1>())));
     TQ_CHECK_LAUNCH("write8");
     return 0;
 }

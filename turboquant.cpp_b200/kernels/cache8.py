@@ -298,8 +298,8 @@ def evict8(codes: torch.Tensor, scales: torch.Tensor, weights: torch.Tensor, len
     rows in each key/value head: the last `recent` and, of those before, the ones with the largest weights (the first of equal ones;
     NaN counts as the smallest), in the order of their places.  A sequence within the budget keeps all its rows.  A new block takes the
     largest byte of its rows, rows of a smaller one are rounded again; sums of weights move along.  The old pages are only read and must
-    not be among the new ones; rows of the new pages behind a sequence's last stay as they were.  Returns the places that were kept,
-    int32 [n_seqs, nkv, budget], -1 where there are fewer."""
+    not be among the new ones; rows of the new pages behind a sequence's last stay as they were; weights start on a 16-byte boundary.
+    Returns the places that were kept, int32 [n_seqs, nkv, budget], -1 where there are fewer."""
     if codes.dim() != 5:
         raise KernelError(f"8-bit cache: codes must be float8_e4m3fn [pages, 2, kv heads, page_size, head size], got {tuple(codes.shape)}")
     _, _, n_kv_heads, _, head_dim = codes.shape
