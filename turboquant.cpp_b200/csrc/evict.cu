@@ -190,10 +190,12 @@ __global__ void __launch_bounds__(SELECT_THREADS) evict8_select_kernel(Cache8 c,
 // ---------------------------------------------------------------------------------------
 // Moving: a warp per 16 rows of the list, a lane for each row and plane on the way to its page and byte.  The new block's byte is the largest of
 // its rows' bytes; rows of a smaller one are rounded again.  Nothing is shared between warps.  2,048 of about 7,000 rows of 32 sequences, 4 heads of 128:
-// 36 us for 134 MB, about the time of reading all of the old pages: 128 bytes in three of every 384.  (A warp per 64 rows and plane, which goes
+// 32 us for 134 MB, about the time of reading all of the old pages: 128 bytes in three of every 384.  (A warp per 64 rows and plane, which goes
 // that way once for four times as many, was slower by a fifth: too few warps;
-// so was a warp that looked up two or four blocks' rows at once.  Rows that lie side by side take 27 us.)
+// so was a warp that looked up two or four blocks' rows at once.  Rows that lie side by side take 24 us.)
 // ---------------------------------------------------------------------------------------
+// HD: the head size, or 0 where it is known at the launch only (then a division for each piece: 36 us for the rows above).
+template <int HD>
 __global__ void __launch_bounds__(256) evict8_move_kernel(Cache8 c, float* __restrict__ weights, const int* __restrict__ kept, const int* __restrict__ new_table,
                                                           int new_stride, int budget) {
     tq_grid_wait();                    // everything below may read what the previous kernel wrote
@@ -203,18 +205,18 @@ __global__ void __launch_bounds__(256) evict8_move_kernel(Cache8 c, float* __res
     const int* list = kept + ((size_t)seq * c.nkv + g) * budget;
     const int place = first + r < budget ? list[first + r] : -1;
     const int page = TQ_CHECKED(new_table[(size_t)seq * new_stride + TQ_CHECKED(c.column(first), new_stride, TQ_IDX_TABLE_COLUMN)], c.n_pages, TQ_IDX_PAGE);
-    const int rows = __popc(__ballot_sync(0xffffffffu, place >= 0) & 0xffffu), row0 = c.row(first), vecs = c.hd / 16;
+    const int rows = __popc(__ballot_sync(0xffffffffu, place >= 0) & 0xffffu), row0 = c.row(first), hd = HD ? HD : c.hd, vecs = hd / 16;
     if (rows == 0) return;                                            // the list ends before these
     unsigned long long from = 0;
     uint32_t byte = 0;
     float weight = 0.f;
     if (place >= 0) {
         const int old = c.page_of(seq, place), row = c.row(place);
-        from = c.codes_at(old, plane, g) + (size_t)row * c.hd;
+        from = c.codes_at(old, plane, g) + (size_t)row * hd;
         byte = c.scales[c.scales_at(old, plane, g) + row / C8_BLOCK];
         if (plane == 0) weight = weights[((size_t)old * c.nkv + g) * c.page_size + row];
     }
-    const size_t to = c.codes_at(page, 0, g) + (size_t)row0 * c.hd, between = (size_t)c.nkv * c.page_size * c.hd;
+    const size_t to = c.codes_at(page, 0, g) + (size_t)row0 * hd, between = (size_t)c.nkv * c.page_size * hd;
     uint32_t top = byte;
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -236,7 +238,7 @@ __global__ void __launch_bounds__(256) evict8_move_kernel(Cache8 c, float* __res
             const uint32_t s = __shfl_sync(0xffffffffu, shift, which & 31);
             if (v < 2 * pieces && (which & 15) < rows) {
                 if (s) x[i] = c8_shift16(x[i], c8_shift_factor((int)min(s, 25u)));
-                *reinterpret_cast<uint4*>(c.codes + to + (which >> 4) * between + (size_t)(which & 15) * c.hd + at) = x[i];
+                *reinterpret_cast<uint4*>(c.codes + to + (which >> 4) * between + (size_t)(which & 15) * hd + at) = x[i];
             }
         }
     }
@@ -277,7 +279,8 @@ TQ_EXPORT int tq_evict8(const void* packed) {
     if (e != cudaSuccess) TQ_FAIL(-1, "evict8: cannot reserve %d bytes of shared memory: %s", cached * 4, cudaGetErrorString(e));
     tq_launch(dim3(nkv, n_seqs), SELECT_THREADS, (size_t)cached * 4, x.stream)(select, c, x.weights, x.lengths, budget, recent, cached, x.kept);
     TQ_CHECK_LAUNCH("evict8_select");
-    tq_launch(dim3(((budget + C8_BLOCK - 1) / C8_BLOCK + 7) / 8, nkv, n_seqs), 256, 0, x.stream)(evict8_move_kernel, c, x.weights, x.kept, x.new_table, x.new_stride, budget);
+    const auto move = hd == 128 ? evict8_move_kernel<128> : hd == 64 ? evict8_move_kernel<64> : evict8_move_kernel<0>;
+    tq_launch(dim3(((budget + C8_BLOCK - 1) / C8_BLOCK + 7) / 8, nkv, n_seqs), 256, 0, x.stream)(move, c, x.weights, x.kept, x.new_table, x.new_stride, budget);
     TQ_CHECK_LAUNCH("evict8_move");
     return 0;
 }
