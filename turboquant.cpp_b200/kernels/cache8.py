@@ -243,8 +243,8 @@ def attention8(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, cu_se
 
 # Steps whose longest run is at least this, and whose queries, heads, elements and the keys they see multiply to this much, go to the tensor-core
 # prompt kernel, where it takes their sizes.  (B200, us, csrc/attention8.cu and the prompt kernel's five launches: 128 rows behind 800, 16
-# heads of 128, 0.2e9: 22 and 31; 28 heads on 4, 0.4e9: 45 and 31; 64 behind 4,000, 16 heads, 0.5e9: 31 and 38; 128 behind 4,000, 1.1e9: 48 and 41;
-# 256 behind 4,000, 2.2e9: 130 and 46.)
+# heads of 128, 0.2e9: 19 and 31; 28 heads on 4, 0.4e9: 39 and 31; 64 behind 4,000, 16 heads, 0.5e9: 28 and 38; 128 behind 4,000, 1.1e9: 44 and 40;
+# 256 behind 4,000, 2.2e9: 119 and 46.)
 PROMPT_MIN_RUN, PROMPT_WORK = 48, 350_000_000
 DENSE_BYTES = 1 << 30        # scratch a step may take for pages in bfloat16; sequences beyond it follow in further launches
 
