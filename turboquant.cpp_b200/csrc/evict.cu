@@ -269,7 +269,7 @@ TQ_EXPORT int tq_evict8(const void* packed) {
     TQ_REQUIRE((long long)x.new_stride * page_size >= budget, "evict8: %d new pages a sequence for a budget of %d rows", x.new_stride, budget);
     TQ_REQUIRE(n_seqs <= 65535 && nkv <= 65535, "evict8: %d sequences, %d heads", n_seqs, nkv);
     TQ_REQUIRE((long long)table_stride * page_size < (1ll << 31), "evict8: page tables of %d pages", table_stride);
-    TQ_REQUIRE((uintptr_t)x.weights % 16 == 0, "evict8: weights must be 16-byte aligned");
+    TQ_REQUIRE(x.weights != nullptr && (uintptr_t)x.weights % 16 == 0, "evict8: weights must be there, and 16-byte aligned");
     const Cache8 c = c8_cache(x.codes, x.scales, page_table, table_stride, page_size, n_pages, nkv, hd);
     const int cached = table_stride * page_size < SELECT_MOST ? table_stride * page_size : SELECT_MOST;
     const bool small = table_stride * page_size - recent <= SELECT_THREADS;

@@ -302,6 +302,8 @@ def evict8(codes: torch.Tensor, scales: torch.Tensor, weights: torch.Tensor, len
     Returns the places that were kept, int32 [n_seqs, nkv, budget], -1 where there are fewer."""
     if codes.dim() != 5:
         raise KernelError(f"8-bit cache: codes must be float8_e4m3fn [pages, 2, kv heads, page_size, head size], got {tuple(codes.shape)}")
+    if weights is None:
+        raise KernelError("evict8: a cache without sums of weights has nothing to choose rows by")
     _, _, n_kv_heads, _, head_dim = codes.shape
     pages, n, width = _sizes(codes, scales, weights, page_table, page_size, n_kv_heads, head_dim)
     check_sizes(page_size, head_dim)
