@@ -32,3 +32,53 @@ def test_the_launcher_refuses_an_eviction_without_weights():
     assert evict(16, 16, 0, 16, 16, 16, 16, 0, 2, 1, PAGE, 3, 1, G, D, 32, 4) != 0
     from turboquant_cpp_b200.csrc.build import load_kernel
     assert b"weights" in load_kernel("evict").tq_last_error()
+
+
+# ---- packed calls ----------------------------------------------------------------------------------------------------------
+def _c_struct(name):
+    """The struct an entry point takes, from its source, as ctypes lays it out (C's rules: padding behind the last member too)."""
+    import os
+    import re
+
+    from conftest import ROOT
+    csrc = os.path.join(ROOT, "turboquant.cpp_b200", "csrc")
+    text = "".join(open(os.path.join(csrc, f), encoding="utf-8").read() for f in ("cache8.cu", "attention8.cu", "evict.cu"))
+    struct = re.search(r"c8_call<(\w+)>", text[text.index(f"TQ_EXPORT int {name}("):]).group(1)
+    fields = []
+    for line in (x.strip() for x in re.search(r"struct " + struct + r" \{(.*?)\};", text, re.S).group(1).split(";")):
+        kind = ctypes.c_void_p if "*" in line or "cudaStream_t" in line else ctypes.c_float if line.startswith("float") else ctypes.c_int
+        fields += [(f"m{len(fields) + i}", kind) for i in range(line.count(",") + 1)] if line else []
+    return type(struct, (ctypes.Structure,), {"_fields_": fields})
+
+
+@pytest.mark.parametrize("name", sorted(cache8._PACKED))
+def test_a_packed_call_has_all_the_bytes_its_launcher_copies(name):
+    from turboquant_cpp_b200.kernels import _call
+    struct, seen = _c_struct(name), []
+
+    class Fn:
+        def __call__(self, data, *size):
+            seen.append((data, size))
+            return 0
+    lib = type("Lib", (), {name: Fn()})()
+    members = list(range(1, len(struct._fields_) + 1))
+    assert _call.packed(lib, name, cache8._PACKED[name])(*members) == 0
+    data, size = seen[0]
+    assert len(data) == ctypes.sizeof(struct) and size == (len(data),)
+    got = struct.from_buffer_copy(data)
+    assert [getattr(got, f) for f, _ in struct._fields_] == members
+
+
+@pytest.mark.parametrize("library,name", [("cache8", "tq_write8"), ("attention8", "tq_attention8"), ("evict", "tq_evict8")])
+def test_a_packed_call_of_another_length_is_refused(library, name):
+    """A layout that no longer is the launcher's: refused before a byte is read."""
+    from turboquant_cpp_b200.csrc.build import load_kernel
+    lib, size = load_kernel(library), ctypes.sizeof(_c_struct(name))
+    fn = getattr(lib, name)
+    was, fn.argtypes = fn.argtypes, [ctypes.c_char_p, ctypes.c_int]
+    try:
+        assert fn(bytes(size), size) == 0                                   # no sequences: nothing to do
+        for other in (0, size - 4, size + 8):
+            assert fn(bytes(size), other) != 0 and b"bytes" in lib.tq_last_error()
+    finally:
+        fn.argtypes = was

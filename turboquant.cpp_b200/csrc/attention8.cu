@@ -969,7 +969,8 @@ struct Attention8Call {
     int act_dtype, table_stride, page_size, window, ranges, score_stride, max_kv_len, n_pages, n_seqs, max_q_len, nh, nkv, hd;
     float scale;
 };
-TQ_EXPORT int tq_attention8(const void* packed) {
+TQ_EXPORT int tq_attention8(const void* packed, int bytes) {
+    C8_REQUIRE_CALL("attention8", Attention8Call);
     const Attention8Call x = c8_call<Attention8Call>(packed);
     const void* q = x.q;
     float *partial = x.partial, *scores = x.scores, *weights = x.weights;

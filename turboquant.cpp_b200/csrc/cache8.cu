@@ -237,7 +237,8 @@ struct Write8Call {
     cudaStream_t stream;
     int act_dtype, bias_dtype, pairing, table_stride, page_size, n_pages, n_seqs, max_q_len, nh, nkv, hd;
 };
-TQ_EXPORT int tq_write8(const void* packed) {
+TQ_EXPORT int tq_write8(const void* packed, int bytes) {
+    C8_REQUIRE_CALL("write8", Write8Call);
     const Write8Call x = c8_call<Write8Call>(packed);
     const void *qkv = x.qkv, *bias = x.bias, *codes = x.codes, *scales = x.scales;
     const float *cos_t = x.cos_t, *sin_t = x.sin_t;

@@ -90,8 +90,10 @@ __device__ __forceinline__ uint4 c8_shift16(uint4 v, uint32_t factor) {
     return make_uint4(c8_shift4(v.x, factor), c8_shift4(v.y, factor), c8_shift4(v.z, factor), c8_shift4(v.w, factor));
 }
 
-// Entry points of calls that single steps make take one packed struct (addresses first, then whole numbers, then floats: no gaps), which costs
-// the caller a fifth of what two dozen arguments do; it is copied, since a Python bytes object need not be aligned for it.
+// Entry points of calls that single steps make take one packed struct (addresses first, then whole numbers, then floats: no gaps but the padding at
+// its end, which the caller sends too) and its length, which costs the caller a fifth of what two dozen arguments do; it is copied, since a
+// Python bytes object need not be aligned for it.
+#define C8_REQUIRE_CALL(what, C) TQ_REQUIRE(packed != nullptr && bytes == (int)sizeof(C), "%s: a call of %d bytes, not %d", what, bytes, (int)sizeof(C))
 template <typename C> inline C c8_call(const void* packed) {
     C c;
     memcpy(&c, packed, sizeof(c));

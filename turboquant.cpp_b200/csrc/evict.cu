@@ -258,7 +258,8 @@ struct Evict8Call {
     cudaStream_t stream;
     int table_stride, new_stride, page_size, n_pages, n_seqs, nkv, hd, budget, recent;
 };
-TQ_EXPORT int tq_evict8(const void* packed) {
+TQ_EXPORT int tq_evict8(const void* packed, int bytes) {
+    C8_REQUIRE_CALL("evict8", Evict8Call);
     const Evict8Call x = c8_call<Evict8Call>(packed);
     const int* page_table = x.page_table;
     const int table_stride = x.table_stride, page_size = x.page_size, n_pages = x.n_pages, n_seqs = x.n_seqs, nkv = x.nkv, hd = x.hd, budget = x.budget, recent = x.recent;
