@@ -82,3 +82,21 @@ def test_a_packed_call_of_another_length_is_refused(library, name):
             assert fn(bytes(size), other) != 0 and b"bytes" in lib.tq_last_error()
     finally:
         fn.argtypes = was
+
+
+# ---- pages whose offsets would not fit ---------------------------------------------------------------------------------------
+@pytest.mark.parametrize("library,name", [("cache8", "tq_write8"), ("attention8", "tq_attention8"), ("evict", "tq_evict8")])
+@pytest.mark.parametrize("page_size,nkv,hd,fits", [(1 << 17, 128, 128, False), (1 << 17, 64, 256, False), (1 << 17, 127, 128, True)])
+def test_a_plane_of_a_page_stays_below_two_to_the_31_codes(library, name, page_size, nkv, hd, fits):
+    """Offsets within a page are 32 bits wide.  (A page that fits is refused for its codes' alignment, the check behind it: nothing is launched.)"""
+    from turboquant_cpp_b200.csrc.build import load_kernel
+    lib, struct = load_kernel(library), _c_struct(name)
+    order = {"tq_write8": [0, 0, 0, 1, page_size, 1, 1, 1, nkv, nkv, hd], "tq_attention8": [0, 1, page_size, 0, 1, 0, 16, 1, 1, 1, nkv, nkv, hd],
+             "tq_evict8": [1, 1, page_size, 1, 1, nkv, hd, 16, 4]}[name]
+    call = cache8._PACKED[name]
+    addresses = [8] * int(call[:call.index("P")])
+    members = addresses + order + ([0.1] if call.endswith("f") else [])
+    assert len(members) == len(struct._fields_)
+    assert getattr(cache8, f"_{library}")(name)(*members) != 0
+    message = lib.tq_last_error()
+    assert (b"codes a plane" in message) == (not fits) and (b"aligned" in message) == fits, message

@@ -314,7 +314,7 @@ __device__ __forceinline__ void attend_tile(const Tile& T, int range, int ranges
     int page = ask < to ? page_at(column) : 0;
     uint32_t kbs[F::STAGES - 1], vbs[F::STAGES - 1];      // the bytes of the blocks on their way, oldest first
     const uint32_t mine = (uint32_t)__cvta_generic_to_shared(ring) + warp * (F::STAGES * F::STAGE_BYTES);
-    // (a page's codes stay below 2^31 bytes: head size, page size and heads as the launcher takes them)
+    // (a page's plane has fewer than 2^31 codes: c8_check)
     const uint32_t plane = (uint32_t)c.nkv * c.page_size * hd, plane_scales = (uint32_t)c.nkv * per_page;
     const uint8_t* codes_g = c.codes + (size_t)T.g * c.page_size * hd;
     const uint8_t* scales_g = c.scales + (size_t)T.g * per_page;

@@ -110,6 +110,8 @@ inline int c8_check(const char* what, const void* codes, const void* scales, int
     TQ_REQUIRE(hd % 16 == 0 && hd >= 16 && hd <= C8_MAX_HEAD_DIM, "%s: head size %d is not a multiple of 16 up to %d", what, hd, C8_MAX_HEAD_DIM);
     TQ_REQUIRE(page_size >= C8_BLOCK && page_size % C8_BLOCK == 0, "%s: page size %d is not a multiple of %d", what, page_size, C8_BLOCK);
     TQ_REQUIRE(n_pages >= 0 && nkv >= 1 && table_stride >= 1, "%s: %d pages, %d key/value heads, page tables %d wide", what, n_pages, nkv, table_stride);
+    // (the attention kernels' offsets within a page are 32 bits wide)
+    TQ_REQUIRE((long long)nkv * page_size < (1ll << 31) / hd, "%s: pages of %d rows of %d heads of %d have 2^31 codes a plane or more", what, page_size, nkv, hd);
     TQ_REQUIRE((uintptr_t)codes % 16 == 0, "%s: the codes must be 16-byte aligned", what);
     (void)scales;
     return 0;
