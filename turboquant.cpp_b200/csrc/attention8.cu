@@ -12,9 +12,12 @@
 // 2^-24 of half the row's largest), float32 ones as two parts of 11 bits each.
 //
 // A block's two bytes are uniform over its 16 keys.  The key's scale goes into the factor that makes a sum a score.  The value's cannot go
-// into float16 weights or values as it is (it spans 2^-126 .. 2^120), so the weights are taken as 2^(s + e - m'), m' the running maximum of s + e: at
-// most 1, and what is lost below float16's range is lost against the largest contribution to the result.  The denominator has a
-// maximum of its own, over s.
+// into float16 weights or values as it is (it spans 2^-126 .. 2^120), so the weights are taken as 2^(s + e - m'), m' the running maximum of s + e, times
+// 2^14: at most 2^14, so that float16 holds them to 11 bits down to 2^-28 of the largest and to multiples of 2^-38 of it (without the
+// factor down to 2^-14 and 2^-24: thousands of keys beside one that most of the weight goes to, 2^-22 of it each, then lose a hundredth of their sum).
+// What is lost below that is lost against the largest contribution to the row's result, over all of its elements: an element that is zero in a
+// block whose byte is 30 above the others' has some eight bits of those.  The denominator has a maximum of its own, over s.  m' is kept as its
+// distance from that one: differences of scores are exact where they matter, sums of a score and an exponent are not once scores are large.
 #include "cache8.cuh"
 
 TQ_DEFINE_LAST_ERROR
@@ -261,6 +264,8 @@ __device__ __forceinline__ void products(float (&s)[F::NT][4], const KeyRegs<F>&
 __device__ __forceinline__ int first_seen(int place, int window) { return window > 0 ? max(0, place + 1 - window) : 0; }
 
 constexpr float LOWEST = -3.402823466e38f;       // a maximum over nothing
+// Weights as float16 operands are times 2^WEIGHT_UP, and so are the sums of values until they are results.
+constexpr float WEIGHT_UP = 14.f, WEIGHT_DOWN = 1.f / 16384.f;
 
 // Scores of a step of single rows lie by key, a key's columns side by side in the next power of two (at most 16, or a multiple of 16).
 __host__ __device__ __forceinline__ int score_columns(int per) { return per <= 2 ? per : per <= 4 ? 4 : per <= 8 ? 8 : (per + 15) / 16 * 16; }
@@ -283,8 +288,8 @@ __device__ __forceinline__ float weight_of(const float* __restrict__ scores, con
 }
 
 // ---------------------------------------------------------------------------------------
-// A range of the keys for a tile of columns.  partial: null, or [T * nh][ranges][hd + 4] for a second launch: the unnormalised sum, the
-// maximum m' it is relative to, the denominator's maximum and the denominator.  scores: null, or (runs of one row) the base-2 scores of the
+// A range of the keys for a tile of columns.  partial: null, or [T * nh][ranges][hd + 4] for a second launch: the unnormalised sum (times
+// 2^WEIGHT_UP), the maximum it is relative to, as what it lies above the denominator's, the denominator's maximum and the denominator.  scores: null, or (runs of one row) the base-2 scores of the
 // tile's `per` columns, [n_seqs * nkv][score_stride][score_columns(per)].
 // lse: null, or [T * nh], log2 of the denominator (where there is no second launch).  Several ranges without `partial`: they are the CTAs of a
 // cluster, which join in their shared memory, each for its part of the result; with `weights` and scores each then adds up its own keys'
@@ -297,7 +302,7 @@ __device__ __forceinline__ void attend_tile(const Tile& T, int range, int ranges
     constexpr int NT = F::NT, NC = F::NC, MT = F::MT, HDP = F::HDP;
     extern __shared__ __align__(16) uint8_t ring[];
     __shared__ Queries<F> Q;
-    __shared__ float s_stat[WARPS][NC][3], s_ranks[CLUSTERED ? CLUSTER : 1][NC][3], s_lse[NC];
+    __shared__ float s_stat[WARPS][NC][3], s_ranks[CLUSTERED ? CLUSTER : 1][NC][3], s_part[CLUSTERED ? CLUSTER : 1][NC], s_norm[NC], s_lse[NC];
     float (*s_o)[NC][HDP + 4] = reinterpret_cast<float (*)[NC][HDP + 4]>(ring);        // [WARPS], once the keys are through
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, hd = F::EXACT ? HDP : c.hd;
     // this range's blocks of 16 keys
@@ -352,7 +357,7 @@ __device__ __forceinline__ void attend_tile(const Tile& T, int range, int ranges
 #pragma unroll
         for (int i = 0; i < F::STEPS; ++i) kept[F::KEEP ? i : 0] = Q.b[0][0][i][lane];
     }
-    float o[NT][MT][4], m[NT][2], mo[NT][2], l[NT][2];        // m: of the scores, mo: of scores and value scales
+    float o[NT][MT][4], m[NT][2], mo[NT][2], l[NT][2];        // m: maximum of the scores, mo: that of scores and value scales, less m
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -415,7 +420,7 @@ __device__ __forceinline__ void attend_tile(const Tile& T, int range, int ranges
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 top[nt][j] = fmaxf(s[nt][j], s[nt][j + 2]);
-                grows |= top[nt][j] > m[nt][j] || top[nt][j] + ve > mo[nt][j];
+                grows |= top[nt][j] > m[nt][j] || top[nt][j] - m[nt][j] + ve > mo[nt][j];
             }
         if (__any_sync(0xffffffffu, grows)) {
 #pragma unroll
@@ -424,15 +429,15 @@ __device__ __forceinline__ void attend_tile(const Tile& T, int range, int ranges
                 for (int j = 0; j < 2; ++j) {
 #pragma unroll
                     for (int x = 4; x < 32; x <<= 1) top[nt][j] = fmaxf(top[nt][j], __shfl_xor_sync(0xffffffffu, top[nt][j], x));
-                    const float mn = fmaxf(m[nt][j], top[nt][j]), mon = fmaxf(mo[nt][j], top[nt][j] + ve);
-                    l[nt][j] *= ex2(m[nt][j] - mn);
+                    const float mn = fmaxf(m[nt][j], top[nt][j]), up = m[nt][j] - mn, was = mo[nt][j] + up, mon = fmaxf(was, top[nt][j] - mn + ve);
+                    l[nt][j] *= ex2(up);
                     m[nt][j] = mn;
-                    if (mon > mo[nt][j]) {
-                        const float down = ex2(mo[nt][j] - mon);
+                    if (mon > was) {
+                        const float down = ex2(was - mon);
 #pragma unroll
                         for (int i = 0; i < MT; ++i) { o[nt][i][j] *= down; o[nt][i][j + 2] *= down; }
-                        mo[nt][j] = mon;
                     }
+                    mo[nt][j] = mon;
                 }
         }
         uint32_t p_hi[NT][2], p_lo[NT][2];
@@ -441,8 +446,9 @@ __device__ __forceinline__ void attend_tile(const Tile& T, int range, int ranges
             float w[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                l[nt][j & 1] += ex2(s[nt][j] - m[nt][j & 1]);
-                w[j] = ex2(s[nt][j] + (ve - mo[nt][j & 1]));
+                const float below = s[nt][j] - m[nt][j & 1];
+                l[nt][j & 1] += ex2(below);
+                w[j] = ex2(below + (ve + WEIGHT_UP - mo[nt][j & 1]));
             }
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
@@ -540,13 +546,16 @@ __device__ __forceinline__ void attend_tile(const Tile& T, int range, int ranges
         }
     __syncthreads();
     for (int col = warp; col < T.n; col += WARPS) {
-        float mw[WARPS], M = LOWEST, MO = LOWEST, L = 0.f;
+        float mw[WARPS], M = LOWEST, MO = LOWEST, L = 0.f;            // (MO: less M)
 #pragma unroll
-        for (int w = 0; w < WARPS; ++w) { MO = fmaxf(MO, s_stat[w][col][0]); M = fmaxf(M, s_stat[w][col][1]); }
+        for (int w = 0; w < WARPS; ++w) M = fmaxf(M, s_stat[w][col][1]);
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) MO = fmaxf(MO, s_stat[w][col][1] - M + s_stat[w][col][0]);
 #pragma unroll
         for (int w = 0; w < WARPS; ++w) {
-            mw[w] = exp2f(s_stat[w][col][0] - MO);
-            L += s_stat[w][col][2] * exp2f(s_stat[w][col][1] - M);
+            const float below = s_stat[w][col][1] - M;
+            mw[w] = exp2f(below + s_stat[w][col][0] - MO);
+            L += s_stat[w][col][2] * exp2f(below);
         }
         if (CLUSTERED) {
             for (int d = lane; d < hd; d += 32) {
@@ -561,20 +570,20 @@ __device__ __forceinline__ void attend_tile(const Tile& T, int range, int ranges
         }
         const size_t at = Q.row[col];
         float* pp = partial != nullptr ? partial + (at * ranges + range) * (hd + 4) : nullptr;
-        const float norm = exp2f(MO - M) / L;
+        const float norm = exp2f(MO) / L;
         for (int d = lane; d < hd; d += 32) {
             float sum = 0.f;
 #pragma unroll
             for (int w = 0; w < WARPS; ++w) sum += s_o[w][col][d] * mw[w];
             if (pp != nullptr) pp[d] = sum;
-            else out[at * hd + d] = tq_from_float<typename F::TA>(sum * norm);
+            else out[at * hd + d] = tq_from_float<typename F::TA>(sum * WEIGHT_DOWN * norm);
         }
         if (pp != nullptr && lane == 0) { pp[hd] = MO; pp[hd + 1] = M; pp[hd + 2] = L; }
         if (pp == nullptr && lse != nullptr && lane == 0) lse[at] = M + log2f(L);
     }
     if (!CLUSTERED) return;
     __syncwarp();
-    // the cluster's sums together: statistics of all ranges first, then every CTA its part of the tile's results
+    // the cluster's sums together: statistics of all ranges first (a warp a column, a lane a range), then every CTA its part of the tile's results
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
     auto remote = [](const float* own, int rank) {
         uint32_t a;
@@ -586,26 +595,35 @@ __device__ __forceinline__ void attend_tile(const Tile& T, int range, int ranges
     for (int i = threadIdx.x; i < ranges * NC * 3; i += WARPS * 32)
         if (i / 3 % NC < T.n) (&s_ranks[0][0][0])[i] = remote(&s_stat[0][0][0] + i % (NC * 3), i / (NC * 3));
     __syncthreads();
+    for (int col = warp; col < T.n; col += WARPS) {
+        const bool mine = lane < ranges;                               // the lane's range
+        const float mor = mine ? s_ranks[lane][col][0] : LOWEST, mr = mine ? s_ranks[lane][col][1] : LOWEST, lr = mine ? s_ranks[lane][col][2] : 0.f;
+        float M = mr;
+#pragma unroll
+        for (int x = 1; x < CLUSTER; x <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
+        const float below = mr - M;
+        float MO = below + mor, L = lr * exp2f(below);
+#pragma unroll
+        for (int x = 1; x < CLUSTER; x <<= 1) {
+            MO = fmaxf(MO, __shfl_xor_sync(0xffffffffu, MO, x));
+            L += __shfl_xor_sync(0xffffffffu, L, x);
+        }
+        if (lane < ranges) s_part[lane][col] = exp2f(below + mor - MO);
+        if (lane == 0) {
+            s_norm[col] = exp2f(MO) / L;
+            s_lse[col] = M + log2f(L);
+            if (lse != nullptr && range == 0) lse[Q.row[col]] = M + log2f(L);
+        }
+    }
+    __syncthreads();
     for (int i = range * WARPS * 32 + threadIdx.x; i < T.n * hd; i += ranges * WARPS * 32) {
         const int col = i / hd, d = i - col * hd;
-        float M = LOWEST, MO = LOWEST, L = 0.f, sum = 0.f;
-        for (int r = 0; r < ranges; ++r) { MO = fmaxf(MO, s_ranks[r][col][0]); M = fmaxf(M, s_ranks[r][col][1]); }
+        float sum = 0.f;
 #pragma unroll 8
-        for (int r = 0; r < ranges; ++r) {
-            L += s_ranks[r][col][2] * exp2f(s_ranks[r][col][1] - M);
-            sum += remote(&s_o[0][col][d], r) * exp2f(s_ranks[r][col][0] - MO);
-        }
-        out[Q.row[col] * hd + d] = tq_from_float<typename F::TA>(sum * (exp2f(MO - M) / L));
-        if (lse != nullptr && d == 0) lse[Q.row[col]] = M + log2f(L);
+        for (int r = 0; r < ranges; ++r) sum += remote(&s_o[0][col][d], r) * s_part[r][col];
+        out[Q.row[col] * hd + d] = tq_from_float<typename F::TA>(sum * WEIGHT_DOWN * s_norm[col]);
     }
     if (weights != nullptr) {
-        if (threadIdx.x < T.n) {
-            float M = LOWEST, L = 0.f;
-            for (int r = 0; r < ranges; ++r) M = fmaxf(M, s_ranks[r][threadIdx.x][1]);
-            for (int r = 0; r < ranges; ++r) L += s_ranks[r][threadIdx.x][2] * exp2f(s_ranks[r][threadIdx.x][1] - M);
-            s_lse[threadIdx.x] = M + log2f(L);
-        }
-        __syncthreads();
         // (the step has one row of the sequence: it sees up to its own place)
         const int last = min(min(to * C8_BLOCK, place1 + 1), score_stride);
 #pragma unroll 2
@@ -658,7 +676,7 @@ __global__ void __launch_bounds__(WARPS * 32) repair8_kernel(const typename F::T
 // ---------------------------------------------------------------------------------------
 constexpr int JOIN_RANGES = 64;
 
-// The statistics of row `at` of q, and each range's factor in s_f[0 .. ranges - 1]; by a warp, which then has them.
+// The statistics of row `at` of q (MO: less M), and each range's factor in s_f[0 .. ranges - 1]; by a warp, which then has them.
 __device__ __forceinline__ void join_stats(const float* __restrict__ partial, size_t at, int ranges, int hd, float& MO, float& M, float& L, float* s_f) {
     const int lane = threadIdx.x & 31;
     const float* p = partial + at * ranges * (hd + 4) + hd;
@@ -670,15 +688,16 @@ __device__ __forceinline__ void join_stats(const float* __restrict__ partial, si
         mo[i] = m[i] = LOWEST;
         l[i] = 0.f;
         if (r < ranges) { mo[i] = p[(size_t)r * (hd + 4)]; m[i] = p[(size_t)r * (hd + 4) + 1]; l[i] = p[(size_t)r * (hd + 4) + 2]; }
-        MO = fmaxf(MO, mo[i]);
         M = fmaxf(M, m[i]);
     }
-    MO = tq_warp_max(MO);
     M = tq_warp_max(M);
+#pragma unroll
+    for (int i = 0; i < JOIN_RANGES / 32; ++i) MO = fmaxf(MO, m[i] - M + mo[i]);
+    MO = tq_warp_max(MO);
 #pragma unroll
     for (int i = 0; i < JOIN_RANGES / 32; ++i) {
         L += l[i] * exp2f(m[i] - M);
-        if (s_f != nullptr && lane + 32 * i < ranges) s_f[lane + 32 * i] = exp2f(mo[i] - MO);
+        if (s_f != nullptr && lane + 32 * i < ranges) s_f[lane + 32 * i] = exp2f(m[i] - M + mo[i] - MO);
     }
     L = tq_warp_sum(L);
 }
@@ -705,7 +724,7 @@ __global__ void __launch_bounds__(128) join8_kernel(Cache8 c, Step S, const floa
             float MO, M, L;
             join_stats(partial, at, ranges, hd, MO, M, L, s_f);
             if (lane == 0) {
-                s_lse[0] = exp2f(MO - M) / L;
+                s_lse[0] = exp2f(MO) / L;
                 if (lse != nullptr) lse[at] = M + log2f(L);
             }
         }
@@ -719,7 +738,7 @@ __global__ void __launch_bounds__(128) join8_kernel(Cache8 c, Step S, const floa
             for (int r = 0; r < 8; ++r) if (r < ranges) sum += v[h][r] * s_f[r];
 #pragma unroll 8
             for (int r = 8; r < ranges; ++r) sum += p[(size_t)r * (hd + 4) + d] * s_f[r];
-            out[at * hd + d] = tq_from_float<TA>(sum * s_lse[0]);
+            out[at * hd + d] = tq_from_float<TA>(sum * WEIGHT_DOWN * s_lse[0]);
         }
         return;
     }
