@@ -83,3 +83,75 @@ def test_scores_far_from_zero(dtype, size, ranges, monkeypatch):
         got, _ = _attend(q, codes, scales, [1], [rows - 1], table, 64, 0, size, H, G, D)
         want = got if want is None else want
         assert torch.equal(got, want), sign
+
+
+# ---- steps launched ahead ----------------------------------------------------------------------------------------------------
+def _begun(model, prompts):
+    import turboquant_cpp_b200 as tq
+    engine = tq.Engine(model, max_tokens=512, cache_dtype="e4m3")
+    seqs = [engine.open() for _ in prompts]
+    engine.step([tq.StepEntry(s, p) for s, p in zip(seqs, prompts)])
+    engine.step([tq.StepEntry(s, [6], [0]) for s in seqs])
+    return engine, seqs
+
+
+def _rows(engine, seq):
+    """The first page of a sequence of up to 16 rows: its codes and bytes, every layer."""
+    page = seq.pages[0][0]
+    return [t for c, b in zip(engine.cache.kv, engine.cache.scales) for t in (c.view(torch.uint8)[page, :, :, :seq.held].cpu(), b[page, :, :, 0].cpu())]
+
+
+def test_a_step_launched_ahead_counts_for_those_that_go_on(tiny_folders):
+    """A row that raises its block's byte has the rows it finds there rounded again, for good: dropping its step does not undo it.  So the step is kept, and
+    leaves what a plain step leaves."""
+    import turboquant_cpp_b200 as tq
+    from turboquant_cpp_b200.engine.step import StepError
+    model = tq.load_model(tiny_folders["A"], "float32", DEV)
+    prompts = [[3, 17, 200, 42, 9], [7, 8, 9], [100, 2]]
+    (engine, (a, b, c)), (other, theirs) = _begun(model, prompts), _begun(model, prompts)
+    before = _rows(engine, a)
+    assert engine.can_step_ahead and all(torch.equal(x, y) for x, y in zip(before, _rows(other, theirs[0])))
+    for token in range(0, 256, 5):
+        tokens = [token, 9, (token + 1) % 256]
+        logits = engine.step_ahead([a, b, c], torch.tensor(tokens, dtype=torch.int32, device=DEV)).clone()
+        with pytest.raises(StepError):
+            engine.drop_ahead()
+        with pytest.raises(StepError):
+            engine.step([tq.StepEntry(a, [1], [0])])
+        with pytest.raises(StepError):
+            engine.commit_ahead([a, c])                  # b is open
+        if a.held == 10:
+            engine.close(b)
+            engine.commit_ahead([c, a])
+        else:
+            engine.commit_ahead()
+        want = other.step([tq.StepEntry(s, [t], [0]) for s, t in zip(theirs, tokens)])
+        assert torch.equal(logits, want) and a.held == theirs[0].held
+        assert all(torch.equal(x, y) for x, y in zip(_rows(engine, a), _rows(other, theirs[0])))
+        if not b.open:
+            break
+    assert any(not torch.equal(x, y) for x, y in zip(before, [t[:, :, :6] if t.dim() == 4 else t for t in _rows(engine, a)]))        # bytes did grow
+    with pytest.raises(StepError):
+        engine.step_ahead([a], torch.tensor([1], dtype=torch.int32, device=DEV)), engine.commit_ahead([c])
+    engine.close(a)
+    engine.drop_ahead()                                  # nobody is left whom it could have changed
+    assert torch.isfinite(engine.step([tq.StepEntry(c, [1], [0])])).all()
+    engine.close(c)
+    engine.cache.book.check_invariants()
+    engine.release()
+    other.release()
+
+
+def test_generation_whose_requests_end_early(tiny_folders, monkeypatch):
+    """Steps ahead of their tokens or not: the same tokens."""
+    import turboquant_cpp_b200 as tq
+    model = tq.load_model(tiny_folders["A"], "float32", DEV)
+    prompts = [[5, 9, 2], list(range(60)), [1] * 20, [200, 100], [77]]
+    out = []
+    for graphs in (True, False):
+        monkeypatch.setenv("TQ_NO_GRAPHS", "0" if graphs else "1")
+        with tq.Model.from_model(model, temperature=0.0, max_tokens=40, context_length=128, max_batch=5, stop_token_ids=list(range(0, 256, 17)), cache_dtype="e4m3") as m:
+            assert m.engine.can_step_ahead == graphs
+            out.append(m.generate_batch(prompts))
+            m.engine.cache.book.check_invariants()
+    assert out[0] == out[1] and len({len(t) for t in out[0]}) > 1 and min(len(t) for t in out[0]) < 40

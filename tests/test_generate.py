@@ -331,3 +331,45 @@ def test_loop_detector_ends_a_request_as_the_reference_does():
         for _ in range(120):
             out.append(rng.randrange(3))
             assert det.push(out[-1]) == closes_a_loop(prompt, out)
+
+
+class FakeCountingEngine(FakeAheadEngine):
+    """... whose steps cannot be undone: one launched ahead is kept for the sequences that go on, and dropped only when all of its are closed."""
+    ahead_counts = True
+
+    def commit_ahead(self, keep=None):
+        seqs, toks = self.pending
+        keep = seqs if keep is None else keep
+        assert all((s.id in self.book.live) == (s in keep) for s in seqs)
+        self.pending = ([s for s in seqs if s in keep], [t for s, t in zip(seqs, toks) if s in keep])
+        super().commit_ahead()
+
+    def drop_ahead(self):
+        assert not any(s.id in self.book.live for s in self.pending[0])
+        super().drop_ahead()
+
+
+@pytest.mark.parametrize("stop,max_new", [((), 6), ((24,), 6), ((24, 3, 7), 12), ((24, 0, 48, 25), 30), ((), 1), ((), 2)])
+def test_steps_that_cannot_be_undone_are_kept_by_those_that_go_on(stop, max_new):
+    prompts = [[1, 2, 3], [4] * 11, [5] * 17, [7], [9, 9], [3] * 290]
+    params = GenParams(max_new_tokens=max_new, stop_token_ids=stop)
+    want = generate(FakeEngine(), ArgmaxSampler(), prompts, params, max_batch=3)
+    eng, smp = FakeCountingEngine(), ArgmaxSampler()
+    got = generate(eng, smp, prompts, params, max_batch=3)
+    assert [(r.tokens, r.finish_reason) for r in got] == [(r.tokens, r.finish_reason) for r in want]
+    assert eng.pending is None and not eng.book.live and eng.book.pools[0].n_free == eng.book.pools[0].n
+    for reqs, steps in smp.calls:
+        assert len(reqs) == len(set(reqs)) and all(0 <= s < max_new for s in steps)
+    if not stop:
+        assert eng.dropped == 0
+
+
+def test_an_error_closes_sequences_before_their_step_is_dropped():
+    eng = FakeCountingEngine()
+
+    def boom(idx, toks):
+        if len(toks) and eng.kept >= 1:
+            raise RuntimeError("stop here")
+    with pytest.raises(RuntimeError, match="stop here"):
+        generate(eng, ArgmaxSampler(), [[1, 2], [3]], GenParams(max_new_tokens=8), on_tokens=boom)
+    assert eng.pending is None and not eng.book.live

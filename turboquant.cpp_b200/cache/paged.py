@@ -45,6 +45,7 @@ class PagedCache:
         self.page_size = int(page_size)
         self.device = torch.device(device)
         self.dtype = dtype
+        self.eight_bits = bool(eight_bits)
         n_pages = max(1, -(-int(max_tokens) // self.page_size))
         self.max_slots = int(max_slots) if max_slots is not None else min(n_pages, 1024)
         self.groups: List[KVNeed] = []

@@ -114,7 +114,8 @@ def generate(engine, sampler, prompts: Sequence[Sequence[int]], params: GenParam
 
     engine:   open(), close(seq), step(entries) -> logits rows, make_entry(seq, tokens, want),
               capacity_tokens, max_slots, page_size, max_position; optionally bounded_rows; optionally can_step_ahead, step_ahead(seqs,
-              sampled tokens) -> logits rows, commit_ahead(), drop_ahead(), token_reader(n); optionally
+              sampled tokens) -> logits rows, commit_ahead(), drop_ahead(), token_reader(n), and ahead_counts with
+              commit_ahead(sequences that go on); optionally
               tokens_to_host(sampled tokens) -> list, which may raise if the step's kernels reported a fault (the
               tokens are then neither appended nor told)
     sampler:  sample(logits, request indices, token indices) -> one token per row (anything with .tolist());
@@ -125,7 +126,8 @@ def generate(engine, sampler, prompts: Sequence[Sequence[int]], params: GenParam
 
     An engine that can (`can_step_ahead`) is kept one decode step ahead of the host: the next step is launched
     from the samples while they are still on the device, and the host reads them meanwhile.  If a sequence
-    turns out to have ended, that step is dropped and run again without it, so the results are the same."""
+    turns out to have ended, that step is dropped and run again without it, so the results are the same; with an engine
+    whose steps cannot be undone (`ahead_counts`) the others keep it."""
     stats = stats if stats is not None else GenStats()
     sync = sync or (lambda: None)
     results = [GenResult() for _ in prompts]
@@ -166,6 +168,7 @@ def generate(engine, sampler, prompts: Sequence[Sequence[int]], params: GenParam
             stats.steps += 1
             t0 = time.perf_counter()
             can_ahead = bool(getattr(engine, "can_step_ahead", False))
+            counts = can_ahead and bool(getattr(engine, "ahead_counts", False))
             reader = engine.token_reader(len(order)) if can_ahead else None
             while True:
                 nxt: List[Tuple[int, int]] = []
@@ -199,6 +202,11 @@ def generate(engine, sampler, prompts: Sequence[Sequence[int]], params: GenParam
                     engine.commit_ahead()                # nobody ended: the step launched ahead is this step
                     logits = ahead[1]
                     ahead = None
+                elif ahead is not None and counts:       # somebody ended: it is the others' step
+                    order = [i for i, _ in nxt]
+                    engine.commit_ahead([live[i] for i in order])
+                    logits = ahead[1][[ahead[0].index(i) for i in order]]
+                    ahead = None
                 else:
                     if ahead is not None:                # somebody ended: that step is void
                         ahead = None
@@ -227,8 +235,8 @@ def generate(engine, sampler, prompts: Sequence[Sequence[int]], params: GenParam
             sync()
             stats.decode_seconds += time.perf_counter() - t0
         finally:
-            if ahead is not None:                        # the batch ended, or an error, before the step's fate
-                engine.drop_ahead()
             for seq in live.values():
                 engine.close(seq)
+            if ahead is not None:                        # the batch ended, or an error, before the step's fate
+                engine.drop_ahead()
     return results

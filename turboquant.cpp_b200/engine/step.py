@@ -318,6 +318,8 @@ class Engine:
         the order of the entries and of each entry's `want`; None if nothing is wanted."""
         if not entries:
             return None
+        if self._ahead is not None and self.ahead_counts:
+            raise StepError("a step launched ahead is still waiting to be kept")
         self._check(entries)
         seqs = [e.seq for e in entries]
         n_new = [len(e.tokens) for e in entries]
@@ -371,12 +373,19 @@ class Engine:
         state, sums of attention weights among it, that a dropped step would have changed)."""
         return self.graphs is not None and self.debug is None and self._stateless and not self.layer_dump and not self.cache_budget
 
+    @property
+    def ahead_counts(self) -> bool:
+        """Whether a step launched ahead counts for every sequence that goes on (`commit_ahead(keep)`; it is dropped only once all of its
+        sequences are closed): over a cache in 8 bits a row that raises its block's scale has the rows it finds there rounded again, for good."""
+        return self.cache.eight_bits
+
     def step_ahead(self, seqs: Sequence[Sequence_], tokens_dev: torch.Tensor) -> torch.Tensor:
         """Launches the decode step whose tokens are `tokens_dev` (int32, one per sequence, on the device: the
         samples of the step before) and returns its logits, without advancing the sequences: the caller reads the
         samples on the host meanwhile and then either keeps the step (`commit_ahead`) or, if a sequence turned
         out to have ended, drops it (`drop_ahead`) and steps again.  A dropped step leaves nothing behind: what it
         wrote into the cache lies beyond the sequences' lengths and is written again by the step that replaces it.
+        Where that is not so (`ahead_counts`), the step is kept for the sequences that go on.
         The logits are the captured step's own buffer: they hold until the next decode step of this batch size."""
         if not self.can_step_ahead:
             raise StepError("this engine cannot launch a step ahead")
@@ -415,10 +424,18 @@ class Engine:
             raise KernelError("step: " + GAVE_UP + "; the tokens sampled from it are withheld")
         return both[:-1]
 
-    def commit_ahead(self) -> None:
+    def commit_ahead(self, keep: Optional[Sequence[Sequence_]] = None) -> None:
+        """The step launched ahead is the next step of its sequences, or of those in `keep`, the others being closed."""
         seqs, n_new = self._ahead
+        if keep is not None:
+            going = {s.id for s in keep}
+            if not going <= {s.id for s in seqs} or any(s.open and s.id not in going for s in seqs):
+                raise StepError("a step launched ahead is kept for all of its sequences that are open, and for no others")
+            seqs, n_new = list(keep), [1] * len(keep)
         self._ahead = None
         self._commit(seqs, n_new)
 
     def drop_ahead(self) -> None:
+        if self._ahead is not None and self.ahead_counts and any(s.open for s in self._ahead[0]):
+            raise StepError("a step launched ahead over a cache in 8 bits cannot be dropped while its sequences are open")
         self._ahead = None
