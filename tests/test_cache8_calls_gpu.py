@@ -155,3 +155,36 @@ def test_generation_whose_requests_end_early(tiny_folders, monkeypatch):
             out.append(m.generate_batch(prompts))
             m.engine.cache.book.check_invariants()
     assert out[0] == out[1] and len({len(t) for t in out[0]}) > 1 and min(len(t) for t in out[0]) < 40
+
+
+# ---- tensors off their 16-byte boundaries --------------------------------------------------------------------------------------
+def _off(t, where):
+    """The same elements one element behind a boundary of 16 bytes."""
+    if not where:
+        return t
+    x = torch.empty(t.numel() + 1, dtype=t.dtype, device=t.device)[1:].view(t.shape)
+    x.copy_(t)
+    assert x.data_ptr() % 16 and x.is_contiguous()
+    return x
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("runs,held", [([1, 1], [70, 5]), ([60, 3], [0, 40])])
+@pytest.mark.parametrize("q_off,out_off", [(True, False), (False, True), (True, True)])
+def test_queries_and_results_may_begin_anywhere(dtype, runs, held, q_off, out_off, monkeypatch):
+    """Whatever the step's size: with the long run the prompt kernel is asked for, which itself wants 16-byte boundaries.  Rows behind the last sequence stay."""
+    from turboquant_cpp_b200.kernels import cache8
+    monkeypatch.setattr(cache8, "PROMPT_WORK", 0)
+    H, G, D = 8, 2, 64
+    table, pages = _pages([n + h for n, h in zip(runs, held)], 64)
+    codes, scales = _cache(pages, G, 64, D)
+    q = torch.randn(sum(runs) + 2, H, D).to(dtype).to(DEV)
+    seen = []
+    for moved in (False, True):
+        out = _off(torch.full((sum(runs) + 2, H * D), 7.0, dtype=dtype, device=DEV), moved and out_off)
+        w = torch.zeros(pages, G, 64, device=DEV)
+        got = cache8.attention8(_off(q, moved and q_off), _on(codes), scales.to(DEV), _cu(runs), _i(held), table.to(DEV), 64, 0, 0.1, out, H, G, D, max(runs),
+                                max(n + h for n, h in zip(runs, held)), weights=w)
+        assert got is out and bool((out[-2:] == 7.0).all())
+        seen.append((out.clone(), w))
+    assert torch.equal(seen[0][0], seen[1][0]) and torch.equal(seen[0][1], seen[1][1])

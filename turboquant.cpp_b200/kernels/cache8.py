@@ -201,8 +201,13 @@ def attention8(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, cu_se
         return out
     max_q_len, max_kv_len = index(max_q_len), index(max_kv_len)
     if max_q_len >= PROMPT_MIN_RUN and prefill_usable(dtype, head_dim, page_size) and T * (max_kv_len - max_q_len // 2) * n_heads * head_dim >= PROMPT_WORK:
-        return _attention8_prompt(q, codes, scales, cu_seqlens, held, page_table, page_size, window, scale, out, n_heads, n_kv_heads, head_dim,
-                                  max_q_len, max_kv_len, weights, status)
+        # the prompt kernel copies and stores 16 bytes at a time: queries and results that begin elsewhere go through a copy
+        if q.is_contiguous() and q.data_ptr() % 16:
+            q = q.clone()
+        to = out.clone() if out.is_contiguous() and out.data_ptr() % 16 else out           # (rows behind the last sequence come back as they were)
+        _attention8_prompt(q, codes, scales, cu_seqlens, held, page_table, page_size, window, scale, to, n_heads, n_kv_heads, head_dim,
+                           max_q_len, max_kv_len, weights, status)
+        return out if to is out else out.copy_(to)
     p_q, p_out, p_codes, p_scales, p_cu, p_held, p_table, p_weights, at = addresses(q, out, codes, scales, cu_seqlens, held, page_table, weights)
     per = n_heads // n_kv_heads
     columns = max_q_len * per
