@@ -188,3 +188,39 @@ def test_queries_and_results_may_begin_anywhere(dtype, runs, held, q_off, out_of
         assert got is out and bool((out[-2:] == 7.0).all())
         seen.append((out.clone(), w))
     assert torch.equal(seen[0][0], seen[1][0]) and torch.equal(seen[0][1], seen[1][1])
+
+
+# ---- scratch ------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("with_weights", [False, True])
+@pytest.mark.parametrize("shape", [(8, 2, 64), (16, 16, 128), (7, 1, 128)], ids=str)
+@pytest.mark.parametrize("runs,held,window", [([64, 0, 50, 1], [6000, 5, 3000, 40], 100), ([200], [4999], 1), ([130, 70], [3, 6400], 64), ([300], [2000], 700)])
+def test_a_windowed_prompt_expands_the_pages_it_sees(shape, runs, held, window, with_weights, monkeypatch):
+    """Scratch for the window's pages of each sequence, not for all that its longest one holds; the result is held to the 64-bit one."""
+    from turboquant_cpp_b200.kernels import cache8
+    monkeypatch.setattr(cache8, "PROMPT_WORK", 0)
+    H, G, D = shape
+    table, pages = _pages([n + h for n, h in zip(runs, held)], 64, windows=[max(0, h + 1 - window) for h in held])
+    codes, scales = _cache(pages, G, 64, D, spread=1.0)
+    q = (torch.randn(sum(runs), H, D) * 1.5).to(torch.bfloat16)
+    scale, weights = 1.0 / math.sqrt(D) / 4, torch.rand(pages, G, 64)
+    args = [q.to(DEV), _on(codes), scales.to(DEV), _cu(runs), _i(held), table.to(DEV)]
+    out, w = torch.full((sum(runs), H * D), float("nan"), dtype=torch.bfloat16, device=DEV), weights.to(DEV) if with_weights else None
+    longest = max(n + h for n, h in zip(runs, held))
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    cache8.attention8(*args, 64, window, scale, out, H, G, D, max(runs), longest, weights=w)
+    took = torch.cuda.max_memory_allocated() - before
+    seen = len(runs) * ((max(runs) + window) // 64 + 2) * 2 * G * 64 * D * 2           # bfloat16 pages of what the sequences may see
+    pieces = 4 * sum(runs) * H * (D + 1) * (longest // 512 + 2)
+    assert took <= 1.01 * seen + pieces + (1 << 20), (took, seen, pieces)
+    want, mags, units, p = plain.attention(q, codes, scales, runs, held, table, 64, window, scale, H, G, D)
+    top = float((codes.view(torch.float8_e4m3fn).float().abs() * torch.pow(2.0, scales.float() - 127).repeat_interleave(16, -1)[..., None]).max())
+    limit = _limit(torch.bfloat16, want, mags, units, D, longest, top)
+    off = (out.cpu().double().view(want.shape) - want).abs()
+    assert bool((off <= limit).all()), float((off / limit).max())
+    if with_weights:
+        want_w = weights.double()
+        plain.add_weights(want_w, p, runs, held, table, 64, H, G)
+        rel = float(2.02 * ((D + 8) * 4 * U * units).max()) + (longest + H // G * max(runs) + 16) * 4 * U
+        assert bool(((w.cpu().double() - want_w).abs() <= rel * want_w.abs() + 1e-30).all())

@@ -24,13 +24,17 @@ __device__ __forceinline__ uint32_t bf16x2_of(uint32_t two, float scale) {
     return *reinterpret_cast<const uint32_t*>(&b);
 }
 
+// the first page of a sequence that a step's rows see
+__device__ __forceinline__ int first_page(int start, int window) { return (window > 0 ? max(0, start + 1 - window) : 0) / PAGE; }
+
 __global__ void __launch_bounds__(256) expand8_kernel(Cache8 c, const int* __restrict__ cu_seqlens, const int* __restrict__ held, int window, uint4* __restrict__ dense,
-                                                      int* __restrict__ dense_table, uint8_t* __restrict__ lost, int width) {
+                                                      int* __restrict__ dense_table, uint8_t* __restrict__ lost, int width, int dense_width) {
     tq_grid_wait();                    // everything below may read what the previous kernel wrote
     tq_grid_launch_dependents();
     const int n = blockIdx.x, g = blockIdx.y, seq = blockIdx.z, start = held[seq], run = cu_seqlens[seq + 1] - cu_seqlens[seq], last = start + run - 1;
-    if (run <= 0 || n * PAGE > last || n < (window > 0 ? max(0, start + 1 - window) : 0) / PAGE) return;
-    const int page = c.page_of(seq, n * PAGE), to = seq * width + n, vecs = c.hd / 16, rows = min(PAGE, last + 1 - n * PAGE);
+    const int first = first_page(start, window);
+    if (run <= 0 || n * PAGE > last || n < first || n - first >= dense_width) return;
+    const int page = c.page_of(seq, n * PAGE), to = seq * dense_width + n - first, vecs = c.hd / 16, rows = min(PAGE, last + 1 - n * PAGE);
     bool nan = false;
     const uint8_t* codes = c.codes + c.codes_at(page, 0, g);
     const uint8_t* scales = c.scales + c.scales_at(page, 0, g);
@@ -70,7 +74,7 @@ __global__ void __launch_bounds__(256) expand8_kernel(Cache8 c, const int* __res
     const bool any = __syncthreads_or(nan);
     if (threadIdx.x == 0) {
         lost[((size_t)seq * c.nkv + g) * width + n] = any ? 1 : 0;
-        if (g == 0) dense_table[to] = to;
+        if (g == 0) dense_table[seq * width + n] = to;
     }
 }
 
@@ -138,13 +142,13 @@ weigh8_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
     auto wait = [&](uint32_t bar, uint32_t parity) { return (bool)__all_sync(0xffffffffu, mbar_wait(bar, parity, &s_abort)); };
     if (warp == 0) {
         const uint32_t elected = elect_one();
-        const int pages = min(2, (start + run - 1) / PAGE - key0 / PAGE + 1);
+        const int pages = min(2, (start + run - 1) / PAGE - key0 / PAGE + 1), first = first_page(start, S.window);
         if (elected) {
             mbar_expect_tx(k_full, (uint32_t)(pages * C::PAGE_BYTES));
             for (int p = 0; p < pages; ++p)
 #pragma unroll
                 for (int c = 0; c < C::KB; ++c)
-                    tma_load_2d(base + c * (BM * 128) + p * (PAGE * 128), &map_k, c * 64, ((seq * S.width + key0 / PAGE + p) * 2 * S.nkv + g) * PAGE, k_full);
+                    tma_load_2d(base + c * (BM * 128) + p * (PAGE * 128), &map_k, c * 64, ((seq * S.width + max(key0 / PAGE + p - first, 0)) * 2 * S.nkv + g) * PAGE, k_full);      // (a page no row sees: any other's keys)
         }
         int i = 0;
         for (; i < n; ++i) {
@@ -256,24 +260,24 @@ int launch_weigh_prompt(const CUtensorMap& mq, const CUtensorMap& mk, const WSha
 
 }  // namespace
 
-// dense [n_seqs * width, 2, nkv, 64, hd] bfloat16: page n of sequence s at s * width + n, which dense_table [n_seqs, width] says;
-// lost [n_seqs, nkv, width] bytes.  Pages the step does not see are left alone in all three.
+// dense [n_seqs * dense_width, 2, nkv, 64, hd] bfloat16: page n of sequence s at s * dense_width + n - the first page its rows see, which
+// dense_table [n_seqs, width] says; lost [n_seqs, nkv, width] bytes.  Pages the step does not see are left alone in all three.
 TQ_EXPORT int tq_expand8(const void* codes, const void* scales, const int* cu_seqlens, const int* held, const int* page_table, int table_stride, int page_size,
-                         int window, void* dense, int* dense_table, void* lost, int width, int n_pages, int n_seqs, int nkv, int hd, cudaStream_t stream) {
+                         int window, void* dense, int* dense_table, void* lost, int width, int dense_width, int n_pages, int n_seqs, int nkv, int hd, cudaStream_t stream) {
     if (n_seqs == 0 || width == 0) return 0;
     int rc = c8_check("expand8", codes, scales, page_size, n_pages, nkv, hd, table_stride);
     if (rc) return rc;
     TQ_REQUIRE(page_size == PAGE && n_seqs <= 65535 && nkv <= 65535 && window >= 0, "expand8: page size %d, %d sequences, %d heads, window %d", page_size, n_seqs, nkv, window);
-    TQ_REQUIRE((long long)n_seqs * width < (1ll << 31) && (uintptr_t)dense % 16 == 0, "expand8: %d pages for each of %d sequences", width, n_seqs);
+    TQ_REQUIRE(dense_width >= 1 && dense_width <= width && (long long)n_seqs * width < (1ll << 31) && (uintptr_t)dense % 16 == 0, "expand8: %d pages for each of %d sequences", width, n_seqs);
     const Cache8 c = c8_cache(codes, scales, page_table, table_stride, page_size, n_pages, nkv, hd);
-    tq_launch(dim3(width, nkv, n_seqs), 256, 0, stream)(expand8_kernel, c, cu_seqlens, held, window, (uint4*)dense, dense_table, (uint8_t*)lost, width);
+    tq_launch(dim3(width, nkv, n_seqs), 256, 0, stream)(expand8_kernel, c, cu_seqlens, held, window, (uint4*)dense, dense_table, (uint8_t*)lost, width, dense_width);
     TQ_CHECK_LAUNCH("expand8");
     return 0;
 }
 
 // q [T, nh, hd] bfloat16, dense as tq_expand8 leaves it, lse [T, nh]: the base-2 logarithm of each row's denominator.  weights [n_pages, nkv, 64]
 // of places below held[s] grow by, those of the step's own rows become, the sum over the step's rows and the head's query heads of their weight.
-TQ_EXPORT int tq_weigh8_prompt(const void* q, const void* dense, int width, const int* cu_seqlens, const int* held, const int* page_table, int table_stride,
+TQ_EXPORT int tq_weigh8_prompt(const void* q, const void* dense, int dense_width, const int* cu_seqlens, const int* held, const int* page_table, int table_stride,
                                int window, float scale, const float* lse, float* weights, int n_pages, int T_, int n_seqs, int max_kv_len, int nh, int nkv, int hd,
                                int* status, cudaStream_t stream) {
     if (n_seqs == 0 || T_ == 0 || max_kv_len == 0) return 0;
@@ -281,9 +285,9 @@ TQ_EXPORT int tq_weigh8_prompt(const void* q, const void* dense, int width, cons
     TQ_REQUIRE(window >= 0 && max_kv_len >= 1 && status != nullptr, "weigh8_prompt: window %d, %d places", window, max_kv_len);
     TQ_REQUIRE(((uintptr_t)q | (uintptr_t)dense) % 16 == 0, "weigh8_prompt: q and the scratch must be 16-byte aligned");
     const int tiles = (max_kv_len + BM - 1) / BM;
-    const long long rows = (long long)n_seqs * width * 2 * nkv * PAGE;
-    TQ_REQUIRE(rows < (1ll << 31) && tiles <= 65535 && (long long)nkv * n_seqs < (1ll << 31), "weigh8_prompt: %d pages for each of %d sequences", width, n_seqs);
-    const WShape S{nh, nkv, width, window, table_stride, n_pages, scale * 1.4426950408889634f};
+    const long long rows = (long long)n_seqs * dense_width * 2 * nkv * PAGE;
+    TQ_REQUIRE(rows < (1ll << 31) && tiles <= 65535 && (long long)nkv * n_seqs < (1ll << 31), "weigh8_prompt: %d pages for each of %d sequences", dense_width, n_seqs);
+    const WShape S{nh, nkv, dense_width, window, table_stride, n_pages, scale * 1.4426950408889634f};
     CUtensorMap mq, mk;
     int rc = make_map(&mq, q, (uint64_t)T_, (uint64_t)nh * hd, BM, "weigh8_prompt");
     if (!rc) rc = make_map(&mk, dense, (uint64_t)rows, (uint64_t)hd, PAGE, "weigh8_prompt");

@@ -33,7 +33,7 @@ MAX_HEAD_DIM = 256
 _PACKED = {"tq_write8": "12P11i", "tq_attention8": "12P13if", "tq_evict8": "8P9i"}        # members of the entry points' structs (_call.packed)
 _SIGNATURES = {              # argument types of the others (_call.declared)
     "tq_weigh8": "pppippp" "iiifpp" "iiiiii" "p", "tq_repair8": "pppppp" "iiifppi" "iiiii" "p",
-    "tq_expand8": "ppppp" "iiipppi" "iiii" "p", "tq_weigh8_prompt": "ppippp" "iifpp" "iiiiiii" "pp",
+    "tq_expand8": "ppppp" "iiipppii" "iiii" "p", "tq_weigh8_prompt": "ppippp" "iifpp" "iiiiiii" "pp",
     "tq_attention_prefill": "ppippp" "iiiiii" "ffpippp" "iiiiiii" "pp", "tq_attention_prefill_split": "ppppp" "iiiifpppp" "iiiiiiii" "pp",
 }
 _entries = {}
@@ -249,9 +249,10 @@ def attention8(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, cu_se
 # Steps whose longest run is at least this, and whose queries, heads, elements and the keys they see multiply to this much, go to the tensor-core
 # prompt kernel, where it takes their sizes.  (B200, us, csrc/attention8.cu and the prompt kernel's five launches: 128 rows behind 800, 16
 # heads of 128, 0.2e9: 19 and 31; 28 heads on 4, 0.4e9: 39 and 31; 64 behind 4,000, 16 heads, 0.5e9: 28 and 38; 128 behind 4,000, 1.1e9: 44 and 40;
-# 256 behind 4,000, 2.2e9: 119 and 46.)
+# 256 behind 4,000, 2.2e9: 119 and 46.)  A window is left out of the count: behind 30,000 with a window of 128, 64 rows, 16 heads: 14 and 23, 28 on 4: 30 and
+# 17; 512 rows: 103 and 31, 231 and 26.
 PROMPT_MIN_RUN, PROMPT_WORK = 48, 350_000_000
-DENSE_BYTES = 1 << 30        # scratch a step may take for pages in bfloat16; sequences beyond it follow in further launches
+DENSE_BYTES = 1 << 30        # scratch a step may take for pages in bfloat16 (or one sequence's, if they are more); sequences beyond it follow in further launches
 
 
 def _attention8_prompt(q, codes, scales, cu_seqlens, held, page_table, page_size, window, scale, out, n_heads, n_kv_heads, head_dim, max_q_len,
@@ -264,11 +265,12 @@ def _attention8_prompt(q, codes, scales, cu_seqlens, held, page_table, page_size
         q, out, codes, scales, cu_seqlens, held, page_table, weights, status)
     width = -(-max_kv_len // page_size)
     page_bytes = 2 * n_kv_heads * page_size * head_dim * 2
-    group = max(1, min(n, DENSE_BYTES // (page_bytes * width)))
+    dense_width = min(width, (window + max_q_len - 2) // page_size + 2) if window > 0 else width         # pages a sequence's rows see
+    group = max(1, min(n, DENSE_BYTES // (page_bytes * dense_width)))
     pieces, piece_pages = prefill_pieces(T, group, max_q_len, max_kv_len, n_heads, n_kv_heads, head_dim, window, _sms(q)) if scale > 0.0 else (1, 0)
     # one allocation: the pages, the rows' denominators and the pieces' results (float32), the page table (int32), the pages' marks (bytes)
     rows = T * n_heads
-    sizes = (group * width * page_bytes, 4 * rows if weights is not None else 0, 4 * rows * pieces * (head_dim + 1) if pieces > 1 else 0, 4 * group * width,
+    sizes = (group * dense_width * page_bytes, 4 * rows if weights is not None else 0, 4 * rows * pieces * (head_dim + 1) if pieces > 1 else 0, 4 * group * width,
              group * n_kv_heads * width)
     scratch = torch.empty(sum(sizes) + 64, dtype=torch.uint8, device=q.device)
     dense = scratch.data_ptr()
@@ -280,19 +282,19 @@ def _attention8_prompt(q, codes, scales, cu_seqlens, held, page_table, page_size
     for i in range(0, n, group):
         m, cu, starts, own = min(group, n - i), p_cu + 4 * i, p_held + 4 * i, p_table + 4 * i * columns
         cache = (p_codes, p_scales, cu, starts, own, columns, page_size, window)
-        check("prompt8", _prompt8("tq_expand8")(*cache, dense, tables, lost, width, pages, m, n_kv_heads, head_dim, at))
+        check("prompt8", _prompt8("tq_expand8")(*cache, dense, tables, lost, width, dense_width, pages, m, n_kv_heads, head_dim, at))
         if pieces > 1:
             check("attention_prefill", _attention_prefill("tq_attention_prefill_split")(
-                p_q, dense, cu, starts, tables, width, page_size, group * width, window, scale, p_out, p_lse, part, part + 4 * rows * pieces * head_dim,
+                p_q, dense, cu, starts, tables, width, page_size, group * dense_width, window, scale, p_out, p_lse, part, part + 4 * rows * pieces * head_dim,
                 pieces, piece_pages, T, m, max_q_len, n_heads, n_kv_heads, head_dim, p_status, at), kernels=2)
         else:
             check("attention_prefill", _attention_prefill("tq_attention_prefill")(
-                p_q, dense, 2, cu, starts, tables, width, page_size, group * width, window, 0, 0, scale, 0.0, 0, 0, 0, p_out, p_lse, T, m, max_q_len,
+                p_q, dense, 2, cu, starts, tables, width, page_size, group * dense_width, window, 0, 0, scale, 0.0, 0, 0, 0, p_out, p_lse, T, m, max_q_len,
                 n_heads, n_kv_heads, head_dim, head_dim, p_status, at))
         check("attention8", _attention8("tq_repair8")(p_q, *cache, scale, p_out, lost, width, pages, m, n_heads, n_kv_heads, head_dim, at))
         if weights is not None:
             check("prompt8", _prompt8("tq_weigh8_prompt")(
-                p_q, dense, width, cu, starts, own, columns, window, scale, p_lse, p_weights, pages, T, m, max_kv_len,
+                p_q, dense, dense_width, cu, starts, own, columns, window, scale, p_lse, p_weights, pages, T, m, max_kv_len,
                 n_heads, n_kv_heads, head_dim, p_status, at))
     return out
 
