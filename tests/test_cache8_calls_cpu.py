@@ -100,3 +100,14 @@ def test_a_plane_of_a_page_stays_below_two_to_the_31_codes(library, name, page_s
     assert getattr(cache8, f"_{library}")(name)(*members) != 0
     message = lib.tq_last_error()
     assert (b"codes a plane" in message) == (not fits) and (b"aligned" in message) == fits, message
+
+
+# ---- options --------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("options", [dict(cache_recent=16), dict(cache_dtype="e4m3", cache_recent=16), dict(cache_recent=-1), dict(cache_dtype="e4m3", cache_recent=1)])
+def test_newest_rows_without_a_budget_are_refused(options):
+    """`cache_recent` says how many of a budget's rows are the newest: without a budget it would do nothing."""
+    import turboquant_cpp_b200 as tq
+    from conftest import TINY_A
+    for make in (lambda m: tq.Model.from_model(m, **options), lambda m: tq.Engine(m, max_tokens=64, **options)):
+        with pytest.raises(ValueError, match="cache"):
+            make(tq.build_model(TINY_A, "bfloat16"))

@@ -159,7 +159,7 @@ class Engine:
         """Checks the cache's options against the model and tells its mixers."""
         if cache_dtype not in ("", "e4m3"):
             raise ValueError(f"cache_dtype '{cache_dtype}': '' (the run's type) or 'e4m3'")
-        if self.cache_budget < 0 or (self.cache_budget and not 0 <= self.cache_recent <= self.cache_budget):
+        if not 0 <= self.cache_recent <= self.cache_budget:                # (no budget: no newest rows of it)
             raise ValueError(f"a cache budget of {self.cache_budget} rows cannot keep the newest {self.cache_recent}")
         if self.cache_budget and not cache_dtype:
             raise ValueError("cache_budget needs a cache in 8 bits (cache_dtype='e4m3')")

@@ -64,7 +64,7 @@ class Model:
         ctx = int(context_length) if context_length and context_length > 0 else min(self._model.max_position, 4096)
         self.context_length = min(ctx, self._model.max_position)
         page = PAGE_SIZE
-        cache = dict(cache_dtype=cache_dtype, cache_budget=cache_budget, cache_recent=cache_recent) if cache_dtype or cache_budget else {}
+        cache = dict(cache_dtype=cache_dtype, cache_budget=cache_budget, cache_recent=cache_recent) if cache_dtype or cache_budget or cache_recent is not None else {}
         per_request = -(-self.context_length // page) * page
         self._engine = Engine(self._model, max_tokens=per_request * self.max_batch, max_slots=max(self.max_batch, 1),
                               device=device, **cache)
