@@ -111,3 +111,19 @@ def test_newest_rows_without_a_budget_are_refused(options):
     for make in (lambda m: tq.Model.from_model(m, **options), lambda m: tq.Engine(m, max_tokens=64, **options)):
         with pytest.raises(ValueError, match="cache"):
             make(tq.build_model(TINY_A, "bfloat16"))
+
+
+# ---- what the kernel ahead wrote ----------------------------------------------------------------------------------------------------
+def test_data_of_the_kernel_ahead_is_not_read_as_read_only():
+    """A kernel launched early may be resident while the kernel ahead still writes the queries, the codes and their bytes: for its lifetime they are not
+    read-only, which __ldg would claim.  (Queries come as `const __restrict__` parameters: those are renewed behind the wait.)"""
+    import os
+    import re
+
+    from conftest import ROOT
+    csrc = os.path.join(ROOT, "turboquant.cpp_b200", "csrc")
+    for name in ("cache8.cu", "cache8.cuh", "attention8.cu", "prompt8.cu", "evict.cu"):
+        text = open(os.path.join(csrc, name), encoding="utf-8").read()
+        assert not re.search(r"__ldg\s*\(", text), name
+        for m in re.finditer(r"__restrict__ q,[^{]*\{(.*?)\n\}\n", text, re.S):
+            assert "q = tq_fresh(q);" in m.group(1) or "tq_grid_wait()" not in m.group(1), (name, m.group(0)[:120])

@@ -100,7 +100,7 @@ template <int HDP> __device__ __forceinline__ int chunk_of(int j, int t) { retur
 // 80; 678 rows of 28 heads of 128 in float32 71 us, now 58).
 __device__ __forceinline__ void load4(float (&x)[4], const __nv_bfloat16* p, bool aligned) {
     if (aligned) {
-        const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
+        const uint2 v = *reinterpret_cast<const uint2*>(p);
         x[0] = __uint_as_float(v.x << 16); x[1] = __uint_as_float(v.x & 0xffff0000u);
         x[2] = __uint_as_float(v.y << 16); x[3] = __uint_as_float(v.y & 0xffff0000u);
     } else {
@@ -110,7 +110,7 @@ __device__ __forceinline__ void load4(float (&x)[4], const __nv_bfloat16* p, boo
 }
 __device__ __forceinline__ void load4(float (&x)[4], const float* p, bool aligned) {
     if (aligned) {
-        const float4 v = __ldg(reinterpret_cast<const float4*>(p));
+        const float4 v = *reinterpret_cast<const float4*>(p);
         x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
     } else {
 #pragma unroll
@@ -328,8 +328,8 @@ __device__ __forceinline__ void attend_tile(const Tile& T, int range, int ranges
             const uint8_t* k = codes_g + (size_t)(uint32_t)page * (2u * plane) + (uint32_t)(inner * (C8_BLOCK * hd));
             copy_block<F>(mine + slot * F::STAGE_BYTES, k, k + plane, hd);
             const uint8_t* b8 = scales_g + (size_t)(uint32_t)page * (2u * plane_scales) + inner;
-            kb = __ldg(b8);
-            vb = __ldg(b8 + plane_scales);
+            kb = *b8;
+            vb = b8[plane_scales];
             ask += WARPS;
             inner += WARPS;
             const int was = column;
@@ -643,6 +643,7 @@ __global__ void __launch_bounds__(WARPS * 32, F::PER_SM) attention8_kernel(const
                                                                                            float* __restrict__ partial, float* __restrict__ scores, int score_stride,
                                                                                            float* __restrict__ lse, float* __restrict__ weights, int ranges) {
     tq_grid_wait();                    // everything below may read what the previous kernel wrote
+    q = tq_fresh(q);
     tq_grid_launch_dependents();
     const int tile = blockIdx.x / ranges, tile_no = tile / c.nkv;
     const Tile T = tile_of(S, blockIdx.z, tile - tile_no * c.nkv, c.nkv, tile_no, F::NC);
@@ -655,6 +656,7 @@ template <class F>
 __global__ void __launch_bounds__(WARPS * 32) repair8_kernel(const typename F::TA* __restrict__ q, Cache8 c, Step S, typename F::TA* __restrict__ out,
                                                              const uint8_t* __restrict__ lost, int lost_stride, int page_size) {
     tq_grid_wait();                    // everything below may read what the previous kernel wrote
+    q = tq_fresh(q);
     tq_grid_launch_dependents();
     const int seq = blockIdx.z, g = blockIdx.y, start = S.held[seq], run = S.cu_seqlens[seq + 1] - S.cu_seqlens[seq];
     if (run <= 0) return;
@@ -774,7 +776,7 @@ __device__ __forceinline__ void load16(float (&x)[16], const __nv_bfloat16* p, b
     if (aligned) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const uint4 v = __ldg(reinterpret_cast<const uint4*>(p) + h);
+            const uint4 v = reinterpret_cast<const uint4*>(p)[h];
             const uint32_t u[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
             for (int e = 0; e < 4; ++e) { x[8 * h + 2 * e] = __uint_as_float(u[e] << 16); x[8 * h + 2 * e + 1] = __uint_as_float(u[e] & 0xffff0000u); }
@@ -788,7 +790,7 @@ __device__ __forceinline__ void load16(float (&x)[16], const float* p, bool alig
     if (aligned) {
 #pragma unroll
         for (int h = 0; h < 4; ++h) {
-            const float4 v = __ldg(reinterpret_cast<const float4*>(p) + h);
+            const float4 v = reinterpret_cast<const float4*>(p)[h];
             x[4 * h] = v.x; x[4 * h + 1] = v.y; x[4 * h + 2] = v.z; x[4 * h + 3] = v.w;
         }
     } else {
@@ -800,6 +802,7 @@ __device__ __forceinline__ void load16(float (&x)[16], const float* p, bool alig
 template <class F, int KB>
 __global__ void __launch_bounds__(WARPS * 32) weigh8_kernel(const typename F::TA* __restrict__ q, Cache8 c, Step S, const float* __restrict__ lse, float* __restrict__ weights) {
     tq_grid_wait();                    // everything below may read what the previous kernel wrote
+    q = tq_fresh(q);
     tq_grid_launch_dependents();
     using TA = typename F::TA;
     constexpr int KEYS = KB * C8_BLOCK;
@@ -826,7 +829,7 @@ __global__ void __launch_bounds__(WARPS * 32) weigh8_kernel(const typename F::TA
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const int at = chunk_of<F::HDP>(j, t) * 16;
-                kr[b][j][h] = there && at < hd ? __ldg(reinterpret_cast<const uint4*>(k + (g + 8 * h) * hd + at)) : make_uint4(0, 0, 0, 0);
+                kr[b][j][h] = there && at < hd ? *reinterpret_cast<const uint4*>(k + (g + 8 * h) * hd + at) : make_uint4(0, 0, 0, 0);
             }
         if (there) ks[b] = c8_scale(c.scales[c.scales_at(page, 0, gh) + row / C8_BLOCK]);
     }

@@ -50,8 +50,8 @@ __global__ void __launch_bounds__(256) expand8_kernel(Cache8 c, const int* __res
             x[k] = make_uint4(0, 0, 0, 0);
             s[k] = 1.f;
             if (i < 2 * pieces && r < rows) {
-                x[k] = __ldg(reinterpret_cast<const uint4*>(codes + plane * plane_codes) + j);
-                s[k] = c8_scale(__ldg(scales + plane * plane_scales + r / C8_BLOCK));
+                x[k] = __ldcg(reinterpret_cast<const uint4*>(codes + plane * plane_codes) + j);
+                s[k] = c8_scale(__ldcg(scales + plane * plane_scales + r / C8_BLOCK));
             }
         }
 #pragma unroll
