@@ -197,3 +197,50 @@ def _engine_options(model, dtype, budget, recent):
     e = Engine.__new__(Engine)
     e.cache_budget, e.cache_recent = budget, budget // 4 if recent is None else recent
     return e._cache_in_8_bits(model, dtype)
+
+
+def test_the_pages_set_aside_stay_as_many():
+    """Moves to fewer pages than are set aside, and of sequences that hold fewer than they move to: the next move still finds its pages."""
+    book = CacheBook([20], [0], page_size=64, max_slots=4)
+    book.keep_spare(256)                          # four pages
+    for length, rows in ((500, 64), (100, 100), (70, 256), (300, 130), (600, 256)):
+        seq = book.open()
+        book.reserve(seq, length)
+        book.commit(seq, length)
+        (pages,) = book.take_for_moves(1, rows)
+        book.moved(seq, pages, min(rows, length))
+        assert len(book.spare[0]) == 4 and seq.held == min(rows, length), (length, rows)
+        book.check_invariants()
+        book.close(seq)
+    assert book.pools[0].n_free == 16
+
+
+def test_an_eviction_that_fails_gives_its_pages_back(monkeypatch):
+    """Its sequences stay as they were: the old pages are only read."""
+    import numpy as np
+    from turboquant_cpp_b200.cache import paged
+    cache = PagedCache([KVNeed(1, 16)], [None], [None], 640, torch.bfloat16, "cpu", eight_bits=True, weights=True)
+    cache.book.keep_spare(64)
+    seq = cache.open()
+    cache.reserve([seq], [200])
+    cache.commit([seq], [200])
+    pages, free = [list(p) for p in seq.pages], cache.book.pools[0].n_free
+
+    def fails(*a):
+        raise RuntimeError("no")
+    monkeypatch.setattr(paged, "evict8", fails)
+    monkeypatch.setattr(torch.Tensor, "pin_memory", lambda t: t)
+    for seqs in ([seq], [seq, seq]):
+        with pytest.raises(RuntimeError, match="no"):
+            cache.evict(seqs, 64, 4)
+        assert seq.pages == pages and seq.held == 200 and len(cache.book.spare[0]) == 1 and cache.book.pools[0].n_free == free
+        cache.book.check_invariants()
+    kept = []
+    monkeypatch.setattr(paged, "evict8", lambda codes, scales, weights, lengths, *a: kept.append(lengths.tolist()))
+    short = cache.open()
+    cache.reserve([short], [64])
+    cache.commit([short], [64])
+    mine = [list(p) for p in short.pages]
+    cache.evict([short, seq], 64, 4)
+    assert kept == [[200]] and (seq.held, short.held) == (64, 64) and short.pages == mine        # within the budget: nothing to give up
+    cache.book.check_invariants()

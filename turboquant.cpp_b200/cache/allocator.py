@@ -88,6 +88,7 @@ class CacheBook:
         self.pools = [IndexPool(n, f"page of group {g}") for g, n in enumerate(n_pages)]
         self.slots = IndexPool(max_slots, "sequence slot")
         self.spare: List[List[int]] = [[] for _ in self.pools]      # pages no sequence holds, for moves (keep_spare)
+        self.n_spare = 0                                            # how many of each group there are between moves
         self._next_id = 0
         self.live: Dict[int, Sequence_] = {}
 
@@ -141,12 +142,12 @@ class CacheBook:
     # ---- eviction: a sequence's rows move to other pages, and there are fewer of them --------------
     def keep_spare(self, rows: int) -> None:
         """Sets pages for `rows` rows aside in every group, so that one sequence can always be moved."""
-        per = -(-int(rows) // self.page_size)
-        self.spare = [pool.take_many(per) for pool in self.pools]
+        self.n_spare = -(-int(rows) // self.page_size)
+        self.spare = [pool.take_many(self.n_spare) for pool in self.pools]
 
     def take_for_moves(self, n: int, rows: int) -> List[List[List[int]]]:
         """New pages for `rows` rows each of up to n sequences (as many as the free pages allow, at least one): per sequence, per group.
-        Follow with `moved` for each of them."""
+        Follow with `moved` for each of them, or with `not_moved`."""
         per = -(-int(rows) // self.page_size)
         if any(len(s) < per for s in self.spare):
             raise CacheMisuse(f"no pages for {rows} rows are set aside")
@@ -160,15 +161,24 @@ class CacheBook:
     def moved(self, seq: Sequence_, pages: List[List[int]], rows: int) -> None:
         """The sequence now holds `rows` rows, on these pages; its old ones are set aside again or free."""
         self._check_open(seq)
-        per = len(pages[0]) if pages else 0
         for g, new in enumerate(pages):
-            for p in seq.pages[g]:
-                if len(self.spare[g]) < per:
-                    self.spare[g].append(p)
-                else:
-                    self.pools[g].give_back(p)
+            self._give_back(g, seq.pages[g])
             seq.pages[g] = list(new)
         seq.evicted = seq.length - rows
+
+    def not_moved(self, pages: List[List[int]]) -> None:
+        """Pages of `take_for_moves` that no sequence moved to are set aside again or free."""
+        for g, back in enumerate(pages):
+            self._give_back(g, back)
+
+    def _give_back(self, g: int, pages: List[int]) -> None:
+        for p in pages:
+            if len(self.spare[g]) < self.n_spare:
+                self.spare[g].append(p)
+            else:
+                self.pools[g].give_back(p)
+        # (a sequence of fewer pages than it moved to)
+        self.spare[g] += self.pools[g].take_many(min(self.n_spare - len(self.spare[g]), self.pools[g].n_free))
 
     def close(self, seq: Sequence_) -> None:
         self._check_open(seq)

@@ -144,20 +144,29 @@ class PagedCache:
 
     # ---- eviction -------------------------------------------------------------------------------
     def evict(self, seqs: Sequence[Sequence_], budget: int, recent: int) -> None:
-        """The sequences keep `budget` rows in every key/value head of every layer (kernels.cache8.evict8), on pages of their own."""
-        todo = list(seqs)
+        """The sequences that hold more than `budget` rows keep that many in every key/value head of every layer (kernels.cache8.evict8), on pages of
+        their own.  An error leaves those that were not done as they were."""
+        todo = [s for s in seqs if s.held > budget]
         while todo:
             moves = self.book.take_for_moves(len(todo), budget)
             now, todo = todo[:len(moves)], todo[len(moves):]
-            tables = self.page_tables(now)
-            fields = [np.array([s.held for s in now], dtype=np.int32)] + tables + [np.array([m[g] for m in moves], dtype=np.int32) for g in range(len(self.groups))]
-            sizes = [f.size for f in fields]
-            parts = torch.split(torch.from_numpy(np.concatenate([f.reshape(-1) for f in fields])).pin_memory().to(self.device, non_blocking=True), sizes)
-            for i, codes in enumerate(self.kv):
-                if codes is None or self.cache_of[i] is not None:
-                    continue
-                g = self.entry_group[i]
-                evict8(codes, self.scales[i], self.weights[i], parts[0], parts[1 + g].view(tables[g].shape),
-                       parts[1 + len(self.groups) + g].view(len(now), -1), self.page_size, budget, recent)
+            try:
+                self._evict_to(now, moves, budget, recent)
+            except BaseException:
+                for m in moves:
+                    self.book.not_moved(m)
+                raise
             for s, m in zip(now, moves):
-                self.book.moved(s, m, min(s.held, budget))
+                self.book.moved(s, m, budget)
+
+    def _evict_to(self, now: Sequence[Sequence_], moves, budget: int, recent: int) -> None:
+        tables = self.page_tables(now)
+        fields = [np.array([s.held for s in now], dtype=np.int32)] + tables + [np.array([m[g] for m in moves], dtype=np.int32) for g in range(len(self.groups))]
+        sizes = [f.size for f in fields]
+        parts = torch.split(torch.from_numpy(np.concatenate([f.reshape(-1) for f in fields])).pin_memory().to(self.device, non_blocking=True), sizes)
+        for i, codes in enumerate(self.kv):
+            if codes is None or self.cache_of[i] is not None:
+                continue
+            g = self.entry_group[i]
+            evict8(codes, self.scales[i], self.weights[i], parts[0], parts[1 + g].view(tables[g].shape),
+                   parts[1 + len(self.groups) + g].view(len(now), -1), self.page_size, budget, recent)
