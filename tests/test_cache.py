@@ -244,3 +244,10 @@ def test_an_eviction_that_fails_gives_its_pages_back(monkeypatch):
     cache.evict([short, seq], 64, 4)
     assert kept == [[200]] and (seq.held, short.held) == (64, 64) and short.pages == mine        # within the budget: nothing to give up
     cache.book.check_invariants()
+
+
+def test_bytes_of_a_token_where_groups_have_pages_of_their_own():
+    """An 8-bit row's scales and sums count by the pages of their own group."""
+    near, far = KVNeed(2, 32, window=64), KVNeed(4, 16)
+    cache = PagedCache([near, far], [None, None], [None, None], 640, torch.bfloat16, "cpu", pages_per_group={near: 2, far: 40}, eight_bits=True, weights=True)
+    assert cache.bytes_per_token() == 2 * 2 * 32 + 2 * 4 * 16 + -(-2 * (2 + 4) // 16) + 4 * (2 + 4)

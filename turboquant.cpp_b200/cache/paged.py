@@ -26,7 +26,7 @@ from typing import Dict, List, Optional, Sequence, Tuple
 import numpy as np
 import torch
 
-from ..kernels.cache8 import evict8, storage as storage8
+from ..kernels.cache8 import BLOCK, evict8, storage as storage8
 from ..parts.base import KVNeed, LayerCache, StateNeed
 from .allocator import CacheBook, CacheFull, Sequence_
 
@@ -138,9 +138,11 @@ class PagedCache:
     def bytes_per_token(self) -> int:
         """Key/value bytes one token adds across all layers that keep a cache."""
         own = [i for i, t in enumerate(self.kv) if t is not None and self.cache_of[i] is None]
-        side = sum(t.numel() * t.element_size() for i in own for t in (self.scales[i], self.weights[i]) if t is not None)
-        tokens = self.kv[own[0]].shape[0] * self.page_size if own else 1
-        return sum(self.kv[i].shape[1] * self.kv[i].shape[2] * self.kv[i].shape[4] * self.kv[i].element_size() for i in own) + -(-side // tokens)
+        rows = sum(self.kv[i].shape[1] * self.kv[i].shape[2] * self.kv[i].shape[4] * self.kv[i].element_size() for i in own)
+        if not self.eight_bits:
+            return rows
+        scales = sum(2 * self.kv[i].shape[2] for i in own)                      # a byte each for BLOCK rows
+        return rows + -(-scales // BLOCK) + sum(4 * self.kv[i].shape[2] for i in own if self.weights[i] is not None)
 
     # ---- eviction -------------------------------------------------------------------------------
     def evict(self, seqs: Sequence[Sequence_], budget: int, recent: int) -> None:
