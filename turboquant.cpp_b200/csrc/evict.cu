@@ -204,9 +204,10 @@ __global__ void __launch_bounds__(256) evict8_move_kernel(Cache8 c, float* __res
     if (first >= budget) return;
     const int* list = kept + ((size_t)seq * c.nkv + g) * budget;
     const int place = first + r < budget ? list[first + r] : -1;
-    const int page = TQ_CHECKED(new_table[(size_t)seq * new_stride + TQ_CHECKED(c.column(first), new_stride, TQ_IDX_TABLE_COLUMN)], c.n_pages, TQ_IDX_PAGE);
+    const int listed = new_table[(size_t)seq * new_stride + TQ_CHECKED(c.column(first), new_stride, TQ_IDX_TABLE_COLUMN)];
     const int rows = __popc(__ballot_sync(0xffffffffu, place >= 0) & 0xffffu), row0 = c.row(first), hd = HD ? HD : c.hd, vecs = hd / 16;
-    if (rows == 0) return;                                            // the list ends before these
+    if (rows == 0) return;                                            // the list ends before these: they need no page
+    const int page = TQ_CHECKED(listed, c.n_pages, TQ_IDX_PAGE);
     unsigned long long from = 0;
     uint32_t byte = 0;
     float weight = 0.f;
