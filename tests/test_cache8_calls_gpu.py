@@ -224,3 +224,32 @@ def test_a_windowed_prompt_expands_the_pages_it_sees(shape, runs, held, window, 
         plain.add_weights(want_w, p, runs, held, table, 64, H, G)
         rel = float(2.02 * ((D + 8) * 4 * U * units).max()) + (longest + H // G * max(runs) + 16) * 4 * U
         assert bool(((w.cpu().double() - want_w).abs() <= rel * want_w.abs() + 1e-30).all())
+
+
+# ---- plans for longer sequences than there are -----------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("shape", [(16, 16, 128), (28, 4, 128), (8, 2, 64), (40, 2, 64), (3, 1, 256)], ids=str)
+@pytest.mark.parametrize("longest", [1024, 8192, 40000])
+@pytest.mark.parametrize("with_weights", [False, True])
+def test_steps_planned_for_the_longest_sequence_there_could_be(dtype, shape, longest, with_weights):
+    """As captured steps are: page tables and ranges for `longest` places, sequences that hold from none to some hundred, one that brings nothing."""
+    from turboquant_cpp_b200.kernels import cache8
+    (H, G, D), runs, held = shape, [1, 1, 0, 1, 1], [700, 0, 30, 63, 64]
+    narrow, pages = _pages([n + h for n, h in zip(runs, held)], 64)
+    table = torch.full((len(runs), longest // 64), -1, dtype=torch.int32)
+    table[:, :narrow.shape[1]] = narrow
+    codes, scales = _cache(pages, G, 64, D)
+    q, scale = (torch.randn(sum(runs), H, D) * 1.5).to(dtype), 1.0 / math.sqrt(D) / 4
+    weights = torch.rand(pages, G, 64)
+    out, w = torch.full((sum(runs), H * D), float("nan"), dtype=dtype, device=DEV), weights.to(DEV) if with_weights else None
+    cache8.attention8(q.to(DEV), _on(codes), scales.to(DEV), _cu(runs), _i(held), table.to(DEV), 64, 0, scale, out, H, G, D, 1, longest, weights=w)
+    want, mags, units, p = plain.attention(q, codes, scales, runs, held, narrow, 64, 0, scale, H, G, D)
+    top = float((codes.view(torch.float8_e4m3fn).float().abs() * torch.pow(2.0, scales.float() - 127).repeat_interleave(16, -1)[..., None]).max())
+    limit = _limit(dtype, want, mags, units, D, max(held) + 1, top)
+    off = (out.cpu().double().view(want.shape) - want).abs()
+    assert bool((off <= limit).all()), float((off / limit).max())
+    if with_weights:
+        want_w = weights.double()
+        plain.add_weights(want_w, p, runs, held, narrow, 64, H, G)
+        rel = float(2.02 * ((D + 8) * 4 * U * units).max()) + (max(held) + 1 + H // G + 16) * 4 * U
+        assert bool(((w.cpu().double() - want_w).abs() <= rel * want_w.abs() + 1e-30).all())
