@@ -253,3 +253,77 @@ def test_steps_planned_for_the_longest_sequence_there_could_be(dtype, shape, lon
         plain.add_weights(want_w, p, runs, held, narrow, 64, H, G)
         rel = float(2.02 * ((D + 8) * 4 * U * units).max()) + (max(held) + 1 + H // G + 16) * 4 * U
         assert bool(((w.cpu().double() - want_w).abs() <= rel * want_w.abs() + 1e-30).all())
+
+
+# ---- scales and queries out of the ordinary ---------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("runs,held", [([1, 1], [200, 30]), ([60, 3], [100, 500])])
+@pytest.mark.parametrize("scale", [-0.05, 0.0, 1e-30])
+def test_scales_of_any_sign(dtype, runs, held, scale, monkeypatch):
+    from turboquant_cpp_b200.kernels import cache8
+    monkeypatch.setattr(cache8, "PROMPT_WORK", 0)
+    H, G, D = 8, 2, 64
+    table, pages = _pages([n + h for n, h in zip(runs, held)], 64)
+    codes, scales = _cache(pages, G, 64, D, spread=1.0)
+    q, weights = torch.randn(sum(runs), H, D).to(dtype), torch.rand(pages, G, 64)
+    want, mags, units, p = plain.attention(q, codes, scales, runs, held, table, 64, 0, scale, H, G, D)
+    want_w = weights.double()
+    plain.add_weights(want_w, p, runs, held, table, 64, H, G)
+    got, got_w = _attend(q, codes, scales, runs, held, table, 64, 0, scale, H, G, D, weights)
+    places = max(n + h for n, h in zip(runs, held))
+    top = float((codes.view(torch.float8_e4m3fn).float().abs() * torch.pow(2.0, scales.float() - 127).repeat_interleave(16, -1)[..., None]).max())
+    limit = _limit(dtype, want, mags, units, D, places, top)
+    assert bool(((got.double().view(want.shape) - want).abs() <= limit).all())
+    rel = float(2.02 * ((D + 8) * 4 * U * units).max()) + (places + H // G * max(runs) + 16) * 4 * U
+    assert bool(((got_w.double() - want_w).abs() <= rel * want_w.abs() + 1e-30).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("runs,held", [([1, 1], [200, 30]), ([60, 3], [100, 500])])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_a_query_that_is_not_finite_is_its_rows_and_heads_alone(dtype, runs, held, bad, monkeypatch):
+    from turboquant_cpp_b200.kernels import cache8
+    monkeypatch.setattr(cache8, "PROMPT_WORK", 0)
+    H, G, D = 8, 2, 64
+    table, pages = _pages([n + h for n, h in zip(runs, held)], 64)
+    codes, scales = _cache(pages, G, 64, D, spread=1.0)
+    q = torch.randn(sum(runs), H, D).to(dtype)
+    want, _ = _attend(q, codes, scales, runs, held, table, 64, 0, 0.1, H, G, D)
+    q[0, 3, 7] = bad
+    got, _ = _attend(q, codes, scales, runs, held, table, 64, 0, 0.1, H, G, D)
+    want, got = want.view(-1, H, D), got.view(-1, H, D)
+    others = torch.ones(want.shape[:2], dtype=torch.bool)
+    others[0, 3] = False
+    assert torch.equal(got[others], want[others])
+    assert math.isinf(bad) or bool(torch.isnan(got[0, 3]).all())
+
+
+# ---- pools of more than 2^32 codes -------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("runs,held", [([1, 1], [300, 64]), ([70, 3], [300, 64])])
+def test_pages_behind_the_first_four_gigabytes(runs, held, monkeypatch):
+    """A pool of 4.7 GB: sequences on its last pages get the bits they get on a small one's; its first pages stay as they are."""
+    from turboquant_cpp_b200.kernels import cache8
+    monkeypatch.setattr(cache8, "PROMPT_WORK", 0)
+    H, G, D, budget = 16, 16, 128, 100
+    T, rows = sum(runs), [n + h for n, h in zip(runs, held)]
+    table, pages = _pages(rows, 64, spare=4)
+    new = torch.tensor([p for p in range(pages) if p not in table.flatten().tolist()], dtype=torch.int32)[:4].view(2, 2)
+    codes, scales = _cache(pages, G, 64, D, spread=1.0)
+    qkv, w0 = torch.randn(T, (H + 2 * G) * D).to(torch.bfloat16).to(DEV), torch.rand(pages, G, 64)
+    seen = []
+    for before in (0, 18000):
+        c, s, w = cache8.storage(before + pages, G, 64, D, DEV, weights=True)
+        c[before:].view(torch.uint8).copy_(codes)
+        s[before:].copy_(scales)
+        w[before:].copy_(w0)
+        on = lambda t: torch.where(t >= 0, t + before, t).to(torch.int32).to(DEV)
+        q, out = torch.empty(T, H, D, dtype=torch.bfloat16, device=DEV), torch.empty(T, H * D, dtype=torch.bfloat16, device=DEV)
+        cu, h = _cu(runs), _i(held)
+        cache8.write_rows8(qkv, None, None, None, "half", torch.zeros(T, dtype=torch.int32, device=DEV), cu, h, on(table), 64, q, c, s, H, G, D, max(runs))
+        cache8.attention8(q, c, s, cu, h, on(table), 64, 0, 0.08, out, H, G, D, max(runs), max(rows), weights=w)
+        kept = cache8.evict8(c, s, w, _i(rows), on(table), on(new), 64, budget, 8)
+        seen.append([t.clone() for t in (q, out, c[before:].view(torch.uint8), s[before:], w[before:], kept)])
+        assert not bool(w[:before].any()) and not bool(c[:before].view(torch.uint8).any()) and bool((s[:before] == 1).all())
+        del c, s, w
+    for a, b in zip(*seen):
+        assert torch.equal(a, b)
