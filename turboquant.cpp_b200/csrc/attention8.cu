@@ -1,14 +1,15 @@
 // Attention over the 8-bit cache (layout and codes: cache8.cuh) for single tokens, short runs and every type and head size.
 //
-//   tq_attention8   softmax(scale q.K) V, causal, with an optional window, the keys of a row cut into ranges that a second launch joins
+//   tq_attention8   softmax(scale q.K) V, causal, with an optional window, the keys of a row cut into ranges: up to 8 join as a cluster, more in a
+//                   second launch
 //   tq_weigh8       sums of softmax weights: what each cached row received from a step's rows and its key/value head's query heads
 //
 // A CTA takes one key/value head of one sequence, a tile of 8 or 16 columns (query heads of one row, or of several rows of the run) and a range
-// of the keys; its four warps take blocks of 16 keys in turn.  Both products run on mma.sync with the cache as the left operand, straight
-// from global memory to registers: a lane's 16 bytes of a key row are its share of four steps of S = K q (which element goes to which place
-// of a sum does not matter as long as the queries lie the same way), and its 16 bytes of four value rows, interleaved two rows at a time by
-// byte permutes, its share of eight steps of O = V^T p.  No byte of the cache passes through shared memory.  Codes become float16 exactly
-// (one conversion for two); so the queries are float16 as well, scaled per row by a power of two (bfloat16 ones are then exact down to
+// of the keys; its four warps take blocks of 16 keys in turn, each through a ring of its own in shared memory that cp.async fills two blocks ahead (in
+// tq_weigh8 keys go straight to registers).  Both products run on mma.sync with the cache as the left operand: a lane's 16 bytes of a key row are its
+// share of four steps of S = K q (which element goes to which place of a sum does not matter as long as the queries lie the same way), and its
+// 16 bytes of four value rows, interleaved two rows at a time by byte permutes, its share of eight steps of O = V^T p.  Codes become float16
+// exactly (one conversion for two); so the queries are float16 as well, scaled per row by a power of two (bfloat16 ones are then exact down to
 // 2^-24 of half the row's largest), float32 ones as two parts of 11 bits each.
 //
 // A block's two bytes are uniform over its 16 keys.  The key's scale goes into the factor that makes a sum a score.  The value's cannot go
@@ -302,7 +303,7 @@ __device__ __forceinline__ void attend_tile(const Tile& T, int range, int ranges
     constexpr int NT = F::NT, NC = F::NC, MT = F::MT, HDP = F::HDP;
     extern __shared__ __align__(16) uint8_t ring[];
     __shared__ Queries<F> Q;
-    __shared__ float s_stat[WARPS][NC][3], s_ranks[CLUSTERED ? CLUSTER : 1][NC][3], s_part[CLUSTERED ? CLUSTER : 1][NC], s_norm[NC], s_lse[NC];
+    __shared__ float s_stat[WARPS][NC][3], s_ranks[CLUSTERED ? CLUSTER : 1][NC][3], s_lse[NC];
     float (*s_o)[NC][HDP + 4] = reinterpret_cast<float (*)[NC][HDP + 4]>(ring);        // [WARPS], once the keys are through
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, hd = F::EXACT ? HDP : c.hd;
     // this range's blocks of 16 keys
@@ -583,7 +584,7 @@ __device__ __forceinline__ void attend_tile(const Tile& T, int range, int ranges
     }
     if (!CLUSTERED) return;
     __syncwarp();
-    // the cluster's sums together: statistics of all ranges first (a warp a column, a lane a range), then every CTA its part of the tile's results
+    // the cluster's sums together: statistics of all ranges first, then every CTA its part of the tile's results
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
     auto remote = [](const float* own, int rank) {
         uint32_t a;
@@ -592,38 +593,55 @@ __device__ __forceinline__ void attend_tile(const Tile& T, int range, int ranges
         asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
         return v;
     };
+    // (a thread's first element of every range is asked for beside the statistics, whose way is as long: one chat of 700 rows in 6 ranges 6.2 us, one
+    // behind the other 6.8)
+    const int element0 = range * WARPS * 32 + (int)threadIdx.x;
+    float v[CLUSTER];
+    auto fetch = [&](int i) {
+#pragma unroll
+        for (int r = 0; r < CLUSTER; ++r) v[r] = r < ranges ? remote(&s_o[0][i / hd][i % hd], r) : 0.f;
+    };
+    if (element0 < T.n * hd) fetch(element0);
     for (int i = threadIdx.x; i < ranges * NC * 3; i += WARPS * 32)
         if (i / 3 % NC < T.n) (&s_ranks[0][0][0])[i] = remote(&s_stat[0][0][0] + i % (NC * 3), i / (NC * 3));
     __syncthreads();
-    for (int col = warp; col < T.n; col += WARPS) {
-        const bool mine = lane < ranges;                               // the lane's range
-        const float mor = mine ? s_ranks[lane][col][0] : LOWEST, mr = mine ? s_ranks[lane][col][1] : LOWEST, lr = mine ? s_ranks[lane][col][2] : 0.f;
-        float M = mr;
+    // a column's denominator and, for each range, the factor of its sums
+    auto join = [&](int col, float (&factors)[CLUSTER], float& MO, float& log_sum) {
+        float M = LOWEST, L = 0.f;
+        MO = LOWEST;
 #pragma unroll
-        for (int x = 1; x < CLUSTER; x <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
-        const float below = mr - M;
-        float MO = below + mor, L = lr * exp2f(below);
+        for (int r = 0; r < CLUSTER; ++r) if (r < ranges) M = fmaxf(M, s_ranks[r][col][1]);
 #pragma unroll
-        for (int x = 1; x < CLUSTER; x <<= 1) {
-            MO = fmaxf(MO, __shfl_xor_sync(0xffffffffu, MO, x));
-            L += __shfl_xor_sync(0xffffffffu, L, x);
+        for (int r = 0; r < CLUSTER; ++r) {
+            factors[r] = LOWEST;
+            if (r >= ranges) continue;
+            const float below = s_ranks[r][col][1] - M;
+            factors[r] = below + s_ranks[r][col][0];
+            MO = fmaxf(MO, factors[r]);
+            L += s_ranks[r][col][2] * ex2(below);
         }
-        if (lane < ranges) s_part[lane][col] = exp2f(below + mor - MO);
-        if (lane == 0) {
-            s_norm[col] = exp2f(MO) / L;
-            s_lse[col] = M + log2f(L);
-            if (lse != nullptr && range == 0) lse[Q.row[col]] = M + log2f(L);
-        }
-    }
-    __syncthreads();
-    for (int i = range * WARPS * 32 + threadIdx.x; i < T.n * hd; i += ranges * WARPS * 32) {
+#pragma unroll
+        for (int r = 0; r < CLUSTER; ++r) factors[r] = ex2(factors[r] - MO);
+        log_sum = M + log2f(L);
+        return L;
+    };
+    float factors[CLUSTER], MO, log_sum;
+    for (int i = element0; i < T.n * hd; i += ranges * WARPS * 32) {
         const int col = i / hd, d = i - col * hd;
+        if (i != element0) fetch(i);
+        const float L = join(col, factors, MO, log_sum);
         float sum = 0.f;
-#pragma unroll 8
-        for (int r = 0; r < ranges; ++r) sum += remote(&s_o[0][col][d], r) * s_part[r][col];
-        out[Q.row[col] * hd + d] = tq_from_float<typename F::TA>(sum * WEIGHT_DOWN * s_norm[col]);
+#pragma unroll
+        for (int r = 0; r < CLUSTER; ++r) sum += v[r] * factors[r];
+        out[Q.row[col] * hd + d] = tq_from_float<typename F::TA>(sum * WEIGHT_DOWN * (exp2f(MO) / L));
+        if (lse != nullptr && d == 0) lse[Q.row[col]] = log_sum;
     }
     if (weights != nullptr) {
+        if (threadIdx.x < T.n) {
+            join(threadIdx.x, factors, MO, log_sum);
+            s_lse[threadIdx.x] = log_sum;
+        }
+        __syncthreads();
         // (the step has one row of the sequence: it sees up to its own place)
         const int last = min(min(to * C8_BLOCK, place1 + 1), score_stride);
 #pragma unroll 2
@@ -979,9 +997,9 @@ int check_step(const char* what, int nh, int nkv, int n_seqs, int longest, int w
 
 // q [T, nh, hd], out [T, nh * hd]; place i sees j <= i with window == 0 or i - j < window.  max_q_len: the longest run.  ranges > 1: the keys
 // of a row are cut into that many ranges, which join as a cluster (up to 8; partial null) or in a second launch (up to 64; partial
-// [T * nh * ranges * (hd + 4)]).  lse [T, nh] float32 or null.  scores [T * nh, score_stride] with weights [n_pages, nkv, page_size], or both
-// null: the weights of a step of single rows are added up by whoever joins, so by clusters only of all of a key/value head's query heads, and of
-// two ranges or more.  scores: [n_seqs * nkv, score_stride, score_columns(nh / nkv)], score_stride at least max_kv_len, the longest held[s] + run.
+// [T * nh * ranges * (hd + 4)]).  lse [T, nh] float32 or null.  scores [n_seqs * nkv, score_stride, score_columns(nh / nkv)] with weights [n_pages,
+// nkv, page_size], or both null: the weights of a step of single rows are added up by whoever joins, so by clusters only of all of a key/value
+// head's query heads, and of two ranges or more.  score_stride: at least max_kv_len, the longest held[s] + run.
 struct Attention8Call {
     const void *q, *codes, *scales;
     const int *cu_seqlens, *held, *page_table;
