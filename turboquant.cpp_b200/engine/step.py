@@ -107,7 +107,8 @@ class Engine:
         """cache_dtype: "e4m3" keeps keys and values in 8 bits with a scale per 16 rows (kernels.cache8; models whose layers are all
         plain attention), "" in the run's own type.  cache_budget > 0 (8-bit caches without windows): after a step, sequences that
         hold `cache_budget` rows and a page more go back to that many, in every key/value head the last cache_recent (default a
-        quarter) and those that received the most attention; steps are then not launched ahead of their tokens.
+        quarter) and those that received the most attention; steps are then not launched ahead of their tokens.  The budget bounds what
+        sequences come to hold, not the pool: max_tokens does that, and has to have room for whole prompts.
         record_routing: decode steps captured into CUDA graphs keep what the parts record into the step's
         `debug` (the experts chosen) in memory of the graph, so that setting `engine.debug = {}` before a step
         fills it from the very launches that generation replays; without it, a step with `debug` set runs

@@ -158,8 +158,10 @@ SETUP, CLUSTER_JOIN, JOIN = 1.5, 1.0, 6.0
 @lru_cache(maxsize=4096)
 def ranges_for(tiles: int, blocks: int, resident: int) -> int:
     """Ranges the keys of a tile of columns are cut into, where the device runs `resident` CTAs at once and a CTA's four warps take a block of 16
-    keys each in turn: the count with the fewest turns.  (B200, 16 heads of 128, 64 sequences of up to 2,048 keys, 1,024 tiles: one
-    range 86 us, two 97, three 95, four 99.)"""
+    keys each in turn: the count with the fewest turns.  (B200, device time, 16 heads of 128, 64 sequences of up to 2,048 keys, 1,024 tiles: one
+    range 80 us, two 94, three 100, four 108.)  `blocks` is what the call says its longest sequence holds: a captured step says the longest there could be and
+    is cut for that (these 64 planned for 8,192 keys: four ranges, 108 us; one of 700 rows 9.6 us where 6 ranges take 6.2; 32 of
+    4,096 rows, seven query heads on a key/value head, with sums: no difference)."""
     turns = lambda n: -(-tiles * n // resident) * (-(-blocks // (4 * n)) + SETUP) + (0.0 if n == 1 else CLUSTER_JOIN if n <= CLUSTER else JOIN)
     most = max(1, min(MAX_RANGES, blocks // 4, max(CLUSTER, resident // tiles)))
     return min((n for n in (1, 2, 3, 4, 5, 6, 7, 8, 12, 16, 24, 32, 48, most) if n <= most), key=lambda n: (turns(n), n))
@@ -185,7 +187,8 @@ def attention8(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, cu_se
                status: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Causal attention of the step's queries q [T, nh, hd] over the pages (the step's own rows are in them already): a row sees its
     sequence's places up to its own (window > 0: the last `window` of them), scores times `scale`; out [T, nh * hd] in q's type.
-    max_q_len: the longest run; max_kv_len: at least the longest held + run.
+    max_q_len: the longest run; max_kv_len: at least the longest held + run.  Large steps of bfloat16 with heads of 64 or 128 take scratch for the pages
+    they see in bfloat16: up to DENSE_BYTES, or one sequence's.
     weights: the softmax weights that each cached row receives from the step's rows, summed over a key/value head's query heads, are
     added to its sum; the sums of the step's own rows start with this step.
     status: the word in which the prompt kernel reports a wait that ran out (default: the device's, kernels.gemm_tc)."""

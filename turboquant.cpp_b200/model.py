@@ -36,7 +36,8 @@ class Model:
         here) leaves the logits alone.  detect_loops ends a request when its last four tokens have come up three
         times among the 64 draws before, as the reference always does (src/engine/tq_generate.c:610-630).
         cache_dtype="e4m3" keeps keys and values in 8 bits; cache_budget > 0 bounds the rows a request keeps of them, cache_recent of
-        which are its newest (engine.Engine; models whose layers are all plain attention)."""
+        which are its newest (engine.Engine; models whose layers are all plain attention).  A request holds its whole prompt for one step, then up to
+        the budget and a page; the cache is sized as without a budget."""
         if not os.path.isdir(path):
             raise FileNotFoundError(f"model folder '{path}' does not exist")
         self._setup(load_model(path, dtype, device), path, temperature, top_p, max_tokens, context_length, seed,

@@ -120,7 +120,7 @@ class AttentionMixer(Mixer):
                            cache.kv if cache.writes else None, cache.scales if cache.writes else None, self.n_heads, self.n_kv_heads, self.head_dim, ctx.max_q_len)
             o = K8.attention8(q, cache.kv, cache.scales, ctx.cu_seqlens, held, cache.page_table, cache.page_size, self.window, self.scale,
                               torch.empty((T, self.q_size), dtype=act, device=xn.device), self.n_heads, self.n_kv_heads, self.head_dim, ctx.max_q_len,
-                              min(ctx.max_kv_len, cache.page_table.shape[1] * cache.page_size),       # positions may exceed the rows that are held
+                              min(ctx.max_kv_len, cache.page_table.shape[1] * cache.page_size),       # the rows' places, where positions go further (captured steps: as wide as the tables)
                               weights=cache.weights, status=ctx.status)
             return self._project(o, T, ctx)
         KA.qkv_rope_cache(qkv, bias, cos, sin, pairing, ctx.positions, ctx.seq_of_token, cache.page_table,
