@@ -63,7 +63,7 @@ def main(argv=None) -> int:
     ap.add_argument("--detect-loops", action="store_true",
                     help="end a request whose last four tokens have come up three times before (the reference always does)")
     ap.add_argument("--cache", choices=["e4m3"], default="", help="keep keys and values in 8 bits with a scale per 16 rows")
-    ap.add_argument("--cache-budget", type=int, default=0, help="most rows a request keeps of an 8-bit cache, by the attention they received (0: all)")
+    ap.add_argument("--cache-budget", type=int, default=0, help="rows a request goes back to in an 8-bit cache, by the attention they received, once it holds a page more (0: all)")
     ap.add_argument("--cache-recent", type=int, default=None, help="of those, the newest (default: a quarter)")
     ap.add_argument("--info", action="store_true")
     ap.add_argument("--profile", action="store_true")
